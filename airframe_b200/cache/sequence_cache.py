@@ -59,9 +59,13 @@ class KVGroup:
         self.held = [[] for _ in range(n_slots)]        # slot -> its pages, in row order
         self.table_host = torch.full((n_slots, self.pages_per_seq), -1, dtype=torch.int32)
         self.dirty = set()
-        self.k = self.v = self.table = None
+        self.k = self.v = self.table = self.k_exp = self.v_exp = None
         if device is not None:
             shape = (len(self.run_ids), n_pages, need.num_kv_heads, PAGE)
+            if need.eight_bits:
+                dtype = torch.float8_e4m3fn
+                self.k_exp = torch.zeros(shape, dtype=torch.uint8, device=device)
+                self.v_exp = torch.zeros(shape, dtype=torch.uint8, device=device)
             self.k = torch.zeros((*shape, need.head_dim), dtype=dtype, device=device)
             if need.value_size:        # (0: the values lie inside the key rows)
                 self.v = torch.zeros((*shape, need.value_size), dtype=dtype, device=device)
@@ -114,8 +118,9 @@ class KVGroup:
         self.dirty.clear()
 
     def bytes_per_token(self) -> int:
-        el = 2 if self.k is None else self.k.element_size()
-        return len(self.run_ids) * self.need.num_kv_heads * (self.need.head_dim + self.need.value_size) * el
+        el = (1 if self.need.eight_bits else 2) if self.k is None else self.k.element_size()
+        row = (self.need.head_dim + self.need.value_size) * el + (2 if self.need.eight_bits else 0)      # (an exponent a row)
+        return len(self.run_ids) * self.need.num_kv_heads * row
 
 
 @dataclass
@@ -127,6 +132,8 @@ class KVView:
     ring_rows: int                      # 0: rows are positions; else rows behind the kept pages are a ring of this many
     need: KVNeed
     keep_first: int = 0                 # the first tokens that stay beside a window: their pages come before the ring
+    k_exp: Optional[torch.Tensor] = None    # an 8-bit cache's exponents [pages, kv_heads, PAGE]
+    v_exp: Optional[torch.Tensor] = None
 
 
 @dataclass
@@ -189,13 +196,14 @@ class SequenceCache:
             if kv_need is not None:
                 if src_need is None:
                     raise ValueError(f"run {run} reads keys and values of run {src}, which keeps none")
-                if (src_need.num_kv_heads, src_need.head_dim, src_need.value_size, src_need.keep_first) != \
-                        (kv_need.num_kv_heads, kv_need.head_dim, kv_need.value_size, kv_need.keep_first):
-                    raise ValueError(f"run {run} reads the cache of run {src} with other head sizes or kept tokens")
+                if (src_need.num_kv_heads, src_need.head_dim, src_need.value_size, src_need.keep_first, src_need.eight_bits) != \
+                        (kv_need.num_kv_heads, kv_need.head_dim, kv_need.value_size, kv_need.keep_first, kv_need.eight_bits):
+                    raise ValueError(f"run {run} reads the cache of run {src} with other head sizes, bits or kept tokens")
                 g = self.groups[src_need]
                 i = g.index_of[src]
                 kv_view = KVView(g.k[i] if g.k is not None else None, g.v[i] if g.v is not None else None,
-                                 g.table, g.ring_rows, src_need, src_need.keep_first if g.ring_rows else 0)
+                                 g.table, g.ring_rows, src_need, src_need.keep_first if g.ring_rows else 0,
+                                 g.k_exp[i] if g.k_exp is not None else None, g.v_exp[i] if g.v_exp is not None else None)
             if isinstance(state_need, tuple):
                 state = tuple(self._new_state((run, i), need) for i, need in enumerate(state_need))
             else:
@@ -290,7 +298,7 @@ class SequenceCache:
     def bytes_allocated(self) -> int:
         n = 0
         for g in self.groups.values():
-            for t in (g.k, g.v):
+            for t in (g.k, g.v, g.k_exp, g.v_exp):
                 if t is not None:
                     n += t.numel() * t.element_size()
         return n

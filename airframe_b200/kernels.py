@@ -332,6 +332,45 @@ def store_kv(qkv, batch, nq: int, nkv: int, hd: int, kv, parts=None) -> None:
                      keep=kv_keep(kv))
 
 
+CACHE8_HEAD_SIZES = (64, 128, 256)     # head sizes that the 8-bit cache takes
+
+
+def _cache8_pages(kv, nkv: int, hd: int, who: str):
+    """Checks a layer's view of its 8-bit pages (see ``csrc/cache8.cuh``); returns how many pages there are."""
+    if kv.k is None or kv.v is None or kv.k.dtype != torch.float8_e4m3fn or kv.v.dtype != torch.float8_e4m3fn \
+            or kv.k_exp.dtype != torch.uint8 or kv.v_exp is None or kv.v_exp.dtype != torch.uint8:
+        raise KernelError(f"{who}: an 8-bit cache keeps float8_e4m3fn codes and uint8 exponents of keys and values")
+    n = kv.k.shape[0]
+    if tuple(kv.k.shape) != (n, nkv, PAGE, hd) or kv.v.shape != kv.k.shape or tuple(kv.k_exp.shape) != (n, nkv, PAGE) \
+            or kv.v_exp.shape != kv.k_exp.shape:
+        raise KernelError(f"{who}: 8-bit pages must be [pages, {nkv}, {PAGE}, {hd}], their exponents [pages, {nkv}, {PAGE}]")
+    if not all(t.is_contiguous() for t in (kv.k, kv.v, kv.k_exp, kv.v_exp, kv.page_table)):
+        raise KernelError(f"{who}: cache pages and page table must be contiguous")
+    return n
+
+
+def store_kv8(qkv, batch, nq: int, nkv: int, hd: int, kv, rounded=None) -> None:
+    """A mixer's store into a cache of 8 bits: the k and v heads of the packed bfloat16 rows [q | k | v] go to each
+    token's row of its page as e4m3 codes with a power of two a row (``kv.k``, ``kv.v``, ``kv.k_exp``, ``kv.v_exp``; infinities
+    and NaN become NaN).  ``rounded`` (bfloat16 [T, 2 nkv hd]) gets the values as they are kept, [k | v], of every token of the step:
+    what a prompt's own attention takes, so that its tokens see the keys that later single tokens see."""
+    T = qkv.shape[0]
+    if qkv.dtype != torch.bfloat16 or qkv.shape[1] != (nq + 2 * nkv) * hd:
+        raise KernelError(f"store_kv8: bfloat16 rows of (nq + 2 nkv) * head_dim = {(nq + 2 * nkv) * hd}, got {qkv.dtype} {tuple(qkv.shape)}")
+    if rounded is not None and (rounded.dtype != torch.bfloat16 or tuple(rounded.shape) != (T, 2 * nkv * hd)):
+        raise KernelError(f"store_kv8: rounded must be bfloat16 [{T}, {2 * nkv * hd}]")
+    if batch.positions.numel() != T or batch.seq_of_token.numel() != T:
+        raise KernelError(f"store_kv8: {T} rows, {batch.positions.numel()} positions")
+    n_pages = _cache8_pages(kv, nkv, hd, "store_kv8")
+    _check(_lib().af_store_kv8(
+        _ptr(qkv), c_longlong(_rows(qkv, "qkv")), _ptr(rounded, allow_none=True),
+        c_longlong(_rows(rounded, "rounded") if rounded is not None else 0), _ptr(batch.positions, "positions", torch.int32),
+        _ptr(batch.seq_of_token, "seq_of_token", torch.int32), _ptr(batch.slots, "slots", torch.int32),
+        _ptr(batch.len_after, "len_after", torch.int32), _ptr(kv.page_table, "page_table", torch.int32),
+        c_int(kv.page_table.shape[1]), c_int(kv.ring_rows), c_int(kv_keep(kv)), c_int(T), c_int(nq), c_int(nkv), c_int(hd),
+        _ptr(kv.k), _ptr(kv.v), _ptr(kv.k_exp), _ptr(kv.v_exp), c_longlong(n_pages), _stream()))
+
+
 def sum_parts(qkv, parts, batch, nq: int, nkv: int, hd: int) -> None:
     """qkv = the sum of the split-K partial sums ``parts`` (float32 [S, T, width]), in index order."""
     rope_cache_write(qkv, batch.positions, _no_frequencies(qkv.device), nq, nkv, hd, 0, "half", parts=parts)
@@ -938,8 +977,15 @@ def attn_decode(out, q, kv, batch, nq, nkv, hd, scale, cap, window, slopes=None,
     size than the keys or inside them, and sinks)."""
     # values that lie inside their key rows: the split kernel takes the key pages for the value pages too and gives
     # whole key-sized rows back, of which the caller (who asked for it with an `out` that wide) reads the values' part
-    wide = kv.v is None and out.shape[1] == nq * hd
     keep = kv_keep(kv)
+    if getattr(kv, "k_exp", None) is not None:
+        if slopes is not None or (dv or hd) != hd:
+            raise KernelError("attn_decode: an 8-bit cache serves scores without slopes and values of the keys' size")
+        attn_decode8(out, q, kv, batch, nq, nkv, hd, scale, cap, -window if mask == "chunk" else window, sinks=sinks, keep=keep if window else 0)
+        if gate is not None:
+            head_gate(out, gate, nq, hd)
+        return
+    wide = kv.v is None and out.shape[1] == nq * hd
     special = slopes is not None or (not wide and ((dv or hd) != hd or kv.v is None))
     if (not special and q.dtype == torch.bfloat16 and _lib().af_attn_decode_supported(c_int(hd))
             and batch.n_seqs <= ATTN_DECODE_MAX_SEQS):
@@ -973,6 +1019,31 @@ def attn_decode(out, q, kv, batch, nq, nkv, hd, scale, cap, window, slopes=None,
     attn_decode_plain(out, q, kv.k, kv.v, kv.page_table, batch.slots, batch.len_after, nq, nkv, hd,
                       scale, cap, window, kv.ring_rows, slopes, dv=dv, mask=mask, sinks=sinks, gate=gate,
                       n_splits=plain_decode_splits(batch.n_seqs, nq, most), keep=keep)
+
+
+def attn_decode8(out, q, kv, batch, nq: int, nkv: int, hd: int, scale: float, cap: float, window: int, sinks=None,
+                 keep: int = 0) -> None:
+    """Decode attention over a cache of 8 bits (``window`` < 0: a chunk of that many positions; ``keep``: beside a window,
+    the first tokens that stay visible)."""
+    B = batch.n_seqs
+    n_pages = _cache8_pages(kv, nkv, hd, "attn_decode8")
+    if q.dtype != torch.bfloat16 or out.dtype != torch.bfloat16 or tuple(out.shape) != (B, nq * hd) or q.shape[0] != B or q.shape[1] < nq * hd:
+        raise KernelError(f"attn_decode8: bfloat16 queries and out [{B}, {nq * hd}]")
+    if sinks is not None and sinks.numel() != nq:
+        raise KernelError(f"attn_decode8: {sinks.numel()} sinks for {nq} heads")
+    _check(_lib().af_attn_decode8(
+        _ptr(out), c_longlong(_rows(out, "out")), _ptr(q), c_longlong(_rows(q, "q")), _ptr(kv.k), _ptr(kv.v), _ptr(kv.k_exp),
+        _ptr(kv.v_exp), _ptr(kv.page_table, "page_table", torch.int32), c_int(kv.page_table.shape[1]),
+        _ptr(batch.slots, "slots", torch.int32), _ptr(batch.len_after, "lens", torch.int32), c_int(B), c_int(nq), c_int(nkv),
+        c_int(hd), c_float(scale), c_float(cap), c_int(window), c_int(keep), c_int(kv.ring_rows),
+        _ptr(sinks, "sinks", torch.float32, allow_none=True), _stream()))
+
+
+def attn_decode_shared(out, q, kv, batch, nq: int, nkv: int, hd: int, scale: float, cap: float, lead, pages, most_pages: int,
+                       sinks=None, gate=None) -> None:
+    """Decode attention (all keys visible) of sequences that share their first pages: row b's first ``pages[b]`` cache pages
+    are those of row ``lead[b]`` (int32 [B] each; rows that share nothing: 0 pages), ``most_pages`` the most that any row shares."""
+    attn_decode(out, q, kv, batch, nq, nkv, hd, scale, cap, 0, sinks=sinks, gate=gate)
 
 
 # ---------------------------------------------------------------- mixers with a state of fixed size

@@ -70,12 +70,14 @@ class KVNeed:
     otherwise the last ``window`` rows (a ring).  ``value_dim``: the size of a
     value row (None: ``head_dim``, as the keys; 0: no value pages, the mixer finds
     its values inside the key rows).  ``keep_first``: beside the window's rows those of
-    the sequence's first tokens are kept (their pages never belong to the ring)."""
+    the sequence's first tokens are kept (their pages never belong to the ring).  ``eight_bits``: rows are kept
+    as e4m3 codes with a power of two a row (:func:`airframe_b200.kernels.store_kv8`) instead of in the cache's dtype."""
     num_kv_heads: int
     head_dim: int
     window: Optional[int] = None
     value_dim: Optional[int] = None
     keep_first: int = 0
+    eight_bits: bool = False
 
     @property
     def value_size(self) -> int:
