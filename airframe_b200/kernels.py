@@ -900,6 +900,19 @@ def attn_decode_plan(page_table, slots, lens, nq: int, nkv: int, window: int, ri
     return plan
 
 
+def _step_plan(kv, batch, nq: int, nkv: int, window: int, keep: int, n_splits: int):
+    """The plan of the step (see :func:`attn_decode_plan`), made once in a pass for all layers that read this group of caches
+    alike (a batch without a place for the step's tables gets a plan for the call)."""
+    aux = getattr(batch, "aux", None)
+    key = ("attn_decode_plan", kv.page_table.data_ptr(), kv.ring_rows, nq, nkv, window, keep, n_splits)
+    plan = aux.get(key) if aux is not None else None
+    if plan is None:
+        plan = attn_decode_plan(kv.page_table, batch.slots, batch.len_after, nq, nkv, window, kv.ring_rows, n_splits, keep)
+        if aux is not None:
+            aux[key] = plan
+    return plan
+
+
 def attn_decode_split(out, q, kcache, vcache, page_table, slots, lens, nq, nkv, hd, scale, cap, window, ring_rows,
                       n_splits: int, scratch=None, plan=None, sinks=None, keep: int = 0) -> None:
     """bfloat16 decode attention, split over the keys (two kernels: partial
@@ -994,13 +1007,7 @@ def attn_decode(out, q, kv, batch, nq, nkv, hd, scale, cap, window, slopes=None,
         n = attn_decode_max_splits(batch.n_seqs, nkv, batch.max_len_after, window, nq=nq, keep=keep)
         # the plan of the step, shared by the layers that read this group of caches alike (a batch without a
         # place for the step's tables gets none: every block then works the cut out itself)
-        plan, aux = None, getattr(batch, "aux", None)
-        if aux is not None:
-            key = ("attn_decode_plan", kv.page_table.data_ptr(), kv.ring_rows, nq, nkv, window, keep, n)
-            if key not in aux:
-                aux[key] = attn_decode_plan(kv.page_table, batch.slots, batch.len_after, nq, nkv, window,
-                                            kv.ring_rows, n, keep)
-            plan = aux[key]
+        plan = _step_plan(kv, batch, nq, nkv, window, keep, n) if getattr(batch, "aux", None) is not None else None
         attn_decode_split(out, q, kv.k, kv.k if wide else kv.v, kv.page_table, batch.slots, batch.len_after, nq, nkv,
                           hd, scale, cap, window, kv.ring_rows, n, plan=plan, sinks=sinks, keep=keep)
         if gate is not None:
@@ -1031,12 +1038,20 @@ def attn_decode8(out, q, kv, batch, nq: int, nkv: int, hd: int, scale: float, ca
         raise KernelError(f"attn_decode8: bfloat16 queries and out [{B}, {nq * hd}]")
     if sinks is not None and sinks.numel() != nq:
         raise KernelError(f"attn_decode8: {sinks.numel()} sinks for {nq} heads")
-    _check(_lib().af_attn_decode8(
+    if B > ATTN_DECODE_MAX_SEQS:
+        raise KernelError(f"attn_decode8: {B} sequences (takes {ATTN_DECODE_MAX_SEQS})")
+    n = attn_decode_max_splits(B, nkv, batch.max_len_after, window, nq=nq, keep=keep)
+    plan = _step_plan(kv, batch, nq, nkv, window, keep, n)
+    lib = _lib()
+    lib.af_attn_decode_scratch.restype = ctypes.c_longlong
+    scratch = torch.empty(lib.af_attn_decode_scratch(c_int(B), c_int(nq), c_int(hd), c_int(n)), dtype=torch.float32, device=q.device)
+    _check(lib.af_attn_decode8(
         _ptr(out), c_longlong(_rows(out, "out")), _ptr(q), c_longlong(_rows(q, "q")), _ptr(kv.k), _ptr(kv.v), _ptr(kv.k_exp),
-        _ptr(kv.v_exp), _ptr(kv.page_table, "page_table", torch.int32), c_int(kv.page_table.shape[1]),
+        _ptr(kv.v_exp), c_longlong(n_pages), _ptr(kv.page_table, "page_table", torch.int32), c_int(kv.page_table.shape[1]),
         _ptr(batch.slots, "slots", torch.int32), _ptr(batch.len_after, "lens", torch.int32), c_int(B), c_int(nq), c_int(nkv),
-        c_int(hd), c_float(scale), c_float(cap), c_int(window), c_int(keep), c_int(kv.ring_rows),
-        _ptr(sinks, "sinks", torch.float32, allow_none=True), _stream()))
+        c_int(hd), c_float(scale), c_float(cap), c_int(window), c_int(keep), c_int(kv.ring_rows), c_int(n),
+        _ptr(scratch, "scratch", torch.float32), _ptr(plan, "plan", torch.int32), _ptr(sinks, "sinks", torch.float32, allow_none=True),
+        _ptr(error_word(q.device), "err", torch.int32), _stream()))
 
 
 def attn_decode_shared(out, q, kv, batch, nq: int, nkv: int, hd: int, scale: float, cap: float, lead, pages, most_pages: int,
