@@ -684,9 +684,9 @@ AF_EXPORT long long af_attn_decode_plan_ints(int batch, int nq, int nkv) {
 // Works out, once for a step, how af_attn_decode cuts the work of the layers that read the same caches the same
 // way (the same slots, lengths, page table, heads, window, ring and n_splits): pass `plan` to each of their calls.
 // It holds for these lengths alone: a step later it is made again.
-AF_EXPORT int af_attn_decode_plan_kept(int* plan, long long plan_ints, const int* page_table, int max_pages,
-                                  const int* slots, const int* lens, int batch, int nq, int nkv, int window,
-                                  int keep, int ring_rows, int n_splits, cudaStream_t stream) {
+static int decode_plan_impl(int* plan, long long plan_ints, const int* page_table, int max_pages, const int* slots, const int* lens,
+                            const int* shared, int batch, int nq, int nkv, int window, int keep, int ring_rows, int n_splits,
+                            cudaStream_t stream) {
   if (batch == 0) return 0;
   AF_REQUIRE(nq > 0 && nkv > 0 && nq % nkv == 0, "af_attn_decode_plan: heads %d, groups %d", nq, nkv);
   AF_REQUIRE(plan != nullptr && ((uintptr_t)plan & 15) == 0 && plan_ints >= af_attn_decode_plan_ints(batch, nq, nkv),
@@ -699,8 +699,30 @@ AF_EXPORT int af_attn_decode_plan_kept(int* plan, long long plan_ints, const int
   const int sms = af_sm_count();
   if (sms <= 0) return -1;
   af_launch(attn_decode_plan_kernel, dim3(1), dim3(256), (size_t)2 * (batch + 1) * sizeof(int), stream, plan, slots,
-            lens, page_table, max_pages, batch, nq, nkv, window, keep, ring_rows, n_splits, sms, nullptr);
+            lens, page_table, max_pages, batch, nq, nkv, window, keep, ring_rows, n_splits, sms, shared);
   AF_CHECK_LAUNCH("af_attn_decode_plan");
+}
+
+AF_EXPORT int af_attn_decode_plan_kept(int* plan, long long plan_ints, const int* page_table, int max_pages,
+                                  const int* slots, const int* lens, int batch, int nq, int nkv, int window,
+                                  int keep, int ring_rows, int n_splits, cudaStream_t stream) {
+  return decode_plan_impl(plan, plan_ints, page_table, max_pages, slots, lens, nullptr, batch, nq, nkv, window, keep, ring_rows, n_splits,
+                          stream);
+}
+
+// The same where each sequence's first shared[b] pages are another kernel's (attention_shared.cu).
+int af_decode_plan_shared(int* plan, long long plan_ints, const int* page_table, int max_pages, const int* slots, const int* lens,
+                          const int* shared, int batch, int nq, int nkv, int n_splits, cudaStream_t stream) {
+  return decode_plan_impl(plan, plan_ints, page_table, max_pages, slots, lens, shared, batch, nq, nkv, 0, 0, 0, n_splits, stream);
+}
+
+// The split pass alone (partial results into `scratch`), each sequence's first shared[b] pages left out.
+int af_decode16_split(const void* q, long long q_stride, const void* kcache, const void* vcache, long long n_pages,
+                      const int* page_table, int max_pages, const int* slots, const int* lens, const int* shared, int batch, int nq,
+                      int nkv, int hd, float scale, float cap, int n_splits, float* scratch, const int* plan, int* err,
+                      cudaStream_t stream) {
+  return attn_decode_impl(nullptr, nullptr, 0, q, q_stride, kcache, vcache, n_pages, page_table, max_pages, slots, lens, batch, nq, nkv, hd,
+                          scale, cap, 0, 0, 0, n_splits, scratch, plan, err, stream, shared, false);
 }
 
 AF_EXPORT int af_attn_decode_plan(int* plan, long long plan_ints, const int* page_table, int max_pages,

@@ -138,7 +138,10 @@ decode8_split_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
     return;
   }
   __syncthreads();
-  if (r0.x < 0) return;                               // (no work)
+  if (r0.x < 0) {                                     // (no work; a grid without any must not end before the kernel in front)
+    if (blockIdx.x == 0) pdl_wait();
+    return;
+  }
   int left = r1.y;
 
   struct Segment {

@@ -1,0 +1,829 @@
+// Decode attention of sequences that share a prefix (completions of one prompt, requests behind one system prompt): the
+// shared cache pages are read once for all of a group's sequences, and their products are one tensor-core product of many rows.
+//
+// Three kernels behind the step's plan (one small kernel a step for all layers):
+//   prefix  the rows of a unit are the query heads of one kv head of all members of a group (up to 128 of them, more in several
+//           units); the units' pages are cut into items, one a block; every row leaves (max, sum, output) of each item
+//   rest    the split kernel of the cache at hand over each sequence's own pages (its plan leaves the shared ones out)
+//   merge   of both, one block a (sequence, head)
+//
+// The prefix kernel.  A block holds its 128 rows' queries in tensor memory and walks its pages, 64 keys at a time:
+//   S = Q K^T     tcgen05.mma, M = 128, N = 64, Q from TMEM, the K page from swizzled shared memory
+//   softmax       two groups of four warps take the pages in turn, a thread a row: all keys are visible (a shared page is full
+//                 and older than every member's token), so there is no mask; P goes back into its S columns of TMEM
+//   O += P V      tcgen05.mma, P from TMEM, O (128 x head_dim, 32 bits) in TMEM for the whole item
+// The groups share O and its reference maximum, which a group hands to the other with every page and which moves only when it is
+// passed by more than 2^8.  Products and softmax of neighbouring pages overlap.
+//   warp 0        TMA producer (16-bit cache)         warp 1  issue of S, TMEM allocation      warp 2  issue of O += P V
+//   warps 4..11   queries, softmax, rescaling, partial results
+//   warps 12..19  8-bit cache only: codes from memory to halves in the swizzled operand layout, 16 bytes a load, the next page's
+//                 loads in flight while this page's are converted
+// In the 8-bit cache a key's factor multiplies its scores, a value's its weights, whose halves are kept relative to the largest
+// such weight (see attention_decode8.cu; the queries are scaled alike).
+// Bound by the prefix's bytes up to some 128 rows; then by the products.
+// Every wait on a barrier is bounded in time; one that runs out sets the error word, and the block frees its TMEM and returns.
+#include "airframe_b200.h"
+#include "cache8.cuh"
+#include "decode_split.cuh"
+#include "umma.cuh"
+
+int af_decode8_split(const void* q, long long q_stride, const void* k, const void* v, const void* k_exp, const void* v_exp,
+                     long long n_pages, const int* page_table, int max_pages, const int* slots, const int* lens, const int* shared,
+                     int batch, int nq, int nkv, int hd, float scale, float cap, int window, int keep, int ring_rows, int n_splits,
+                     float* scratch, const int* plan, int* err, cudaStream_t stream);
+int af_decode16_split(const void* q, long long q_stride, const void* kcache, const void* vcache, long long n_pages,
+                      const int* page_table, int max_pages, const int* slots, const int* lens, const int* shared, int batch, int nq,
+                      int nkv, int hd, float scale, float cap, int n_splits, float* scratch, const int* plan, int* err,
+                      cudaStream_t stream);
+int af_decode_plan_shared(int* plan, long long plan_ints, const int* page_table, int max_pages, const int* slots, const int* lens,
+                          const int* shared, int batch, int nq, int nkv, int n_splits, cudaStream_t stream);
+
+namespace {
+
+// ---------------------------------------------------------------- the plan
+//
+// 32-bit integers: [0, 16) items, units, sequences, heads, kv heads, blocks; then
+//   shared [batch]      the pages of each sequence that the prefix kernel takes (0: none)
+//   loc    [batch][2]   its group's first unit (-1: none), its place among the group's members
+//   order  [batch]      the groups' members, group after group
+//   units  [n][8]       where its members begin in `order`, members, kv head, tile of 128 rows; pages, items, first partial row, slot
+//   items  [n][2]       unit, part of its pages
+constexpr int SH_HEAD = 16, SH_ROWS = 128, SH_MAX_BATCH = DA_MAX_BATCH;
+
+__host__ __device__ inline int sh_max_units(int batch, int nq, int nkv) { return nkv * (batch * (nq / nkv) / SH_ROWS + batch / 2 + 1); }
+struct ShPlan {
+  int shared, loc, order, units, items, total;
+};
+__host__ __device__ inline ShPlan sh_layout(int batch, int nq, int nkv, int blocks) {
+  ShPlan p;
+  const int b4 = (batch + 3) / 4 * 4, units = sh_max_units(batch, nq, nkv);
+  p.shared = SH_HEAD;
+  p.loc = p.shared + b4;
+  p.order = p.loc + 2 * b4;
+  p.units = p.order + b4;
+  p.items = p.units + 8 * units;
+  p.total = p.items + 2 * (blocks + units);
+  return p;
+}
+
+// One block.  A group is the live rows of one `lead` that share at least a page; alone in it a row keeps its pages.  Fewer
+// pages than a row claims are taken where another of the group shares fewer, and never the page of its new token.
+__global__ void __launch_bounds__(512)
+attn_shared_plan_kernel(int* __restrict__ plan, const int* __restrict__ lead, const int* __restrict__ pages, const int* __restrict__ slots,
+                        const int* __restrict__ lens, int batch, int nq, int nkv, int blocks) {
+  extern __shared__ int sp_smem[];
+  int* gid = sp_smem;                  // [batch] the row's group, -1: none
+  int* cnt = gid + batch;              // [batch] by group: members
+  int* few = cnt + batch;              //           the pages all of them share
+  int* unit0 = few + batch;            //           first unit
+  int* item0 = unit0 + batch;          //           first item
+  int* memb0 = item0 + batch;          //           first place in `order`
+  int* row0 = memb0 + batch;           //           first partial row
+  __shared__ long long total_s;
+  pdl_wait();
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int group = nq / nkv;
+  const ShPlan L = sh_layout(batch, nq, nkv, blocks);
+  for (int b = tid; b < batch; b += blockDim.x) cnt[b] = 0, few[b] = 0x7fffffff;
+  __syncthreads();
+  for (int b = tid; b < batch; b += blockDim.x) {
+    const int len = lens[b], p = slots[b] >= 0 && len > 0 ? min(pages[b], (len - 1) / AF_PAGE) : 0, g = lead[b];
+    gid[b] = p > 0 && g >= 0 && g < batch ? g : -1;
+    if (gid[b] >= 0) {
+      atomicAdd(&cnt[g], 1);
+      atomicMin(&few[g], p);
+    }
+  }
+  __syncthreads();
+  if (warp == 0) {
+    // places of the groups: units first, then (their pages known) items and partial rows
+    int units = 0, members = 0;
+    long long total = 0;
+    for (int base = 0; base < batch; base += 32) {
+      const int g = base + lane;
+      const bool on = g < batch && cnt[g] >= 2;
+      const int c = on ? cnt[g] : 0, u = on ? nkv * ((c * group + SH_ROWS - 1) / SH_ROWS) : 0;
+      int vu = u, vm = c;
+      long long vt = on ? (long long)u * few[g] : 0;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int a = __shfl_up_sync(0xffffffffu, vu, o), m = __shfl_up_sync(0xffffffffu, vm, o);
+        if (lane >= o) vu += a, vm += m;
+      }
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) vt += __shfl_xor_sync(0xffffffffu, vt, o);
+      if (on) unit0[g] = units + vu - u, memb0[g] = members + vm - c;
+      units += __shfl_sync(0xffffffffu, vu, 31);
+      members += __shfl_sync(0xffffffffu, vm, 31);
+      total += vt;
+    }
+    int items = 0, rows = 0;
+    for (int base = 0; base < batch; base += 32) {
+      const int g = base + lane;
+      const bool on = g < batch && cnt[g] >= 2;
+      const int c = on ? cnt[g] : 0, u = on ? nkv * ((c * group + SH_ROWS - 1) / SH_ROWS) : 0;
+      // items of a unit: its share of the blocks, rounded down, so that no block gets a second one
+      const int s = on ? (int)max(1ll, min((long long)few[g], (long long)few[g] * blocks / total)) : 0;
+      int vi = u * s, vr = nkv * c * group * s;
+      const int i1 = vi, r1 = vr;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int a = __shfl_up_sync(0xffffffffu, vi, o), m = __shfl_up_sync(0xffffffffu, vr, o);
+        if (lane >= o) vi += a, vr += m;
+      }
+      if (on) item0[g] = items + vi - i1, row0[g] = rows + vr - r1;
+      items += __shfl_sync(0xffffffffu, vi, 31);
+      rows += __shfl_sync(0xffffffffu, vr, 31);
+    }
+    if (lane == 0) {
+      total_s = total;
+      plan[0] = items, plan[1] = units, plan[2] = batch, plan[3] = nq, plan[4] = nkv, plan[5] = blocks;
+    }
+  }
+  __syncthreads();
+  const long long total = total_s;
+  for (int b = tid; b < batch; b += blockDim.x) {
+    const int g = gid[b];
+    const bool on = g >= 0 && cnt[g] >= 2;
+    int place = 0;
+    if (on)
+      for (int j = 0; j < b; ++j) place += gid[j] == g ? 1 : 0;
+    plan[L.shared + b] = on ? few[g] : 0;
+    plan[L.loc + 2 * b] = on ? unit0[g] : -1;
+    plan[L.loc + 2 * b + 1] = place;
+    if (on) plan[L.order + memb0[g] + place] = b;
+  }
+  for (int g = warp; g < batch; g += (int)blockDim.x >> 5) {
+    const int c = cnt[g];
+    if (c < 2) continue;
+    int b = 0;                                            // a member's slot: its page table holds the shared pages
+    for (int base = 0; base < batch; base += 32) {
+      const uint32_t with = __ballot_sync(0xffffffffu, base + lane < batch && gid[min(base + lane, batch - 1)] == g);
+      if (with) {
+        b = base + __ffs(with) - 1;
+        break;
+      }
+    }
+    const int rows = c * group, tiles = (rows + SH_ROWS - 1) / SH_ROWS, u = nkv * tiles;
+    const int s = (int)max(1ll, min((long long)few[g], (long long)few[g] * blocks / total));
+    for (int x = lane; x < u; x += 32) {
+      int* r = plan + L.units + 8 * (unit0[g] + x);
+      const int kvh = x / tiles, tile = x - kvh * tiles;
+      r[0] = memb0[g], r[1] = c, r[2] = kvh, r[3] = tile;
+      r[4] = few[g], r[5] = s, r[6] = row0[g] + (kvh * rows + tile * SH_ROWS) * s, r[7] = slots[b];
+    }
+    for (int x = lane; x < u * s; x += 32) {
+      plan[L.items + 2 * (item0[g] + x)] = unit0[g] + x / s;
+      plan[L.items + 2 * (item0[g] + x) + 1] = x - x / s * s;
+    }
+  }
+}
+
+// ---------------------------------------------------------------- the prefix kernel
+
+constexpr float SH_NONE = -3.0e38f;      // a reference before the first key
+constexpr float SH_MOVES = 8.f;          // the reference moves when it is passed by more than this
+constexpr float SH_SHIFT = 6.f;          // (8 bits) halves of weights are kept times 2^6
+constexpr int SH_EXPS = 16;              // (8 bits) pages whose factors are kept: more than the K stages and the two at work
+
+template <int HD, int BITS>
+struct Sh {
+  static constexpr int WARPS = BITS == 8 ? 20 : 12, THREADS = WARPS * 32;
+  static constexpr int TILE = AF_PAGE * HD * 2;                              // bytes of a page's keys, or values, as operand
+  static constexpr int STAGES = HD == 256 ? 3 : (HD == 128 ? 6 : 8);         // pages in flight
+  static constexpr int SMEM = 2 * STAGES * TILE + 1024;
+};
+
+struct ShArgs {
+  const __nv_bfloat16* q;
+  long long q_stride;
+  const uint8_t *k, *v, *k_exp, *v_exp;     // (8 bits)
+  long long n_pages;
+  const int *page_table, *plan;
+  int max_pages, batch, nq, nkv;
+  float scale, cap;
+  float *part_o, *part_ml;                  // [partial row][HD], [partial row][2]
+  int* err;
+};
+
+// f16 x f16 -> f32, as umma_idesc
+__host__ __device__ constexpr uint32_t sh_idesc(int bn, bool f16, bool b_mn_major) {
+  return (1u << 4) | (f16 ? 0u : (1u << 7) | (1u << 10)) | ((b_mn_major ? 1u : 0u) << 16) | ((uint32_t)(bn >> 3) << 17) |
+         ((uint32_t)(128 >> 4) << 24);
+}
+
+// What an item is: every role reads it from the plan.
+struct ShItem {
+  int rows, first, pages, row0, members0, group0, kvh, slot;      // rows of the tile; page range; partial row; ...
+};
+
+template <int HD, int BITS>
+__global__ void __launch_bounds__(Sh<HD, BITS>::THREADS, 1)
+attn_shared_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, ShArgs a) {
+  using C = Sh<HD, BITS>;
+  constexpr int SUB = HD / 64, STAGES = C::STAGES;
+  constexpr uint32_t Q_COL = 128, O_COL = 256;       // TMEM columns: S (and P) [0, 64) [64, 128), Q [128, 128 + HD / 2), O [256, 256 + HD)
+  constexpr uint32_t IDESC_S = sh_idesc(AF_PAGE, BITS == 8, false), IDESC_O = sh_idesc(HD, BITS == 8, true);
+  constexpr float LOG2E = 1.4426950408889634f;
+  extern __shared__ unsigned char sh_raw[];
+  unsigned char* k_s = (unsigned char*)(((uintptr_t)sh_raw + 1023) & ~(uintptr_t)1023);      // [stage][sub-tile][64 keys][128 B]
+  unsigned char* v_s = k_s + STAGES * C::TILE;
+  __shared__ uint64_t k_full[STAGES], k_empty[STAGES], v_full[STAGES], v_empty[STAGES], s_full[2], p_full[2], pv_done[2], m_ready[2], q_ready,
+      l_full;
+  __shared__ float mref_s[2][SH_ROWS], l_s[2][SH_ROWS];
+  __shared__ float wref_s[BITS == 8 ? 2 : 1][BITS == 8 ? SH_ROWS : 1];
+  __shared__ __align__(16) float ks_s[BITS == 8 ? SH_EXPS : 1][AF_PAGE], lv_s[BITS == 8 ? SH_EXPS : 1][AF_PAGE];
+  __shared__ uint32_t tmem_base_s;
+  __shared__ int give_up_s;
+  volatile int* give_up = &give_up_s;
+
+  pdl_launch_dependents();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int group = a.nq / a.nkv;
+  const ShPlan L = sh_layout(a.batch, a.nq, a.nkv, (int)gridDim.x);
+  const int n_items = a.plan[0];
+  if (a.plan[2] != a.batch || a.plan[3] != a.nq || a.plan[4] != a.nkv || a.plan[5] != (int)gridDim.x) {
+    if (threadIdx.x == 0 && a.err) atomicExch(a.err, 1);      // (a plan made for another launch)
+    return;
+  }
+  if ((int)blockIdx.x >= n_items) {
+    if (blockIdx.x == 0) pdl_wait();      // (without items the kernel must not end before the one in front: the next one waits for this one alone)
+    return;
+  }
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < STAGES; ++s) {
+      mbar_init(&k_full[s], BITS == 8 ? 8 : 1);
+      mbar_init(&k_empty[s], 1);
+      mbar_init(&v_full[s], BITS == 8 ? 8 : 1);
+      mbar_init(&v_empty[s], 1);
+    }
+    for (int s = 0; s < 2; ++s) {
+      mbar_init(&s_full[s], 1);
+      mbar_init(&p_full[s], 4);
+      mbar_init(&pv_done[s], 1);
+      mbar_init(&m_ready[s], 4);
+    }
+    mbar_init(&q_ready, 8);
+    mbar_init(&l_full, 8);
+    give_up_s = 0;
+    mbar_fence_init();
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_base_s)), "r"(512u));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::);
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = tmem_base_s;
+
+  auto item_of = [&](int w) {
+    const int u = a.plan[L.items + 2 * w], z = a.plan[L.items + 2 * w + 1];
+    const int4 x = *reinterpret_cast<const int4*>(a.plan + L.units + 8 * u), y = *reinterpret_cast<const int4*>(a.plan + L.units + 8 * u + 4);
+    ShItem it;
+    it.group0 = x.w * SH_ROWS;                                        // the tile's first row among the group's
+    it.rows = min(SH_ROWS, x.y * group - it.group0);
+    it.first = (int)((long long)z * y.x / y.y);
+    it.pages = (int)((long long)(z + 1) * y.x / y.y) - it.first;
+    it.row0 = y.z + z * it.rows;
+    it.members0 = x.x;
+    it.kvh = x.z;
+    it.slot = y.w;
+    return it;
+  };
+  auto page_id = [&](const ShItem& it, int j) {
+    const int entry = it.first + j;
+    const int page = AF_INDEX_OK(entry < a.max_pages, entry) && entry < a.max_pages ? a.page_table[(size_t)it.slot * a.max_pages + entry] : 0;
+    return AF_INDEX_OK(page >= 0 && page < a.n_pages, page) && page >= 0 && page < a.n_pages ? page : 0;
+  };
+
+  // Pages are counted through over the block's items (`jj`): a page's group, stage and phases follow from its count.
+  if (warp == 0) {
+    // ---- the 16-bit cache's pages.  They are older than the kernels in front: nothing to wait for
+    if (BITS == 16 && lane == 0) {
+      int jj = 0;
+      for (int w = blockIdx.x; w < n_items && !*give_up; w += gridDim.x) {
+        const ShItem it = item_of(w);
+        int next = page_id(it, 0);
+        for (int j = 0; j < it.pages; ++j, ++jj) {
+          const int s = jj % STAGES, row = (next * a.nkv + it.kvh) * AF_PAGE;
+          const uint32_t ph = ((jj / STAGES) & 1) ^ 1;
+          if (j + 1 < it.pages) next = page_id(it, j + 1);
+          if (!mbar_wait(&k_empty[s], ph, give_up)) break;
+          mbar_expect_tx(&k_full[s], C::TILE);
+#pragma unroll
+          for (int c = 0; c < SUB; ++c) tma_load_2d(k_s + s * C::TILE + c * 8192, &map_k, c * 64, row, &k_full[s]);
+          if (!mbar_wait(&v_empty[s], ph, give_up)) break;
+          mbar_expect_tx(&v_full[s], C::TILE);
+#pragma unroll
+          for (int c = 0; c < SUB; ++c) tma_load_2d(v_s + s * C::TILE + c * 8192, &map_v, c * 64, row, &v_full[s]);
+        }
+      }
+      if (*give_up) grace_period();
+    }
+  } else if (warp == 1) {
+    if (lane == 0) {
+      int jj = 0, n = 0;
+      bool ok = true;
+      for (int w = blockIdx.x; w < n_items && ok; w += gridDim.x, ++n) {
+        const ShItem it = item_of(w);
+        ok = mbar_wait(&q_ready, n & 1, give_up);       // (and everything of the item before is read)
+        for (int j = 0; j < it.pages && ok; ++j, ++jj) {
+          const int s = jj % STAGES;
+          ok = mbar_wait(&k_full[s], (jj / STAGES) & 1, give_up);
+          if (ok && j >= 2) ok = mbar_wait(&pv_done[jj & 1], ((jj - 2) >> 1) & 1, give_up);      // P of two pages before is consumed
+          if (!ok) break;
+          tc_fence_after();
+          const uint32_t kt = smem_u32(k_s + s * C::TILE);
+#pragma unroll
+          for (int ks = 0; ks < HD / 16; ++ks)
+            umma_f16_ts(tmem + (jj & 1) * 64, tmem + Q_COL + ks * 8, umma_desc(kt + (ks >> 2) * 8192) + 2 * (ks & 3), IDESC_S, ks > 0 ? 1u : 0u);
+          umma_commit(&s_full[jj & 1]);
+          umma_commit(&k_empty[s]);
+        }
+      }
+    }
+  } else if (warp == 2) {
+    if (lane == 0) {
+      int jj = 0;
+      bool ok = true;
+      for (int w = blockIdx.x; w < n_items && ok; w += gridDim.x) {
+        const ShItem it = item_of(w);
+        for (int j = 0; j < it.pages && ok; ++j, ++jj) {
+          const int s = jj % STAGES;
+          ok = mbar_wait(&v_full[s], (jj / STAGES) & 1, give_up) && mbar_wait(&p_full[jj & 1], (jj >> 1) & 1, give_up);
+          if (!ok) break;
+          tc_fence_after();
+          const uint32_t vt = smem_u32(v_s + s * C::TILE);
+#pragma unroll
+          for (int kk = 0; kk < AF_PAGE / 16; ++kk)
+            umma_f16_ts(tmem + O_COL, tmem + (jj & 1) * 64 + kk * 8, umma_desc_mn(vt + kk * 2048, 8192), IDESC_O, (j > 0 || kk > 0) ? 1u : 0u);
+          umma_commit(&v_empty[s]);
+          umma_commit(&pv_done[jj & 1]);
+        }
+      }
+    }
+  } else if (warp >= 4 && warp < 12) {
+    // ---- queries, softmax, partial results.  A thread has a row; group g takes the pages whose count is g modulo 2
+    const int grp = (warp - 4) >> 2, quarter = warp & 3, row = quarter * 32 + lane;
+    const uint32_t lane_addr = tmem + ((uint32_t)(quarter * 32) << 16);
+    const float ecap = a.cap > 0.f ? 2.f * LOG2E / a.cap : 0.f, capl = a.cap * LOG2E;
+    int jj = 0, n = 0;
+    bool ok = true;
+    pdl_wait();
+    for (int w = blockIdx.x; w < n_items && ok; w += gridDim.x, ++n) {
+      const ShItem it = item_of(w);
+      const bool live = row < it.rows;
+      const bool any = quarter * 32 < it.rows;             // (warps without a row only keep the barriers' count)
+      float cs = a.cap > 0.f ? a.scale : a.scale * LOG2E;
+      if (any) {
+        // ---- half of the row's query into TMEM, two elements a column
+        const int rr = it.group0 + row, member = rr / group;
+        const int b = live ? a.plan[L.order + it.members0 + member] : 0;
+        const __nv_bfloat16* qr = a.q + (size_t)b * a.q_stride + (size_t)(it.kvh * group + (live ? rr - member * group : 0)) * HD;
+        constexpr int HALF = HD / 2, PIECES = HALF / 8;
+        float f1 = 1.f, f2 = 1.f;
+        if constexpr (BITS == 8) {
+          uint32_t top = 0;
+          for (int c = 0; c < HD / 8; ++c) {
+            const uint4 x = live ? *reinterpret_cast<const uint4*>(qr + c * 8) : make_uint4(0u, 0u, 0u, 0u);
+            const uint32_t ws[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const uint32_t lo = ws[e] & 0x7fffu, hi = (ws[e] >> 16) & 0x7fffu;
+              top = max(top, max(lo < 0x7f80u ? lo : 0u, hi < 0x7f80u ? hi : 0u));
+            }
+          }
+          const int k = top == 0 ? 14 : max((int)(top >> 7) - 127, -126), up = 14 - k;
+          f1 = c8_pow2(up / 2), f2 = c8_pow2(up - up / 2);
+          cs *= c8_pow2(-(up / 2)) * c8_pow2(-(up - up / 2));
+        }
+#pragma unroll
+        for (int c0 = 0; c0 < PIECES; c0 += 4) {
+          uint32_t wd[16];
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            const uint4 x = live ? *reinterpret_cast<const uint4*>(qr + grp * HALF + (c0 + c) * 8) : make_uint4(0u, 0u, 0u, 0u);
+            wd[4 * c] = x.x, wd[4 * c + 1] = x.y, wd[4 * c + 2] = x.z, wd[4 * c + 3] = x.w;
+          }
+          if constexpr (BITS == 8) {
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+              const __half2 h = __floats2half2_rn(__uint_as_float(wd[e] << 16) * f1 * f2, __uint_as_float(wd[e] & 0xffff0000u) * f1 * f2);
+              wd[e] = *reinterpret_cast<const uint32_t*>(&h);
+            }
+          }
+          tmem_st16(lane_addr + Q_COL + grp * (HALF / 2) + c0 * 4, reinterpret_cast<const float*>(wd));
+        }
+        tmem_wait_st();
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&q_ready);
+
+      float m_known = SH_NONE, l = 0.f;                     // this thread's sum is relative to m_known
+      for (int j = 0; j < it.pages && ok; ++j, ++jj) {
+        if ((jj & 1) != grp) continue;
+        ok = mbar_wait(&s_full[grp], (jj >> 1) & 1, give_up);
+        if (!ok) break;
+        if (!any) {
+          if (lane == 0) {
+            mbar_arrive(&m_ready[grp]);
+            mbar_arrive(&p_full[grp]);
+          }
+          continue;
+        }
+        tc_fence_after();
+        float s[AF_PAGE];
+        tmem_ld32(lane_addr + grp * 64, s);
+        tmem_ld32(lane_addr + grp * 64 + 32, s + 32);
+        tmem_wait_ld();
+        const float* ksp = ks_s[BITS == 8 ? jj % SH_EXPS : 0];
+        const float* lvp = lv_s[BITS == 8 ? jj % SH_EXPS : 0];
+        float mx = SH_NONE, mw = SH_NONE;
+        if constexpr (BITS == 8) {
+#pragma unroll
+          for (int c = 0; c < AF_PAGE; c += 4) {
+            const float4 f = *reinterpret_cast<const float4*>(ksp + c);
+            s[c] *= cs * f.x, s[c + 1] *= cs * f.y, s[c + 2] *= cs * f.z, s[c + 3] *= cs * f.w;
+          }
+        } else {
+#pragma unroll
+          for (int c = 0; c < AF_PAGE; ++c) s[c] *= cs;
+        }
+        if (a.cap > 0.f) {
+#pragma unroll
+          for (int c = 0; c < AF_PAGE; ++c) s[c] = capl - 2.f * capl * __fdividef(1.f, 1.f + fast_exp2(s[c] * ecap));
+        }
+#pragma unroll
+        for (int c = 0; c < AF_PAGE; ++c) mx = fmaxf(mx, s[c]);
+        if constexpr (BITS == 8) {
+#pragma unroll
+          for (int c = 0; c < AF_PAGE; c += 4) {
+            const float4 f = *reinterpret_cast<const float4*>(lvp + c);
+            mw = fmaxf(mw, fmaxf(fmaxf(s[c] + f.x, s[c + 1] + f.y), fmaxf(s[c + 2] + f.z, s[c + 3] + f.w)));
+          }
+        }
+        // the references after the page before, published by the other group
+        float m_prev = SH_NONE, w_prev = SH_NONE;
+        if (j > 0) {
+          ok = mbar_wait(&m_ready[grp ^ 1], ((jj - 1) >> 1) & 1, give_up);
+          if (!ok) break;
+          m_prev = mref_s[grp ^ 1][row];
+          if constexpr (BITS == 8) w_prev = wref_s[grp ^ 1][row];
+        }
+        const float m_new = mx > m_prev + SH_MOVES ? mx : m_prev;
+        mref_s[grp][row] = m_new;
+        float w_new = m_new;                                // the reference of O
+        if constexpr (BITS == 8) {
+          w_new = mw > w_prev + SH_MOVES ? mw : w_prev;
+          wref_s[grp][row] = w_new;
+        } else {
+          w_prev = m_prev;
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&m_ready[grp]);
+        if (j > 0 && __any_sync(0xffffffffu, w_new != w_prev)) {
+          // O is rescaled once the product of the page before is complete (the next one waits for this page's P)
+          ok = mbar_wait(&pv_done[grp ^ 1], ((jj - 1) >> 1) & 1, give_up);
+          if (!ok) break;
+          tc_fence_after();
+          const float f = fast_exp2(w_prev - w_new);
+#pragma unroll 1
+          for (int c0 = 0; c0 < HD; c0 += 16) {
+            float o[16];
+            tmem_ld16(lane_addr + O_COL + c0, o);
+            tmem_wait_ld();
+#pragma unroll
+            for (int c = 0; c < 16; ++c) o[c] *= f;
+            tmem_st16(lane_addr + O_COL + c0, o);
+          }
+          tmem_wait_st();
+        }
+        float sum4[4] = {0.f, 0.f, 0.f, 0.f};
+        uint32_t packed[AF_PAGE / 2];
+        if constexpr (BITS == 8) {
+#pragma unroll
+          for (int c = 0; c < AF_PAGE; c += 4) {
+            const float4 f = *reinterpret_cast<const float4*>(lvp + c);
+            float p[4];
+            const float fv[4] = {f.x, f.y, f.z, f.w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              p[e] = fast_exp2(s[c + e] - m_new);
+              sum4[e] += p[e];
+              p[e] = fast_exp2(s[c + e] + fv[e] - w_new + SH_SHIFT);
+            }
+            const __half2 h0 = __floats2half2_rn(p[0], p[1]), h1 = __floats2half2_rn(p[2], p[3]);
+            packed[c / 2] = *reinterpret_cast<const uint32_t*>(&h0);
+            packed[c / 2 + 1] = *reinterpret_cast<const uint32_t*>(&h1);
+          }
+        } else {
+#pragma unroll
+          for (int c = 0; c < AF_PAGE; c += 2) {
+            const __nv_bfloat162 pb = __floats2bfloat162_rn(fast_exp2(s[c] - m_new), fast_exp2(s[c + 1] - m_new));
+            sum4[(c >> 1) & 3] += __low2float(pb) + __high2float(pb);      // (of the rounded weights that the product sees)
+            packed[c / 2] = *reinterpret_cast<const uint32_t*>(&pb);
+          }
+        }
+        l = l * fast_exp2(m_known - m_new) + ((sum4[0] + sum4[1]) + (sum4[2] + sum4[3]));
+        m_known = m_new;
+        tmem_st32(lane_addr + grp * 64, reinterpret_cast<const float*>(packed));
+        tmem_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&p_full[grp]);
+      }
+      if (!ok) break;
+      // ---- the item's partial results
+      const int last = jj - 1;
+      ok = mbar_wait(&pv_done[last & 1], (last >> 1) & 1, give_up);
+      if (!ok) break;
+      tc_fence_after();
+      const float m_fin = any ? mref_s[last & 1][row] : 0.f;
+      if (any) l_s[grp][row] = l * fast_exp2(m_known - m_fin);
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&l_full);
+      ok = mbar_wait(&l_full, n & 1, give_up);
+      if (!ok) break;
+      if (any) {
+        float f = 1.f;
+        if constexpr (BITS == 8) f = fast_exp2(wref_s[last & 1][row] - SH_SHIFT - m_fin);
+        const size_t at = (size_t)it.row0 + row;
+#pragma unroll 1
+        for (int c0 = 0; c0 < HD / 2; c0 += 32) {
+          float o[32];
+          const int col = grp * (HD / 2) + c0;
+          tmem_ld32(lane_addr + O_COL + col, o);
+          tmem_wait_ld();
+          if (live) {
+#pragma unroll
+            for (int c = 0; c < 32; c += 4)
+              *reinterpret_cast<float4*>(a.part_o + at * HD + col + c) = make_float4(o[c] * f, o[c + 1] * f, o[c + 2] * f, o[c + 3] * f);
+          }
+        }
+        if (live && grp == 0) *reinterpret_cast<float2*>(a.part_ml + at * 2) = make_float2(m_fin, l_s[0][row] + l_s[1][row]);
+      }
+    }
+  } else if (BITS == 8 && warp >= 12) {
+    // ---- codes to halves.  A page's keys (and values) are 64 rows of HD / 16 pieces of 16 codes; a thread takes PER of them
+    constexpr int P_ROW = HD / 16, PER = AF_PAGE * P_ROW / 256;
+    const int ct = threadIdx.x - 12 * 32;
+    int jj = 0;
+    bool ok = true;
+    uint4 kc[PER], vc[PER];
+    int ke = 0, ve = 0;
+    auto load = [&](const ShItem& it, int page) {
+      const size_t at = (size_t)(page * a.nkv + it.kvh) * AF_PAGE;
+      const uint4* kp = reinterpret_cast<const uint4*>(a.k + at * HD);
+      const uint4* vp = reinterpret_cast<const uint4*>(a.v + at * HD);
+#pragma unroll
+      for (int i = 0; i < PER; ++i) kc[i] = __ldg(kp + ct + i * 256), vc[i] = __ldg(vp + ct + i * 256);
+      if (ct < AF_PAGE) ke = a.k_exp[at + ct], ve = a.v_exp[at + ct];
+    };
+    auto convert = [&](unsigned char* tile, const uint4* codes) {
+#pragma unroll
+      for (int i = 0; i < PER; ++i) {
+        const int x = ct + i * 256, r = x / P_ROW, p = x - r * P_ROW;
+        const uint32_t w[4] = {codes[i].x, codes[i].y, codes[i].z, codes[i].w};
+        uint4 h[2];
+        h[0] = make_uint4(c8_half2(w[0]), c8_half2(w[0] >> 16), c8_half2(w[1]), c8_half2(w[1] >> 16));
+        h[1] = make_uint4(c8_half2(w[2]), c8_half2(w[2] >> 16), c8_half2(w[3]), c8_half2(w[3] >> 16));
+        unsigned char* base = tile + (p >> 2) * 8192 + r * 128;
+        const int c = (p & 3) * 2, first = (p >> 2) & 1;      // (neighbouring sub-tiles begin with the other piece: other banks)
+        *reinterpret_cast<uint4*>(base + (((c + first) ^ (r & 7)) << 4)) = first ? h[1] : h[0];
+        *reinterpret_cast<uint4*>(base + (((c + 1 - first) ^ (r & 7)) << 4)) = first ? h[0] : h[1];
+      }
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      __syncwarp();
+    };
+    ShItem it = item_of(blockIdx.x);
+    load(it, page_id(it, 0));
+    for (int w = blockIdx.x; w < n_items && ok; w += gridDim.x) {
+      it = item_of(w);
+      if (w != (int)blockIdx.x) load(it, page_id(it, 0));
+      for (int j = 0; j < it.pages && ok; ++j, ++jj) {
+        const int s = jj % STAGES;
+        const uint32_t ph = ((jj / STAGES) & 1) ^ 1;
+        const int next = j + 1 < it.pages ? page_id(it, j + 1) : -1;
+        ok = mbar_wait(&k_empty[s], ph, give_up);
+        if (!ok) break;
+        convert(k_s + s * C::TILE, kc);
+        if (ct < AF_PAGE) {
+          ks_s[jj % SH_EXPS][ct] = __uint_as_float((uint32_t)ke << 23);
+          lv_s[jj % SH_EXPS][ct] = (float)(ve - 127);
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&k_full[s]);
+        ok = mbar_wait(&v_empty[s], ph, give_up);
+        if (!ok) break;
+        convert(v_s + s * C::TILE, vc);
+        if (lane == 0) mbar_arrive(&v_full[s]);
+        if (next >= 0) load(it, next);
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u));
+  if (threadIdx.x == 0 && give_up_s && a.err) atomicExch(a.err, 1);
+}
+
+// ---------------------------------------------------------------- merge
+
+constexpr int SHM_THREADS = 256, SHM_MOST = 1024;     // partial results of a (sequence, head) that the block weighs
+
+// out[b, h] from the items of the shared pages and the splits of the sequence's own.
+template <int HD>
+__global__ void __launch_bounds__(SHM_THREADS)
+attn_shared_merge_kernel(__nv_bfloat16* __restrict__ out, long long out_stride, const float* pre_o, const float* pre_ml, const float* own_o,
+                         const float* own_ml, int nq, int nkv, int own_room, const int* __restrict__ shared_plan, const int* __restrict__ own_plan,
+                         int blocks, const float* __restrict__ sinks) {
+  pdl_launch_dependents();
+  const int b = blockIdx.x, h = blockIdx.y, batch = gridDim.x, tid = threadIdx.x, lane = tid & 31;
+  const int group = nq / nkv, kvh = h / group, units_per_seq = nkv * ((group + 15) / 16);
+  const ShPlan L = sh_layout(batch, nq, nkv, blocks);
+  const int n_own = own_plan[DA_PLAN_HEAD + b * units_per_seq + kvh * ((group + 15) / 16) + (h % group) / 16];
+  int n_pre = 0, rows = 0;
+  size_t pre0 = 0;
+  const int unit0 = shared_plan[L.loc + 2 * b];
+  if (unit0 >= 0) {
+    const int rr = shared_plan[L.loc + 2 * b + 1] * group + h % group;
+    const int members = shared_plan[L.units + 8 * unit0 + 1], tiles = (members * group + SH_ROWS - 1) / SH_ROWS;
+    const int* u = shared_plan + L.units + 8 * (unit0 + kvh * tiles + rr / SH_ROWS);
+    rows = min(SH_ROWS, members * group - rr / SH_ROWS * SH_ROWS);
+    n_pre = u[5];
+    pre0 = (size_t)u[6] + rr % SH_ROWS;
+  }
+  const size_t own0 = ((size_t)b * nq + h) * own_room;
+  __shared__ float f_s[SHM_MOST], l_s[SHM_MOST];
+  __shared__ float4 red_s[SHM_THREADS];
+  pdl_wait();
+  pre_o = pdl_fresh(pre_o), pre_ml = pdl_fresh(pre_ml), own_o = pdl_fresh(own_o), own_ml = pdl_fresh(own_ml);
+  const int n = n_own + n_pre;         // (own splits first)
+  constexpr int ROW = HD / 4, GROUPS = SHM_THREADS / ROW;
+  const int grp = tid / ROW, d = (tid - grp * ROW) * 4;
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  float M = sinks ? sinks[h] * 1.4426950408889634f : -INFINITY, Ls = sinks ? 1.f : 0.f;
+  // (more partial results than the block weighs at a time: several rounds)
+  for (int base = 0; base < n; base += SHM_MOST) {
+    const int m = min(SHM_MOST, n - base);
+    __syncthreads();
+    float mine = -INFINITY;
+    for (int i = tid; i < m; i += SHM_THREADS) {
+      const int x = base + i;
+      const float2 ml = __ldcg(reinterpret_cast<const float2*>(x < n_own ? own_ml + (own0 + x) * 2 : pre_ml + (pre0 + (size_t)(x - n_own) * rows) * 2));
+      f_s[i] = ml.x;
+      l_s[i] = ml.y;
+    }
+    __syncthreads();
+    for (int i = lane; i < m; i += 32) mine = fmaxf(mine, f_s[i]);
+    const float now = fmaxf(M, warp_max(mine)), ref = now == -INFINITY ? 0.f : now;
+    const float back = M == -INFINITY ? 0.f : fast_exp2(M - ref);
+    acc.x *= back, acc.y *= back, acc.z *= back, acc.w *= back;
+    float part = 0.f;
+    for (int i = lane; i < m; i += 32) part += l_s[i] * fast_exp2(f_s[i] - ref);
+    Ls = Ls * back + warp_sum(part);
+    M = now;
+    for (int i0 = grp; i0 < m; i0 += 8 * GROUPS) {
+      float4 v[8];
+#pragma unroll
+      for (int u = 0; u < 8; ++u) {
+        const int i = i0 + u * GROUPS, x = base + i;
+        v[u] = i < m ? __ldcg(reinterpret_cast<const float4*>((x < n_own ? own_o + (own0 + x) * HD : pre_o + (pre0 + (size_t)(x - n_own) * rows) * HD) + d))
+                     : make_float4(0.f, 0.f, 0.f, 0.f);
+      }
+#pragma unroll
+      for (int u = 0; u < 8; ++u) {
+        const int i = i0 + u * GROUPS;
+        const float f = i < m ? fast_exp2(f_s[i] - ref) : 0.f;
+        acc.x += v[u].x * f, acc.y += v[u].y * f, acc.z += v[u].z * f, acc.w += v[u].w * f;
+      }
+    }
+  }
+  red_s[tid] = acc;
+  __syncthreads();
+  if (tid < ROW) {
+    for (int u = 1; u < GROUPS; ++u) {
+      const float4 x = red_s[u * ROW + tid];
+      acc.x += x.x, acc.y += x.y, acc.z += x.z, acc.w += x.w;
+    }
+    const float inv = Ls == 0.f ? 0.f : 1.f / Ls;
+    __nv_bfloat162* dst = reinterpret_cast<__nv_bfloat162*>(out + (size_t)b * out_stride + (size_t)h * HD + d);
+    dst[0] = __floats2bfloat162_rn(acc.x * inv, acc.y * inv);
+    dst[1] = __floats2bfloat162_rn(acc.z * inv, acc.w * inv);
+  }
+}
+
+template <int HD, int BITS>
+int launch_shared(const ShArgs& a, const void* k, const void* v, int blocks, cudaStream_t stream) {
+  CUtensorMap mk = {}, mv = {};
+  if (BITS == 16) {
+    int rc = af_make_map_bf16(&mk, k, a.n_pages * a.nkv * AF_PAGE, HD, HD, AF_PAGE);
+    if (rc) return rc;
+    rc = af_make_map_bf16(&mv, v, a.n_pages * a.nkv * AF_PAGE, HD, HD, AF_PAGE);
+    if (rc) return rc;
+  }
+  static bool configured[AF_MAX_DEVICES] = {};
+  const int dev = af_current_device();
+  if (dev < 0) return -1;
+  if (!configured[dev]) {
+    const cudaError_t e = cudaFuncSetAttribute(attn_shared_kernel<HD, BITS>, cudaFuncAttributeMaxDynamicSharedMemorySize, Sh<HD, BITS>::SMEM);
+    if (e != cudaSuccess) return af_fail((int)e, "af_attn_decode_shared: %s", cudaGetErrorString(e));
+    configured[dev] = true;
+  }
+  af_launch(attn_shared_kernel<HD, BITS>, dim3(blocks), dim3(Sh<HD, BITS>::THREADS), Sh<HD, BITS>::SMEM, stream, mk, mv, a);
+  AF_CHECK_LAUNCH("af_attn_decode_shared (prefix)");
+}
+
+}  // namespace
+
+// 32-bit integers of the two plans of a shared step (the prefix kernel's, then the split kernel's), 0 where the sizes are refused.
+AF_EXPORT long long af_attn_shared_plan_ints(int batch, int nq, int nkv) {
+  if (batch <= 0 || batch > SH_MAX_BATCH || nq <= 0 || nkv <= 0 || nq % nkv) return 0;
+  const int sms = af_sm_count();
+  if (sms <= 0) return 0;
+  return (sh_layout(batch, nq, nkv, sms).total + 3) / 4 * 4 + af_attn_decode_plan_ints(batch, nq, nkv);
+}
+
+// The most partial rows that the prefix kernel leaves (see af_attn_decode_shared).
+AF_EXPORT long long af_attn_shared_rows(int batch, int nq, int nkv) {
+  const int sms = af_sm_count();
+  if (sms <= 0 || batch <= 0 || nq <= 0 || nkv <= 0) return 0;
+  // units with several items have at most a block each and up to 128 rows, the others one item
+  const int rows = batch * (nq / nkv) < SH_ROWS ? batch * (nq / nkv) : SH_ROWS;
+  return (long long)rows * sms + (long long)batch * nq;
+}
+
+// The plans of a step: row b's first pages[b] cache pages are those of row lead[b].
+AF_EXPORT int af_attn_shared_plan(int* plan, long long plan_ints, const int* lead, const int* pages, const int* page_table, int max_pages,
+                                  const int* slots, const int* lens, int batch, int nq, int nkv, int n_splits, cudaStream_t stream) {
+  if (batch == 0) return 0;
+  const long long need = af_attn_shared_plan_ints(batch, nq, nkv);
+  AF_REQUIRE(need > 0, "af_attn_shared_plan: %d sequences (takes %d), %d heads in %d groups", batch, SH_MAX_BATCH, nq, nkv);
+  AF_REQUIRE(plan != nullptr && ((uintptr_t)plan & 15) == 0 && plan_ints >= need, "af_attn_shared_plan: a plan of %lld integers, 16-byte aligned",
+             need);
+  const int sms = af_sm_count(), smem = 7 * batch * (int)sizeof(int);
+  static bool configured[AF_MAX_DEVICES] = {};
+  const int dev = af_current_device();
+  if (dev < 0) return -1;
+  if (!configured[dev]) {
+    const cudaError_t e = cudaFuncSetAttribute(attn_shared_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 7 * SH_MAX_BATCH * (int)sizeof(int));
+    if (e != cudaSuccess) return af_fail((int)e, "af_attn_shared_plan: %s", cudaGetErrorString(e));
+    configured[dev] = true;
+  }
+  af_launch(attn_shared_plan_kernel, dim3(1), dim3(512), smem, stream, plan, lead, pages, slots, lens, batch, nq, nkv,
+            sms);
+  AF_COUNT_LAUNCH("af_attn_shared_plan");
+  const ShPlan L = sh_layout(batch, nq, nkv, sms);
+  const int at = (L.total + 3) / 4 * 4;
+  return af_decode_plan_shared(plan + at, plan_ints - at, page_table, max_pages, slots, lens, plan + L.shared, batch, nq, nkv, n_splits, stream);
+}
+
+// out [batch, nq * hd] bfloat16 = attention of one new token per sequence over all its keys, the shared pages read once a
+// group.  bits 16: k, v are bfloat16 pages; 8: codes, with k_exp, v_exp.  own_scratch: af_attn_decode_scratch(batch, nq, hd,
+// n_splits) floats; pre_scratch: af_attn_shared_rows(...) * (hd + 2) floats; plan: af_attn_shared_plan's.
+AF_EXPORT int af_attn_decode_shared(void* out, long long out_stride, const void* q, long long q_stride, int bits, const void* k, const void* v,
+                                    const void* k_exp, const void* v_exp, long long n_pages, const int* page_table, int max_pages,
+                                    const int* slots, const int* lens, int batch, int nq, int nkv, int hd, float scale, float cap, int n_splits,
+                                    float* own_scratch, float* pre_scratch, const int* plan, const float* sinks, int* err,
+                                    cudaStream_t stream) {
+  if (batch == 0) return 0;
+  AF_REQUIRE(bits == 8 || bits == 16, "af_attn_decode_shared: a cache of 8 or 16 bits, not %d", bits);
+  AF_REQUIRE(nq > 0 && nkv > 0 && nq % nkv == 0 && batch > 0 && batch <= SH_MAX_BATCH, "af_attn_decode_shared: %d sequences, %d heads, %d groups",
+             batch, nq, nkv);
+  AF_REQUIRE(hd == 64 || hd == 128 || hd == 256, "af_attn_decode_shared: head_dim %d (takes 64, 128, 256)", hd);
+  AF_REQUIRE(q_stride % 8 == 0 && out_stride % 2 == 0 &&
+                 (((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)own_scratch | (uintptr_t)pre_scratch | (uintptr_t)plan) & 15) == 0 &&
+                 ((uintptr_t)out & 3) == 0,
+             "af_attn_decode_shared: rows must be 16-byte aligned (out: 4)");
+  AF_REQUIRE(own_scratch != nullptr && pre_scratch != nullptr && plan != nullptr, "af_attn_decode_shared: scratch and plan");
+  AF_REQUIRE(n_pages > 0 && n_pages * nkv * AF_PAGE < (1ll << 31), "af_attn_decode_shared: %lld cache pages", n_pages);
+  const int sms = af_sm_count();
+  if (sms <= 0) return -1;
+  const ShPlan L = sh_layout(batch, nq, nkv, sms);
+  const int at = (L.total + 3) / 4 * 4;
+  const long long rows = af_attn_shared_rows(batch, nq, nkv);
+  ShArgs a{(const __nv_bfloat16*)q, q_stride, (const uint8_t*)k, (const uint8_t*)v, (const uint8_t*)k_exp, (const uint8_t*)v_exp, n_pages,
+           page_table, plan, max_pages, batch, nq, nkv, scale, cap, pre_scratch, pre_scratch + rows * hd, err};
+  int rc;
+  if (bits == 16)
+    rc = hd == 64 ? launch_shared<64, 16>(a, k, v, sms, stream)
+                  : (hd == 128 ? launch_shared<128, 16>(a, k, v, sms, stream) : launch_shared<256, 16>(a, k, v, sms, stream));
+  else
+    rc = hd == 64 ? launch_shared<64, 8>(a, k, v, sms, stream)
+                  : (hd == 128 ? launch_shared<128, 8>(a, k, v, sms, stream) : launch_shared<256, 8>(a, k, v, sms, stream));
+  if (rc) return rc;
+  if (bits == 16)
+    rc = af_decode16_split(q, q_stride, k, v, n_pages, page_table, max_pages, slots, lens, plan + L.shared, batch, nq, nkv, hd, scale, cap,
+                           n_splits, own_scratch, plan + at, err, stream);
+  else
+    rc = af_decode8_split(q, q_stride, k, v, k_exp, v_exp, n_pages, page_table, max_pages, slots, lens, plan + L.shared, batch, nq, nkv, hd,
+                          scale, cap, 0, 0, 0, n_splits, own_scratch, plan + at, err, stream);
+  if (rc) return rc;
+  const auto merge = hd == 64 ? attn_shared_merge_kernel<64> : (hd == 128 ? attn_shared_merge_kernel<128> : attn_shared_merge_kernel<256>);
+  af_launch(merge, dim3(batch, nq), dim3(SHM_THREADS), 0, stream, (__nv_bfloat16*)out, out_stride, (const float*)a.part_o, (const float*)a.part_ml,
+            (const float*)own_scratch, (const float*)own_scratch + (size_t)batch * nq * n_splits * hd, nq, nkv, n_splits, plan, plan + at, sms,
+            sinks);
+  AF_CHECK_LAUNCH("af_attn_decode_shared (merge)");
+}

@@ -1054,11 +1054,60 @@ def attn_decode8(out, q, kv, batch, nq: int, nkv: int, hd: int, scale: float, ca
         _ptr(error_word(q.device), "err", torch.int32), _stream()))
 
 
+def attn_decode_shared_supported(dtype, hd: int, n_seqs: int) -> bool:
+    """Whether :func:`attn_decode_shared` reads shared pages once for these (else it is :func:`attn_decode`)."""
+    return dtype == torch.bfloat16 and hd in FAST_HEAD_SIZES and n_seqs <= ATTN_DECODE_MAX_SEQS
+
+
 def attn_decode_shared(out, q, kv, batch, nq: int, nkv: int, hd: int, scale: float, cap: float, lead, pages, most_pages: int,
                        sinks=None, gate=None) -> None:
     """Decode attention (all keys visible) of sequences that share their first pages: row b's first ``pages[b]`` cache pages
     are those of row ``lead[b]`` (int32 [B] each; rows that share nothing: 0 pages), ``most_pages`` the most that any row shares."""
-    attn_decode(out, q, kv, batch, nq, nkv, hd, scale, cap, 0, sinks=sinks, gate=gate)
+    B = batch.n_seqs
+    if lead.numel() != B or pages.numel() != B or most_pages < 0:
+        raise KernelError(f"attn_decode_shared: a lead and a number of pages for each of {B} rows")
+    eight = getattr(kv, "k_exp", None) is not None
+    if kv.ring_rows or kv.v is None or tuple(kv.v.shape) != tuple(kv.k.shape) or tuple(kv.k.shape[1:]) != (nkv, PAGE, hd):
+        raise KernelError(f"attn_decode_shared: pages [pages, {nkv}, {PAGE}, {hd}] of all keys and values (no ring)")
+    if (most_pages == 0 or not attn_decode_shared_supported(q.dtype, hd, B) or not (eight or kv.k.dtype == torch.bfloat16)
+            or q.stride(0) % 8 or q.data_ptr() % 16):
+        attn_decode(out, q, kv, batch, nq, nkv, hd, scale, cap, 0, sinks=sinks, gate=gate)
+        return
+    if out.dtype != torch.bfloat16 or tuple(out.shape) != (B, nq * hd) or q.shape[0] != B or q.shape[1] < nq * hd:
+        raise KernelError(f"attn_decode_shared: bfloat16 queries and out [{B}, {nq * hd}]")
+    if sinks is not None and sinks.numel() != nq:
+        raise KernelError(f"attn_decode_shared: {sinks.numel()} sinks for {nq} heads")
+    n_pages = _cache8_pages(kv, nkv, hd, "attn_decode_shared") if eight else kv.k.shape[0]
+    lib = _lib()
+    for f in (lib.af_attn_shared_plan_ints, lib.af_attn_shared_rows, lib.af_attn_decode_scratch):
+        f.restype = ctypes.c_longlong
+    table = kv.page_table
+    n = attn_decode_max_splits(B, nkv, batch.max_len_after, 0, nq=nq)
+    aux = getattr(batch, "aux", None)
+    key = ("attn_shared_plan", table.data_ptr(), nq, nkv, n, lead.data_ptr(), pages.data_ptr())
+    plan = aux.get(key) if aux is not None else None
+    if plan is None:
+        ints = lib.af_attn_shared_plan_ints(c_int(B), c_int(nq), c_int(nkv))
+        plan = torch.empty(max(ints, 0), dtype=torch.int32, device=q.device)
+        _check(lib.af_attn_shared_plan(
+            _ptr(plan, "plan", torch.int32), c_longlong(ints), _ptr(lead, "lead", torch.int32), _ptr(pages, "pages", torch.int32),
+            _ptr(table, "page_table", torch.int32), c_int(table.shape[1]), _ptr(batch.slots, "slots", torch.int32),
+            _ptr(batch.len_after, "lens", torch.int32), c_int(B), c_int(nq), c_int(nkv), c_int(n), _stream()))
+        if aux is not None:
+            aux[key] = plan
+    n_own = lib.af_attn_decode_scratch(c_int(B), c_int(nq), c_int(hd), c_int(n))
+    n_pre = lib.af_attn_shared_rows(c_int(B), c_int(nq), c_int(nkv)) * (hd + 2)
+    n_own = (n_own + 3) // 4 * 4
+    scratch = torch.empty(n_own + n_pre, dtype=torch.float32, device=q.device)
+    _check(lib.af_attn_decode_shared(
+        _ptr(out), c_longlong(_rows(out, "out")), _ptr(q), c_longlong(_rows(q, "q")), c_int(8 if eight else 16), _ptr(kv.k), _ptr(kv.v),
+        _ptr(kv.k_exp if eight else None, allow_none=True), _ptr(kv.v_exp if eight else None, allow_none=True), c_longlong(n_pages),
+        _ptr(table, "page_table", torch.int32), c_int(table.shape[1]), _ptr(batch.slots, "slots", torch.int32),
+        _ptr(batch.len_after, "lens", torch.int32), c_int(B), c_int(nq), c_int(nkv), c_int(hd), c_float(scale), c_float(cap), c_int(n),
+        _ptr(scratch, "scratch", torch.float32), _ptr(scratch[n_own:]), _ptr(plan, "plan", torch.int32),
+        _ptr(sinks, "sinks", torch.float32, allow_none=True), _ptr(error_word(q.device), "err", torch.int32), _stream()))
+    if gate is not None:
+        head_gate(out, gate, nq, hd)
 
 
 # ---------------------------------------------------------------- mixers with a state of fixed size
