@@ -12,6 +12,12 @@ first tokens in sight, their pages come before the ring's and stay.  Pages are t
 sequence grows and given back, with the slot, when it ends; both are used
 again by later sequences.
 
+A sequence can be *forked*: the new one has the same tokens in the cache.  Where all keys are kept it shares the whole pages (a
+page belongs to all of its owners and is free when the last gives it back); the page that is begun, the pages of a window and the
+state are copied.  Nothing ever writes a whole page again, so owners do not see each other.  Sequences that go back to one trunk are
+a *family*; ``shared_claims`` says for the rows of a step how many first pages they share, which decode attention then reads once
+(:func:`airframe_b200.kernels.attn_decode_shared`).
+
 Beside the pages lies per-sequence state of fixed size for mixers that ask
 for it: ``[runs, slots, *shape]``, zeroed when a slot is taken.
 
@@ -95,6 +101,27 @@ class KVGroup:
             self.table_host[slot, have + j] = p
         self.dirty.add(slot)
 
+    def pages_to_fork(self, length: int) -> int:
+        """Pages that a fork of a sequence of this length takes at once."""
+        if self.ring_rows:
+            return pages_for(self.rows_held(length))
+        return 1 if length % PAGE else 0
+
+    def fork(self, src: int, dst: int, length: int) -> None:
+        """Give ``dst`` (which holds nothing) the rows of ``src``: its whole pages shared, the others copied."""
+        n = pages_for(self.rows_held(length))
+        whole = 0 if self.ring_rows else length // PAGE
+        new = self.pages.take_many(n - whole)
+        for p in self.held[src][:whole]:
+            self.pages.share(p)
+        self.held[dst] = self.held[src][:whole] + new
+        self.table_host[dst, :n] = torch.tensor(self.held[dst], dtype=torch.int32)
+        self.dirty.add(dst)
+        for t in (self.k, self.v, self.k_exp, self.v_exp):
+            if t is not None:
+                for a, b in zip(self.held[src][whole:n], new):
+                    t[:, b].copy_(t[:, a])
+
     def release(self, slot: int) -> None:
         for p in self.held[slot]:
             self.pages.give_back(p)
@@ -172,6 +199,9 @@ class SequenceCache:
         self.slots = IndexPool(self.n_slots, "cache slot")
         self.lens = [0] * self.n_slots
         self.room = [0] * self.n_slots       # tokens that fit into the pages a slot holds in every group
+        # of forked sequences: slot -> (family, the first pages it shares with the family's trunk)
+        self._family: dict = {}
+        self._families = 0
         self.device = device
         self.dtype = dtype
         self.groups: dict = {}
@@ -239,9 +269,56 @@ class SequenceCache:
             raise PoolError(f"cache slot {slot} is not held (freed twice or never taken)")
         for g in self.groups.values():
             g.release(slot)
+        self._family.pop(slot, None)
         self.lens[slot] = 0
         self.room[slot] = 0
         self.slots.give_back(slot)
+
+    def fork(self, slot: int) -> int:
+        """A new slot whose sequence has the tokens of ``slot``'s, or an error and nothing changed.  The copies are queued on the
+        current stream, behind the steps that wrote what they copy."""
+        n = self.length(slot)
+        if n == 0:
+            raise ValueError(f"the sequence in slot {slot} has no tokens to share")
+        for g in self.groups.values():
+            if g.pages_to_fork(n) > g.pages.n_free:
+                raise CacheFull(f"{g.pages_to_fork(n)} more cache pages wanted, {g.pages.n_free} of {g.n_pages} free "
+                                f"(window {g.need.window})")
+        new = self.slots.take()
+        for g in self.groups.values():
+            g.fork(slot, new, n)
+        for st in self.states.values():
+            if st is not None:
+                st[new].copy_(st[slot])
+        self.lens[new] = n
+        self.room[new] = min((g.room(new) for g in self.groups.values()), default=self.max_context)
+        if slot not in self._family:
+            self._family[slot] = (self._families, 1 << 30)         # (the trunk shares all it has)
+            self._families += 1
+        family, pages = self._family[slot]
+        self._family[new] = (family, min(pages, n // PAGE))
+        return new
+
+    def shared_claims(self, slots):
+        """For the rows of a step (slots, -1 or None: none): (lead, pages, most): row i's first ``pages[i]`` pages are those of row
+        ``lead[i]`` in every group that keeps all keys, ``most`` the most pages that are read again and again without: a group's shared
+        pages times its rows but one.  None where no two rows share a page."""
+        if not self._family:
+            return None
+        rows: dict = {}
+        for i, s in enumerate(slots):
+            f = self._family.get(s)
+            if f is not None:
+                rows.setdefault(f[0], []).append((i, min(f[1], self.lens[s] // PAGE)))
+        lead, pages, saved = list(range(len(slots))), [0] * len(slots), 0
+        for members in rows.values():
+            n = min(p for _, p in members)
+            if len(members) < 2 or n == 0:
+                continue
+            for i, _ in members:
+                lead[i], pages[i] = members[0][0], n
+            saved += n * (len(members) - 1)
+        return (lead, pages, saved) if saved else None
 
     def length(self, slot: int) -> int:
         if not self.slots.is_held(slot):
@@ -282,13 +359,17 @@ class SequenceCache:
         for g in self.groups.values():
             g.flush()
 
-    def fits(self, token_counts) -> bool:
+    def fits(self, token_counts, shared=None) -> bool:
         """Whether sequences that come to hold these many tokens fit together:
         a slot each, and in every group the pages they hold there (a group with
-        a window holds at most its ring of a sequence)."""
+        a window holds at most its ring of a sequence).  ``shared``: of each
+        sequence the first tokens whose whole pages are another's (forks)."""
         if len(token_counts) > self.n_slots:
             return False
-        return all(sum(pages_for(g.rows_held(n)) for n in token_counts) <= g.n_pages for g in self.groups.values())
+        if shared is None:
+            shared = [0] * len(token_counts)
+        return all(sum(pages_for(g.rows_held(n)) - (0 if g.ring_rows else s // PAGE) for n, s in zip(token_counts, shared)) <= g.n_pages
+                   for g in self.groups.values())
 
     # ------------------------------------------------------------------ figures
 

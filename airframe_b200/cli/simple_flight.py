@@ -6,6 +6,8 @@ by default, generation stops at the end token, and it closes with "Flight
 Complete".  Prompts are token ids ("5,17,3"), positional or after
 ``--prompt-ids``; several prompts make a batch.  ``--random NAME`` runs a named
 configuration with seeded random weights instead of a folder.
+``--completions N`` makes N of every prompt, which runs once and whose cache
+they share; ``--kv-dtype float8_e4m3`` keeps keys and values in 8 bits.
 Sampling options carry the names of ``SamplingParams``
 (``src/runtime/gpu.rs:25-47``).
 """
@@ -45,6 +47,8 @@ def main(argv=None) -> int:
     ap.add_argument("--stop-token-id", type=int, action="append", default=[])
     ap.add_argument("--ignore-eos", action="store_true")
     ap.add_argument("--max-context", type=int, default=None)
+    ap.add_argument("--completions", type=int, default=1, metavar="N", help="completions of every prompt")
+    ap.add_argument("--kv-dtype", default=None, choices=["float8_e4m3"], help="keep keys and values in 8 bits (default: in --dtype)")
     ap.add_argument("--device", default="cuda:0")
     args = ap.parse_args(argv)
     if not args.model and not args.random:
@@ -61,7 +65,9 @@ def main(argv=None) -> int:
     for p in prompts:
         print(f"Tokens: {p}")
     print("Loading airframe_b200...")
-    need = sum((len(p) + args.max_tokens + 63) // 64 * 64 for p in prompts)
+    if args.completions < 1:
+        ap.error("--completions must be 1 or more")
+    need = args.completions * sum((len(p) + args.max_tokens + 63) // 64 * 64 for p in prompts)
     if args.random:
         from ..config import config_from_dict
         from ..config.presets import preset
@@ -70,15 +76,15 @@ def main(argv=None) -> int:
         except KeyError as e:
             ap.error(str(e.args[0]))
         rt = GpuRuntime.random(cfg, seed=args.seed, dtype=dtype, device=args.device, max_tokens=need,
-                               max_context=args.max_context, on_device=True)
+                               max_context=args.max_context, on_device=True, kv_dtype=args.kv_dtype)
     else:
         rt = GpuRuntime.load(args.model, dtype=dtype, device=args.device, max_tokens=need,
-                             max_context=args.max_context)
+                             max_context=args.max_context, kv_dtype=args.kv_dtype)
     print(f"Weights loaded: {len(rt.model.weight_decls())}")
     params = SamplingParams(max_tokens=args.max_tokens, temperature=args.temperature, top_p=args.top_p,
                             repetition_penalty=args.repetition_penalty, seed=args.seed,
                             stop_token_ids=list(args.stop_token_id), ignore_eos=args.ignore_eos)
-    single = len(prompts) == 1
+    single = len(prompts) == 1 and args.completions == 1
 
     def on_token(index, token):
         if single:
@@ -87,7 +93,9 @@ def main(argv=None) -> int:
     if single:
         print("\nOutput: ", end="", flush=True)
     t0 = time.time()
-    outs = rt.generate(prompts, params, on_token)
+    outs = rt.generate(prompts, params, on_token, completions=args.completions)
+    if args.completions > 1:
+        outs = [o for of_prompt in outs for o in of_prompt]
     dt = time.time() - t0
     if single:
         print()

@@ -23,6 +23,14 @@ class StepEntry:
 
 
 @dataclass
+class SharedPrefix:
+    """First cache pages that the sequences of a decode step share (of every layer that keeps all keys)."""
+    lead: torch.Tensor                  # int32 [B] the row whose first pages a row's are (its own: it shares none)
+    pages: torch.Tensor                 # int32 [B] how many
+    most_pages: int                     # host: the most that any row may share
+
+
+@dataclass
 class StepBatch:
     is_prefill: bool
     n_tokens: int
@@ -43,11 +51,13 @@ class StepBatch:
     # what parts make once per forward pass and share between layers (a table of rotary cosines and sines,
     # the tokens' rows in a group's cache pages); emptied when a pass begins
     aux: dict = field(default_factory=dict)
+    shared: Optional[SharedPrefix] = None         # a decode step of sequences that share their first pages
 
 
-def build_batch(entries, lens_before, device, pad_to: int = 0) -> StepBatch:
+def build_batch(entries, lens_before, device, pad_to: int = 0, claims=None) -> StepBatch:
     """Lay out ``entries`` (validated by the caller) on the device with one copy.
-    ``pad_to`` > B adds padding sequences (slot -1, token 0) to a decode step."""
+    ``pad_to`` > B adds padding sequences (slot -1, token 0) to a decode step.
+    ``claims``: (lead, pages) of a decode step's rows (see :class:`SharedPrefix`)."""
     is_prefill = all(n == 0 for n in lens_before)
     seq_lens = [len(e.tokens) for e in entries]
     B = len(entries)
@@ -72,7 +82,10 @@ def build_batch(entries, lens_before, device, pad_to: int = 0) -> StepBatch:
             len_after.append(0)
             starts.append(len(tokens))
     T, Bp, R = len(tokens), len(slots), len(want_rows)
-    flat = tokens + positions + seq_of + slots + len_after + starts + want_rows
+    lead, pages = [], []
+    if claims is not None:
+        lead, pages = list(claims[0]) + list(range(B, Bp)), list(claims[1]) + [0] * (Bp - B)
+    flat = tokens + positions + seq_of + slots + len_after + starts + want_rows + lead + pages
     host = torch.tensor(flat, dtype=torch.int32)
     if device.type == "cuda":
         host = host.pin_memory()
@@ -86,8 +99,11 @@ def build_batch(entries, lens_before, device, pad_to: int = 0) -> StepBatch:
         o += n
         return t
 
-    return StepBatch(
+    batch = StepBatch(
         is_prefill=is_prefill, n_tokens=T, n_seqs=Bp, max_len=max(seq_lens), seq_lens=seq_lens,
         tokens=cut(T), positions=cut(T), seq_of_token=cut(T), slots=cut(Bp), len_after=cut(Bp),
         seq_starts=cut(Bp + 1), want_rows=cut(R) if R else None, n_want=R,
         max_len_after=max(len_after), want_counts=[len(e.want) for e in entries])
+    if claims is not None:
+        batch.shared = SharedPrefix(cut(Bp), cut(Bp), max(pages))
+    return batch

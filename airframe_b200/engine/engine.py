@@ -15,7 +15,9 @@ import torch
 from .. import transfers
 
 from ..cache import PoolError, SequenceCache
-from .batch import StepBatch, StepEntry, build_batch
+from .. import kernels
+from ..kernels_const import PAGE
+from .batch import SharedPrefix, StepBatch, StepEntry, build_batch
 from .model import Model
 
 
@@ -53,6 +55,26 @@ class Engine:
 
     def free_slot(self, slot: int) -> None:
         self.cache.free_slot(slot)
+
+    def fork(self, slot: int, n: int = 1) -> list:
+        """``n`` new slots whose sequences go on from where ``slot``'s is.  Where all keys are kept its whole cache pages are
+        shared (memory, and in decode steps that carry several of them the pages' reading); the rest is copied.  All or none."""
+        if n < 1:
+            raise ValueError(f"a sequence is forked into one or more, not {n}")
+        new = []
+        try:
+            for _ in range(n):
+                new.append(self.cache.fork(slot))
+        except Exception:
+            for s in new:
+                self.cache.free_slot(s)
+            raise
+        return new
+
+    def _claims(self, slots):
+        """(lead, pages) of a decode step whose shared pages are worth the shared kernels, else None."""
+        claims = self.cache.shared_claims(slots)
+        return claims[:2] if claims is not None and claims[2] >= kernels.SHARED_PAGES_FROM else None
 
     def length(self, slot: int) -> int:
         return self.cache.length(slot)
@@ -112,7 +134,8 @@ class Engine:
             if not borrow:
                 logits = logits.clone()
         else:
-            batch = build_batch(entries, lens, self.device, pad_to=pad_to)
+            claims = self._claims([e.slot for e in entries]) if lens[0] > 0 else None
+            batch = build_batch(entries, lens, self.device, pad_to=pad_to, claims=claims)
             logits = self.model.forward(batch, self.cache, probe, greedy=greedy)
         self.cache.commit(growth)
         return logits
@@ -177,9 +200,12 @@ class Engine:
         B = len(slots)
         Bp = self.padded_batch(B)
         key = (Bp, "greedy") if greedy else Bp
+        claims = self._claims(slots)
+        if claims is not None:              # (a graph of its own: its attention is the shared prefix's)
+            key = (Bp, "greedy" if greedy else "logits", "shared")
         g = self._graphs.get(key)
         if g is None:
-            g = self._capture(Bp, greedy)
+            g = self._capture(Bp, greedy, claims is not None)
             self._graphs[key] = g
         # two pinned staging buffers in turn: one may still be in flight when the next step is laid out
         k = g["turn"] = g["turn"] ^ 1
@@ -195,6 +221,9 @@ class Engine:
             lay[Bp + B:2 * Bp] = 0
             lay[2 * Bp + B:3 * Bp] = -1
             lay[3 * Bp + B:] = 0
+        if claims is not None:                # (the rows behind the sequences share nothing)
+            lay[4 * Bp:5 * Bp] = claims[0] + list(range(B, Bp))
+            lay[5 * Bp:] = claims[1] + [0] * (Bp - B)
         g["dynamic"].copy_(host, non_blocking=True)
         transfers.count_h2d(host)
         sent.record()
@@ -205,19 +234,22 @@ class Engine:
         self._last_graph = g
         return g["logits"][:B]
 
-    def _capture(self, Bp: int, greedy: bool = False) -> dict:
+    def _capture(self, Bp: int, greedy: bool = False, shared: bool = False) -> dict:
         dev = self.device
-        # [tokens | positions | slots | len_after] change every step; the rest is fixed
-        dynamic = torch.zeros(4 * Bp, dtype=torch.int32, device=dev)
+        # [tokens | positions | slots | len_after] (and [lead | pages]) change every step; the rest is fixed
+        width = (6 if shared else 4) * Bp
+        dynamic = torch.zeros(width, dtype=torch.int32, device=dev)
         dynamic[2 * Bp: 3 * Bp] = -1
         fixed = torch.cat([torch.arange(Bp, dtype=torch.int32), torch.arange(Bp + 1, dtype=torch.int32),
                            torch.arange(Bp, dtype=torch.int32)]).to(dev)
         batch = StepBatch(
             is_prefill=False, n_tokens=Bp, n_seqs=Bp, max_len=1, seq_lens=[1] * Bp,
             tokens=dynamic[:Bp], positions=dynamic[Bp: 2 * Bp], seq_of_token=fixed[:Bp],
-            slots=dynamic[2 * Bp: 3 * Bp], len_after=dynamic[3 * Bp:], seq_starts=fixed[Bp: 2 * Bp + 1],
+            slots=dynamic[2 * Bp: 3 * Bp], len_after=dynamic[3 * Bp: 4 * Bp], seq_starts=fixed[Bp: 2 * Bp + 1],
             want_rows=fixed[2 * Bp + 1:], n_want=Bp,
             max_len_after=self.max_context)          # kernels size their splits for the longest context
+        if shared:
+            batch.shared = SharedPrefix(dynamic[4 * Bp: 5 * Bp], dynamic[5 * Bp:], self.max_context // PAGE)
         # a run outside the graph first: kernels set their attributes and load lazily
         side = torch.cuda.Stream(device=dev)
         side.wait_stream(torch.cuda.current_stream(dev))
@@ -225,13 +257,12 @@ class Engine:
             self.model.forward(batch, self.cache, greedy=greedy)
         torch.cuda.current_stream(dev).wait_stream(side)
         torch.cuda.synchronize(dev)
-        from .. import kernels
         graph = torch.cuda.CUDAGraph()
         n0 = kernels.launch_count()
         with torch.cuda.graph(graph):
             logits = self.model.forward(batch, self.cache, greedy=greedy)
         return {"graph": graph, "dynamic": dynamic, "logits": logits, "batch": batch, "fixed": fixed,
                 "launches": kernels.launch_count() - n0, "turn": 0,
-                "host": (hosts := [torch.empty(4 * Bp, dtype=torch.int32).pin_memory() for _ in range(2)]),
+                "host": (hosts := [torch.empty(width, dtype=torch.int32).pin_memory() for _ in range(2)]),
                 "host_np": [h.numpy() for h in hosts],
                 "sent": [torch.cuda.Event() for _ in range(2)]}

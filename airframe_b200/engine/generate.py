@@ -24,6 +24,10 @@ applies in time; a stop token it sees one step late: that sequence's next
 step is already queued, its result is dropped and nothing of it is emitted.
 The tokens are the same either way.
 
+Several ``completions`` of every prompt: the prompt runs once and the others are forks of it (``engine.fork``): they share its
+cache pages, and decode steps read these once for all.  Completion c of prompt i is request i * completions + c, with a
+generator and an end of its own.
+
 A ``logits_processor`` is the loop's control hook (reference: ``InferenceControl::intervene``
 with its decisions Allow / ForceToken / EarlyExit / BlockAndTerminate, ``src/control.rs:29-52``,
 applied per token at ``src/runtime/engine.rs:183-205``).  It is called for every live
@@ -39,6 +43,8 @@ from __future__ import annotations
 
 from dataclasses import dataclass, field
 from typing import Callable, Optional
+
+import torch
 
 from ..kernels_const import PAGE
 from .batch import StepEntry
@@ -63,6 +69,7 @@ class _Sequence:
     state: object = None
     out: list = field(default_factory=list)
     length: int = 0            # tokens in the cache
+    trunk: Optional[int] = None    # a completion that goes on from another's prompt: that one's place in the batch
     finish: Optional[str] = None
 
 
@@ -98,8 +105,9 @@ class GenerationLoop:
         """The most tokens a request can come to hold."""
         return min(prompt_len + max(params.max_tokens - 1, 0), self.engine.max_context)
 
-    def plan_batches(self, prompts, params) -> list:
-        """Requests in order, as many to a batch as slots and cache pages allow."""
+    def plan_batches(self, prompts, params, completions: int = 1) -> list:
+        """Requests in order, as many to a batch as slots and cache pages allow (completions of one prompt in a batch hold its
+        whole pages once, where the cache says so)."""
         total_pages = self.engine.cache.total_pages
         limit = self.engine.cache.n_slots
         if self.max_batch:
@@ -107,16 +115,26 @@ class GenerationLoop:
         # a cache whose groups of layers have storage of their own answers for each of them
         fits = getattr(self.engine.cache, "fits", None)
         batches, cur, cur_pages = [], [], 0
+
+        def shares(i, batch):
+            """Tokens of request i whose pages an earlier completion of the same prompt in the batch holds."""
+            return len(prompts[i]) if fits is not None and any(j // completions == i // completions for j in batch if j < i) else 0
+
+        def together(batch):
+            if completions == 1:
+                return fits([self.tokens_held(len(prompts[j]), params) for j in batch])
+            return fits([self.tokens_held(len(prompts[j]), params) for j in batch], [shares(j, batch) for j in batch])
+
         for i, p in enumerate(prompts):
             held = self.tokens_held(len(p), params)
             need = _pages(held)
             if need > total_pages or (fits is not None and not fits([held])):
                 raise RequestError(f"request {i} needs {need} cache pages, the cache has {total_pages}")
-            if cur and (len(cur) >= limit or cur_pages + need > total_pages
-                        or (fits is not None and not fits([self.tokens_held(len(prompts[j]), params) for j in cur]
-                                                          + [held]))):
+            need -= shares(i, cur) // PAGE
+            if cur and (len(cur) >= limit or cur_pages + need > total_pages or (fits is not None and not together(cur + [i]))):
                 batches.append(cur)
                 cur, cur_pages = [], 0
+                need = _pages(held)
             cur.append(i)
             cur_pages += need
         if cur:
@@ -126,12 +144,16 @@ class GenerationLoop:
     # ------------------------------------------------------------------ running
 
     def generate(self, prompts, params, on_token: Optional[Callable] = None,
-                 logits_processor: Optional[Callable] = None) -> list:
-        """New token ids per request, in request order.  ``on_token(request
+                 logits_processor: Optional[Callable] = None, completions: int = 1) -> list:
+        """New token ids per request, in request order (with ``completions`` of
+        every prompt: the first prompt's, then the second's, ...).  ``on_token(request
         index, token id)`` is called for every emitted token;
         ``logits_processor(request index, step, logits row, tokens so far)``
         before every choice (see the module's text)."""
+        if completions < 1:
+            raise RequestError(f"one completion of a prompt or more, not {completions}")
         self.check(prompts, params)
+        prompts = [p for p in prompts for _ in range(completions)]
         results = [[] for _ in prompts]
         self.finish_reasons = [None] * len(prompts)
         self.batches_run = []
@@ -141,12 +163,17 @@ class GenerationLoop:
         stops = set(params.stop_token_ids)
         if not params.ignore_eos:
             stops |= self.model_stop_ids
-        for batch in self.plan_batches(prompts, params):
+        for batch in self.plan_batches(prompts, params, completions):
             self.batches_run.append(list(batch))
             seqs = [_Sequence(i, list(prompts[i])) for i in batch]
+            trunks: dict = {}
+            for r, s in enumerate(seqs):
+                first = trunks.setdefault(s.index // completions, r)
+                s.trunk = first if first != r else None
             try:
                 for s in seqs:
-                    s.slot = self.engine.take_slot()
+                    if s.trunk is None:
+                        s.slot = self.engine.take_slot()
                     s.state = self.sampler.new_state(params, s.index)
                 self._run_batch(seqs, params, stops, on_token, logits_processor)
             finally:
@@ -158,6 +185,21 @@ class GenerationLoop:
                 results[s.index] = s.out
                 self.finish_reasons[s.index] = s.finish
         return results
+
+    def _start(self, seqs, **kw):
+        """The step of a batch's prompts; then the completions that go on from another's prompt are forked from it.  Returns the
+        result (logits or tokens) of every sequence."""
+        own = [s for s in seqs if s.trunk is None]
+        result = self.engine.step([StepEntry(s.slot, s.prompt, [len(s.prompt) - 1]) for s in own], **kw)
+        for s in seqs:
+            s.length = len(s.prompt)
+            if s.trunk is not None:
+                s.slot = self.engine.fork(seqs[s.trunk].slot)[0]
+        if len(own) < len(seqs):
+            place = {id(s): r for r, s in enumerate(own)}
+            rows = [place[id(s if s.trunk is None else seqs[s.trunk])] for s in seqs]
+            result = result[torch.tensor(rows, device=result.device)]
+        return result
 
     def _end(self, s: _Sequence, reason: str) -> None:
         s.finish = reason
@@ -175,9 +217,7 @@ class GenerationLoop:
 
     def _run_batch_in_step(self, seqs, params, stops, on_token, processor=None) -> None:
         """Every step waits for the tokens of the step before."""
-        logits = self.engine.step([StepEntry(s.slot, s.prompt, [len(s.prompt) - 1]) for s in seqs])
-        for s in seqs:
-            s.length = len(s.prompt)
+        logits = self._start(seqs)
         active = list(seqs)
         while active:
             decisions = [None] * len(active)
@@ -229,9 +269,7 @@ class GenerationLoop:
         # not logits, and the sampler only brings them to the host
         fused = bool(params.greedy and getattr(eng, "fused_greedy", False) and hasattr(smp, "adopt"))
         kw = {"greedy": True} if fused else {}
-        logits = eng.step([StepEntry(s.slot, s.prompt, [len(s.prompt) - 1]) for s in seqs], **kw)
-        for s in seqs:
-            s.length = len(s.prompt)
+        logits = self._start(seqs, **kw)
         n = len(seqs)
         sampled = [1] * n                       # samples asked for per row, the one in flight included
         pend = (smp.adopt(logits, [s.state for s in seqs]) if fused

@@ -26,10 +26,14 @@ def _build_layers(spec: ModelSpec, ctx: BuildContext):
 
 
 class Model:
-    def __init__(self, spec: ModelSpec, compute_dtype=torch.bfloat16, device="cuda:0"):
+    def __init__(self, spec: ModelSpec, compute_dtype=torch.bfloat16, device="cuda:0", kv_dtype=None):
+        """``kv_dtype``: None, or float8_e4m3fn: the layers' keys and values are kept in 8 bits where their mixer can
+        (``attention``; others keep the compute dtype)."""
         spec.validate()
+        if kv_dtype not in (None, torch.float8_e4m3fn):
+            raise ConfigError(f"kv_dtype must be float8_e4m3fn or None, got {kv_dtype}")
         self.spec = spec
-        self.ctx = BuildContext(compute_dtype=compute_dtype, device=torch.device(device))
+        self.ctx = BuildContext(compute_dtype=compute_dtype, device=torch.device(device), kv_dtype=kv_dtype)
         self.embedding = build_part("embedding", spec.embedding, self.ctx)
         self.blocks = _build_layers(spec, self.ctx)
         self.junctions = [build_part("junction", j, self.ctx) for j in spec.junctions]
@@ -40,6 +44,8 @@ class Model:
             if getattr(b, "streams", 1) != self.streams:
                 raise ConfigError(f"a block of kind '{b.kind}' keeps {getattr(b, 'streams', 1)} residual streams, "
                                   f"the model {self.streams}")
+        if kv_dtype is not None and not any(n[0] is not None and n[0].eight_bits for n in self.cache_needs()):
+            raise ConfigError("kv_dtype: no layer of this model keeps keys and values that 8 bits can hold")
         self.loaded = False
         self.prompts_as_one = False      # (a prompt's layers launched by one call: see parts/prompt_run.py)
 

@@ -27,6 +27,14 @@ def _dtype(name) -> torch.dtype:
     return _DTYPES[name]
 
 
+def _kv_dtype(name):
+    if name is None or name == torch.float8_e4m3fn:
+        return name
+    if name in ("float8_e4m3", "fp8"):
+        return torch.float8_e4m3fn
+    raise ValueError(f"kv_dtype must be None (the compute dtype) or 'float8_e4m3', got {name!r}")
+
+
 def _require_gpu(device) -> torch.device:
     device = torch.device(device)
     if device.type != "cuda" or not torch.cuda.is_available():
@@ -47,14 +55,16 @@ class GpuRuntime:
     # ------------------------------------------------------------------ construction
 
     @classmethod
-    def _build(cls, config, source, dtype, device, max_tokens, max_context, max_sequences, spec_edit=None):
+    def _build(cls, config, source, dtype, device, max_tokens, max_context, max_sequences, spec_edit=None,
+               kv_dtype=None):
         device = _require_gpu(device)
         dt = _dtype(dtype)
+        kv_dtype = _kv_dtype(kv_dtype)
         torch.cuda.set_device(device)
         spec = config.model_spec()
         if spec_edit is not None:
             spec_edit(spec)
-        model = Model(spec, dt, device)
+        model = Model(spec, dt, device, kv_dtype)
         model.load(load_weights(source, model.weight_decls(), dt, device))
         limit = model.spec.max_positions
         ctx = min(max_context or DEFAULT_SAFE_CTX, limit)
@@ -63,35 +73,41 @@ class GpuRuntime:
 
     @classmethod
     def load(cls, path, dtype="bfloat16", device="cuda:0", max_tokens: Optional[int] = None,
-             max_context: Optional[int] = None, max_sequences: Optional[int] = None, spec_edit=None) -> "GpuRuntime":
+             max_context: Optional[int] = None, max_sequences: Optional[int] = None, spec_edit=None, kv_dtype=None) -> "GpuRuntime":
         """Load a model folder (config.json, model.safetensors).  ``max_tokens``
         sizes the cache: the most tokens that live sequences hold together.
         ``spec_edit(spec)`` may change the :class:`~airframe_b200.config.ModelSpec`
-        before the model is built (options of parts that config.json does not carry)."""
+        before the model is built (options of parts that config.json does not carry).  ``kv_dtype``: None, or
+        "float8_e4m3": keys and values are kept in 8 bits by the layers that can (twice the tokens in the same memory, half
+        the bytes of a decode step's attention; see ``csrc/cache8.cuh``)."""
         config = config_from_folder(path)
         source = SafetensorsFolder(path)
         try:
-            return cls._build(config, source, dtype, device, max_tokens, max_context, max_sequences, spec_edit)
+            return cls._build(config, source, dtype, device, max_tokens, max_context, max_sequences, spec_edit, kv_dtype)
         finally:
             source.close()
 
     @classmethod
     def random(cls, config: ModelConfig, seed: int = 0, dtype="bfloat16", device="cuda:0",
                max_tokens: Optional[int] = None, max_context: Optional[int] = None,
-               max_sequences: Optional[int] = None, on_device: bool = False, spec_edit=None) -> "GpuRuntime":
+               max_sequences: Optional[int] = None, on_device: bool = False, spec_edit=None, kv_dtype=None) -> "GpuRuntime":
         """A model of ``config`` with seeded random weights, without a folder.
         ``on_device`` draws them on the GPU (fast for large models; the values
         then differ from a folder written with the same seed)."""
         decls = Model(config.model_spec(), torch.bfloat16, "cpu").weight_decls()
         store = torch.float32 if _dtype(dtype) == torch.float32 else torch.bfloat16
         source = RandomSource(decls, seed, store_dtype=store, device=device if on_device else "cpu")
-        return cls._build(config, source, dtype, device, max_tokens, max_context, max_sequences, spec_edit)
+        return cls._build(config, source, dtype, device, max_tokens, max_context, max_sequences, spec_edit, kv_dtype)
 
     # ------------------------------------------------------------------ use
 
-    def generate(self, prompt, params=None, on_token=None, logits_processor=None):
+    def generate(self, prompt, params=None, on_token=None, logits_processor=None, completions: int = 1):
         """``prompt``: token ids of one request, or a list of such lists.
         Returns the new token ids (a list, or a list of lists).
+        ``completions`` > 1: so many for every prompt, each drawn with a generator of
+        its own (with greedy decoding they are alike); the prompt runs once and its
+        cache is shared.  A prompt's result is then the list of its completions, and
+        completion c of prompt i has the request index i * completions + c.
         ``on_token(request index, token id)`` sees every emitted token;
         ``logits_processor`` is the control hook of
         :mod:`airframe_b200.engine.generate` (the reference's third argument of
@@ -104,7 +120,9 @@ class GpuRuntime:
         params = params or SamplingParams()
         single = len(prompt) > 0 and isinstance(prompt[0], int)
         out = self._loop.generate([list(prompt)] if single else [list(p) for p in prompt], params, on_token,
-                                  logits_processor)
+                                  logits_processor, completions)
+        if completions > 1:
+            out = [out[i: i + completions] for i in range(0, len(out), completions)]
         return out[0] if single else out
 
     def step(self, entries, probe=None):

@@ -1054,6 +1054,11 @@ def attn_decode8(out, q, kv, batch, nq: int, nkv: int, hd: int, scale: float, ca
         _ptr(error_word(q.device), "err", torch.int32), _stream()))
 
 
+# From how many cache pages on that a decode step need not read again (a group's shared pages times its sequences but one) the
+# shared kernels are taken.
+SHARED_PAGES_FROM = 64
+
+
 def attn_decode_shared_supported(dtype, hd: int, n_seqs: int) -> bool:
     """Whether :func:`attn_decode_shared` reads shared pages once for these (else it is :func:`attn_decode`)."""
     return dtype == torch.bfloat16 and hd in FAST_HEAD_SIZES and n_seqs <= ATTN_DECODE_MAX_SEQS

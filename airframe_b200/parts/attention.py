@@ -15,6 +15,10 @@ before any rotation) and values taken from the raw key projection (no
 projection goes into 32-bit rows and one kernel norms, rotates, packs
 [q | k | v] and writes the cache.
 
+With a cache of 8 bits (``kv_dtype`` of the build context) the mixer stores its rows as e4m3 codes with a power of two a row
+and attends over those; a prompt attends over its own rows as they are kept, so that it makes no difference in how many
+steps its tokens came.
+
 More options that go the same way: biases of the q, k and v projections; q and k
 divided by their root mean square per head *after* the rotation (no weight); values
 of another size than the keys (``value_dim``); a chunked mask (``mask`` = "chunk": a
@@ -125,6 +129,12 @@ class Attention(Mixer):
             fit = next((p for p in kernels.FAST_HEAD_SIZES if p >= big), 0)
             if fit and fit <= 2 * big and (fit != self.hd or fit != self.dv):
                 self.pad = fit
+        self.eight_bits = ctx.kv_dtype is not None
+        if self.eight_bits:
+            size, value = (self.pad, self.pad) if self.pad else (self.hd, self.dv)
+            if ctx.compute_dtype != torch.bfloat16 or size not in kernels.CACHE8_HEAD_SIZES or value != size:
+                raise ConfigError(f"attention: a cache of 8 bits goes with bfloat16 and keys and values of one size in "
+                                  f"{kernels.CACHE8_HEAD_SIZES}, not with {ctx.compute_dtype}, {size} and {value}")
         self.q_norm_w = self.k_norm_w = self.bias = self.sinks = None
         self.w_qkv = None
         self.w_o = None
@@ -133,8 +143,8 @@ class Attention(Mixer):
     def kv_need(self):
         # (a chunk's keys all lie within the last ``window`` positions: the ring of a window serves it)
         if self.pad:
-            return KVNeed(self.nkv, self.pad, self.window, keep_first=self.keep)
-        return KVNeed(self.nkv, self.hd, self.window, None if self.dv == self.hd else self.dv, self.keep)
+            return KVNeed(self.nkv, self.pad, self.window, keep_first=self.keep, eight_bits=self.eight_bits)
+        return KVNeed(self.nkv, self.hd, self.window, None if self.dv == self.hd else self.dv, self.keep, self.eight_bits)
 
     def weight_decls(self):
         q, k, v, o = self.names
@@ -180,7 +190,7 @@ class Attention(Mixer):
         # bfloat16 with a head size and a K that the tensor-core product takes: the rows of every head in the
         # order in which the product's epilogue rotates pairs and writes the cache (used only when the position
         # encoding says, step by step, that it is such a rotation)
-        self.rope_epilogue = (bool(self.params.get("rope_epilogue")) and not self.packs and dt == torch.bfloat16 and self.hd % 32 == 0
+        self.rope_epilogue = (bool(self.params.get("rope_epilogue")) and not self.packs and not self.eight_bits and dt == torch.bfloat16 and self.hd % 32 == 0
                               and self.hidden % 8 == 0 and self.w_qkv.is_cuda
                               and self.position.rotates_half_pairs(self.hd))
         if self.rope_epilogue:
@@ -194,7 +204,8 @@ class Attention(Mixer):
 
     def decode_bytes(self, lens) -> int:
         weights = (self.w_qkv.numel() + self.w_o.numel()) * self._el()
-        kv_row = self.nkv * (2 * self.pad if self.pad else self.hd + self.dv) * self._el()
+        values = 2 * self.pad if self.pad else self.hd + self.dv
+        kv_row = self.nkv * (values + 2 if self.eight_bits else values * self._el())
         return weights + sum(kv_row * self._visible(n - 1) for n in lens)
 
     def _visible(self, pos: int) -> int:
@@ -259,7 +270,7 @@ class Attention(Mixer):
             rope.rotary_dim if rope is not None else 0, rope.pairing if rope is not None else "half",
             q_weight=self.q_norm_w, k_weight=self.k_norm_w,
             eps=float(self.qk_norm["eps"]) if self.qk_norm is not None else 0.0,
-            v_from_k=self.v_from_k, kv=view.kv if view.writes else None, bias=self.bias,
+            v_from_k=self.v_from_k, kv=view.kv if view.writes and not self.eight_bits else None, bias=self.bias,
             norm_after=self.norm_after, magnitude=rope.magnitude if rope is not None else 1.0, dv=self.dv,
             pitch=self.pad, whole_norm=self.norm_whole,
             table=rope.precise_table(batch) if rope is not None else None)
@@ -285,7 +296,7 @@ class Attention(Mixer):
                 qkv = torch.empty(x.shape[0], (nq + 2 * nkv) * hd, dtype=x.dtype, device=x.device)
             # positions into q and k, then k and v into the cache: the store is this mixer's; an encoding
             # that can do both in one kernel says so
-            if not view.writes:
+            if not view.writes or self.eight_bits:
                 self.position.encode(qkv, batch, nq, nkv, hd, parts=parts)
             elif not self.position.encode_and_store(qkv, batch, nq, nkv, hd, kv, parts=parts):
                 self.position.encode(qkv, batch, nq, nkv, hd, parts=parts)
@@ -297,6 +308,11 @@ class Attention(Mixer):
         q = qkv[:, : nq * hd]
         k = qkv[:, nq * hd: (nq + nkv) * hd]
         v = qkv[:, (nq + nkv) * hd:]
+        if self.eight_bits and view.writes:
+            rounded = torch.empty(x.shape[0], 2 * nkv * hd, dtype=x.dtype, device=x.device) if batch.is_prefill else None
+            kernels.store_kv8(qkv, batch, nq, nkv, hd, kv, rounded=rounded)
+            if batch.is_prefill:
+                k, v = rounded[:, : nkv * hd], rounded[:, nkv * hd:]
         ctx = torch.empty(x.shape[0], nq * dv, dtype=x.dtype, device=x.device)
         window = self.window or 0
         more = {"dv": dv, "mask": self.mask, "sinks": self.sinks, "gate": gate}
@@ -307,6 +323,10 @@ class Attention(Mixer):
                 batch.step_kv[view.cache_id] = (k.clone(), v.clone())
             kernels.attn_prefill(ctx, q, k, v, batch, nq, nkv, hd, self.scale, self.softcap, window, slopes,
                                  keep=self.keep, **more)
+        elif batch.shared is not None and not window and slopes is None and dv == hd:
+            s = batch.shared
+            kernels.attn_decode_shared(ctx, q, kv, batch, nq, nkv, hd, self.scale, self.softcap, s.lead, s.pages, s.most_pages,
+                                       sinks=self.sinks, gate=gate)
         else:
             kernels.attn_decode(ctx, q, kv, batch, nq, nkv, hd, self.scale, self.softcap, window, slopes, **more)
         return linear_split(ctx, self.w_o, wide=bool(self.params.get("wide_output", False)), prompt=of_prompt(batch))

@@ -51,6 +51,8 @@ class BuildContext:
     """What every part is told besides its own parameters."""
     compute_dtype: torch.dtype      # bfloat16 or float32: activations, matrices, cache
     device: torch.device
+    # None: keys and values are kept in the compute dtype; float8_e4m3fn: parts that can, keep them in 8 bits
+    kv_dtype: Optional[torch.dtype] = None
 
 
 def build_part(category: str, spec: PartSpec, ctx: BuildContext, **children):

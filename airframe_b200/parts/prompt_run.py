@@ -39,7 +39,7 @@ def _alike(block):
         return None
     norms = [block.norms[r] for r in SandwichBlock.roles]
     rope = m.position
-    fits = (block.ctx.compute_dtype == torch.bfloat16 and not (m.packs or m.pad or m.rope_epilogue or m.sinks is not None)
+    fits = (block.ctx.compute_dtype == torch.bfloat16 and not (m.eight_bits or m.packs or m.pad or m.rope_epilogue or m.sinks is not None)
             and m.mask == "window" and f.interleaved and f.w_gu.shape[0] == 2 * f.inter
             and not (m.params.get("wide_output") or f.params.get("wide_output"))
             and all(type(n) is RmsNorm and n.offset == norms[0].offset for n in norms)

@@ -126,7 +126,13 @@ class Rope(PositionEncoding):
         if self.rotary_dim > hd:
             raise ConfigError(f"rope: rotary_dim {self.rotary_dim} exceeds head_dim {hd}")
         kernels.rope_cache_write(qkv, batch.positions, self.inv_freq, nq, nkv, hd, self.rotary_dim,
-                                 self.pairing, parts=parts)
+                                 self.pairing, parts=parts, table=self._prompt_table(qkv, batch, hd, parts))
+
+    def _prompt_table(self, qkv, batch, hd, parts):
+        """Many rows (a prompt): the cosines and sines come from the step's table, made once for all layers."""
+        if qkv.shape[0] >= kernels.ROPE_TABLE_ROWS and parts is None and self.rotates_half_pairs(hd):
+            return self.rotary_table(batch, hd)
+        return None
 
     def encode_and_store(self, qkv, batch, nq, nkv, hd, kv, parts=None) -> bool:
         """The rotation and the mixer's cache store as one kernel (the rotated
@@ -134,11 +140,7 @@ class Rope(PositionEncoding):
         self._plain_only()
         if self.rotary_dim > hd:
             raise ConfigError(f"rope: rotary_dim {self.rotary_dim} exceeds head_dim {hd}")
-        # many rows (a prompt): the cosines and sines come from the step's table, made once for all layers
-        table = None
-        if (qkv.shape[0] >= kernels.ROPE_TABLE_ROWS and parts is None
-                and self.rotates_half_pairs(hd)):
-            table = self.rotary_table(batch, hd)
+        table = self._prompt_table(qkv, batch, hd, parts)
         kernels.rope_cache_write(qkv, batch.positions, self.inv_freq, nq, nkv, hd, self.rotary_dim,
                                  self.pairing, seq_of_token=batch.seq_of_token, slots=batch.slots,
                                  len_after=batch.len_after, kcache=kv.k, vcache=kv.v,

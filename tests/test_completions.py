@@ -1,0 +1,330 @@
+"""Forked sequences and caches of 8 bits through the engine, the generation loop and the command line: what the cache keeps of
+them, that they give what separate sequences give, and that a prompt runs once."""
+import pytest
+import torch
+
+import plain_gemma2 as plain
+import replay
+import tiny_fiferax
+import tiny_retudra
+from test_cache8 import quantise, values
+from test_generate_loop import FakeEngine, P, ScriptSampler
+from tiny import CONFIGS, WIDE_D, make_folder
+from tolerances import BF16_SPLITS, FP32_SPLITS, VS_PLAIN, rel_err
+
+from airframe_b200.cache import CacheFull, IndexPool, PoolError, SequenceCache
+from airframe_b200.config import ConfigError, config_from_dict
+from airframe_b200.engine import GenerationLoop, Model, RequestError, StepEntry
+from airframe_b200.parts import KVNeed, StateNeed
+
+F8 = torch.float8_e4m3fn
+
+
+# ---------------------------------------------------------------------------------------------- bookkeeping, no GPU
+
+def test_pool_shares_and_gives_back():
+    p = IndexPool(3, "page")
+    a = p.take()
+    p.share(a)
+    p.share(a)
+    assert p.owners(a) == 3 and p.n_held == 1 and p.owners(2) == 0
+    p.give_back(a)
+    p.give_back(a)
+    assert p.is_held(a) and p.n_free == 2
+    p.give_back(a)
+    assert not p.is_held(a) and p.n_free == 3
+    with pytest.raises(PoolError):
+        p.give_back(a)
+    with pytest.raises(PoolError):
+        p.share(a)
+
+
+def test_fork_shares_whole_pages_and_copies_the_rest():
+    full, ring, eight = KVNeed(2, 16), KVNeed(1, 8, 100, keep_first=3), KVNeed(1, 64, eight_bits=True)
+    c = SequenceCache([(full, None, None), (ring, StateNeed((3,)), None), (eight, (StateNeed((2, 2)), StateNeed((1,), "int32")), None)], 64 * 40, 1024,
+                      torch.float32, "cpu", max_sequences=4)
+    a = c.take_slot()
+    c.reserve({a: 150})
+    c.commit({a: 150})
+    for g in c.groups.values():
+        for t in (g.k, g.v):
+            t.copy_(torch.randint(0, 100, t.shape).to(t.dtype))
+        if g.k_exp is not None:
+            g.k_exp.random_(0, 255)
+            g.v_exp.random_(0, 255)
+    for st in c.states.values():
+        if st is not None:
+            st.copy_(torch.randint(0, 9, st.shape))
+    free = {n: g.pages.n_free for n, g in c.groups.items()}
+    b = c.fork(a)
+    assert c.length(b) == 150
+    f, r, e = c.groups[full], c.groups[ring], c.groups[eight]
+    assert f.held[b][:2] == f.held[a][:2] and f.held[b][2] != f.held[a][2] and f.pages.owners(f.held[a][0]) == 2
+    assert not set(r.held[a]) & set(r.held[b]) and len(r.held[b]) == len(r.held[a]) == 3
+    assert free[full] - f.pages.n_free == 1 and free[ring] - r.pages.n_free == 3
+    for g in c.groups.values():
+        assert g.table_host[b, : len(g.held[b])].tolist() == g.held[b]
+        for x, y in zip(g.held[a], g.held[b]):
+            assert torch.equal(g.k[:, x].float(), g.k[:, y].float()) and torch.equal(g.v[:, x].float(), g.v[:, y].float())
+            if g.k_exp is not None:
+                assert torch.equal(g.k_exp[:, x], g.k_exp[:, y]) and torch.equal(g.v_exp[:, x], g.v_exp[:, y])
+    for st in c.states.values():
+        if st is not None:
+            assert torch.equal(st[a], st[b])
+    # the original ends: the shared pages stay with the fork, and are free when it ends too
+    c.free_slot(a)
+    assert f.pages.owners(f.held[b][0]) == 1
+    c.reserve({b: 193})
+    c.free_slot(b)
+    assert all(g.pages.n_held == 0 for g in c.groups.values()) and c.slots.n_held == 0
+
+
+def test_fork_refusals_change_nothing():
+    need = KVNeed(1, 8)
+    c = SequenceCache([(need, None, None)], 64 * 4, 256, torch.float32, "cpu", max_sequences=3)
+    a = c.take_slot()
+    with pytest.raises(ValueError, match="no tokens"):
+        c.fork(a)
+    with pytest.raises(PoolError):
+        c.fork(2)
+    c.reserve({a: 200})
+    c.commit({a: 200})
+    assert c.groups[need].pages.n_free == 0
+    with pytest.raises(CacheFull):
+        c.fork(a)                                    # (the begun page needs a copy)
+    assert c.slots.n_held == 1 and c.groups[need].pages.owners(c.groups[need].held[a][0]) == 1
+    c.free_slot(a)
+    b = c.take_slot()
+    c.reserve({b: 192})
+    c.commit({b: 192})
+    x, y = c.fork(b), c.fork(b)                      # (whole pages only: nothing to copy)
+    assert c.groups[need].pages.n_held == 3
+    with pytest.raises(CacheFull):
+        c.fork(b)                                    # (no slot)
+    assert c.groups[need].pages.owners(c.groups[need].held[b][0]) == 3
+    for s in (b, x, y):
+        c.free_slot(s)
+    assert c.groups[need].pages.n_held == 0
+
+
+def test_shared_claims():
+    c = SequenceCache([(KVNeed(1, 8), None, None)], 64 * 100, 2000, torch.float32, "cpu", max_sequences=8)
+    a, z = c.take_slot(), c.take_slot()
+    for s, n in ((a, 200), (z, 300)):
+        c.reserve({s: n})
+        c.commit({s: n})
+    assert c.shared_claims([a, z]) is None
+    b = c.fork(a)                                    # shares 3 pages with a
+    c.reserve({a: 400})
+    c.commit({a: 400})
+    d = c.fork(a)                                    # shares 6 with a, 3 with b
+    e = c.fork(b)                                    # 3
+    y = c.fork(z)                                    # another family: 4
+    assert c.shared_claims([a, b]) == ([0, 0], [3, 3], 3)
+    assert c.shared_claims([z, d, a]) == ([0, 1, 1], [0, 6, 6], 6)
+    assert c.shared_claims([y, b, -1, d, z, e, None]) == ([0, 1, 2, 1, 0, 1, 6], [4, 3, 0, 3, 4, 3, 0], 3 * 2 + 4)
+    assert c.shared_claims([a, z]) is None
+    held = c.groups[KVNeed(1, 8)].held
+    assert held[a][:6] == held[d][:6] and held[a][:3] == held[b][:3] == held[e][:3]
+    c.free_slot(a)                                   # its slot is another sequence's now
+    n = c.take_slot()
+    assert n == a and c.shared_claims([n, b, e]) == ([0, 1, 1], [0, 3, 3], 3)
+
+
+def test_fits_counts_shared_pages_once():
+    full, ring = KVNeed(1, 8), KVNeed(1, 8, 64)
+    c = SequenceCache([(full, None, None), (ring, None, None)], 64 * 10, 2000, torch.float32, None, max_sequences=4)
+    assert not c.fits([320, 320, 320]) and c.fits([320, 320, 320], [0, 300, 300])
+    assert not c.fits([320] * 5, [0, 300, 300, 300, 300])             # (slots)
+
+
+def test_refused_builds():
+    spec = lambda name: config_from_dict(CONFIGS[name]).model_spec()
+    with pytest.raises(ConfigError, match="8 bits"):
+        Model(spec("A"), torch.bfloat16, "cpu", F8)                    # head size 16
+    with pytest.raises(ConfigError, match="8 bits"):
+        Model(spec("D"), torch.float32, "cpu", F8)
+    with pytest.raises(ConfigError, match="kv_dtype"):
+        Model(spec("D"), torch.bfloat16, "cpu", torch.float8_e5m2)
+    needs = Model(spec("D"), torch.bfloat16, "cpu", F8).cache_needs()
+    assert all(n[0].eight_bits for n in needs)
+    from airframe_b200.engine.runtime import _kv_dtype
+    with pytest.raises(ValueError, match="kv_dtype"):
+        _kv_dtype("int8")
+    with pytest.raises(ValueError, match="other head sizes, bits"):
+        SequenceCache([(KVNeed(2, 64), None, None), (KVNeed(2, 64, eight_bits=True), None, 0)], 640, 512)
+
+
+class ForkingEngine(FakeEngine):
+    def fork(self, slot, n=1):
+        new = []
+        for _ in range(n):
+            s = self.take_slot()
+            self.lens[s] = self.lens[slot]
+            self.forks.append((slot, s))
+            new.append(s)
+        return new
+
+    def step(self, entries, borrow=False):
+        super().step(entries, borrow)
+        return torch.tensor([e.slot for e in entries])
+
+
+def test_loop_runs_a_prompt_once():
+    eng = ForkingEngine()
+    eng.forks = []
+    script = {0: [5, 9], 1: [6, 7, 8, 1], 2: [9], 3: [4, 4, 4, 4], 4: [3, 9], 5: [2, 2, 9]}
+    loop = GenerationLoop(eng, ScriptSampler(script), stop_token_ids=[9])
+    out = loop.generate([[1, 2, 3], [7]], P(max_tokens=4), completions=3)
+    assert out == [[5], [6, 7, 8, 1], [], [4, 4, 4, 4], [3], [2, 2]]
+    assert eng.steps[0] == [(0, [1, 2, 3]), (1, [7])]                   # two prompts, six sequences
+    assert eng.forks == [(0, 2), (0, 3), (1, 4), (1, 5)] and eng.pool.n_held == 0
+    assert loop.finish_reasons == ["stop", "length", "stop", "length", "stop", "stop"]
+    with pytest.raises(RequestError):
+        loop.generate([[1]], P(max_tokens=1), completions=0)
+
+
+def test_loop_plans_completions():
+    """Slots end a batch inside a prompt's completions: the next batch runs the prompt again."""
+    eng = ForkingEngine(slots=2)
+    eng.forks = []
+    loop = GenerationLoop(eng, ScriptSampler({i: [i] for i in range(3)}))
+    assert loop.generate([[1, 2]], P(max_tokens=1), completions=3) == [[0], [1], [2]]
+    assert loop.batches_run == [[0, 1], [2]] and len(eng.steps) == 2
+    # and shared pages count once where the cache says so
+    eng.cache = SequenceCache([(KVNeed(1, 8), None, None)], 64 * 8, 1000, torch.float32, None, max_sequences=9)
+    eng.max_context = 1000
+    loop = GenerationLoop(eng, None)
+    assert loop.plan_batches([[1] * 300] * 4, P(max_tokens=30), 4) == [[0, 1], [2, 3]]       # 6 pages and, the 4 whole ones shared, 2: of 8
+    assert loop.plan_batches([[1] * 300] * 4, P(max_tokens=30)) == [[0], [1], [2], [3]]
+
+
+# ---------------------------------------------------------------------------------------------- on the GPU
+
+def _runtime(tmp_path, cfg, dtype, **kw):
+    from airframe_b200.engine import GpuRuntime
+    return GpuRuntime.load(make_folder(cfg, seed=5, store_dtype="bfloat16", root=tmp_path), dtype=dtype, max_tokens=64 * 60, **kw)
+
+
+def _forked(rt, prompt, tails, graphs=True):
+    """The prompt once, forked for every tail; logits at the tails' tokens, a step for all a time."""
+    eng = rt.engine
+    eng.use_graphs = graphs and eng.model.graph_safe
+    s = eng.take_slot()
+    rt.step([StepEntry(s, prompt, [])])
+    slots = [s] + eng.fork(s, len(tails) - 1)
+    got = [[] for _ in tails]
+    for i in range(max(map(len, tails))):
+        live = [r for r, t in enumerate(tails) if i < len(t)]
+        logits = rt.step([StepEntry(slots[r], [tails[r][i]], [0]) for r in live])
+        for k, r in enumerate(live):
+            got[r].append(logits[k].cpu())
+        for r, t in enumerate(tails):
+            if i + 1 == len(t):
+                eng.free_slot(slots[r])
+    assert eng.cache.slots.n_held == 0 and all(n == 0 for n in eng.cache.pages_held().values())
+    return [torch.stack(g) for g in got]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("name,dtype,kv", [("H", "bfloat16", None), ("D", "bfloat16", None), ("C", "bfloat16", None), ("A", "float32", None),
+                                           ("H", "bfloat16", "float8_e4m3"), ("D", "bfloat16", "float8_e4m3")])
+@pytest.mark.parametrize("graphs", [True, False])
+def test_forks_go_on_like_separate_sequences(tmp_path, monkeypatch, name, dtype, kv, graphs):
+    """Forks with other tails (shared pages, copied begun pages and rings; one ends early) against sequences of their own."""
+    from airframe_b200 import kernels
+    monkeypatch.setattr(kernels, "SHARED_PAGES_FROM", 1)
+    cfg = dict(CONFIGS[name], max_position_embeddings=512)
+    rt = _runtime(tmp_path, cfg, dtype, kv_dtype=kv)
+    shared = []
+    whole = kernels.attn_decode_shared
+    monkeypatch.setattr(kernels, "attn_decode_shared", lambda *a, **k: (shared.append(1), whole(*a, **k))[1])
+    V = cfg["vocab_size"]
+    prompt = replay.random_ids(V, 200, 3)
+    tails = [replay.random_ids(V, n, 40 + n) for n in (70, 3, 70, 69)]
+    got = _forked(rt, prompt, tails, graphs)
+    assert shared                                              # (the layers that keep all keys went that way)
+    limit = FP32_SPLITS if dtype == "float32" else BF16_SPLITS
+    for t, g in zip(tails, got):
+        rt.engine.use_graphs = False
+        ref = replay.run_tail(rt, prompt + t, len(t))[-len(t):]
+        assert rel_err(g, ref) < limit
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("make,cfg", [(tiny_fiferax.make_folder, tiny_fiferax.CONFIGS["A"]), (tiny_retudra.make_folder, tiny_retudra.CONFIGS["A"])])
+def test_forks_of_sequences_with_states(tmp_path, make, cfg):
+    from airframe_b200.engine import GpuRuntime
+    rt = GpuRuntime.load(make(cfg, seed=5, root=tmp_path), dtype="float32", max_tokens=64 * 30)
+    V = rt.model.spec.vocab_size
+    prompt = replay.random_ids(V, 50, 3)
+    tails = [replay.random_ids(V, n, 40 + n) for n in (12, 9)]
+    for t, g in zip(tails, _forked(rt, prompt, tails)):
+        assert rel_err(g, replay.run_tail(rt, prompt + t, len(t))[-len(t):]) < FP32_SPLITS
+
+
+# An 8-bit value is off by half a step at most, 2^-4 of itself (e4m3): logits are held to that fraction of the largest, beside what
+# the bfloat16 engine is held to; two ways of cutting the work round bfloat16 rows that differ in their last bit to neighbouring
+# codes here and there: the same bound.
+EIGHT_BITS = 2.0 ** -4
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("name", ["H", "D", "E", "F"])
+def test_engine_with_a_cache_of_8_bits(tmp_path, monkeypatch, name):
+    """Against the plain model with its keys and values rounded as the cache rounds them, and one step against single tokens."""
+    cfg_d = CONFIGS[name]
+    folder = make_folder(cfg_d, seed=11, store_dtype="bfloat16", root=tmp_path)
+    cfg, w = plain.read_model_folder(folder)
+    ids = replay.random_ids(cfg["vocab_size"], 150, 8)
+    attention = plain.attention
+
+    def rounded(q, k, v, *a):
+        k, v = (values(*quantise(t.to(torch.bfloat16))).to(t.dtype) for t in (k, v))
+        return attention(q, k, v, *a)
+
+    monkeypatch.setattr(plain, "attention", rounded)
+    ref = plain.logits(cfg, w, ids)
+    from airframe_b200.engine import GpuRuntime
+    rt = GpuRuntime.load(folder, max_tokens=64 * 24, kv_dtype="float8_e4m3")
+    full = rt.engine.cache
+    assert all(v.kv.k.dtype == F8 for v in full.views)
+    one = replay.run_whole(rt, ids)
+    assert rel_err(one, ref) < VS_PLAIN["bfloat16"] + EIGHT_BITS
+    assert rel_err(replay.run_tail(rt, ids, 100), one) < EIGHT_BITS
+    bits16 = GpuRuntime.load(folder, max_tokens=64 * 24)
+    assert full.bytes_allocated() < 0.52 * bits16.engine.cache.bytes_allocated()
+
+
+@pytest.mark.gpu
+def test_completions_of_a_prompt(tmp_path, monkeypatch):
+    """The same tokens as so many requests of their own (whose generators are seeded alike), greedy and drawn; prompt steps once."""
+    from airframe_b200 import kernels
+    from airframe_b200.engine import GpuRuntime
+    from airframe_b200.sampling import SamplingParams
+    monkeypatch.setattr(kernels, "SHARED_PAGES_FROM", 1)
+    cfg = dict(CONFIGS["A"], max_position_embeddings=512)
+    rt = GpuRuntime.load(make_folder(cfg, seed=5, store_dtype="float32", root=tmp_path), dtype="float32", max_tokens=64 * 60)
+    prompts = [replay.random_ids(256, 130, 1), replay.random_ids(256, 7, 2)]
+    for params in (SamplingParams(max_tokens=20, temperature=0.0, repetition_penalty=1.0, ignore_eos=True),
+                   SamplingParams(max_tokens=20, temperature=1.5, repetition_penalty=1.0, ignore_eos=True),
+                   SamplingParams(max_tokens=20, temperature=1.5, repetition_penalty=1.2)):
+        separate = rt.generate([p for p in prompts for _ in range(3)], params)
+        seen = []
+        got = rt.generate(prompts, params, on_token=lambda i, t: seen.append(i), completions=3)
+        assert [c for of_prompt in got for c in of_prompt] == separate
+        assert set(seen) <= set(range(6))
+        assert rt.generate(prompts[0], params, completions=3) == separate[:3]
+    assert rt.engine.cache.slots.n_held == 0 and all(n == 0 for n in rt.engine.cache.pages_held().values())
+
+
+@pytest.mark.gpu
+def test_command_line(tmp_path, capsys):
+    from airframe_b200.cli.simple_flight import main
+    folder = make_folder(WIDE_D, seed=3, store_dtype="bfloat16", root=tmp_path)
+    argv = ["--model", str(folder), "2,17,3", "--max-tokens", "5", "--temperature", "0.9", "--ignore-eos"]
+    assert main(argv + ["--completions", "3", "--kv-dtype", "float8_e4m3"]) == 0
+    text = capsys.readouterr().out
+    assert all(f"Output {i}:" in text for i in range(3)) and "15 tokens" in text
+    with pytest.raises(SystemExit):
+        main(argv + ["--completions", "0"])
