@@ -11,7 +11,7 @@
 //    meets the end of a unit; taken when the splits are no more than the blocks and none is more than two
 //    pages above the share (sequences of equal or of mixed lengths, one long one among short ones);
 //  * else the run cut: all units' pages end to end, each block an equal run of them, in which every unit counts
-//    DA_BREAK_PAGES more than its pages.  A run may end one unit and begin the next: the block works them as
+//    a break (DA_BREAK_PAGES) more than its pages.  A run may end one unit and begin the next: the block works them as
 //    segments, one after the other, and leaves a partial result for each (many short sequences; more units than blocks).
 // Pass 1: a block of two groups of 4 warps
 // walks its pages, the groups taking alternate
@@ -112,7 +112,7 @@ __device__ __forceinline__ uint32_t da_piece(uint32_t tile, int r, int c) {
 __global__ void __launch_bounds__(256)
 attn_decode_plan_kernel(int* __restrict__ plan, const int* __restrict__ slots, const int* __restrict__ lens,
                         const int* __restrict__ page_table, int max_pages, int batch, int nq, int nkv, int window,
-                        int keep, int ring_rows, int room, int grid_blocks, const int* __restrict__ shared) {
+                        int keep, int ring_rows, int room, int grid_blocks, const int* __restrict__ shared, int brk) {
   extern __shared__ int dp_smem[];
   int* pages_s = dp_smem;                 // [batch + 1]
   int* splits_s = dp_smem + batch + 1;    // [batch + 1]
@@ -120,14 +120,14 @@ attn_decode_plan_kernel(int* __restrict__ plan, const int* __restrict__ slots, c
   pdl_wait();
   const int group = nq / nkv, tiles = (group + 15) / 16, units_per_seq = nkv * tiles;
   if (threadIdx.x < 32) {
-    const DaPlan pl = da_plan(slots, lens, batch, window, keep, shared, units_per_seq, grid_blocks, room, 0, pages_s, splits_s);
+    const DaPlan pl = da_plan(slots, lens, batch, window, keep, shared, brk, units_per_seq, grid_blocks, room, 0, pages_s, splits_s);
     if (threadIdx.x == 0) plan_s = pl;
   }
   __syncthreads();
   const DaPlan pl = plan_s;
   if (threadIdx.x == 0) {
     plan[0] = room;
-    plan[1] = grid_blocks;
+    plan[1] = da_plan_mark(grid_blocks, brk);
     plan[2] = batch;
     plan[3] = units_per_seq;
     plan[4] = pl.even;
@@ -139,7 +139,7 @@ attn_decode_plan_kernel(int* __restrict__ plan, const int* __restrict__ slots, c
     const int b = u / units_per_seq, y = u - b * units_per_seq;
     const int width = pages_s[b + 1] - pages_s[b];      // (the run cut: with a break)
     plan[DA_PLAN_HEAD + u] = pl.even ? da_even_splits(width, pl.share, room, pl.even)
-                                     : da_run_splits(pages_s[b] * units_per_seq + y * width, width - DA_BREAK_PAGES, pl.share);
+                                     : da_run_splits(pages_s[b] * units_per_seq + y * width, width - brk, pl.share, brk);
   }
   int* recs = plan + da_plan_records_at(batch, units_per_seq);
   for (int w = threadIdx.x; w < grid_blocks; w += blockDim.x) {
@@ -215,7 +215,7 @@ attn_decode_split_kernel(const __grid_constant__ CUtensorMap map_k, const __grid
     fs.p_in = r1.x, fs.run_left = r1.y, pos0 = r1.z, slot0 = r1.w;
     ids0[0] = r2.x, ids0[1] = r2.y, ids0[2] = r2.z, ids0[3] = r2.w;
     if (a.shared != nullptr) shared0 = ld_keep_int(reinterpret_cast<const int*>(rec + 3), keep);
-    if (head.x != a.n_splits || head.y != (int)gridDim.x || head.z != a.batch || head.w != units_per_seq) {
+    if (head.x != a.n_splits || head.y != da_plan_mark((int)gridDim.x, DA_BREAK_PAGES) || head.z != a.batch || head.w != units_per_seq) {
       // (a plan made for another launch: nothing is read or written by it)
       if (tid == 0 && a.err) atomicExch(a.err, 1);
       return;
@@ -223,7 +223,7 @@ attn_decode_split_kernel(const __grid_constant__ CUtensorMap map_k, const __grid
     __syncthreads();     // (the barriers are set up)
   } else {
     if (warp == 0) {
-      const DaPlan pl = da_plan(a.slots, a.lens, a.batch, a.window, a.keep, a.shared, units_per_seq, (int)gridDim.x, a.n_splits, 0,
+      const DaPlan pl = da_plan(a.slots, a.lens, a.batch, a.window, a.keep, a.shared, DA_BREAK_PAGES, units_per_seq, (int)gridDim.x, a.n_splits, 0,
                                 pages_s, splits_s);
       if (lane == 0) plan_s = pl;
     }
@@ -685,7 +685,7 @@ AF_EXPORT long long af_attn_decode_plan_ints(int batch, int nq, int nkv) {
 // way (the same slots, lengths, page table, heads, window, ring and n_splits): pass `plan` to each of their calls.
 // It holds for these lengths alone: a step later it is made again.
 static int decode_plan_impl(int* plan, long long plan_ints, const int* page_table, int max_pages, const int* slots, const int* lens,
-                            const int* shared, int batch, int nq, int nkv, int window, int keep, int ring_rows, int n_splits,
+                            const int* shared, int batch, int nq, int nkv, int window, int keep, int ring_rows, int n_splits, int brk,
                             cudaStream_t stream) {
   if (batch == 0) return 0;
   AF_REQUIRE(nq > 0 && nkv > 0 && nq % nkv == 0, "af_attn_decode_plan: heads %d, groups %d", nq, nkv);
@@ -694,12 +694,12 @@ static int decode_plan_impl(int* plan, long long plan_ints, const int* page_tabl
   AF_REQUIRE(keep >= 0 && (keep == 0 || window != 0), "af_attn_decode_plan: %d kept tokens with window %d", keep, window);
   AF_REQUIRE(n_splits >= 1 && ring_rows % AF_PAGE == 0, "af_attn_decode_plan: splits %d, ring rows %d", n_splits, ring_rows);
   const int units_per_seq = nkv * ((nq / nkv + 15) / 16);
-  AF_REQUIRE(batch <= DA_MAX_BATCH && (long long)batch * (max_pages + 1 + DA_BREAK_PAGES) * units_per_seq < (1ll << 31),
+  AF_REQUIRE(batch <= DA_MAX_BATCH && (long long)batch * (max_pages + 1 + brk) * units_per_seq < (1ll << 31),
              "af_attn_decode_plan: %d sequences of up to %d pages (takes %d sequences)", batch, max_pages, DA_MAX_BATCH);
   const int sms = af_sm_count();
   if (sms <= 0) return -1;
   af_launch(attn_decode_plan_kernel, dim3(1), dim3(256), (size_t)2 * (batch + 1) * sizeof(int), stream, plan, slots,
-            lens, page_table, max_pages, batch, nq, nkv, window, keep, ring_rows, n_splits, sms, shared);
+            lens, page_table, max_pages, batch, nq, nkv, window, keep, ring_rows, n_splits, sms, shared, brk);
   AF_CHECK_LAUNCH("af_attn_decode_plan");
 }
 
@@ -707,13 +707,22 @@ AF_EXPORT int af_attn_decode_plan_kept(int* plan, long long plan_ints, const int
                                   const int* slots, const int* lens, int batch, int nq, int nkv, int window,
                                   int keep, int ring_rows, int n_splits, cudaStream_t stream) {
   return decode_plan_impl(plan, plan_ints, page_table, max_pages, slots, lens, nullptr, batch, nq, nkv, window, keep, ring_rows, n_splits,
-                          stream);
+                          DA_BREAK_PAGES, stream);
 }
 
-// The same where each sequence's first shared[b] pages are another kernel's (attention_shared.cu).
+// The same for af_attn_decode8 (attention_decode8.cu).
+AF_EXPORT int af_attn_decode8_plan(int* plan, long long plan_ints, const int* page_table, int max_pages, const int* slots,
+                                   const int* lens, int batch, int nq, int nkv, int window, int keep, int ring_rows, int n_splits,
+                                   cudaStream_t stream) {
+  return decode_plan_impl(plan, plan_ints, page_table, max_pages, slots, lens, nullptr, batch, nq, nkv, window, keep, ring_rows, n_splits,
+                          D8_BREAK_PAGES, stream);
+}
+
+// The same (for a cache of so many bits) where each sequence's first shared[b] pages are another kernel's (attention_shared.cu).
 int af_decode_plan_shared(int* plan, long long plan_ints, const int* page_table, int max_pages, const int* slots, const int* lens,
-                          const int* shared, int batch, int nq, int nkv, int n_splits, cudaStream_t stream) {
-  return decode_plan_impl(plan, plan_ints, page_table, max_pages, slots, lens, shared, batch, nq, nkv, 0, 0, 0, n_splits, stream);
+                          const int* shared, int batch, int nq, int nkv, int n_splits, int bits, cudaStream_t stream) {
+  return decode_plan_impl(plan, plan_ints, page_table, max_pages, slots, lens, shared, batch, nq, nkv, 0, 0, 0, n_splits,
+                          bits == 8 ? D8_BREAK_PAGES : DA_BREAK_PAGES, stream);
 }
 
 // The split pass alone (partial results into `scratch`), each sequence's first shared[b] pages left out.

@@ -31,17 +31,21 @@ constexpr float D8_SHIFT = 6.f;          // weights are kept times 2^6
 
 template <int HD, int NT>
 struct D8 {
-  // (the accumulators of 16 heads of 256 take 128 registers: half as many warps)
-  static constexpr int THREADS = HD * NT > 256 ? 256 : 512;
-  static constexpr int WARPS = THREADS / 32, GROUPS = WARPS / 4;
-  static constexpr int CODES = AF_PAGE * HD;                             // bytes of a page's keys, and of its values
-  static constexpr int STAGES = HD == 256 ? 6 : (HD == 128 ? 12 : 16);
-  // barriers: a page's must not be met by another group's pages (a multiple of GROUPS), nor be armed before the page in the
+  // (the accumulators of 16 heads of 256 take 128 registers, those of 8 heads 64 beside 32 of queries: fewer warps)
+  static constexpr int THREADS = HD * NT == 512 ? 256 : (HD * NT == 256 ? 384 : 512);
+  static constexpr int WARPS = THREADS / 32;
+  // keys of a piece: half a page where heads are large, so that all warps have pieces in shared memory
+  static constexpr int KEYS = HD == 256 ? 32 : 64, PER_PAGE = AF_PAGE / KEYS, TILES = KEYS / 16;
+  static constexpr int AT_ONCE = NT == 2 && TILES == 4 ? 2 : TILES;      // tiles of a piece that are worked together
+  static constexpr int CODES = KEYS * HD;                                // bytes of a piece's keys, and of its values
+  static constexpr int SUB = KEYS * 128;                                 // bytes of a sub-tile of 128 dims
+  static constexpr int STAGES = HD == 64 ? 16 : 12;
+  // barriers: a piece's must not be met by another warp's pieces (a multiple of WARPS), nor be armed before the piece in the
   // same stage was consumed (a multiple of STAGES)
-  static constexpr int NBAR = HD == 256 ? 12 : STAGES;
+  static constexpr int NBAR = HD == 64 ? 16 : (WARPS == 16 ? 48 : (WARPS == 12 ? 12 : 24));
   static constexpr int RING = STAGES * 2 * CODES;
-  static constexpr int SMEM = RING + STAGES * 2 * AF_PAGE + 1024;
-  static_assert(NBAR % GROUPS == 0 && NBAR % STAGES == 0, "barriers");
+  static constexpr int SMEM = RING + STAGES * 2 * KEYS + 1024;
+  static_assert(NBAR % WARPS == 0 && NBAR % STAGES == 0, "barriers");
   static_assert(WARPS * 8 * NT * HD * 4 <= RING, "the merge's buffer");
 };
 
@@ -91,24 +95,179 @@ __device__ __forceinline__ void d8_bulk(void* dst, const void* src, uint32_t byt
                "l"(src), "r"(bytes), "r"(smem_u32(bar))
                : "memory");
 }
-// Address of the 16-byte piece `p` of key row `r` in a page's codes, as TMA wrote them: sub-tiles of [64 rows][128 bytes]
-// (HD 64: [64 rows][64 bytes]) with the hardware's swizzle.
-template <int HD>
-__device__ __forceinline__ uint32_t d8_piece(uint32_t tile, int r, int p) {
-  if constexpr (HD == 64) return tile + (uint32_t)(r * 64 + ((p ^ ((r >> 1) & 3)) << 4));
-  return tile + (uint32_t)((p >> 3) * 8192 + r * 128 + (((p & 7) ^ (r & 7)) << 4));
-}
+// S^T, softmax and O^T of N tiles of 16 keys (all of a piece, or one), beginning with tile `t0`.
+template <int HD, int NT, int N>
+struct D8Step {
+  using C = D8<HD, NT>;
+  // k_l, v_l, e_l: this lane's addresses of the piece's keys, values and exponents (tile 0); swap: what the odd halves' addresses
+  // differ by (the swizzle); lo, hi, keep: the visible keys, counted from the piece's first
+  __device__ static __forceinline__ void run(uint32_t k_l, uint32_t v_l, uint32_t ke_l, int t0, bool whole, int lo, int hi, int keep,
+                                             int g, int t, bool capped, float ecap, float capl, const uint32_t (&qf)[NT][HD / 16][2],
+                                             const float (&cq)[NT][2], float (&o)[HD / 16][NT][4], float (&rs)[NT][2], float (&ra)[NT][2],
+                                             float (&l)[NT][2]) {
+    constexpr int ROW = HD == 64 ? 64 : 128;              // bytes between rows of a sub-tile
+    k_l += t0 * 16 * ROW;
+    v_l += t0 * 16 * ROW;
+    ke_l += t0 * 16;
+    float sc[N][NT][4], wt[N][NT][4];
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+#pragma unroll
+      for (int n = 0; n < NT; ++n) sc[i][n][0] = sc[i][n][1] = sc[i][n][2] = sc[i][n][3] = 0.f;
+    // ---- S^T = K Q^T
+#pragma unroll
+    for (int c = 0; c < HD / 64; ++c) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const uint32_t at = (c & 1 ? k_l ^ 64u : k_l) + (c >> 1) * C::SUB + i * 16 * ROW;
+        const uint4 x = d8_lds4(at), y = d8_lds4(at + 8 * ROW);
+        const uint32_t xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          uint32_t a0, a1, a2, a3;
+          c8_half4(xs[j], a0, a2);
+          c8_half4(ys[j], a1, a3);
+#pragma unroll
+          for (int n = 0; n < NT; ++n) d8_mma(sc[i][n], a0, a1, a2, a3, qf[n][c * 4 + j][0], qf[n][c * 4 + j][1]);
+        }
+      }
+    }
+    // ---- scale, softcap, mask; the weights' exponents; whether a reference moves
+    const int kr = t0 * 16 + d8_perm(g);                  // this lane's keys: kr + 16 i, and 8 behind
+    bool moves = false;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      float ks[2], lv[2];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        ks[h] = __uint_as_float((uint32_t)d8_lds_u8(ke_l + i * 16 + 8 * h) << 23);
+        lv[h] = (float)(d8_lds_u8(ke_l + C::KEYS + i * 16 + 8 * h) - 127);
+      }
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sc[i][n][e] *= cq[n][e & 1] * ks[e >> 1];
+      if (capped) {
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) sc[i][n][e] = capl - 2.f * capl * __fdividef(1.f, 1.f + fast_exp2(sc[i][n][e] * ecap));
+      }
+      if (!whole) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int j = kr + 16 * i + 8 * (e >> 1);
+          const bool on = (j >= lo || j < keep) && j <= hi;
+#pragma unroll
+          for (int n = 0; n < NT; ++n) sc[i][n][e] = on ? sc[i][n][e] : -INFINITY;
+        }
+      }
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) wt[i][n][e] = sc[i][n][e] + lv[e >> 1];
+    }
+    float ms[NT][2], ma[NT][2];
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        float x = fmaxf(sc[0][n][h], sc[0][n][h + 2]), y = fmaxf(wt[0][n][h], wt[0][n][h + 2]);
+#pragma unroll
+        for (int i = 1; i < N; ++i) {
+          x = fmaxf(x, fmaxf(sc[i][n][h], sc[i][n][h + 2]));
+          y = fmaxf(y, fmaxf(wt[i][n][h], wt[i][n][h + 2]));
+        }
+        ms[n][h] = x, ma[n][h] = y;
+        moves = moves || x > rs[n][h] + D8_MOVES || y > ra[n][h] + D8_MOVES;
+      }
+    if (__any_sync(0xffffffffu, moves)) {
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          float x = ms[n][h], y = ma[n][h];
+#pragma unroll
+          for (int w = 4; w < 32; w <<= 1) {
+            x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, w));
+            y = fmaxf(y, __shfl_xor_sync(0xffffffffu, y, w));
+          }
+          x = fmaxf(x, rs[n][h]), y = fmaxf(y, ra[n][h]);
+          l[n][h] *= fast_exp2(rs[n][h] - x);
+          const float f = fast_exp2(ra[n][h] - y);
+          rs[n][h] = x, ra[n][h] = y;
+#pragma unroll
+          for (int m = 0; m < HD / 16; ++m) o[m][n][h] *= f, o[m][n][h + 2] *= f;
+        }
+    }
+    uint32_t pb[N][NT][2];
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        float w[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          l[n][e & 1] += fast_exp2(sc[i][n][e] - rs[n][e & 1]);
+          w[e] = fast_exp2(wt[i][n][e] - (ra[n][e & 1] - D8_SHIFT));
+        }
+        const __half2 p0 = __floats2half2_rn(w[0], w[1]), p1 = __floats2half2_rn(w[2], w[3]);
+        pb[i][n][0] = d8_transpose(*reinterpret_cast<const uint32_t*>(&p0));
+        pb[i][n][1] = d8_transpose(*reinterpret_cast<const uint32_t*>(&p1));
+      }
+    // ---- O^T += V^T P^T: this lane's fragments hold the keys t, t + 4, t + 8, t + 12 of a tile
+    constexpr int VW = HD == 64 ? 2 : 4;                  // words of a row that a lane takes at a time
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+#pragma unroll
+      for (int c = 0; c < HD / (32 * VW); ++c) {
+        uint32_t w[4][VW];
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          const uint32_t at = (x & 1 ? v_l ^ (HD == 64 ? 32u : 64u) : v_l) + c * C::SUB + (i * 16 + 4 * x) * ROW;
+          if constexpr (HD == 64) {
+            const uint2 v = d8_lds2(at);
+            w[x][0] = v.x, w[x][1] = v.y;
+          } else {
+            const uint4 v = d8_lds4(at);
+            w[x][0] = v.x, w[x][1] = v.y, w[x][2] = v.z, w[x][3] = v.w;
+          }
+          if (!whole) {
+            // (a hidden key's codes may be any bytes, NaN among them: its weight of 0 does not make them 0)
+            const int j = (t0 + i) * 16 + t + 4 * x;
+            if (!((j >= lo || j < keep) && j <= hi)) {
+#pragma unroll
+              for (int k = 0; k < VW; ++k) w[x][k] = 0u;
+            }
+          }
+        }
+#pragma unroll
+        for (int j = 0; j < VW; ++j) {
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            const uint32_t sel = u ? 0x7362u : 0x5140u;
+            uint32_t a0, a1, a2, a3;
+            c8_half4(__byte_perm(w[0][j], w[1][j], sel), a0, a1);
+            c8_half4(__byte_perm(w[2][j], w[3][j], sel), a2, a3);
+#pragma unroll
+            for (int n = 0; n < NT; ++n) d8_mma(o[c * 2 * VW + 2 * j + u][n], a0, a1, a2, a3, pb[i][n][0], pb[i][n][1]);
+          }
+        }
+      }
+    }
+  }
+};
 
 template <int HD, int NT>
 __global__ void __launch_bounds__(D8<HD, NT>::THREADS, 1)
 decode8_split_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, Decode8Args a) {
   using C = D8<HD, NT>;
-  constexpr int STAGES = C::STAGES, GROUPS = C::GROUPS, WARPS = C::WARPS, NBAR = C::NBAR;
+  constexpr int STAGES = C::STAGES, WARPS = C::WARPS, NBAR = C::NBAR, PER = C::PER_PAGE;
   constexpr int ROWS = 8 * NT;
   constexpr float LOG2E = 1.4426950408889634f;
   extern __shared__ unsigned char d8_raw[];
   unsigned char* ring = (unsigned char*)(((uintptr_t)d8_raw + 1023) & ~(uintptr_t)1023);
-  unsigned char* exps = ring + C::RING;                        // [stage][k exponents 64 | v exponents 64]
+  unsigned char* exps = ring + C::RING;                        // [stage][k exponents | v exponents]
   __shared__ uint64_t full[NBAR];
   __shared__ float rs_s[WARPS][ROWS], ra_s[WARPS][ROWS], l_s[WARPS][ROWS];
   __shared__ float f_s[WARPS][ROWS], ml_s[ROWS][2];
@@ -119,7 +278,6 @@ decode8_split_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
   const int group = a.nq / a.nkv;
   const int tiles = (group + 15) / 16, units_per_seq = a.nkv * tiles;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int grp = warp >> 2, wq = warp & 3;
   const int g = lane >> 2, t = lane & 3;
   if (tid == 0) {
     for (int s = 0; s < NBAR; ++s) mbar_init(&full[s], 1);
@@ -133,7 +291,7 @@ decode8_split_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
   const int4 head = ld_keep_int4(reinterpret_cast<const int4*>(a.plan), keep_policy);
   const int4 r0 = ld_keep_int4(rec, keep_policy), r1 = ld_keep_int4(rec + 1, keep_policy), r2 = ld_keep_int4(rec + 2, keep_policy);
   const int4 r3 = ld_keep_int4(rec + 3, keep_policy);
-  if (head.x != a.n_splits || head.y != (int)gridDim.x || head.z != a.batch || head.w != units_per_seq) {
+  if (head.x != a.n_splits || head.y != da_plan_mark((int)gridDim.x, D8_BREAK_PAGES) || head.z != a.batch || head.w != units_per_seq) {
     if (tid == 0 && a.err) atomicExch(a.err, 1);      // (a plan made for another launch: nothing is read or written by it)
     return;
   }
@@ -171,8 +329,8 @@ decode8_split_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
     }
     const int P = da_pages(a.slots, a.lens, b, a.window, a.keep, a.shared);
     nx.z = 0;
-    nx.n_pages = min(P, left - DA_BREAK_PAGES);
-    left -= DA_BREAK_PAGES + P;
+    nx.n_pages = min(P, left - D8_BREAK_PAGES);
+    left -= D8_BREAK_PAGES + P;
     of_unit(nx, b, y, 0, a.lens[b] - 1, a.slots[b], a.shared != nullptr ? a.shared[b] : 0);
     return nx;
   };
@@ -183,24 +341,27 @@ decode8_split_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
     return AF_INDEX_OK(entry < a.max_pages, entry) && entry < a.max_pages ? safe(sg.pt[entry]) : 0;
   };
   const uint64_t read_once = l2_policy_read_once();
-  auto issue = [&](int kvh, int page, int ii) {        // cache page `page`, the block's page number ii, into its stage
-    const int s = ii % STAGES, unit = page * a.nkv + kvh;
+  // piece `half` of cache page `page`, the block's piece number ii, into its stage
+  auto issue = [&](int kvh, int page, int half, int ii) {
+    const int s = ii % STAGES, row = (page * a.nkv + kvh) * AF_PAGE + half * C::KEYS;
     unsigned char* st = ring + (size_t)s * 2 * C::CODES;
     uint64_t* bar = &full[ii % NBAR];
-    mbar_expect_tx(bar, 2 * C::CODES + 2 * AF_PAGE);
+    mbar_expect_tx(bar, 2 * C::CODES + 2 * C::KEYS);
 #pragma unroll
     for (int c = 0; c < (HD + 127) / 128; ++c) {
-      tma_load_2d_once(st + c * 8192, &map_k, c * 128, unit * AF_PAGE, bar, read_once);
-      tma_load_2d_once(st + C::CODES + c * 8192, &map_v, c * 128, unit * AF_PAGE, bar, read_once);
+      tma_load_2d_once(st + c * C::SUB, &map_k, c * 128, row, bar, read_once);
+      tma_load_2d_once(st + C::CODES + c * C::SUB, &map_v, c * 128, row, bar, read_once);
     }
-    d8_bulk(exps + s * 2 * AF_PAGE, a.k_exp + (size_t)unit * AF_PAGE, AF_PAGE, bar);
-    d8_bulk(exps + s * 2 * AF_PAGE + AF_PAGE, a.v_exp + (size_t)unit * AF_PAGE, AF_PAGE, bar);
+    d8_bulk(exps + s * 2 * C::KEYS, a.k_exp + row, C::KEYS, bar);
+    d8_bulk(exps + s * 2 * C::KEYS + C::KEYS, a.v_exp + row, C::KEYS, bar);
   };
-  auto issue_from = [&](const Segment& sg, int from, int to, int ii0, bool skip_last) {
+  auto issue_from = [&](const Segment& sg, int from, int to, int ii0, bool skip_last) {      // (pieces of the segment)
     int i = from;
+    int page = -1, id = 0;
     for (; i < to; ++i) {
-      if (skip_last && page_of(sg, i) == sg.last_pp) break;
-      issue(sg.kvh, page_id(sg, i), ii0 + i);
+      if (skip_last && page_of(sg, i / PER) == sg.last_pp) break;
+      if (i / PER != page) page = i / PER, id = page_id(sg, page);
+      issue(sg.kvh, id, i % PER, ii0 + i);
     }
     return i;
   };
@@ -217,19 +378,19 @@ decode8_split_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
     const int ids0[4] = {r2.x, r2.y, r2.z, r2.w};
     bool go = true;
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      go = go && k < STAGES && k < sg.n_pages && page_of(sg, k) != sg.last_pp;
+    for (int k = 0; k < 4 * PER; ++k) {
+      go = go && k < STAGES && k < sg.n_pages * PER && page_of(sg, k / PER) != sg.last_pp;
       if (go) {
-        issue(sg.kvh, safe(ids0[k]), k);
+        issue(sg.kvh, safe(ids0[k / PER]), k % PER, k);
         ++issued;
       }
     }
-    if (issued == 4) issued = issue_from(sg, 4, min(STAGES, sg.n_pages), 0, true);
+    if (issued == 4 * PER) issued = issue_from(sg, issued, min(STAGES, sg.n_pages * PER), 0, true);
   }
   pdl_wait();
   while (true) {
-    const int b = sg.b, n_pages = sg.n_pages, n_rows = sg.n_rows, row_head0 = sg.row_head0;
-    if (tid == 0) issued = issue_from(sg, issued, min(STAGES, n_pages), i_base, false);
+    const int b = sg.b, n = sg.n_pages * PER, n_rows = sg.n_rows, row_head0 = sg.row_head0;
+    if (tid == 0) issued = issue_from(sg, issued, min(STAGES, n), i_base, false);
 
     // ---- the queries as B fragments (head g of every tile of 8), halves brought to [2^14, 2^15)
     uint32_t qf[NT][HD / 16][2];
@@ -283,149 +444,38 @@ decode8_split_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
 #pragma unroll
     for (int n = 0; n < NT; ++n) rs[n][0] = rs[n][1] = ra[n][0] = ra[n][1] = D8_NONE, l[n][0] = l[n][1] = 0.f;
 
-    // group `grp` takes the pages whose count since the block began is grp modulo GROUPS
-    for (int i = (grp + GROUPS - i_base % GROUPS) % GROUPS; i < n_pages; i += GROUPS) {
-      const int ii = i_base + i, s = ii % STAGES;
-      const bool refill = (tid & 127) == 0 && i + STAGES < n_pages;
-      const int refill_page = refill ? page_id(sg, i + STAGES) : 0;
-      const int ok = mbar_wait(&full[ii % NBAR], (ii / NBAR) & 1, give_up) ? 1 : 0;
-      int all_ok;      // the four warps of the group go on or give up together
-      asm volatile(
-          "{\n\t.reg .pred p, q;\n\t"
-          "setp.ne.b32 q, %1, 0;\n\t"
-          "barrier.red.and.pred.aligned p, %2, 128, q;\n\t"
-          "selp.u32 %0, 1, 0, p;\n\t}"
-          : "=r"(all_ok)
-          : "r"(ok), "r"(1 + grp)
-          : "memory");
-      if (!all_ok) break;
-      const uint32_t k_t = smem_u32(ring + (size_t)s * 2 * C::CODES), v_t = k_t + C::CODES;
-      const uint32_t e_t = smem_u32(exps + s * 2 * AF_PAGE);
-      const int kr = wq * 16 + d8_perm(g);              // this lane's keys: rows kr and kr + 8 of the page
-      // ---- S^T = K Q^T
-      float sc[NT][4];
-#pragma unroll
-      for (int n = 0; n < NT; ++n) sc[n][0] = sc[n][1] = sc[n][2] = sc[n][3] = 0.f;
-#pragma unroll
-      for (int c = 0; c < HD / 64; ++c) {
-        const uint4 x = d8_lds4(d8_piece<HD>(k_t, kr, c * 4 + t)), y = d8_lds4(d8_piece<HD>(k_t, kr + 8, c * 4 + t));
-        const uint32_t xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w};
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const uint32_t a0 = c8_half2(xs[j]), a2 = c8_half2(xs[j] >> 16), a1 = c8_half2(ys[j]), a3 = c8_half2(ys[j] >> 16);
-#pragma unroll
-          for (int n = 0; n < NT; ++n) d8_mma(sc[n], a0, a1, a2, a3, qf[n][c * 4 + j][0], qf[n][c * 4 + j][1]);
-        }
-      }
-      // ---- scale, softcap, mask; the weights' exponents
-      const int base = page_of(sg, i) * AF_PAGE;
-      const bool whole = base + AF_PAGE - 1 <= sg.pos && (base >= sg.lo || base + AF_PAGE - 1 < a.keep);
-      float ks[2], lv[2];
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        ks[h] = __uint_as_float((uint32_t)d8_lds_u8(e_t + kr + 8 * h) << 23);
-        lv[h] = (float)(d8_lds_u8(e_t + AF_PAGE + kr + 8 * h) - 127);
-      }
-      float wt[NT][4];                                   // scores with the values' exponents
-      bool moves = false;
-#pragma unroll
-      for (int n = 0; n < NT; ++n)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          float v = sc[n][e] * (cq[n][e & 1] * ks[e >> 1]);
-          if (a.cap > 0.f) v = capl - 2.f * capl * __fdividef(1.f, 1.f + fast_exp2(v * ecap));
-          if (!whole) {
-            const int j = base + kr + 8 * (e >> 1);
-            if (!((j >= sg.lo || j < a.keep) && j <= sg.pos)) v = -INFINITY;
-          }
-          sc[n][e] = v;
-          wt[n][e] = v == -INFINITY ? v : v + lv[e >> 1];
-          moves = moves || v > rs[n][e & 1] + D8_MOVES || wt[n][e] > ra[n][e & 1] + D8_MOVES;
-        }
-      if (__any_sync(0xffffffffu, moves)) {
-#pragma unroll
-        for (int n = 0; n < NT; ++n)
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            float ms = fmaxf(sc[n][h], sc[n][h + 2]), ma = fmaxf(wt[n][h], wt[n][h + 2]);
-#pragma unroll
-            for (int x = 4; x < 32; x <<= 1) {
-              ms = fmaxf(ms, __shfl_xor_sync(0xffffffffu, ms, x));
-              ma = fmaxf(ma, __shfl_xor_sync(0xffffffffu, ma, x));
-            }
-            ms = fmaxf(ms, rs[n][h]), ma = fmaxf(ma, ra[n][h]);
-            l[n][h] *= fast_exp2(rs[n][h] - ms);
-            const float f = fast_exp2(ra[n][h] - ma);
-            rs[n][h] = ms, ra[n][h] = ma;
-#pragma unroll
-            for (int m = 0; m < HD / 16; ++m) o[m][n][h] *= f, o[m][n][h + 2] *= f;
-          }
-      }
-      uint32_t pb[NT][2];
-#pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        float w[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          l[n][e & 1] += fast_exp2(sc[n][e] - rs[n][e & 1]);
-          w[e] = fast_exp2(wt[n][e] - ra[n][e & 1] + D8_SHIFT);
-        }
-        const __half2 p0 = __floats2half2_rn(w[0], w[1]), p1 = __floats2half2_rn(w[2], w[3]);
-        pb[n][0] = d8_transpose(*reinterpret_cast<const uint32_t*>(&p0));
-        pb[n][1] = d8_transpose(*reinterpret_cast<const uint32_t*>(&p1));
-      }
-      // ---- O^T += V^T P^T: this lane's fragments hold the keys t, t + 4, t + 8, t + 12 of the warp's 16
-      const int vr = wq * 16 + t;
-      bool seen[4] = {true, true, true, true};
-      if (!whole) {
-        // (a hidden key's codes may be any bytes, NaN among them: its weight of 0 does not make them 0)
-#pragma unroll
-        for (int x = 0; x < 4; ++x) {
-          const int j = base + vr + 4 * x;
-          seen[x] = (j >= sg.lo || j < a.keep) && j <= sg.pos;
-        }
-      }
-      constexpr int VW = HD == 64 ? 2 : 4;               // words of a row that a lane takes at a time
-#pragma unroll
-      for (int c = 0; c < HD / (32 * VW); ++c) {
-        uint32_t w[4][VW];
-#pragma unroll
-        for (int x = 0; x < 4; ++x) {
-          if constexpr (HD == 64) {
-            const uint2 v = d8_lds2(d8_piece<HD>(v_t, vr + 4 * x, g >> 1) + (g & 1) * 8);
-            w[x][0] = v.x, w[x][1] = v.y;
-          } else {
-            const uint4 v = d8_lds4(d8_piece<HD>(v_t, vr + 4 * x, c * 8 + d8_perm(g)));
-            w[x][0] = v.x, w[x][1] = v.y, w[x][2] = v.z, w[x][3] = v.w;
-          }
-          if (!whole && !seen[x]) {
-#pragma unroll
-            for (int j = 0; j < VW; ++j) w[x][j] = 0u;
-          }
-        }
-#pragma unroll
-        for (int j = 0; j < VW; ++j) {
-#pragma unroll
-          for (int u = 0; u < 2; ++u) {
-            const uint32_t sel = u ? 0x7362u : 0x5140u;
-            const uint32_t ab = __byte_perm(w[0][j], w[1][j], sel), cd = __byte_perm(w[2][j], w[3][j], sel);
-            const uint32_t a0 = c8_half2(ab), a1 = c8_half2(ab >> 16), a2 = c8_half2(cd), a3 = c8_half2(cd >> 16);
-#pragma unroll
-            for (int n = 0; n < NT; ++n) d8_mma(o[c * 2 * VW + 2 * j + u][n], a0, a1, a2, a3, pb[n][0], pb[n][1]);
-          }
-        }
-      }
-      // the group is done with the stage: its first thread refills it
-      asm volatile("bar.sync %0, 128;" ::"r"(1 + grp) : "memory");
-      if (refill && !*give_up) issue(sg.kvh, refill_page, ii + STAGES);
+    // A warp takes a piece at a time; where the pieces are fewer than the warps, a tile of 16 keys.
+    const bool few = n <= STAGES && n * C::TILES <= 2 * WARPS;
+    const int items = few ? n * C::TILES : n;
+    // this lane's place in a piece (see D8Step)
+    const int pg = d8_perm(g);
+    const uint32_t k_off = HD == 64 ? pg * 64 + ((t ^ ((pg >> 1) & 3)) << 4) : pg * 128 + ((t ^ pg) << 4);
+    const uint32_t v_off = C::CODES + (HD == 64 ? t * 64 + (((g >> 1) ^ (t >> 1)) << 4) + (g & 1) * 8 : t * 128 + ((pg ^ t) << 4));
+    for (int x = warp; x < items; x += WARPS) {
+      const int i = few ? x / C::TILES : x, ii = i_base + i, s = ii % STAGES;
+      const bool refill = lane == 0 && i + STAGES < n;
+      const int refill_page = refill ? page_id(sg, (i + STAGES) / PER) : 0;
+      if (!mbar_wait(&full[ii % NBAR], (ii / NBAR) & 1, give_up)) break;
+      const uint32_t st = smem_u32(ring) + s * 2 * C::CODES, e_l = smem_u32(exps) + s * 2 * C::KEYS + pg;
+      const int base = page_of(sg, i / PER) * AF_PAGE + (i % PER) * C::KEYS;
+      const int lo = sg.lo - base, hi = sg.pos - base, keep = a.keep - base;       // (visible: [lo, hi] and what is before keep)
+      const bool whole = C::KEYS - 1 <= hi && (lo <= 0 || C::KEYS - 1 < keep);
+      if (few)
+        D8Step<HD, NT, 1>::run(st + k_off, st + v_off, e_l, x % C::TILES, whole, lo, hi, keep, g, t, a.cap > 0.f, ecap, capl, qf, cq, o, rs, ra, l);
+      else
+#pragma unroll 1
+        for (int t0 = 0; t0 < C::TILES; t0 += C::AT_ONCE)
+          D8Step<HD, NT, C::AT_ONCE>::run(st + k_off, st + v_off, e_l, t0, whole, lo, hi, keep, g, t, a.cap > 0.f, ecap, capl, qf, cq, o, rs, ra, l);
+      __syncwarp();
+      if (refill && !*give_up) issue(sg.kvh, refill_page, (i + STAGES) % PER, ii + STAGES);
     }
     if (*give_up && tid == 0) grace_period();
     __syncthreads();
     const bool gave_up = *give_up != 0;
 
     // ---- merge the warps through shared memory (the stages that the next segment's first pages do not take)
-    i_base += n_pages;
-    const bool more = left > DA_BREAK_PAGES && !gave_up;
+    i_base += n;
+    const bool more = left > D8_BREAK_PAGES && !gave_up;
     const int buf_bytes = WARPS * n_rows * HD * 4, buf_stages = (buf_bytes + 2 * C::CODES - 1) / (2 * C::CODES);
     Segment nx = sg;
     issued = 0;
@@ -436,7 +486,7 @@ decode8_split_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
     const int room = first >= buf_stages ? STAGES - buf_stages : max(0, buf0 - first);
     if (more) {
       nx = next_unit(sg);
-      if (tid == 0) issued = issue_from(nx, 0, min(room, nx.n_pages), i_base, false);
+      if (tid == 0) issued = issue_from(nx, 0, min(room, nx.n_pages * PER), i_base, false);
     }
     float* o_s = reinterpret_cast<float*>(ring + (size_t)buf0 * 2 * C::CODES);     // [warp][row][HD]
 #pragma unroll
@@ -493,13 +543,13 @@ decode8_split_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
   if (tid == 0 && give_up_s && a.err) atomicExch(a.err, 1);
 }
 
-// Tensor map of the codes as a matrix of bytes [rows, HD]: boxes of 64 rows by up to 128 bytes, swizzled.
+// Tensor map of the codes as a matrix of bytes [rows, HD]: boxes of a piece's rows by up to 128 bytes, swizzled.
 int d8_map(CUtensorMap* map, const void* base, long long rows, int hd) {
   AfEncodeTiledFn enc = af_encode_tiled();
   if (enc == nullptr) return af_fail(-1, "the driver has no cuTensorMapEncodeTiled");
   cuuint64_t dims[2] = {(cuuint64_t)hd, (cuuint64_t)rows};
   cuuint64_t strides[1] = {(cuuint64_t)hd};
-  cuuint32_t box[2] = {hd < 128 ? 64u : 128u, (cuuint32_t)AF_PAGE};
+  cuuint32_t box[2] = {hd < 128 ? 64u : 128u, hd == 256 ? 32u : (cuuint32_t)AF_PAGE};
   cuuint32_t estr[2] = {1, 1};
   const CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
                          hd < 128 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
@@ -542,7 +592,7 @@ int af_decode8_split(const void* q, long long q_stride, const void* k, const voi
   AF_REQUIRE(q_stride % 2 == 0 && ((uintptr_t)q & 3) == 0, "af_attn_decode8: queries must be 4-byte aligned");
   AF_REQUIRE(n_pages > 0 && n_pages * nkv * AF_PAGE < (1ll << 31), "af_attn_decode8: %lld cache pages", n_pages);
   const int group = nq / nkv, units_per_seq = nkv * ((group + 15) / 16);
-  AF_REQUIRE(batch <= DA_MAX_BATCH && (long long)batch * (max_pages + 1 + DA_BREAK_PAGES) * units_per_seq < (1ll << 31),
+  AF_REQUIRE(batch <= DA_MAX_BATCH && (long long)batch * (max_pages + 1 + D8_BREAK_PAGES) * units_per_seq < (1ll << 31),
              "af_attn_decode8: %d sequences of up to %d pages (takes %d sequences)", batch, max_pages, DA_MAX_BATCH);
   CUtensorMap mk, mv;
   int rc = d8_map(&mk, k, n_pages * nkv * AF_PAGE, hd);

@@ -36,7 +36,7 @@ int af_decode16_split(const void* q, long long q_stride, const void* kcache, con
                       int nkv, int hd, float scale, float cap, int n_splits, float* scratch, const int* plan, int* err,
                       cudaStream_t stream);
 int af_decode_plan_shared(int* plan, long long plan_ints, const int* page_table, int max_pages, const int* slots, const int* lens,
-                          const int* shared, int batch, int nq, int nkv, int n_splits, cudaStream_t stream);
+                          const int* shared, int batch, int nq, int nkv, int n_splits, int bits, cudaStream_t stream);
 
 namespace {
 
@@ -757,8 +757,9 @@ AF_EXPORT long long af_attn_shared_rows(int batch, int nq, int nkv) {
 
 // The plans of a step: row b's first pages[b] cache pages are those of row lead[b].
 AF_EXPORT int af_attn_shared_plan(int* plan, long long plan_ints, const int* lead, const int* pages, const int* page_table, int max_pages,
-                                  const int* slots, const int* lens, int batch, int nq, int nkv, int n_splits, cudaStream_t stream) {
+                                  const int* slots, const int* lens, int batch, int nq, int nkv, int n_splits, int bits, cudaStream_t stream) {
   if (batch == 0) return 0;
+  AF_REQUIRE(bits == 8 || bits == 16, "af_attn_shared_plan: a cache of 8 or 16 bits, not %d", bits);
   const long long need = af_attn_shared_plan_ints(batch, nq, nkv);
   AF_REQUIRE(need > 0, "af_attn_shared_plan: %d sequences (takes %d), %d heads in %d groups", batch, SH_MAX_BATCH, nq, nkv);
   AF_REQUIRE(plan != nullptr && ((uintptr_t)plan & 15) == 0 && plan_ints >= need, "af_attn_shared_plan: a plan of %lld integers, 16-byte aligned",
@@ -777,7 +778,7 @@ AF_EXPORT int af_attn_shared_plan(int* plan, long long plan_ints, const int* lea
   AF_COUNT_LAUNCH("af_attn_shared_plan");
   const ShPlan L = sh_layout(batch, nq, nkv, sms);
   const int at = (L.total + 3) / 4 * 4;
-  return af_decode_plan_shared(plan + at, plan_ints - at, page_table, max_pages, slots, lens, plan + L.shared, batch, nq, nkv, n_splits, stream);
+  return af_decode_plan_shared(plan + at, plan_ints - at, page_table, max_pages, slots, lens, plan + L.shared, batch, nq, nkv, n_splits, bits, stream);
 }
 
 // out [batch, nq * hd] bfloat16 = attention of one new token per sequence over all its keys, the shared pages read once a

@@ -22,7 +22,16 @@ __device__ __forceinline__ float c8_pow2(int p) { return __uint_as_float((uint32
 __device__ __forceinline__ uint32_t c8_pack2(float a, float b) {
   return __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
 }
-// Two codes as halves (every e4m3 value is a half): one instruction.
+// Four codes as two pairs of halves (every e4m3 value is a half): one instruction a pair.
+__device__ __forceinline__ void c8_half4(uint32_t codes, uint32_t& lo, uint32_t& hi) {
+  asm("{\n\t.reg .b16 a, b;\n\t"
+      "mov.b32 {a, b}, %2;\n\t"
+      "cvt.rn.f16x2.e4m3x2 %0, a;\n\t"
+      "cvt.rn.f16x2.e4m3x2 %1, b;\n\t}"
+      : "=r"(lo), "=r"(hi)
+      : "r"(codes));
+}
+// Two codes.
 __device__ __forceinline__ uint32_t c8_half2(uint32_t codes) {
   const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(codes & 0xffffu), __NV_E4M3);
   return (uint32_t)h.x | ((uint32_t)h.y << 16);

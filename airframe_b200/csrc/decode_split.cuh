@@ -60,14 +60,18 @@ __device__ __forceinline__ int da_even_splits(int P, int share, int room, int ho
 
 // What a block loses at the end of a unit inside its run (merging, the next unit's queries, the first page's
 // wait), in pages: the even cut is taken if its largest split is no more than this above the share, and in the run cut a unit
-// of P pages takes P + DA_BREAK_PAGES of a run, the break first.  (Runs of equal pages left the blocks that met
+// of P pages takes P and a break of a run, the break first.  (Runs of equal pages left the blocks that met
 // many short sequences behind.  Measured with heads of 256, two a tile: 64 sequences of 10 to 2,048 tokens, 256 units of which 88 have one page: a decode step of 26 layers
 // 2,412 -> 2,267 us.)
 constexpr int DA_BREAK_PAGES = 2;
+// The same for the 8-bit cache, whose pages take half as long.
+constexpr int D8_BREAK_PAGES = 4;
+__device__ __forceinline__ int da_plan_mark(int blocks, int brk) { return blocks | (brk << 16); }
 
 struct DaPlan {
   int share;        // pages a block should get (the run cut: with the units' breaks)
   int n_blocks;     // blocks that work in the run cut
+  int brk;          // the break
   int even;         // 0: the run cut; else the even cut, and how it rounds (da_even_splits)
   int pages_before; // pages of the sequences before `b_query` (each counted once, not per unit; the run cut: with breaks)
 };
@@ -76,7 +80,7 @@ struct DaPlan {
 // checked that batch x (pages + break) x units stays below 2^31.  If `pages_s` is given it gets the pages of the sequences
 // before b (the run cut: with a break for each that has any), and `splits_s` their splits in the even cut (b = 0 .. batch).
 __device__ __forceinline__ DaPlan da_plan(const int* slots, const int* lens, int batch, int window, int keep,
-                                          const int* shared, int units_per_seq, int grid_blocks, int room, int b_query, int* pages_s, int* splits_s) {
+                                          const int* shared, int brk, int units_per_seq, int grid_blocks, int room, int b_query, int* pages_s, int* splits_s) {
   const int lane = threadIdx.x & 31;
   int carry = 0, most = 0, before = 0, P_first = 0, live = 0, live_before = 0;
   if (pages_s && lane == 0) pages_s[0] = 0;
@@ -98,6 +102,7 @@ __device__ __forceinline__ DaPlan da_plan(const int* slots, const int* lens, int
   }
   most = __reduce_max_sync(0xffffffffu, most);
   DaPlan pl;
+  pl.brk = brk;
   pl.pages_before = __reduce_add_sync(0xffffffffu, before);
   const int total = carry * units_per_seq;
   pl.n_blocks = da_blocks_used(grid_blocks, room, units_per_seq, most);
@@ -123,18 +128,18 @@ __device__ __forceinline__ DaPlan da_plan(const int* slots, const int* lens, int
   int how = 0, worst = 0;
   if (fits1 && (!fits2 || worst1 <= worst2)) how = 1, worst = worst1;
   else if (fits2) how = 2, worst = worst2;
-  pl.even = (how != 0 && worst <= pl.share + DA_BREAK_PAGES) ? how : 0;
+  pl.even = (how != 0 && worst <= pl.share + brk) ? how : 0;
   if (!pl.even) {
     live = __reduce_add_sync(0xffffffffu, live);
-    pl.pages_before += DA_BREAK_PAGES * __reduce_add_sync(0xffffffffu, live_before);
-    pl.share = max(1, ((carry + DA_BREAK_PAGES * live) * units_per_seq + pl.n_blocks - 1) / pl.n_blocks);
+    pl.pages_before += brk * __reduce_add_sync(0xffffffffu, live_before);
+    pl.share = max(1, ((carry + brk * live) * units_per_seq + pl.n_blocks - 1) / pl.n_blocks);
     if (pages_s) {
       int breaks = 0;
       for (int base = 0; base < batch; base += 32) {
         const int i = base + lane;
         const int P = base == 0 ? P_first : (i < batch ? da_pages(slots, lens, i, window, keep, shared) : 0);
         const uint32_t with = __ballot_sync(0xffffffffu, P > 0);
-        if (i < batch) pages_s[i + 1] += DA_BREAK_PAGES * (breaks + __popc(with & (0xffffffffu >> (31 - lane))));
+        if (i < batch) pages_s[i + 1] += brk * (breaks + __popc(with & (0xffffffffu >> (31 - lane))));
         breaks += __popc(with);
       }
     }
@@ -201,8 +206,8 @@ __device__ __forceinline__ DaFirst da_first_segment(const DaPlan& pl, const int*
   const int b = da_find(pages_s, batch, units_per_seq, gpos);
   const int width = pages_s[b + 1] - pages_s[b];
   const int y = (gpos - pages_s[b] * units_per_seq) / width;
-  const int unit0 = pages_s[b] * units_per_seq + y * width, page0 = unit0 + DA_BREAK_PAGES;
-  const int p_in = max(0, gpos - page0), n_pages = min(width - DA_BREAK_PAGES, gend - page0) - p_in;
+  const int unit0 = pages_s[b] * units_per_seq + y * width, page0 = unit0 + pl.brk;
+  const int p_in = max(0, gpos - page0), n_pages = min(width - pl.brk, gend - page0) - p_in;
   if (n_pages <= 0) return fs;                // (the run lies in a break)
   fs.b = b;
   fs.y = y;
@@ -213,8 +218,8 @@ __device__ __forceinline__ DaFirst da_first_segment(const DaPlan& pl, const int*
   return fs;
 }
 // The runs that hold pages of a unit whose break begins at unit0.
-__device__ __forceinline__ int da_run_splits(int unit0, int P, int share) {
-  return P > 0 ? (unit0 + DA_BREAK_PAGES + P - 1) / share - (unit0 + DA_BREAK_PAGES) / share + 1 : 0;
+__device__ __forceinline__ int da_run_splits(int unit0, int P, int share, int brk) {
+  return P > 0 ? (unit0 + brk + P - 1) / share - (unit0 + brk) / share + 1 : 0;
 }
 
 // ---------------------------------------------------------------- the plan of a step
@@ -223,7 +228,7 @@ __device__ __forceinline__ int da_run_splits(int unit0, int P, int share) {
 // layers) can share it: a small kernel works it out once, and each layer's blocks read their first segment from
 // it with one load, where otherwise each block loads slots and lengths, works out the cut and loads page ids,
 // one after the other, before its first copy can start.  The plan, 32-bit integers:
-//   [0, 8)                    room (splits a unit may have), grid blocks, sequences, units a sequence, how cut
+//   [0, 8)                    room (splits a unit may have), grid blocks | break << 16, sequences, units a sequence, how cut
 //   [8, 8 + sequences*units)  the splits of every unit, for the merge
 //   then 16 a block           n_pages (< 0: no work), b, y, z, p_in, run_left, position of the new token, slot,
 //                             the cache pages of the segment's first four pages, the sequence's pages left to another kernel
@@ -262,7 +267,7 @@ __global__ void attn_decode_merge_kernel(__nv_bfloat16* __restrict__ out, long l
     n_splits = ld_keep_int(plan + DA_PLAN_HEAD + b * units_per_seq + (h / group) * tiles + (h % group) / 16, l2_policy_keep());
   } else {
     if (threadIdx.x < 32) {
-      const DaPlan pl = da_plan(slots, lens, batch, window, keep, nullptr, units_per_seq, grid_blocks, max_splits, b, nullptr,
+      const DaPlan pl = da_plan(slots, lens, batch, window, keep, nullptr, DA_BREAK_PAGES, units_per_seq, grid_blocks, max_splits, b, nullptr,
                                 nullptr);
       if (threadIdx.x == 0) plan_s = pl;
     }
@@ -272,7 +277,7 @@ __global__ void attn_decode_merge_kernel(__nv_bfloat16* __restrict__ out, long l
       n_splits = da_even_splits(P, plan_s.share, max_splits, plan_s.even);
     } else {
       const int y = (h / group) * tiles + (h % group) / 16;
-      n_splits = da_run_splits(plan_s.pages_before * units_per_seq + y * (P + DA_BREAK_PAGES), P, plan_s.share);
+      n_splits = da_run_splits(plan_s.pages_before * units_per_seq + y * (P + DA_BREAK_PAGES), P, plan_s.share, DA_BREAK_PAGES);
     }
   }
   pdl_wait();

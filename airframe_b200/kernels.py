@@ -881,11 +881,11 @@ def attn_decode_max_splits(batch: int, nkv: int, max_len: int, window: int, bloc
 
 
 def attn_decode_plan(page_table, slots, lens, nq: int, nkv: int, window: int, ring_rows: int, n_splits: int,
-                     keep: int = 0):
+                     keep: int = 0, bits: int = 16):
     """The plan of a decode step for :func:`attn_decode_split`: how the work is
     cut among the blocks, worked out by one small kernel for all layers that
     read the same caches the same way (these slots, lengths, page table, heads,
-    window, ring and ``n_splits``).  It holds for these lengths alone."""
+    window, ring and ``n_splits``).  It holds for these lengths alone.  ``bits`` 8: for :func:`attn_decode8`."""
     lib = _lib()
     lib.af_attn_decode_plan_ints.restype = ctypes.c_longlong
     B = slots.shape[0]
@@ -893,21 +893,21 @@ def attn_decode_plan(page_table, slots, lens, nq: int, nkv: int, window: int, ri
     if n <= 0:
         raise KernelError(f"attn_decode_plan: {B} sequences, {nq} heads in {nkv} groups")
     plan = torch.empty(n, dtype=torch.int32, device=slots.device)
-    _check(lib.af_attn_decode_plan_kept(
+    _check((lib.af_attn_decode8_plan if bits == 8 else lib.af_attn_decode_plan_kept)(
         _ptr(plan, "plan", torch.int32), c_longlong(n), _ptr(page_table, "page_table", torch.int32),
         c_int(page_table.shape[1]), _ptr(slots, "slots", torch.int32), _ptr(lens, "lens", torch.int32), c_int(B),
         c_int(nq), c_int(nkv), c_int(window), c_int(keep), c_int(ring_rows), c_int(n_splits), _stream()))
     return plan
 
 
-def _step_plan(kv, batch, nq: int, nkv: int, window: int, keep: int, n_splits: int):
+def _step_plan(kv, batch, nq: int, nkv: int, window: int, keep: int, n_splits: int, bits: int = 16):
     """The plan of the step (see :func:`attn_decode_plan`), made once in a pass for all layers that read this group of caches
     alike (a batch without a place for the step's tables gets a plan for the call)."""
     aux = getattr(batch, "aux", None)
-    key = ("attn_decode_plan", kv.page_table.data_ptr(), kv.ring_rows, nq, nkv, window, keep, n_splits)
+    key = ("attn_decode_plan", kv.page_table.data_ptr(), kv.ring_rows, nq, nkv, window, keep, n_splits, bits)
     plan = aux.get(key) if aux is not None else None
     if plan is None:
-        plan = attn_decode_plan(kv.page_table, batch.slots, batch.len_after, nq, nkv, window, kv.ring_rows, n_splits, keep)
+        plan = attn_decode_plan(kv.page_table, batch.slots, batch.len_after, nq, nkv, window, kv.ring_rows, n_splits, keep, bits)
         if aux is not None:
             aux[key] = plan
     return plan
@@ -1041,7 +1041,7 @@ def attn_decode8(out, q, kv, batch, nq: int, nkv: int, hd: int, scale: float, ca
     if B > ATTN_DECODE_MAX_SEQS:
         raise KernelError(f"attn_decode8: {B} sequences (takes {ATTN_DECODE_MAX_SEQS})")
     n = attn_decode_max_splits(B, nkv, batch.max_len_after, window, nq=nq, keep=keep)
-    plan = _step_plan(kv, batch, nq, nkv, window, keep, n)
+    plan = _step_plan(kv, batch, nq, nkv, window, keep, n, 8)
     lib = _lib()
     lib.af_attn_decode_scratch.restype = ctypes.c_longlong
     scratch = torch.empty(lib.af_attn_decode_scratch(c_int(B), c_int(nq), c_int(hd), c_int(n)), dtype=torch.float32, device=q.device)
@@ -1089,7 +1089,7 @@ def attn_decode_shared(out, q, kv, batch, nq: int, nkv: int, hd: int, scale: flo
     table = kv.page_table
     n = attn_decode_max_splits(B, nkv, batch.max_len_after, 0, nq=nq)
     aux = getattr(batch, "aux", None)
-    key = ("attn_shared_plan", table.data_ptr(), nq, nkv, n, lead.data_ptr(), pages.data_ptr())
+    key = ("attn_shared_plan", table.data_ptr(), nq, nkv, n, eight, lead.data_ptr(), pages.data_ptr())
     plan = aux.get(key) if aux is not None else None
     if plan is None:
         ints = lib.af_attn_shared_plan_ints(c_int(B), c_int(nq), c_int(nkv))
@@ -1097,7 +1097,8 @@ def attn_decode_shared(out, q, kv, batch, nq: int, nkv: int, hd: int, scale: flo
         _check(lib.af_attn_shared_plan(
             _ptr(plan, "plan", torch.int32), c_longlong(ints), _ptr(lead, "lead", torch.int32), _ptr(pages, "pages", torch.int32),
             _ptr(table, "page_table", torch.int32), c_int(table.shape[1]), _ptr(batch.slots, "slots", torch.int32),
-            _ptr(batch.len_after, "lens", torch.int32), c_int(B), c_int(nq), c_int(nkv), c_int(n), _stream()))
+            _ptr(batch.len_after, "lens", torch.int32), c_int(B), c_int(nq), c_int(nkv), c_int(n), c_int(8 if eight else 16),
+            _stream()))
         if aux is not None:
             aux[key] = plan
     n_own = lib.af_attn_decode_scratch(c_int(B), c_int(nq), c_int(hd), c_int(n))
