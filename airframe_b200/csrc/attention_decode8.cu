@@ -31,22 +31,25 @@ constexpr float D8_SHIFT = 6.f;          // weights are kept times 2^6
 
 template <int HD, int NT>
 struct D8 {
-  // (the accumulators of 16 heads of 256 take 128 registers, those of 8 heads 64 beside 32 of queries: fewer warps)
-  static constexpr int THREADS = HD * NT == 512 ? 256 : (HD * NT == 256 ? 384 : 512);
-  static constexpr int WARPS = THREADS / 32;
-  // keys of a piece: half a page where heads are large, so that all warps have pieces in shared memory
-  static constexpr int KEYS = HD == 256 ? 32 : 64, PER_PAGE = AF_PAGE / KEYS, TILES = KEYS / 16;
+  // Warps that compute (one more brings the pieces in; registers are dealt to four warps at a time): the accumulators of 16 heads
+  // of 256 take 128 registers, those of 8 heads 64 beside 32 of queries.
+  static constexpr int WARPS = HD * NT == 512 ? 7 : (HD * NT == 256 ? 11 : 15), THREADS = (WARPS + 1) * 32;
+  // A stage holds a page.  What a warp takes at a time is a piece of it, 8 KB of keys and values: a page's pieces are worked side by
+  // side, so that a stage is soon free again and as many bytes are on their way as are being worked.
+  static constexpr int KEYS = 4096 / HD, TILES = KEYS / 16;              // keys of a piece, and its tiles of 16 keys
   static constexpr int AT_ONCE = NT == 2 && TILES == 4 ? 2 : TILES;      // tiles of a piece that are worked together
-  static constexpr int CODES = KEYS * HD;                                // bytes of a piece's keys, and of its values
-  static constexpr int SUB = KEYS * 128;                                 // bytes of a sub-tile of 128 dims
-  static constexpr int STAGES = HD == 64 ? 16 : 12;
-  // barriers: a piece's must not be met by another warp's pieces (a multiple of WARPS), nor be armed before the piece in the
-  // same stage was consumed (a multiple of STAGES)
-  static constexpr int NBAR = HD == 64 ? 16 : (WARPS == 16 ? 48 : (WARPS == 12 ? 12 : 24));
+  static constexpr int CODES = AF_PAGE * HD;                             // bytes of a page's keys, and of its values
+  static constexpr int SUB = AF_PAGE * 128;                              // bytes of a sub-tile of 128 dims
+  static constexpr int STAGES = HD == 256 ? 6 : (HD == 128 ? 12 : 20);
+  // Barriers of the pages: the producer fills in order, so a page is only on its way when all pages STAGES before it are consumed; a
+  // warp's next piece lies at most WARPS / (pieces of a page) + 1 pages behind its last one, and must not meet the barrier of a page
+  // that is still on its way.
+  static constexpr int NBAR = 2 * STAGES;
   static constexpr int RING = STAGES * 2 * CODES;
-  static constexpr int SMEM = RING + STAGES * 2 * KEYS + 1024;
-  static_assert(NBAR % WARPS == 0 && NBAR % STAGES == 0, "barriers");
-  static_assert(WARPS * 8 * NT * HD * 4 <= RING, "the merge's buffer");
+  static constexpr int EXPS = 32;                                        // pages whose exponents are kept: eight more than stages
+  static constexpr int MERGE = 24 << 10, ROUND = MERGE / (WARPS * HD * 4);       // the merge's buffer, and the rows it takes at a time
+  static constexpr int SMEM = RING + MERGE + EXPS * 2 * AF_PAGE + 1024;
+  static_assert(NBAR >= STAGES + WARPS * TILES / 4 + 2 && EXPS >= STAGES + 8 && ROUND >= 1, "barriers and buffers");
 };
 
 struct Decode8Args {
@@ -90,17 +93,33 @@ __device__ __forceinline__ int d8_lds_u8(uint32_t addr) {
   asm volatile("ld.shared.u8 %0, [%1];" : "=r"(v) : "r"(addr));
   return (int)v;
 }
-__device__ __forceinline__ void d8_bulk(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
-  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(smem_u32(dst)),
-               "l"(src), "r"(bytes), "r"(smem_u32(bar))
-               : "memory");
+// Whether the barrier's phase is complete, without a wait.
+__device__ __forceinline__ bool d8_is_complete(uint64_t* bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(smem_u32(bar)), "r"(parity)
+      : "memory");
+  return ok != 0;
 }
-// S^T, softmax and O^T of N tiles of 16 keys (all of a piece, or one), beginning with tile `t0`.
+// All of a page's codes, keys or values: rows [row, row + 64) of every sub-tile of 128 dims (see d8_map).
+__device__ __forceinline__ void d8_load(void* dst, const CUtensorMap* map, int row, uint64_t* bar, uint64_t policy) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes.L2::cache_hint [%0], [%1, {%3, %4, %3}], [%2], %5;" ::"r"(
+          smem_u32(dst)),
+      "l"(map), "r"(smem_u32(bar)), "r"(0), "r"(row), "l"(policy)
+      : "memory");
+}
+
+// S^T, softmax and O^T of N tiles of 16 keys, beginning with tile `t0` of a page.
 template <int HD, int NT, int N>
 struct D8Step {
   using C = D8<HD, NT>;
-  // k_l, v_l, e_l: this lane's addresses of the piece's keys, values and exponents (tile 0); swap: what the odd halves' addresses
-  // differ by (the swizzle); lo, hi, keep: the visible keys, counted from the piece's first
+  // k_l, v_l, ke_l: this lane's addresses of the page's keys, values and exponents (tile 0); lo, hi, keep: the visible keys, counted
+  // from the page's first
   __device__ static __forceinline__ void run(uint32_t k_l, uint32_t v_l, uint32_t ke_l, int t0, bool whole, int lo, int hi, int keep,
                                              int g, int t, bool capped, float ecap, float capl, const uint32_t (&qf)[NT][HD / 16][2],
                                              const float (&cq)[NT][2], float (&o)[HD / 16][NT][4], float (&rs)[NT][2], float (&ra)[NT][2],
@@ -141,7 +160,7 @@ struct D8Step {
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         ks[h] = __uint_as_float((uint32_t)d8_lds_u8(ke_l + i * 16 + 8 * h) << 23);
-        lv[h] = (float)(d8_lds_u8(ke_l + C::KEYS + i * 16 + 8 * h) - 127);
+        lv[h] = (float)(d8_lds_u8(ke_l + AF_PAGE + i * 16 + 8 * h) - 127);
       }
 #pragma unroll
       for (int n = 0; n < NT; ++n)
@@ -258,19 +277,25 @@ struct D8Step {
   }
 };
 
+// What a segment of a block's work is: some of the pages of one unit.  The producer warp works it out, the others read it.
+struct D8Segment {
+  int b, kvh, row_head0, n_rows, z, n_pages, x_begin, kept, skip, lo, pos, more;
+};
+
 template <int HD, int NT>
 __global__ void __launch_bounds__(D8<HD, NT>::THREADS, 1)
 decode8_split_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, Decode8Args a) {
   using C = D8<HD, NT>;
-  constexpr int STAGES = C::STAGES, WARPS = C::WARPS, NBAR = C::NBAR, PER = C::PER_PAGE;
+  constexpr int STAGES = C::STAGES, WARPS = C::WARPS, NBAR = C::NBAR, SEGS = 4;
   constexpr int ROWS = 8 * NT;
   constexpr float LOG2E = 1.4426950408889634f;
   extern __shared__ unsigned char d8_raw[];
   unsigned char* ring = (unsigned char*)(((uintptr_t)d8_raw + 1023) & ~(uintptr_t)1023);
-  unsigned char* exps = ring + C::RING;                        // [stage][k exponents | v exponents]
-  __shared__ uint64_t full[NBAR];
+  float* o_s = reinterpret_cast<float*>(ring + C::RING);       // the merge's buffer: [warp][row of the round][HD]
+  unsigned char* exps = ring + C::RING + C::MERGE;             // [page modulo EXPS][k exponents | v exponents]
+  __shared__ uint64_t full[NBAR], empty[STAGES], seg_full[SEGS], seg_empty[SEGS];
+  __shared__ D8Segment seg_s[SEGS];
   __shared__ float rs_s[WARPS][ROWS], ra_s[WARPS][ROWS], l_s[WARPS][ROWS];
-  __shared__ float f_s[WARPS][ROWS], ml_s[ROWS][2];
   __shared__ int give_up_s;
   volatile int* give_up = &give_up_s;
 
@@ -278,19 +303,20 @@ decode8_split_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
   const int group = a.nq / a.nkv;
   const int tiles = (group + 15) / 16, units_per_seq = a.nkv * tiles;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int g = lane >> 2, t = lane & 3;
-  if (tid == 0) {
-    for (int s = 0; s < NBAR; ++s) mbar_init(&full[s], 1);
-    give_up_s = 0;
-    mbar_fence_init();
-  }
-  // what the block begins with, from the step's plan
+  const int4 head = ld_keep_int4(reinterpret_cast<const int4*>(a.plan), l2_policy_keep());
   const int4* rec = reinterpret_cast<const int4*>(a.plan + da_plan_records_at(a.batch, units_per_seq)) +
                     (size_t)blockIdx.x * (DA_PLAN_REC / 4);
-  const uint64_t keep_policy = l2_policy_keep();
-  const int4 head = ld_keep_int4(reinterpret_cast<const int4*>(a.plan), keep_policy);
-  const int4 r0 = ld_keep_int4(rec, keep_policy), r1 = ld_keep_int4(rec + 1, keep_policy), r2 = ld_keep_int4(rec + 2, keep_policy);
-  const int4 r3 = ld_keep_int4(rec + 3, keep_policy);
+  const int4 r0 = ld_keep_int4(rec, l2_policy_keep());
+  if (warp == 0) {
+    for (int s = lane; s < NBAR; s += 32) mbar_init(&full[s], 2);      // (the copies, and the exponents)
+    for (int s = lane; s < STAGES; s += 32) mbar_init(&empty[s], AF_PAGE / 16);
+    if (lane < SEGS) {
+      mbar_init(&seg_full[lane], 1);
+      mbar_init(&seg_empty[lane], WARPS);
+    }
+    if (lane == 0) give_up_s = 0;
+    mbar_fence_init();
+  }
   if (head.x != a.n_splits || head.y != da_plan_mark((int)gridDim.x, D8_BREAK_PAGES) || head.z != a.batch || head.w != units_per_seq) {
     if (tid == 0 && a.err) atomicExch(a.err, 1);      // (a plan made for another launch: nothing is read or written by it)
     return;
@@ -300,105 +326,181 @@ decode8_split_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
     if (blockIdx.x == 0) pdl_wait();
     return;
   }
-  int left = r1.y;
 
-  struct Segment {
-    int b, kvh, row_head0, n_rows, z, n_pages, x_begin, kept, skip, last_pp, lo, pos, y;
+  if (warp == WARPS) {
+    // ---- the producer: segments, and their pieces through the ring without a pause between segments
+    const int4 r1 = ld_keep_int4(rec + 1, l2_policy_keep()), r2 = ld_keep_int4(rec + 2, l2_policy_keep());
+    const int4 r3 = ld_keep_int4(rec + 3, l2_policy_keep());
+    int left = r1.y;                                  // what the block's run holds behind the segment's unit
     const int* pt;
-  };
-  auto of_unit = [&](Segment& sg, int b, int y, int p_in, int pos, int slot, int shared) {
-    sg.b = b;
-    sg.y = y;
-    sg.kvh = y / tiles;
-    sg.row_head0 = sg.kvh * group + (y % tiles) * 16;
-    sg.n_rows = min(16, sg.kvh * group + group - sg.row_head0);
-    sg.pos = pos;
-    sg.lo = da_lo(pos, a.window);
-    sg.last_pp = pos / AF_PAGE;
-    const DaList l = da_list(pos, a.window, a.keep, shared);
-    sg.kept = l.kept, sg.skip = l.skip;
-    sg.x_begin = p_in;
-    sg.pt = a.page_table + (size_t)slot * a.max_pages;
-  };
-  auto next_unit = [&](const Segment& sg) {           // (the run cut: see attention_decode.cu)
-    Segment nx;
-    int b = sg.b, y = sg.y + 1;
-    if (y >= units_per_seq) {
-      y = 0;
-      do ++b; while (b < a.batch - 1 && da_pages(a.slots, a.lens, b, a.window, a.keep, a.shared) == 0);
-    }
-    const int P = da_pages(a.slots, a.lens, b, a.window, a.keep, a.shared);
-    nx.z = 0;
-    nx.n_pages = min(P, left - D8_BREAK_PAGES);
-    left -= D8_BREAK_PAGES + P;
-    of_unit(nx, b, y, 0, a.lens[b] - 1, a.slots[b], a.shared != nullptr ? a.shared[b] : 0);
-    return nx;
-  };
-  auto page_of = [&](const Segment& sg, int i) { return da_page_of(sg.kept, sg.skip, sg.x_begin + i); };
-  auto safe = [&](int page) { return AF_INDEX_OK(page >= 0 && page < a.n_pages, page) && page >= 0 && page < a.n_pages ? page : 0; };
-  auto page_id = [&](const Segment& sg, int i) {
-    const int entry = af_cache_row(page_of(sg, i) * AF_PAGE, a.ring_rows, a.keep) / AF_PAGE;
-    return AF_INDEX_OK(entry < a.max_pages, entry) && entry < a.max_pages ? safe(sg.pt[entry]) : 0;
-  };
-  const uint64_t read_once = l2_policy_read_once();
-  // piece `half` of cache page `page`, the block's piece number ii, into its stage
-  auto issue = [&](int kvh, int page, int half, int ii) {
-    const int s = ii % STAGES, row = (page * a.nkv + kvh) * AF_PAGE + half * C::KEYS;
-    unsigned char* st = ring + (size_t)s * 2 * C::CODES;
-    uint64_t* bar = &full[ii % NBAR];
-    mbar_expect_tx(bar, 2 * C::CODES + 2 * C::KEYS);
-#pragma unroll
-    for (int c = 0; c < (HD + 127) / 128; ++c) {
-      tma_load_2d_once(st + c * C::SUB, &map_k, c * 128, row, bar, read_once);
-      tma_load_2d_once(st + C::CODES + c * C::SUB, &map_v, c * 128, row, bar, read_once);
-    }
-    d8_bulk(exps + s * 2 * C::KEYS, a.k_exp + row, C::KEYS, bar);
-    d8_bulk(exps + s * 2 * C::KEYS + C::KEYS, a.v_exp + row, C::KEYS, bar);
-  };
-  auto issue_from = [&](const Segment& sg, int from, int to, int ii0, bool skip_last) {      // (pieces of the segment)
-    int i = from;
-    int page = -1, id = 0;
-    for (; i < to; ++i) {
-      if (skip_last && page_of(sg, i / PER) == sg.last_pp) break;
-      if (i / PER != page) page = i / PER, id = page_id(sg, page);
-      issue(sg.kvh, id, i % PER, ii0 + i);
-    }
-    return i;
-  };
-
-  int i_base = 0;
-  Segment sg;
-  sg.z = r0.w;
-  sg.n_pages = r0.x;
-  of_unit(sg, r0.y, r0.z, r1.x, r1.z, r1.w, r3.x);
-  int issued = 0;
-  if (tid == 0) {
-    // pages of earlier tokens are on their way before the wait for the kernel in front; the new token's waits.  The first
-    // four pages' ids are in the plan.
-    const int ids0[4] = {r2.x, r2.y, r2.z, r2.w};
-    bool go = true;
-#pragma unroll
-    for (int k = 0; k < 4 * PER; ++k) {
-      go = go && k < STAGES && k < sg.n_pages * PER && page_of(sg, k / PER) != sg.last_pp;
-      if (go) {
-        issue(sg.kvh, safe(ids0[k / PER]), k % PER, k);
-        ++issued;
+    D8Segment sg;
+    int y;
+    auto of_unit = [&](int b, int y, int p_in, int pos, int slot, int shared) {
+      sg.b = b;
+      sg.kvh = y / tiles;
+      sg.row_head0 = sg.kvh * group + (y % tiles) * 16;
+      sg.n_rows = min(16, sg.kvh * group + group - sg.row_head0);
+      sg.pos = pos;
+      sg.lo = da_lo(pos, a.window);
+      const DaList l = da_list(pos, a.window, a.keep, shared);
+      sg.kept = l.kept, sg.skip = l.skip;
+      sg.x_begin = p_in;
+      pt = a.page_table + (size_t)slot * a.max_pages;
+    };
+    auto safe = [&](int page) { return AF_INDEX_OK(page >= 0 && page < a.n_pages, page) && page >= 0 && page < a.n_pages ? page : 0; };
+    auto page_id = [&](int i) {
+      const int entry = af_cache_row(da_page_of(sg.kept, sg.skip, sg.x_begin + i) * AF_PAGE, a.ring_rows, a.keep) / AF_PAGE;
+      return AF_INDEX_OK(entry < a.max_pages, entry) && entry < a.max_pages ? safe(pt[entry]) : 0;
+    };
+    const uint64_t read_once = l2_policy_read_once();
+    sg.z = r0.w;
+    sg.n_pages = r0.x;
+    y = r0.z;
+    of_unit(r0.y, y, r1.x, r1.z, r1.w, r3.x);
+    bool waited = false;                              // for the kernel in front
+    int ii = 0, stage = 0, bar = 0;                   // pages so far; their stage and barrier
+    uint32_t phase = 0;
+    for (int k = 0;; ++k) {
+      sg.more = left > D8_BREAK_PAGES ? 1 : 0;        // (the even cut: one segment)
+      if (k >= SEGS && !mbar_wait(&seg_empty[k % SEGS], ((k / SEGS) & 1) ^ 1, give_up)) break;
+      if (lane == 0) {
+        seg_s[k % SEGS] = sg;
+        mbar_arrive(&seg_full[k % SEGS]);
       }
+      if (waited && lane < sg.n_rows * (HD / 64))     // (the unit's queries: asked into L1 now, read when their segment begins)
+        asm volatile("prefetch.global.L1 [%0];" ::"l"(a.q + (size_t)sg.b * a.q_stride + (size_t)(sg.row_head0 + lane / (HD / 64)) * HD +
+                                                       (lane % (HD / 64)) * 64));
+      const int last_pp = sg.pos / AF_PAGE;           // the page of the new token, which the kernel in front wrote
+      // Eight pages at a time (of a block's first segment first the four whose ids are in the plan).  A lane has a quarter (16 bytes)
+      // of a page's exponents, asked for a round ahead, and sends its page's copies off when the stage is free: as many pages as are
+      // free in a row go out at once.  The page of the new token, a segment's last, was written by the kernel in front.
+      const int quarter = lane & 3, mine = lane >> 2;
+      uint4 kx = make_uint4(0u, 0u, 0u, 0u), vx = kx;
+      auto is_last = [&](int i) { return da_page_of(sg.kept, sg.skip, sg.x_begin + i) == last_pp; };
+      auto load = [&](int page) {
+        const size_t at = (size_t)(page * a.nkv + sg.kvh) * AF_PAGE + quarter * 16;
+        kx = __ldcg(reinterpret_cast<const uint4*>(a.k_exp + at));
+        vx = __ldcg(reinterpret_cast<const uint4*>(a.v_exp + at));
+      };
+      int id = 0;
+      auto ask = [&](int i) {
+        if (i < sg.n_pages) {
+          id = k == 0 && i < 4 ? safe(i == 0 ? r2.x : (i == 1 ? r2.y : (i == 2 ? r2.z : r2.w))) : page_id(i);
+          if (waited || !is_last(i)) load(id);
+        }
+      };
+      int m = k == 0 ? 4 : 8;
+      if (mine < m) ask(mine);
+      bool ok = true;
+      for (int i0 = 0; i0 < sg.n_pages && ok; i0 += m, m = 8) {
+        m = min(m, sg.n_pages - i0);
+        const int here = id;
+        bool late = !waited && is_last(i0 + m - 1);
+        const int at = stage + mine, my_stage = at >= 2 * STAGES ? at - 2 * STAGES : (at >= STAGES ? at - STAGES : at);
+        const uint32_t my_phase = (at >= 2 * STAGES ? phase : (at >= STAGES ? phase ^ 1 : phase)) ^ 1;
+        const int my_bar = bar + mine >= NBAR ? bar + mine - NBAR : bar + mine;
+        int done = 0;
+        while (done < m) {
+          if (late && done == m - 1) {
+            pdl_wait();
+            waited = true;
+            late = false;
+            if (mine == done) load(here);
+          }
+          __syncwarp();
+          const bool open = ii + mine < STAGES || d8_is_complete(&empty[my_stage], my_phase);
+          const int most = late ? m - 1 : m;
+          const uint32_t shut = __ballot_sync(0xffffffffu, mine >= done && !(open && mine < most));
+          const int upto = shut ? (__ffs(shut) - 1) >> 2 : 8;
+          if (upto > done) {
+            if (quarter == 0 && mine >= done && mine < upto) {
+              const int row = (here * a.nkv + sg.kvh) * AF_PAGE;
+              unsigned char* st = ring + (size_t)my_stage * 2 * C::CODES;
+              mbar_expect_tx(&full[my_bar], 2 * C::CODES);
+              d8_load(st, &map_k, row, &full[my_bar], read_once);
+              d8_load(st + C::CODES, &map_v, row, &full[my_bar], read_once);
+            }
+            // (and their exponents: the round's later pages may need these pages' stages)
+            if (mine >= done && mine < upto) {
+              uint4* e = reinterpret_cast<uint4*>(exps + ((ii + mine) % C::EXPS) * 2 * AF_PAGE) + quarter;
+              e[0] = kx;
+              e[AF_PAGE / 16] = vx;
+            }
+            __syncwarp();
+            if (quarter == 0 && mine >= done && mine < upto) mbar_arrive(&full[my_bar]);
+            done = upto;
+          } else if (done < most) {
+            // nothing is free: the page's wait, bounded in time (every lane the same barrier)
+            const int w = stage + done;
+            ok = mbar_wait(&empty[w >= 2 * STAGES ? w - 2 * STAGES : (w >= STAGES ? w - STAGES : w)],
+                           (w >= 2 * STAGES ? phase : (w >= STAGES ? phase ^ 1 : phase)) ^ 1, give_up);
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) break;
+          }
+        }
+        if (!ok) break;
+        ask(i0 + m + mine);
+        ii += m;
+        stage += m;
+        while (stage >= STAGES) stage -= STAGES, phase ^= 1;
+        bar = bar + m >= NBAR ? bar + m - NBAR : bar + m;
+      }
+      if (!ok || !sg.more) break;
+      // the run cut goes on with the unit behind: the same sequence's next, or the first of the next sequence that has pages
+      int b = sg.b;
+      if (++y >= units_per_seq) {
+        y = 0;
+        do ++b; while (b < a.batch - 1 && da_pages(a.slots, a.lens, b, a.window, a.keep, a.shared) == 0);
+      }
+      const int P = da_pages(a.slots, a.lens, b, a.window, a.keep, a.shared);
+      sg.z = 0;
+      sg.n_pages = min(P, left - D8_BREAK_PAGES);
+      left -= D8_BREAK_PAGES + P;
+      of_unit(b, y, 0, a.lens[b] - 1, a.slots[b], a.shared != nullptr ? a.shared[b] : 0);
     }
-    if (issued == 4 * PER) issued = issue_from(sg, issued, min(STAGES, sg.n_pages * PER), 0, true);
+    if (*give_up && lane == 0) {
+      grace_period();
+      if (a.err) atomicExch(a.err, 1);
+    }
+    return;
   }
+
+  // ---- the other warps
+  const int g = lane >> 2, t = lane & 3;
+  const float ecap = a.cap > 0.f ? 2.f * LOG2E / a.cap : 0.f, capl = a.cap * LOG2E;
+  // this lane's place in a piece (see D8Step)
+  const int pg = d8_perm(g);
+  const uint32_t k_off = HD == 64 ? pg * 64 + ((t ^ ((pg >> 1) & 3)) << 4) : pg * 128 + ((t ^ pg) << 4);
+  const uint32_t v_off = C::CODES + (HD == 64 ? t * 64 + (((g >> 1) ^ (t >> 1)) << 4) + (g & 1) * 8 : t * 128 + ((pg ^ t) << 4));
+  // a barrier of these warps with a vote: they go on or give up together
+  auto all_of = [&](bool ok) {
+    int all;
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\t"
+        "setp.ne.b32 q, %1, 0;\n\t"
+        "barrier.red.and.pred.aligned p, 1, %2, q;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(all)
+        : "r"(ok ? 1 : 0), "n"(WARPS * 32)
+        : "memory");
+    return all != 0;
+  };
   pdl_wait();
-  while (true) {
-    const int b = sg.b, n = sg.n_pages * PER, n_rows = sg.n_rows, row_head0 = sg.row_head0;
-    if (tid == 0) issued = issue_from(sg, issued, min(STAGES, n), i_base, false);
+  int i_base = 0;
+  for (int k = 0;; ++k) {
+    if (!all_of(mbar_wait(&seg_full[k % SEGS], (k / SEGS) & 1, give_up))) break;
+    const D8Segment sg = seg_s[k % SEGS];
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&seg_empty[k % SEGS]);
+    const int n = sg.n_pages, n_rows = sg.n_rows, row_head0 = sg.row_head0;
 
     // ---- the queries as B fragments (head g of every tile of 8), halves brought to [2^14, 2^15)
     uint32_t qf[NT][HD / 16][2];
     float cq[NT][2];                     // per column (head) of this lane: the factor of its scores
 #pragma unroll
-    for (int n = 0; n < NT; ++n) {
-      const bool on = n * 8 + g < n_rows;
-      const __nv_bfloat16* qr = a.q + (size_t)b * a.q_stride + (size_t)(row_head0 + n * 8 + g) * HD + t * 16;
+    for (int n8 = 0; n8 < NT; ++n8) {
+      const bool on = n8 * 8 + g < n_rows;
+      const __nv_bfloat16* qr = a.q + (size_t)sg.b * a.q_stride + (size_t)(row_head0 + n8 * 8 + g) * HD + t * 16;
       uint32_t top = 0;
 #pragma unroll
       for (int c = 0; c < HD / 64; ++c) {
@@ -406,8 +508,8 @@ decode8_split_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
         for (int j = 0; j < 4; ++j) {
           const uint32_t* p = reinterpret_cast<const uint32_t*>(qr + c * 64 + j * 4);
           const uint32_t x = on ? p[0] : 0u, y = on ? p[1] : 0u;
-          qf[n][c * 4 + j][0] = x;
-          qf[n][c * 4 + j][1] = y;
+          qf[n8][c * 4 + j][0] = x;
+          qf[n8][c * 4 + j][1] = y;
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             const uint32_t w = h ? y : x, lo = w & 0x7fffu, hi = (w >> 16) & 0x7fffu;
@@ -418,140 +520,123 @@ decode8_split_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
       top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
       top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
       // (the scaling in two steps: 2^(14 - k) alone may pass the largest power of two)
-      const int k = top == 0 ? 14 : max((int)(top >> 7) - 127, -126), up = 14 - k;
+      const int kx = top == 0 ? 14 : max((int)(top >> 7) - 127, -126), up = 14 - kx;
       const float f1 = c8_pow2(up / 2), f2 = c8_pow2(up - up / 2);
-      // cq = scale 2^-up in two steps, too
       const float cs = (a.cap > 0.f ? a.scale : a.scale * LOG2E) * c8_pow2(-(up / 2)) * c8_pow2(-(up - up / 2));
 #pragma unroll
       for (int i = 0; i < HD / 16; ++i)
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          const uint32_t w = qf[n][i][h];
+          const uint32_t w = qf[n8][i][h];
           const __half2 v = __floats2half2_rn(__uint_as_float(w << 16) * f1 * f2, __uint_as_float(w & 0xffff0000u) * f1 * f2);
-          qf[n][i][h] = *reinterpret_cast<const uint32_t*>(&v);
+          qf[n8][i][h] = *reinterpret_cast<const uint32_t*>(&v);
         }
-      cq[n][0] = __shfl_sync(0xffffffffu, cs, t * 8);
-      cq[n][1] = __shfl_sync(0xffffffffu, cs, t * 8 + 4);
+      cq[n8][0] = __shfl_sync(0xffffffffu, cs, t * 8);
+      cq[n8][1] = __shfl_sync(0xffffffffu, cs, t * 8 + 4);
     }
-    const float ecap = a.cap > 0.f ? 2.f * LOG2E / a.cap : 0.f, capl = a.cap * LOG2E;
-
     float o[HD / 16][NT][4];
 #pragma unroll
     for (int m = 0; m < HD / 16; ++m)
 #pragma unroll
-      for (int n = 0; n < NT; ++n) o[m][n][0] = o[m][n][1] = o[m][n][2] = o[m][n][3] = 0.f;
+      for (int n8 = 0; n8 < NT; ++n8) o[m][n8][0] = o[m][n8][1] = o[m][n8][2] = o[m][n8][3] = 0.f;
     float rs[NT][2], ra[NT][2], l[NT][2];
 #pragma unroll
-    for (int n = 0; n < NT; ++n) rs[n][0] = rs[n][1] = ra[n][0] = ra[n][1] = D8_NONE, l[n][0] = l[n][1] = 0.f;
+    for (int n8 = 0; n8 < NT; ++n8) rs[n8][0] = rs[n8][1] = ra[n8][0] = ra[n8][1] = D8_NONE, l[n8][0] = l[n8][1] = 0.f;
 
-    // A warp takes a piece at a time; where the pieces are fewer than the warps, a tile of 16 keys.
-    const bool few = n <= STAGES && n * C::TILES <= 2 * WARPS;
-    const int items = few ? n * C::TILES : n;
-    // this lane's place in a piece (see D8Step)
-    const int pg = d8_perm(g);
-    const uint32_t k_off = HD == 64 ? pg * 64 + ((t ^ ((pg >> 1) & 3)) << 4) : pg * 128 + ((t ^ pg) << 4);
-    const uint32_t v_off = C::CODES + (HD == 64 ? t * 64 + (((g >> 1) ^ (t >> 1)) << 4) + (g & 1) * 8 : t * 128 + ((pg ^ t) << 4));
+    // A warp takes a piece at a time; where the keys are few, a tile of 16.
+    const int each = n * 4 <= 2 * WARPS ? 1 : C::TILES, items = n * 4 / each;
+    bool ok = true;
     for (int x = warp; x < items; x += WARPS) {
-      const int i = few ? x / C::TILES : x, ii = i_base + i, s = ii % STAGES;
-      const bool refill = lane == 0 && i + STAGES < n;
-      const int refill_page = refill ? page_id(sg, (i + STAGES) / PER) : 0;
-      if (!mbar_wait(&full[ii % NBAR], (ii / NBAR) & 1, give_up)) break;
-      const uint32_t st = smem_u32(ring) + s * 2 * C::CODES, e_l = smem_u32(exps) + s * 2 * C::KEYS + pg;
-      const int base = page_of(sg, i / PER) * AF_PAGE + (i % PER) * C::KEYS;
+      const int tile = x * each & 3, i = x * each >> 2, ii = i_base + i, s = ii % STAGES;
+      ok = mbar_wait(&full[ii % NBAR], (ii / NBAR) & 1, give_up);
+      if (!ok) break;
+      const uint32_t st = smem_u32(ring) + s * 2 * C::CODES, e_l = smem_u32(exps) + ii % C::EXPS * 2 * AF_PAGE + pg;
+      const int base = da_page_of(sg.kept, sg.skip, sg.x_begin + i) * AF_PAGE;
       const int lo = sg.lo - base, hi = sg.pos - base, keep = a.keep - base;       // (visible: [lo, hi] and what is before keep)
-      const bool whole = C::KEYS - 1 <= hi && (lo <= 0 || C::KEYS - 1 < keep);
-      if (few)
-        D8Step<HD, NT, 1>::run(st + k_off, st + v_off, e_l, x % C::TILES, whole, lo, hi, keep, g, t, a.cap > 0.f, ecap, capl, qf, cq, o, rs, ra, l);
-      else
+      const bool whole = AF_PAGE - 1 <= hi && (lo <= 0 || AF_PAGE - 1 < keep);
+      if (C::AT_ONCE > 1 && each == 1) {
+        D8Step<HD, NT, 1>::run(st + k_off, st + v_off, e_l, tile, whole, lo, hi, keep, g, t, a.cap > 0.f, ecap, capl, qf, cq, o, rs, ra, l);
+      } else {
 #pragma unroll 1
-        for (int t0 = 0; t0 < C::TILES; t0 += C::AT_ONCE)
+        for (int t0 = tile; t0 < tile + each; t0 += C::AT_ONCE)
           D8Step<HD, NT, C::AT_ONCE>::run(st + k_off, st + v_off, e_l, t0, whole, lo, hi, keep, g, t, a.cap > 0.f, ecap, capl, qf, cq, o, rs, ra, l);
+      }
       __syncwarp();
-      if (refill && !*give_up) issue(sg.kvh, refill_page, (i + STAGES) % PER, ii + STAGES);
+      if (lane == 0)
+        asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0], %1;" ::"r"(smem_u32(&empty[s])), "r"(each) : "memory");
     }
-    if (*give_up && tid == 0) grace_period();
-    __syncthreads();
-    const bool gave_up = *give_up != 0;
-
-    // ---- merge the warps through shared memory (the stages that the next segment's first pages do not take)
     i_base += n;
-    const bool more = left > D8_BREAK_PAGES && !gave_up;
-    const int buf_bytes = WARPS * n_rows * HD * 4, buf_stages = (buf_bytes + 2 * C::CODES - 1) / (2 * C::CODES);
-    Segment nx = sg;
-    issued = 0;
-    // The buffer is `buf_stages` stages in a row (they do not wrap): those just before the next page's stage, so that all
-    // others can be filled, or where these are too few the last ones, and the pages up to them can.
-    const int first = i_base % STAGES;
-    const int buf0 = first >= buf_stages ? first - buf_stages : STAGES - buf_stages;
-    const int room = first >= buf_stages ? STAGES - buf_stages : max(0, buf0 - first);
-    if (more) {
-      nx = next_unit(sg);
-      if (tid == 0) issued = issue_from(nx, 0, min(room, nx.n_pages * PER), i_base, false);
-    }
-    float* o_s = reinterpret_cast<float*>(ring + (size_t)buf0 * 2 * C::CODES);     // [warp][row][HD]
+
+    // ---- merge the warps through shared memory, some rows (heads) a round
 #pragma unroll
-    for (int n = 0; n < NT; ++n)
+    for (int n8 = 0; n8 < NT; ++n8)
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        float v = l[n][h];
+        float v = l[n8][h];
         v += __shfl_xor_sync(0xffffffffu, v, 4);
         v += __shfl_xor_sync(0xffffffffu, v, 8);
         v += __shfl_xor_sync(0xffffffffu, v, 16);
-        const int row = n * 8 + 2 * t + h;
-        if (g == 0) rs_s[warp][row] = rs[n][h], ra_s[warp][row] = ra[n][h], l_s[warp][row] = v;
-        if (row < n_rows) {
-          float* dst = o_s + ((size_t)warp * n_rows + row) * HD;
+        const int row = n8 * 8 + 2 * t + h;
+        if (g == 0) rs_s[warp][row] = rs[n8][h], ra_s[warp][row] = ra[n8][h], l_s[warp][row] = v;
+      }
+    bool going = true;
+    for (int row0 = 0; row0 < n_rows; row0 += C::ROUND) {
+      const int R = min(C::ROUND, n_rows - row0);
 #pragma unroll
-          for (int m = 0; m < HD / 16; ++m) {
-            const int d = HD == 64 ? g * 8 + m * 2 : (m >> 3) * 128 + d8_perm(g) * 16 + (m & 7) * 2;
-            *reinterpret_cast<float2*>(dst + d) = make_float2(o[m][n][h], o[m][n][h + 2]);
+      for (int n8 = 0; n8 < NT; ++n8)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int r = n8 * 8 + 2 * t + h - row0;
+          if (r >= 0 && r < R) {
+            float* dst = o_s + (warp * C::ROUND + r) * HD;
+#pragma unroll
+            for (int m = 0; m < HD / 16; ++m) {
+              const int d = HD == 64 ? g * 8 + m * 2 : (m >> 3) * 128 + pg * 16 + (m & 7) * 2;
+              *reinterpret_cast<float2*>(dst + d) = make_float2(o[m][n8][h], o[m][n8][h + 2]);
+            }
           }
         }
+      if (row0 == 0) {
+        going = all_of(ok);
+        if (!going) break;
+      } else {
+        all_of(true);
       }
-    __syncthreads();
-    if (tid < n_rows) {
-      float M = D8_NONE, L = 0.f;
-      for (int w = 0; w < WARPS; ++w) M = fmaxf(M, rs_s[w][tid]);
-      for (int w = 0; w < WARPS; ++w) {
-        L += l_s[w][tid] * fast_exp2(rs_s[w][tid] - M);
-        f_s[w][tid] = fast_exp2(ra_s[w][tid] - D8_SHIFT - M);
+      for (int i = tid; i < R * (HD / 4); i += WARPS * 32) {
+        const int r = i / (HD / 4), d = (i - r * (HD / 4)) * 4, row = row0 + r;
+        float M = D8_NONE;
+#pragma unroll
+        for (int w = 0; w < WARPS; ++w) M = fmaxf(M, rs_s[w][row]);
+        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+        float L = 0.f;
+#pragma unroll
+        for (int w = 0; w < WARPS; ++w) {
+          const float4 x = *reinterpret_cast<const float4*>(o_s + (w * C::ROUND + r) * HD + d);
+          const float f = fast_exp2(ra_s[w][row] - D8_SHIFT - M);
+          L += l_s[w][row] * fast_exp2(rs_s[w][row] - M);
+          v.x += x.x * f, v.y += x.y * f, v.z += x.z * f, v.w += x.w * f;
+        }
+        const size_t pidx = ((size_t)sg.b * a.nq + row_head0 + row) * a.n_splits + sg.z;
+        *reinterpret_cast<float4*>(a.part_o + pidx * HD + d) = v;
+        if (d == 0) *reinterpret_cast<float2*>(a.part_ml + pidx * 2) = make_float2(M == D8_NONE ? -INFINITY : M, L);
       }
-      ml_s[tid][0] = M == D8_NONE ? -INFINITY : M;
-      ml_s[tid][1] = L;
+      if (row0 + C::ROUND < n_rows) all_of(true);      // (the buffer is written again; a segment's first vote does it for the next segment)
     }
-    __syncthreads();
-    for (int i = tid; i < n_rows * (HD / 4); i += C::THREADS) {
-      const int row = i / (HD / 4), d = (i - row * (HD / 4)) * 4;
-      float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-      for (int w = 0; w < WARPS; ++w) {
-        const float4 x = *reinterpret_cast<const float4*>(o_s + ((size_t)w * n_rows + row) * HD + d);
-        const float f = f_s[w][row];
-        v.x += x.x * f, v.y += x.y * f, v.z += x.z * f, v.w += x.w * f;
-      }
-      const size_t pidx = ((size_t)b * a.nq + row_head0 + row) * a.n_splits + sg.z;
-      *reinterpret_cast<float4*>(a.part_o + pidx * HD + d) = v;
-      if (d == 0) *reinterpret_cast<float2*>(a.part_ml + pidx * 2) = make_float2(ml_s[row][0], ml_s[row][1]);
-    }
-    if (!more) break;
-    // (the buffer is one of the next segment's stages; what was read and written here by the generic proxy comes before the
-    // copies that follow)
-    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-    __syncthreads();
-    sg = nx;
+    if (!going || !sg.more) break;
   }
-  if (tid == 0 && give_up_s && a.err) atomicExch(a.err, 1);
 }
 
-// Tensor map of the codes as a matrix of bytes [rows, HD]: boxes of a piece's rows by up to 128 bytes, swizzled.
+// Tensor map of the codes: [HD / 128 sub-tiles][rows][128 bytes] (HD 64: one of 64 bytes), the sub-tiles of a row beside one
+// another in memory; boxes of a page's rows in all sub-tiles, swizzled.
 int d8_map(CUtensorMap* map, const void* base, long long rows, int hd) {
   AfEncodeTiledFn enc = af_encode_tiled();
   if (enc == nullptr) return af_fail(-1, "the driver has no cuTensorMapEncodeTiled");
-  cuuint64_t dims[2] = {(cuuint64_t)hd, (cuuint64_t)rows};
-  cuuint64_t strides[1] = {(cuuint64_t)hd};
-  cuuint32_t box[2] = {hd < 128 ? 64u : 128u, hd == 256 ? 32u : (cuuint32_t)AF_PAGE};
-  cuuint32_t estr[2] = {1, 1};
-  const CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+  const cuuint32_t width = hd < 128 ? 64u : 128u, subs = (cuuint32_t)hd / width;
+  cuuint64_t dims[3] = {width, (cuuint64_t)rows, subs};
+  cuuint64_t strides[2] = {(cuuint64_t)hd, width};
+  cuuint32_t box[3] = {width, (cuuint32_t)AF_PAGE, subs};
+  cuuint32_t estr[3] = {1, 1, 1};
+  const CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
                          hd < 128 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                          CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) return af_fail(-1, "cuTensorMapEncodeTiled failed (%d)", (int)r);

@@ -317,6 +317,14 @@ def test_decode_many_sequences(K):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("hd", [64, 128, 256])
+def test_decode_more_pages_than_stages(K, hd):
+    """Blocks whose segments are longer than the ring of pages in shared memory, one unit after the other, and one long unit."""
+    check_decode(K, [1500 + 37 * i for i in range(30)], 16, 8, hd, window=1400)
+    check_decode(K, [40000], 2, 1, hd)
+
+
+@pytest.mark.gpu
 def test_decode_scales(K):
     """Values whose rows differ by 2^40 in size, keys and queries of large and small size."""
     check_decode(K, [400, 90], 8, 2, 128, v_scale=20)
