@@ -711,9 +711,8 @@ AF_EXPORT int af_attn_decode_plan_kept(int* plan, long long plan_ints, const int
 }
 
 // The same for af_attn_decode8 (attention_decode8.cu).
-AF_EXPORT int af_attn_decode8_plan(int* plan, long long plan_ints, const int* page_table, int max_pages, const int* slots,
-                                   const int* lens, int batch, int nq, int nkv, int window, int keep, int ring_rows, int n_splits,
-                                   cudaStream_t stream) {
+int af_decode8_plan(int* plan, long long plan_ints, const int* page_table, int max_pages, const int* slots, const int* lens, int batch,
+                    int nq, int nkv, int window, int keep, int ring_rows, int n_splits, cudaStream_t stream) {
   return decode_plan_impl(plan, plan_ints, page_table, max_pages, slots, lens, nullptr, batch, nq, nkv, window, keep, ring_rows, n_splits,
                           D8_BREAK_PAGES, stream);
 }

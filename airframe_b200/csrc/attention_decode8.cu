@@ -23,6 +23,9 @@
 #include "cache8.cuh"
 #include "decode_split.cuh"
 
+int af_decode8_plan(int* plan, long long plan_ints, const int* page_table, int max_pages, const int* slots, const int* lens, int batch,
+                    int nq, int nkv, int window, int keep, int ring_rows, int n_splits, cudaStream_t stream);
+
 namespace {
 
 constexpr float D8_NONE = -3.0e38f;      // a reference before the first key (finite: exp2(-inf - it) is 0)
@@ -699,24 +702,44 @@ int af_decode8_split(const void* q, long long q_stride, const void* k, const voi
   return launch_decode8<256, 2>(mk, mv, a, sms, stream);
 }
 
+// What af_attn_decode8 is given, as one block of 64-bit words.
+struct AfDecode8 {
+  void* out;
+  const void *q, *k, *v, *k_exp, *v_exp, *page_table, *slots, *lens;
+  float* scratch;
+  int* plan;
+  const void* sinks;
+  int* err;
+  cudaStream_t stream;
+  long long out_stride, q_stride, n_pages, max_pages, batch, nq, nkv, hd, window, keep, ring_rows, n_splits, plan_ints;
+  double scale, cap;
+};
+
 // out [batch, nq * hd] bfloat16 = attention of one new token per sequence over its rows of the 8-bit cache (lens counts the new
 // token, which the cache holds already; sequences with slot < 0 or no token give zeros).  window > 0: the last `window`
-// positions; < 0: the position's own chunk of -window; the first `keep` stay visible beside either.
-AF_EXPORT int af_attn_decode8(void* out, long long out_stride, const void* q, long long q_stride, const void* k, const void* v,
-                              const void* k_exp, const void* v_exp, long long n_pages, const int* page_table, int max_pages,
-                              const int* slots, const int* lens, int batch, int nq, int nkv, int hd, float scale, float cap, int window,
-                              int keep, int ring_rows, int n_splits, float* scratch, const int* plan, const float* sinks, int* err,
-                              cudaStream_t stream) {
-  if (batch == 0) return 0;
-  AF_REQUIRE(out_stride % 2 == 0 && ((uintptr_t)out & 3) == 0, "af_attn_decode8: out must be 4-byte aligned");
-  const int rc = af_decode8_split(q, q_stride, k, v, k_exp, v_exp, n_pages, page_table, max_pages, slots, lens, nullptr, batch, nq, nkv, hd,
-                                  scale, cap, window, keep, ring_rows, n_splits, scratch, plan, err, stream);
+// positions; < 0: the position's own chunk of -window; the first `keep` stay visible beside either.  plan_ints > 0: the step's plan
+// is made first, into `plan`'s so many integers; 0: it holds the plan of a call for the same slots, lengths, page table, heads,
+// window, ring and n_splits.
+AF_EXPORT int af_attn_decode8(const AfDecode8* c) {
+  if (c->batch == 0) return 0;
+  AF_REQUIRE(c->out_stride % 2 == 0 && ((uintptr_t)c->out & 3) == 0, "af_attn_decode8: out must be 4-byte aligned");
+  AF_REQUIRE(c->batch > 0 && c->batch <= DA_MAX_BATCH, "af_attn_decode8: %lld sequences (takes %d)", c->batch, DA_MAX_BATCH);
+  const int batch = (int)c->batch, nq = (int)c->nq, nkv = (int)c->nkv, hd = (int)c->hd, n_splits = (int)c->n_splits;
+  const int *page_table = (const int*)c->page_table, *slots = (const int*)c->slots, *lens = (const int*)c->lens;
+  if (c->plan_ints > 0) {
+    const int rc = af_decode8_plan(c->plan, c->plan_ints, page_table, (int)c->max_pages, slots, lens, batch, nq, nkv, (int)c->window, (int)c->keep,
+                                   (int)c->ring_rows, n_splits, c->stream);
+    if (rc) return rc;
+  }
+  const int rc = af_decode8_split(c->q, c->q_stride, c->k, c->v, c->k_exp, c->v_exp, c->n_pages, page_table, (int)c->max_pages, slots, lens,
+                                  nullptr, batch, nq, nkv, hd, (float)c->scale, (float)c->cap, (int)c->window, (int)c->keep, (int)c->ring_rows,
+                                  n_splits, c->scratch, c->plan, c->err, c->stream);
   if (rc) return rc;
   const int sms = af_sm_count();
-  const float* part_ml = scratch + (size_t)batch * nq * n_splits * hd;
+  const float* part_ml = c->scratch + (size_t)batch * nq * n_splits * hd;
   const int threads = n_splits > DA_MERGE_FEW && batch * nq <= 32 ? DA_MERGE_THREADS : (hd < 128 ? hd : 128);
   const auto merge = hd == 64 ? attn_decode_merge_kernel<64> : (hd == 128 ? attn_decode_merge_kernel<128> : attn_decode_merge_kernel<256>);
-  af_launch(merge, dim3(batch, nq), dim3(threads), 0, stream, (__nv_bfloat16*)out, out_stride, (const float*)scratch, part_ml, nq, nkv,
-            n_splits, slots, lens, window, keep, sms, plan, sinks);
+  af_launch(merge, dim3(batch, nq), dim3(threads), 0, c->stream, (__nv_bfloat16*)c->out, c->out_stride, (const float*)c->scratch, part_ml, nq, nkv,
+            n_splits, slots, lens, (int)c->window, (int)c->keep, sms, (const int*)c->plan, (const float*)c->sinks);
   AF_CHECK_LAUNCH("af_attn_decode8 (merge)");
 }

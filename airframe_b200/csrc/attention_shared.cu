@@ -756,75 +756,92 @@ AF_EXPORT long long af_attn_shared_rows(int batch, int nq, int nkv) {
 }
 
 // The plans of a step: row b's first pages[b] cache pages are those of row lead[b].
-AF_EXPORT int af_attn_shared_plan(int* plan, long long plan_ints, const int* lead, const int* pages, const int* page_table, int max_pages,
-                                  const int* slots, const int* lens, int batch, int nq, int nkv, int n_splits, int bits, cudaStream_t stream) {
-  if (batch == 0) return 0;
-  AF_REQUIRE(bits == 8 || bits == 16, "af_attn_shared_plan: a cache of 8 or 16 bits, not %d", bits);
+static int shared_plans(int* plan, long long plan_ints, const int* lead, const int* pages, const int* page_table, int max_pages,
+                        const int* slots, const int* lens, int batch, int nq, int nkv, int n_splits, int bits, cudaStream_t stream) {
   const long long need = af_attn_shared_plan_ints(batch, nq, nkv);
-  AF_REQUIRE(need > 0, "af_attn_shared_plan: %d sequences (takes %d), %d heads in %d groups", batch, SH_MAX_BATCH, nq, nkv);
-  AF_REQUIRE(plan != nullptr && ((uintptr_t)plan & 15) == 0 && plan_ints >= need, "af_attn_shared_plan: a plan of %lld integers, 16-byte aligned",
-             need);
+  AF_REQUIRE(need > 0, "af_attn_decode_shared: %d sequences (takes %d), %d heads in %d groups", batch, SH_MAX_BATCH, nq, nkv);
+  AF_REQUIRE(plan_ints >= need, "af_attn_decode_shared: a plan of %lld integers", need);
   const int sms = af_sm_count(), smem = 7 * batch * (int)sizeof(int);
   static bool configured[AF_MAX_DEVICES] = {};
   const int dev = af_current_device();
   if (dev < 0) return -1;
   if (!configured[dev]) {
     const cudaError_t e = cudaFuncSetAttribute(attn_shared_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 7 * SH_MAX_BATCH * (int)sizeof(int));
-    if (e != cudaSuccess) return af_fail((int)e, "af_attn_shared_plan: %s", cudaGetErrorString(e));
+    if (e != cudaSuccess) return af_fail((int)e, "af_attn_decode_shared: %s", cudaGetErrorString(e));
     configured[dev] = true;
   }
   af_launch(attn_shared_plan_kernel, dim3(1), dim3(512), smem, stream, plan, lead, pages, slots, lens, batch, nq, nkv,
             sms);
-  AF_COUNT_LAUNCH("af_attn_shared_plan");
+  AF_COUNT_LAUNCH("af_attn_decode_shared (plan)");
   const ShPlan L = sh_layout(batch, nq, nkv, sms);
   const int at = (L.total + 3) / 4 * 4;
   return af_decode_plan_shared(plan + at, plan_ints - at, page_table, max_pages, slots, lens, plan + L.shared, batch, nq, nkv, n_splits, bits, stream);
 }
 
+// What af_attn_decode_shared is given, as one block of 64-bit words.
+struct AfShared {
+  void* out;
+  const void *q, *k, *v, *k_exp, *v_exp, *page_table, *slots, *lens, *lead, *pages;
+  float *own_scratch, *pre_scratch;
+  int* plan;
+  const void* sinks;
+  int* err;
+  cudaStream_t stream;
+  long long out_stride, q_stride, n_pages, max_pages, batch, nq, nkv, hd, n_splits, plan_ints, bits;
+  double scale, cap;
+};
+
 // out [batch, nq * hd] bfloat16 = attention of one new token per sequence over all its keys, the shared pages read once a
 // group.  bits 16: k, v are bfloat16 pages; 8: codes, with k_exp, v_exp.  own_scratch: af_attn_decode_scratch(batch, nq, hd,
-// n_splits) floats; pre_scratch: af_attn_shared_rows(...) * (hd + 2) floats; plan: af_attn_shared_plan's.
-AF_EXPORT int af_attn_decode_shared(void* out, long long out_stride, const void* q, long long q_stride, int bits, const void* k, const void* v,
-                                    const void* k_exp, const void* v_exp, long long n_pages, const int* page_table, int max_pages,
-                                    const int* slots, const int* lens, int batch, int nq, int nkv, int hd, float scale, float cap, int n_splits,
-                                    float* own_scratch, float* pre_scratch, const int* plan, const float* sinks, int* err,
-                                    cudaStream_t stream) {
-  if (batch == 0) return 0;
-  AF_REQUIRE(bits == 8 || bits == 16, "af_attn_decode_shared: a cache of 8 or 16 bits, not %d", bits);
-  AF_REQUIRE(nq > 0 && nkv > 0 && nq % nkv == 0 && batch > 0 && batch <= SH_MAX_BATCH, "af_attn_decode_shared: %d sequences, %d heads, %d groups",
-             batch, nq, nkv);
-  AF_REQUIRE(hd == 64 || hd == 128 || hd == 256, "af_attn_decode_shared: head_dim %d (takes 64, 128, 256)", hd);
-  AF_REQUIRE(q_stride % 8 == 0 && out_stride % 2 == 0 &&
-                 (((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)own_scratch | (uintptr_t)pre_scratch | (uintptr_t)plan) & 15) == 0 &&
-                 ((uintptr_t)out & 3) == 0,
+// n_splits) floats; pre_scratch: af_attn_shared_rows(...) * (hd + 2) floats.  plan_ints > 0: the step's plans are made first, into
+// `plan`'s so many integers; 0: it holds those of a call for the same lead, pages, slots, lengths, page table, heads and n_splits.
+AF_EXPORT int af_attn_decode_shared(const AfShared* c) {
+  if (c->batch == 0) return 0;
+  AF_REQUIRE(c->bits == 8 || c->bits == 16, "af_attn_decode_shared: a cache of 8 or 16 bits, not %lld", c->bits);
+  AF_REQUIRE(c->nq > 0 && c->nkv > 0 && c->nq % c->nkv == 0 && c->batch > 0 && c->batch <= SH_MAX_BATCH,
+             "af_attn_decode_shared: %lld sequences, heads %lld, groups %lld", c->batch, c->nq, c->nkv);
+  AF_REQUIRE(c->hd == 64 || c->hd == 128 || c->hd == 256, "af_attn_decode_shared: head_dim %lld (takes 64, 128, 256)", c->hd);
+  AF_REQUIRE(c->q_stride % 8 == 0 && c->out_stride % 2 == 0 &&
+                 (((uintptr_t)c->q | (uintptr_t)c->k | (uintptr_t)c->v | (uintptr_t)c->own_scratch | (uintptr_t)c->pre_scratch | (uintptr_t)c->plan) &
+                  15) == 0 &&
+                 ((uintptr_t)c->out & 3) == 0,
              "af_attn_decode_shared: rows must be 16-byte aligned (out: 4)");
-  AF_REQUIRE(own_scratch != nullptr && pre_scratch != nullptr && plan != nullptr, "af_attn_decode_shared: scratch and plan");
-  AF_REQUIRE(n_pages > 0 && n_pages * nkv * AF_PAGE < (1ll << 31), "af_attn_decode_shared: %lld cache pages", n_pages);
+  AF_REQUIRE(c->own_scratch != nullptr && c->pre_scratch != nullptr && c->plan != nullptr, "af_attn_decode_shared: scratch and plan");
+  AF_REQUIRE(c->n_pages > 0 && c->n_pages * c->nkv * AF_PAGE < (1ll << 31), "af_attn_decode_shared: %lld cache pages", c->n_pages);
   const int sms = af_sm_count();
   if (sms <= 0) return -1;
+  const int batch = (int)c->batch, nq = (int)c->nq, nkv = (int)c->nkv, hd = (int)c->hd, n_splits = (int)c->n_splits, max_pages = (int)c->max_pages;
+  const int *page_table = (const int*)c->page_table, *slots = (const int*)c->slots, *lens = (const int*)c->lens;
+  int rc;
+  if (c->plan_ints > 0) {
+    rc = shared_plans(c->plan, c->plan_ints, (const int*)c->lead, (const int*)c->pages, page_table, max_pages, slots, lens, batch, nq, nkv, n_splits,
+                      (int)c->bits, c->stream);
+    if (rc) return rc;
+  }
   const ShPlan L = sh_layout(batch, nq, nkv, sms);
   const int at = (L.total + 3) / 4 * 4;
   const long long rows = af_attn_shared_rows(batch, nq, nkv);
-  ShArgs a{(const __nv_bfloat16*)q, q_stride, (const uint8_t*)k, (const uint8_t*)v, (const uint8_t*)k_exp, (const uint8_t*)v_exp, n_pages,
-           page_table, plan, max_pages, batch, nq, nkv, scale, cap, pre_scratch, pre_scratch + rows * hd, err};
-  int rc;
-  if (bits == 16)
-    rc = hd == 64 ? launch_shared<64, 16>(a, k, v, sms, stream)
-                  : (hd == 128 ? launch_shared<128, 16>(a, k, v, sms, stream) : launch_shared<256, 16>(a, k, v, sms, stream));
+  ShArgs a{(const __nv_bfloat16*)c->q, c->q_stride, (const uint8_t*)c->k, (const uint8_t*)c->v, (const uint8_t*)c->k_exp, (const uint8_t*)c->v_exp,
+           c->n_pages, page_table, c->plan, max_pages, batch, nq, nkv, (float)c->scale, (float)c->cap, c->pre_scratch, c->pre_scratch + rows * hd,
+           c->err};
+  const bool eight = c->bits == 8;
+  if (hd == 64)
+    rc = eight ? launch_shared<64, 8>(a, c->k, c->v, sms, c->stream) : launch_shared<64, 16>(a, c->k, c->v, sms, c->stream);
+  else if (hd == 128)
+    rc = eight ? launch_shared<128, 8>(a, c->k, c->v, sms, c->stream) : launch_shared<128, 16>(a, c->k, c->v, sms, c->stream);
   else
-    rc = hd == 64 ? launch_shared<64, 8>(a, k, v, sms, stream)
-                  : (hd == 128 ? launch_shared<128, 8>(a, k, v, sms, stream) : launch_shared<256, 8>(a, k, v, sms, stream));
+    rc = eight ? launch_shared<256, 8>(a, c->k, c->v, sms, c->stream) : launch_shared<256, 16>(a, c->k, c->v, sms, c->stream);
   if (rc) return rc;
-  if (bits == 16)
-    rc = af_decode16_split(q, q_stride, k, v, n_pages, page_table, max_pages, slots, lens, plan + L.shared, batch, nq, nkv, hd, scale, cap,
-                           n_splits, own_scratch, plan + at, err, stream);
+  if (eight)
+    rc = af_decode8_split(c->q, c->q_stride, c->k, c->v, c->k_exp, c->v_exp, c->n_pages, page_table, max_pages, slots, lens, c->plan + L.shared,
+                          batch, nq, nkv, hd, a.scale, a.cap, 0, 0, 0, n_splits, c->own_scratch, c->plan + at, c->err, c->stream);
   else
-    rc = af_decode8_split(q, q_stride, k, v, k_exp, v_exp, n_pages, page_table, max_pages, slots, lens, plan + L.shared, batch, nq, nkv, hd,
-                          scale, cap, 0, 0, 0, n_splits, own_scratch, plan + at, err, stream);
+    rc = af_decode16_split(c->q, c->q_stride, c->k, c->v, c->n_pages, page_table, max_pages, slots, lens, c->plan + L.shared, batch, nq, nkv, hd,
+                           a.scale, a.cap, n_splits, c->own_scratch, c->plan + at, c->err, c->stream);
   if (rc) return rc;
   const auto merge = hd == 64 ? attn_shared_merge_kernel<64> : (hd == 128 ? attn_shared_merge_kernel<128> : attn_shared_merge_kernel<256>);
-  af_launch(merge, dim3(batch, nq), dim3(SHM_THREADS), 0, stream, (__nv_bfloat16*)out, out_stride, (const float*)a.part_o, (const float*)a.part_ml,
-            (const float*)own_scratch, (const float*)own_scratch + (size_t)batch * nq * n_splits * hd, nq, nkv, n_splits, plan, plan + at, sms,
-            sinks);
+  af_launch(merge, dim3(batch, nq), dim3(SHM_THREADS), 0, c->stream, (__nv_bfloat16*)c->out, c->out_stride, (const float*)a.part_o,
+            (const float*)a.part_ml, (const float*)c->own_scratch, (const float*)c->own_scratch + (size_t)batch * nq * n_splits * hd, nq, nkv,
+            n_splits, (const int*)c->plan, (const int*)c->plan + at, sms, (const float*)c->sinks);
   AF_CHECK_LAUNCH("af_attn_decode_shared (merge)");
 }

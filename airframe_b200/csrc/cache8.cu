@@ -98,22 +98,29 @@ int launch_store8(const Store8Args& a, cudaStream_t stream) {
 // 1 when the 8-bit cache takes this head size.
 AF_EXPORT int af_cache8_supported(int hd) { return hd == 64 || hd == 128 || hd == 256 ? 1 : 0; }
 
+// What af_store_kv8 is given, as one block of 64-bit words.
+struct AfStore8 {
+  const void *qkv, *rounded, *positions, *seq_of_token, *slots, *len_after, *page_table, *k, *v, *k_exp, *v_exp;
+  cudaStream_t stream;
+  long long ld, rounded_ld, n_pages, max_pages, ring_rows, keep, T, nq, nkv, hd;
+};
+
 // The k and v heads of the packed bfloat16 rows [q | k | v] (T of them, ld elements apart) into the 8-bit pages of their
 // sequences; `rounded` (null, or rows [k | v], rounded_ld elements apart): the values as they are kept.
-AF_EXPORT int af_store_kv8(const void* qkv, long long ld, void* rounded, long long rounded_ld, const int* positions,
-                           const int* seq_of_token, const int* slots, const int* len_after, const int* page_table,
-                           int max_pages, int ring_rows, int keep, int T, int nq, int nkv, int hd, void* k, void* v, void* k_exp,
-                           void* v_exp, long long n_pages, cudaStream_t stream) {
-  if (T == 0) return 0;
-  AF_REQUIRE(T > 0 && nq > 0 && nkv > 0, "af_store_kv8: %d tokens, %d heads, %d kv heads", T, nq, nkv);
-  AF_REQUIRE(af_cache8_supported(hd), "af_store_kv8: head_dim %d (takes 64, 128, 256)", hd);
-  AF_REQUIRE(ring_rows >= 0 && ring_rows % AF_PAGE == 0 && keep >= 0 && max_pages > 0 && n_pages > 0,
-             "af_store_kv8: ring rows %d, %d kept, %d page entries", ring_rows, keep, max_pages);
-  AF_REQUIRE(ld % 8 == 0 && rounded_ld % 8 == 0 && (((uintptr_t)qkv | (uintptr_t)rounded | (uintptr_t)k | (uintptr_t)v) & 15) == 0,
+AF_EXPORT int af_store_kv8(const AfStore8* c) {
+  if (c->T == 0) return 0;
+  AF_REQUIRE(c->T > 0 && c->T < (1ll << 31) && c->nq > 0 && c->nkv > 0, "af_store_kv8: %lld tokens, %lld heads, %lld kv heads", c->T, c->nq, c->nkv);
+  AF_REQUIRE(af_cache8_supported((int)c->hd), "af_store_kv8: head_dim %lld (takes 64, 128, 256)", c->hd);
+  AF_REQUIRE(c->ring_rows >= 0 && c->ring_rows % AF_PAGE == 0 && c->keep >= 0 && c->max_pages > 0 && c->n_pages > 0,
+             "af_store_kv8: ring rows %lld, %lld kept, %lld page entries", c->ring_rows, c->keep, c->max_pages);
+  AF_REQUIRE(c->ld % 8 == 0 && c->rounded_ld % 8 == 0 &&
+                 (((uintptr_t)c->qkv | (uintptr_t)c->rounded | (uintptr_t)c->k | (uintptr_t)c->v) & 15) == 0,
              "af_store_kv8: rows must be 16-byte aligned");
-  Store8Args a{(const __nv_bfloat16*)qkv, ld, (__nv_bfloat16*)rounded, rounded_ld, positions, seq_of_token, slots, len_after, page_table,
-               max_pages, T, nq, nkv, ring_rows, keep, n_pages, (uint8_t*)k, (uint8_t*)v, (uint8_t*)k_exp, (uint8_t*)v_exp};
-  if (hd == 64) return launch_store8<64>(a, stream);
-  if (hd == 128) return launch_store8<128>(a, stream);
-  return launch_store8<256>(a, stream);
+  Store8Args a{(const __nv_bfloat16*)c->qkv, c->ld, (__nv_bfloat16*)c->rounded, c->rounded_ld, (const int*)c->positions,
+               (const int*)c->seq_of_token, (const int*)c->slots, (const int*)c->len_after, (const int*)c->page_table, (int)c->max_pages,
+               (int)c->T, (int)c->nq, (int)c->nkv, (int)c->ring_rows, (int)c->keep, c->n_pages, (uint8_t*)c->k, (uint8_t*)c->v,
+               (uint8_t*)c->k_exp, (uint8_t*)c->v_exp};
+  if (c->hd == 64) return launch_store8<64>(a, c->stream);
+  if (c->hd == 128) return launch_store8<128>(a, c->stream);
+  return launch_store8<256>(a, c->stream);
 }

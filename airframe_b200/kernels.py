@@ -8,6 +8,7 @@ sizes.  Nothing here computes on the host and nothing falls back to torch.
 from __future__ import annotations
 
 import ctypes
+import struct
 from ctypes import c_float, c_int, c_longlong, c_void_p
 
 import torch
@@ -334,18 +335,41 @@ def store_kv(qkv, batch, nq: int, nkv: int, hd: int, kv, parts=None) -> None:
 
 CACHE8_HEAD_SIZES = (64, 128, 256)     # head sizes that the 8-bit cache takes
 
+# What the entry points below take as one block of 64-bit words (pointers, whole numbers, then 64-bit floats): a ctypes argument
+# costs the host some 0.3 us, a packed one 0.05.
+_STORE8 = struct.Struct("<12Q10q")
+_DECODE8 = struct.Struct("<14Q13q2d")
+_SHARED = struct.Struct("<17Q11q2d")
+
+
+def _here(who: str, *tensors) -> int:
+    """The current device, on which all tensors have to live: kernels go to its current stream."""
+    dev = tensors[0].get_device()
+    for t in tensors:
+        if t.get_device() != dev or dev < 0:
+            raise KernelError(f"{who}: tensors must live on the current CUDA device (there is no CPU implementation)")
+    if dev != _current_device():
+        raise KernelError(f"{who}: tensors must live on the current CUDA device, which is {_current_device()}, not {dev}")
+    return dev
+
+
+def _typed(who: str, dtype, **tensors) -> None:
+    for name, t in tensors.items():
+        if t.dtype != dtype or not t.is_contiguous():
+            raise KernelError(f"{who}: {name} must be contiguous {dtype}, got {t.dtype} of strides {t.stride()}")
+
 
 def _cache8_pages(kv, nkv: int, hd: int, who: str):
     """Checks a layer's view of its 8-bit pages (see ``csrc/cache8.cuh``); returns how many pages there are."""
-    if kv.k is None or kv.v is None or kv.k.dtype != torch.float8_e4m3fn or kv.v.dtype != torch.float8_e4m3fn \
-            or kv.k_exp.dtype != torch.uint8 or kv.v_exp is None or kv.v_exp.dtype != torch.uint8:
+    k, v, ke, ve = kv.k, kv.v, kv.k_exp, kv.v_exp
+    if k is None or v is None or ve is None or k.dtype != torch.float8_e4m3fn or v.dtype != torch.float8_e4m3fn \
+            or ke.dtype != torch.uint8 or ve.dtype != torch.uint8:
         raise KernelError(f"{who}: an 8-bit cache keeps float8_e4m3fn codes and uint8 exponents of keys and values")
-    n = kv.k.shape[0]
-    if tuple(kv.k.shape) != (n, nkv, PAGE, hd) or kv.v.shape != kv.k.shape or tuple(kv.k_exp.shape) != (n, nkv, PAGE) \
-            or kv.v_exp.shape != kv.k_exp.shape:
+    n = k.shape[0]
+    if k.shape != (n, nkv, PAGE, hd) or v.shape != k.shape or ke.shape != (n, nkv, PAGE) or ve.shape != ke.shape:
         raise KernelError(f"{who}: 8-bit pages must be [pages, {nkv}, {PAGE}, {hd}], their exponents [pages, {nkv}, {PAGE}]")
-    if not all(t.is_contiguous() for t in (kv.k, kv.v, kv.k_exp, kv.v_exp, kv.page_table)):
-        raise KernelError(f"{who}: cache pages and page table must be contiguous")
+    if not (k.is_contiguous() and v.is_contiguous() and ke.is_contiguous() and ve.is_contiguous()):
+        raise KernelError(f"{who}: cache pages must be contiguous")
     return n
 
 
@@ -355,20 +379,20 @@ def store_kv8(qkv, batch, nq: int, nkv: int, hd: int, kv, rounded=None) -> None:
     and NaN become NaN).  ``rounded`` (bfloat16 [T, 2 nkv hd]) gets the values as they are kept, [k | v], of every token of the step:
     what a prompt's own attention takes, so that its tokens see the keys that later single tokens see."""
     T = qkv.shape[0]
-    if qkv.dtype != torch.bfloat16 or qkv.shape[1] != (nq + 2 * nkv) * hd:
+    if qkv.dtype != torch.bfloat16 or qkv.shape != (T, (nq + 2 * nkv) * hd):
         raise KernelError(f"store_kv8: bfloat16 rows of (nq + 2 nkv) * head_dim = {(nq + 2 * nkv) * hd}, got {qkv.dtype} {tuple(qkv.shape)}")
-    if rounded is not None and (rounded.dtype != torch.bfloat16 or tuple(rounded.shape) != (T, 2 * nkv * hd)):
+    if rounded is not None and (rounded.dtype != torch.bfloat16 or rounded.shape != (T, 2 * nkv * hd)):
         raise KernelError(f"store_kv8: rounded must be bfloat16 [{T}, {2 * nkv * hd}]")
-    if batch.positions.numel() != T or batch.seq_of_token.numel() != T:
-        raise KernelError(f"store_kv8: {T} rows, {batch.positions.numel()} positions")
+    positions, seq, slots, lens, table = batch.positions, batch.seq_of_token, batch.slots, batch.len_after, kv.page_table
+    if positions.numel() != T or seq.numel() != T or slots.numel() != lens.numel():
+        raise KernelError(f"store_kv8: {T} rows, {positions.numel()} positions, {seq.numel()} places of sequences")
     n_pages = _cache8_pages(kv, nkv, hd, "store_kv8")
-    _check(_lib().af_store_kv8(
-        _ptr(qkv), c_longlong(_rows(qkv, "qkv")), _ptr(rounded, allow_none=True),
-        c_longlong(_rows(rounded, "rounded") if rounded is not None else 0), _ptr(batch.positions, "positions", torch.int32),
-        _ptr(batch.seq_of_token, "seq_of_token", torch.int32), _ptr(batch.slots, "slots", torch.int32),
-        _ptr(batch.len_after, "len_after", torch.int32), _ptr(kv.page_table, "page_table", torch.int32),
-        c_int(kv.page_table.shape[1]), c_int(kv.ring_rows), c_int(kv_keep(kv)), c_int(T), c_int(nq), c_int(nkv), c_int(hd),
-        _ptr(kv.k), _ptr(kv.v), _ptr(kv.k_exp), _ptr(kv.v_exp), c_longlong(n_pages), _stream()))
+    _typed("store_kv8", torch.int32, positions=positions, seq_of_token=seq, slots=slots, len_after=lens, page_table=table)
+    dev = _here("store_kv8", qkv, positions, seq, slots, lens, table, kv.k, kv.v, kv.k_exp, kv.v_exp, *(() if rounded is None else (rounded,)))
+    _check(_lib().af_store_kv8(_STORE8.pack(
+        qkv.data_ptr(), 0 if rounded is None else rounded.data_ptr(), positions.data_ptr(), seq.data_ptr(), slots.data_ptr(), lens.data_ptr(),
+        table.data_ptr(), kv.k.data_ptr(), kv.v.data_ptr(), kv.k_exp.data_ptr(), kv.v_exp.data_ptr(), _raw_stream(dev),
+        _rows(qkv, "qkv"), 0 if rounded is None else _rows(rounded, "rounded"), n_pages, table.shape[1], kv.ring_rows, kv_keep(kv), T, nq, nkv, hd)))
 
 
 def sum_parts(qkv, parts, batch, nq: int, nkv: int, hd: int) -> None:
@@ -529,6 +553,17 @@ def error_word(device) -> torch.Tensor:
     if key not in _ERR:
         _ERR[key] = torch.zeros(1, dtype=torch.int32, device=device)
     return _ERR[key]
+
+
+_ERR_POINTERS = {}
+
+
+def _error_pointer(dev: int) -> int:
+    """The address of :func:`error_word` of a device ordinal."""
+    p = _ERR_POINTERS.get(dev)
+    if p is None:
+        p = _ERR_POINTERS[dev] = error_word(torch.device("cuda", dev)).data_ptr()
+    return p
 
 
 def check_device_errors(device) -> None:
@@ -881,11 +916,11 @@ def attn_decode_max_splits(batch: int, nkv: int, max_len: int, window: int, bloc
 
 
 def attn_decode_plan(page_table, slots, lens, nq: int, nkv: int, window: int, ring_rows: int, n_splits: int,
-                     keep: int = 0, bits: int = 16):
+                     keep: int = 0):
     """The plan of a decode step for :func:`attn_decode_split`: how the work is
     cut among the blocks, worked out by one small kernel for all layers that
     read the same caches the same way (these slots, lengths, page table, heads,
-    window, ring and ``n_splits``).  It holds for these lengths alone.  ``bits`` 8: for :func:`attn_decode8`."""
+    window, ring and ``n_splits``).  It holds for these lengths alone."""
     lib = _lib()
     lib.af_attn_decode_plan_ints.restype = ctypes.c_longlong
     B = slots.shape[0]
@@ -893,21 +928,21 @@ def attn_decode_plan(page_table, slots, lens, nq: int, nkv: int, window: int, ri
     if n <= 0:
         raise KernelError(f"attn_decode_plan: {B} sequences, {nq} heads in {nkv} groups")
     plan = torch.empty(n, dtype=torch.int32, device=slots.device)
-    _check((lib.af_attn_decode8_plan if bits == 8 else lib.af_attn_decode_plan_kept)(
+    _check(lib.af_attn_decode_plan_kept(
         _ptr(plan, "plan", torch.int32), c_longlong(n), _ptr(page_table, "page_table", torch.int32),
         c_int(page_table.shape[1]), _ptr(slots, "slots", torch.int32), _ptr(lens, "lens", torch.int32), c_int(B),
         c_int(nq), c_int(nkv), c_int(window), c_int(keep), c_int(ring_rows), c_int(n_splits), _stream()))
     return plan
 
 
-def _step_plan(kv, batch, nq: int, nkv: int, window: int, keep: int, n_splits: int, bits: int = 16):
+def _step_plan(kv, batch, nq: int, nkv: int, window: int, keep: int, n_splits: int):
     """The plan of the step (see :func:`attn_decode_plan`), made once in a pass for all layers that read this group of caches
     alike (a batch without a place for the step's tables gets a plan for the call)."""
     aux = getattr(batch, "aux", None)
-    key = ("attn_decode_plan", kv.page_table.data_ptr(), kv.ring_rows, nq, nkv, window, keep, n_splits, bits)
+    key = ("attn_decode_plan", kv.page_table.data_ptr(), kv.ring_rows, nq, nkv, window, keep, n_splits)
     plan = aux.get(key) if aux is not None else None
     if plan is None:
-        plan = attn_decode_plan(kv.page_table, batch.slots, batch.len_after, nq, nkv, window, kv.ring_rows, n_splits, keep, bits)
+        plan = attn_decode_plan(kv.page_table, batch.slots, batch.len_after, nq, nkv, window, kv.ring_rows, n_splits, keep)
         if aux is not None:
             aux[key] = plan
     return plan
@@ -1028,30 +1063,64 @@ def attn_decode(out, q, kv, batch, nq, nkv, hd, scale, cap, window, slopes=None,
                       n_splits=plain_decode_splits(batch.n_seqs, nq, most), keep=keep)
 
 
+_PLAN_INTS = {}
+
+
+def _plan_ints(entry: str, B: int, nq: int, nkv: int) -> int:
+    """What ``entry`` of the library answers for these sizes (asked once a device and size)."""
+    key = (entry, _current_device(), B, nq, nkv)
+    n = _PLAN_INTS.get(key)
+    if n is None:
+        f = getattr(_lib(), entry)
+        f.restype = ctypes.c_longlong
+        n = int(f(c_int(B), c_int(nq), c_int(nkv)))
+        if n <= 0:
+            raise KernelError(f"{entry}: {B} sequences (takes {ATTN_DECODE_MAX_SEQS}), heads {nq}, groups {nkv}")
+        _PLAN_INTS[key] = n
+    return n
+
+
+def _decode_rows(who: str, out, q, batch, nq: int, hd: int, sinks) -> int:
+    """Checks the rows of a decode step; returns how many sequences there are."""
+    B = batch.n_seqs
+    if q.dtype != torch.bfloat16 or out.dtype != torch.bfloat16 or out.shape != (B, nq * hd) or q.dim() != 2 or q.shape[0] != B \
+            or q.shape[1] < nq * hd:
+        raise KernelError(f"{who}: bfloat16 queries and out [{B}, {nq * hd}]")
+    if B > ATTN_DECODE_MAX_SEQS or batch.slots.numel() != B or batch.len_after.numel() != B:
+        raise KernelError(f"{who}: {B} sequences (takes {ATTN_DECODE_MAX_SEQS}), {batch.slots.numel()} slots, {batch.len_after.numel()} lengths")
+    if sinks is not None and (sinks.numel() != nq or sinks.dtype != torch.float32 or not sinks.is_contiguous()):
+        raise KernelError(f"{who}: {sinks.numel()} sinks for {nq} heads, in float32")
+    return B
+
+
 def attn_decode8(out, q, kv, batch, nq: int, nkv: int, hd: int, scale: float, cap: float, window: int, sinks=None,
                  keep: int = 0) -> None:
     """Decode attention over a cache of 8 bits (``window`` < 0: a chunk of that many positions; ``keep``: beside a window,
     the first tokens that stay visible)."""
-    B = batch.n_seqs
+    B = _decode_rows("attn_decode8", out, q, batch, nq, hd, sinks)
     n_pages = _cache8_pages(kv, nkv, hd, "attn_decode8")
-    if q.dtype != torch.bfloat16 or out.dtype != torch.bfloat16 or tuple(out.shape) != (B, nq * hd) or q.shape[0] != B or q.shape[1] < nq * hd:
-        raise KernelError(f"attn_decode8: bfloat16 queries and out [{B}, {nq * hd}]")
-    if sinks is not None and sinks.numel() != nq:
-        raise KernelError(f"attn_decode8: {sinks.numel()} sinks for {nq} heads")
-    if B > ATTN_DECODE_MAX_SEQS:
-        raise KernelError(f"attn_decode8: {B} sequences (takes {ATTN_DECODE_MAX_SEQS})")
+    table, slots, lens = kv.page_table, batch.slots, batch.len_after
+    _typed("attn_decode8", torch.int32, page_table=table, slots=slots, len_after=lens)
+    dev = _here("attn_decode8", out, q, table, slots, lens, kv.k, kv.v, kv.k_exp, kv.v_exp, *(() if sinks is None else (sinks,)))
+    if B == 0:
+        return
     n = attn_decode_max_splits(B, nkv, batch.max_len_after, window, nq=nq, keep=keep)
-    plan = _step_plan(kv, batch, nq, nkv, window, keep, n, 8)
-    lib = _lib()
-    lib.af_attn_decode_scratch.restype = ctypes.c_longlong
-    scratch = torch.empty(lib.af_attn_decode_scratch(c_int(B), c_int(nq), c_int(hd), c_int(n)), dtype=torch.float32, device=q.device)
-    _check(lib.af_attn_decode8(
-        _ptr(out), c_longlong(_rows(out, "out")), _ptr(q), c_longlong(_rows(q, "q")), _ptr(kv.k), _ptr(kv.v), _ptr(kv.k_exp),
-        _ptr(kv.v_exp), c_longlong(n_pages), _ptr(kv.page_table, "page_table", torch.int32), c_int(kv.page_table.shape[1]),
-        _ptr(batch.slots, "slots", torch.int32), _ptr(batch.len_after, "lens", torch.int32), c_int(B), c_int(nq), c_int(nkv),
-        c_int(hd), c_float(scale), c_float(cap), c_int(window), c_int(keep), c_int(kv.ring_rows), c_int(n),
-        _ptr(scratch, "scratch", torch.float32), _ptr(plan, "plan", torch.int32), _ptr(sinks, "sinks", torch.float32, allow_none=True),
-        _ptr(error_word(q.device), "err", torch.int32), _stream()))
+    # the plan of the step, made in front of its first layer's attention and shared by the layers that read alike
+    aux = getattr(batch, "aux", None)
+    key = ("attn_decode8_plan", table.data_ptr(), kv.ring_rows, nq, nkv, window, keep, n)
+    plan = aux.get(key) if aux is not None else None
+    ints = 0
+    if plan is None:
+        ints = _plan_ints("af_attn_decode_plan_ints", B, nq, nkv)
+        plan = torch.empty(ints, dtype=torch.int32, device=q.device)
+        if aux is not None:
+            aux[key] = plan
+    scratch = torch.empty(B * nq * n * (hd + 2), dtype=torch.float32, device=q.device)
+    _check(_lib().af_attn_decode8(_DECODE8.pack(
+        out.data_ptr(), q.data_ptr(), kv.k.data_ptr(), kv.v.data_ptr(), kv.k_exp.data_ptr(), kv.v_exp.data_ptr(), table.data_ptr(),
+        slots.data_ptr(), lens.data_ptr(), scratch.data_ptr(), plan.data_ptr(), 0 if sinks is None else sinks.data_ptr(),
+        _error_pointer(dev), _raw_stream(dev), _rows(out, "out"), _rows(q, "q"), n_pages, table.shape[1], B, nq, nkv, hd, window, keep,
+        kv.ring_rows, n, ints, scale, cap)))
 
 
 # From how many cache pages on that a decode step need not read again (a group's shared pages times its sequences but one) the
@@ -1072,46 +1141,39 @@ def attn_decode_shared(out, q, kv, batch, nq: int, nkv: int, hd: int, scale: flo
     if lead.numel() != B or pages.numel() != B or most_pages < 0:
         raise KernelError(f"attn_decode_shared: a lead and a number of pages for each of {B} rows")
     eight = getattr(kv, "k_exp", None) is not None
-    if kv.ring_rows or kv.v is None or tuple(kv.v.shape) != tuple(kv.k.shape) or tuple(kv.k.shape[1:]) != (nkv, PAGE, hd):
+    if kv.ring_rows or kv.v is None or kv.v.shape != kv.k.shape or kv.k.shape[1:] != (nkv, PAGE, hd):
         raise KernelError(f"attn_decode_shared: pages [pages, {nkv}, {PAGE}, {hd}] of all keys and values (no ring)")
     if (most_pages == 0 or not attn_decode_shared_supported(q.dtype, hd, B) or not (eight or kv.k.dtype == torch.bfloat16)
             or q.stride(0) % 8 or q.data_ptr() % 16):
         attn_decode(out, q, kv, batch, nq, nkv, hd, scale, cap, 0, sinks=sinks, gate=gate)
         return
-    if out.dtype != torch.bfloat16 or tuple(out.shape) != (B, nq * hd) or q.shape[0] != B or q.shape[1] < nq * hd:
-        raise KernelError(f"attn_decode_shared: bfloat16 queries and out [{B}, {nq * hd}]")
-    if sinks is not None and sinks.numel() != nq:
-        raise KernelError(f"attn_decode_shared: {sinks.numel()} sinks for {nq} heads")
+    _decode_rows("attn_decode_shared", out, q, batch, nq, hd, sinks)
     n_pages = _cache8_pages(kv, nkv, hd, "attn_decode_shared") if eight else kv.k.shape[0]
-    lib = _lib()
-    for f in (lib.af_attn_shared_plan_ints, lib.af_attn_shared_rows, lib.af_attn_decode_scratch):
-        f.restype = ctypes.c_longlong
-    table = kv.page_table
+    table, slots, lens = kv.page_table, batch.slots, batch.len_after
+    _typed("attn_decode_shared", torch.int32, page_table=table, slots=slots, len_after=lens, lead=lead, pages=pages)
+    if not eight:
+        _typed("attn_decode_shared", torch.bfloat16, k=kv.k, v=kv.v)
+    dev = _here("attn_decode_shared", out, q, table, slots, lens, lead, pages, kv.k, kv.v, *((kv.k_exp, kv.v_exp) if eight else ()),
+                *(() if sinks is None else (sinks,)))
+    if B == 0:
+        return
     n = attn_decode_max_splits(B, nkv, batch.max_len_after, 0, nq=nq)
     aux = getattr(batch, "aux", None)
     key = ("attn_shared_plan", table.data_ptr(), nq, nkv, n, eight, lead.data_ptr(), pages.data_ptr())
     plan = aux.get(key) if aux is not None else None
+    ints = 0
     if plan is None:
-        ints = lib.af_attn_shared_plan_ints(c_int(B), c_int(nq), c_int(nkv))
-        plan = torch.empty(max(ints, 0), dtype=torch.int32, device=q.device)
-        _check(lib.af_attn_shared_plan(
-            _ptr(plan, "plan", torch.int32), c_longlong(ints), _ptr(lead, "lead", torch.int32), _ptr(pages, "pages", torch.int32),
-            _ptr(table, "page_table", torch.int32), c_int(table.shape[1]), _ptr(batch.slots, "slots", torch.int32),
-            _ptr(batch.len_after, "lens", torch.int32), c_int(B), c_int(nq), c_int(nkv), c_int(n), c_int(8 if eight else 16),
-            _stream()))
+        ints = _plan_ints("af_attn_shared_plan_ints", B, nq, nkv)
+        plan = torch.empty(ints, dtype=torch.int32, device=q.device)
         if aux is not None:
             aux[key] = plan
-    n_own = lib.af_attn_decode_scratch(c_int(B), c_int(nq), c_int(hd), c_int(n))
-    n_pre = lib.af_attn_shared_rows(c_int(B), c_int(nq), c_int(nkv)) * (hd + 2)
-    n_own = (n_own + 3) // 4 * 4
-    scratch = torch.empty(n_own + n_pre, dtype=torch.float32, device=q.device)
-    _check(lib.af_attn_decode_shared(
-        _ptr(out), c_longlong(_rows(out, "out")), _ptr(q), c_longlong(_rows(q, "q")), c_int(8 if eight else 16), _ptr(kv.k), _ptr(kv.v),
-        _ptr(kv.k_exp if eight else None, allow_none=True), _ptr(kv.v_exp if eight else None, allow_none=True), c_longlong(n_pages),
-        _ptr(table, "page_table", torch.int32), c_int(table.shape[1]), _ptr(batch.slots, "slots", torch.int32),
-        _ptr(batch.len_after, "lens", torch.int32), c_int(B), c_int(nq), c_int(nkv), c_int(hd), c_float(scale), c_float(cap), c_int(n),
-        _ptr(scratch, "scratch", torch.float32), _ptr(scratch[n_own:]), _ptr(plan, "plan", torch.int32),
-        _ptr(sinks, "sinks", torch.float32, allow_none=True), _ptr(error_word(q.device), "err", torch.int32), _stream()))
+    n_own = (B * nq * n * (hd + 2) + 3) // 4 * 4
+    scratch = torch.empty(n_own + _plan_ints("af_attn_shared_rows", B, nq, nkv) * (hd + 2), dtype=torch.float32, device=q.device)
+    _check(_lib().af_attn_decode_shared(_SHARED.pack(
+        out.data_ptr(), q.data_ptr(), kv.k.data_ptr(), kv.v.data_ptr(), kv.k_exp.data_ptr() if eight else 0, kv.v_exp.data_ptr() if eight else 0,
+        table.data_ptr(), slots.data_ptr(), lens.data_ptr(), lead.data_ptr(), pages.data_ptr(), scratch.data_ptr(),
+        scratch.data_ptr() + 4 * n_own, plan.data_ptr(), 0 if sinks is None else sinks.data_ptr(), _error_pointer(dev), _raw_stream(dev),
+        _rows(out, "out"), _rows(q, "q"), n_pages, table.shape[1], B, nq, nkv, hd, n, ints, 8 if eight else 16, scale, cap)))
     if gate is not None:
         head_gate(out, gate, nq, hd)
 
