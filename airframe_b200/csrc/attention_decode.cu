@@ -107,62 +107,15 @@ __device__ __forceinline__ uint32_t da_piece(uint32_t tile, int r, int c) {
 }
 
 
-// One block.  It does not release its dependents early: the kernel behind it starts when the plan is complete, and
-// so does every kernel after that one, so all of them may read the plan before they wait for anything.
+// One block (see da_write_plan).  It does not release its dependents early: the kernel behind it starts when the plan is complete,
+// and so does every kernel after that one, so all of them may read the plan before they wait for anything.
 __global__ void __launch_bounds__(256)
 attn_decode_plan_kernel(int* __restrict__ plan, const int* __restrict__ slots, const int* __restrict__ lens,
                         const int* __restrict__ page_table, int max_pages, int batch, int nq, int nkv, int window,
-                        int keep, int ring_rows, int room, int grid_blocks, const int* __restrict__ shared, int brk) {
+                        int keep, int ring_rows, int room, int grid_blocks, int brk) {
   extern __shared__ int dp_smem[];
-  int* pages_s = dp_smem;                 // [batch + 1]
-  int* splits_s = dp_smem + batch + 1;    // [batch + 1]
-  __shared__ DaPlan plan_s;
   pdl_wait();
-  const int group = nq / nkv, tiles = (group + 15) / 16, units_per_seq = nkv * tiles;
-  if (threadIdx.x < 32) {
-    const DaPlan pl = da_plan(slots, lens, batch, window, keep, shared, brk, units_per_seq, grid_blocks, room, 0, pages_s, splits_s);
-    if (threadIdx.x == 0) plan_s = pl;
-  }
-  __syncthreads();
-  const DaPlan pl = plan_s;
-  if (threadIdx.x == 0) {
-    plan[0] = room;
-    plan[1] = da_plan_mark(grid_blocks, brk);
-    plan[2] = batch;
-    plan[3] = units_per_seq;
-    plan[4] = pl.even;
-    plan[5] = pl.share;
-    plan[6] = pl.n_blocks;
-    plan[7] = 0;
-  }
-  for (int u = threadIdx.x; u < batch * units_per_seq; u += blockDim.x) {
-    const int b = u / units_per_seq, y = u - b * units_per_seq;
-    const int width = pages_s[b + 1] - pages_s[b];      // (the run cut: with a break)
-    plan[DA_PLAN_HEAD + u] = pl.even ? da_even_splits(width, pl.share, room, pl.even)
-                                     : da_run_splits(pages_s[b] * units_per_seq + y * width, width - brk, pl.share, brk);
-  }
-  int* recs = plan + da_plan_records_at(batch, units_per_seq);
-  for (int w = threadIdx.x; w < grid_blocks; w += blockDim.x) {
-    const DaFirst fs = da_first_segment(pl, pages_s, splits_s, batch, units_per_seq, w);
-    int* r = recs + (size_t)w * DA_PLAN_REC;
-    int pos = 0, slot = 0, first = 0, ids[4] = {0, 0, 0, 0};
-    if (fs.n_pages >= 0) {
-      pos = lens[fs.b] - 1;
-      slot = slots[fs.b];
-      if (shared != nullptr) first = shared[fs.b];
-      const DaList l = da_list(pos, window, keep, first);
-      for (int i = 0; i < 4 && i < fs.n_pages; ++i) {
-        const int entry = af_cache_row(da_page_of(l.kept, l.skip, fs.p_in + i) * AF_PAGE, ring_rows, keep) / AF_PAGE;
-        int page = AF_INDEX_OK(entry < max_pages, entry) ? page_table[(size_t)slot * max_pages + entry] : 0;
-        if (!AF_INDEX_OK(page >= 0, page)) page = 0;
-        ids[i] = page;
-      }
-    }
-    reinterpret_cast<int4*>(r)[0] = make_int4(fs.n_pages, fs.b, fs.y, fs.z);
-    reinterpret_cast<int4*>(r)[1] = make_int4(fs.p_in, fs.run_left, pos, slot);
-    reinterpret_cast<int4*>(r)[2] = make_int4(ids[0], ids[1], ids[2], ids[3]);
-    reinterpret_cast<int4*>(r)[3] = make_int4(first, 0, 0, 0);
-  }
+  da_write_plan(plan, slots, lens, page_table, max_pages, batch, nq, nkv, window, keep, ring_rows, room, grid_blocks, nullptr, brk, dp_smem);
 }
 
 // The heads of one kv group are the (up to 16) rows of an m16n8k16 tile; the
@@ -685,7 +638,7 @@ AF_EXPORT long long af_attn_decode_plan_ints(int batch, int nq, int nkv) {
 // way (the same slots, lengths, page table, heads, window, ring and n_splits): pass `plan` to each of their calls.
 // It holds for these lengths alone: a step later it is made again.
 static int decode_plan_impl(int* plan, long long plan_ints, const int* page_table, int max_pages, const int* slots, const int* lens,
-                            const int* shared, int batch, int nq, int nkv, int window, int keep, int ring_rows, int n_splits, int brk,
+                            int batch, int nq, int nkv, int window, int keep, int ring_rows, int n_splits, int brk,
                             cudaStream_t stream) {
   if (batch == 0) return 0;
   AF_REQUIRE(nq > 0 && nkv > 0 && nq % nkv == 0, "af_attn_decode_plan: heads %d, groups %d", nq, nkv);
@@ -699,29 +652,22 @@ static int decode_plan_impl(int* plan, long long plan_ints, const int* page_tabl
   const int sms = af_sm_count();
   if (sms <= 0) return -1;
   af_launch(attn_decode_plan_kernel, dim3(1), dim3(256), (size_t)2 * (batch + 1) * sizeof(int), stream, plan, slots,
-            lens, page_table, max_pages, batch, nq, nkv, window, keep, ring_rows, n_splits, sms, shared, brk);
+            lens, page_table, max_pages, batch, nq, nkv, window, keep, ring_rows, n_splits, sms, brk);
   AF_CHECK_LAUNCH("af_attn_decode_plan");
 }
 
 AF_EXPORT int af_attn_decode_plan_kept(int* plan, long long plan_ints, const int* page_table, int max_pages,
                                   const int* slots, const int* lens, int batch, int nq, int nkv, int window,
                                   int keep, int ring_rows, int n_splits, cudaStream_t stream) {
-  return decode_plan_impl(plan, plan_ints, page_table, max_pages, slots, lens, nullptr, batch, nq, nkv, window, keep, ring_rows, n_splits,
+  return decode_plan_impl(plan, plan_ints, page_table, max_pages, slots, lens, batch, nq, nkv, window, keep, ring_rows, n_splits,
                           DA_BREAK_PAGES, stream);
 }
 
 // The same for af_attn_decode8 (attention_decode8.cu).
 int af_decode8_plan(int* plan, long long plan_ints, const int* page_table, int max_pages, const int* slots, const int* lens, int batch,
                     int nq, int nkv, int window, int keep, int ring_rows, int n_splits, cudaStream_t stream) {
-  return decode_plan_impl(plan, plan_ints, page_table, max_pages, slots, lens, nullptr, batch, nq, nkv, window, keep, ring_rows, n_splits,
+  return decode_plan_impl(plan, plan_ints, page_table, max_pages, slots, lens, batch, nq, nkv, window, keep, ring_rows, n_splits,
                           D8_BREAK_PAGES, stream);
-}
-
-// The same (for a cache of so many bits) where each sequence's first shared[b] pages are another kernel's (attention_shared.cu).
-int af_decode_plan_shared(int* plan, long long plan_ints, const int* page_table, int max_pages, const int* slots, const int* lens,
-                          const int* shared, int batch, int nq, int nkv, int n_splits, int bits, cudaStream_t stream) {
-  return decode_plan_impl(plan, plan_ints, page_table, max_pages, slots, lens, shared, batch, nq, nkv, 0, 0, 0, n_splits,
-                          bits == 8 ? D8_BREAK_PAGES : DA_BREAK_PAGES, stream);
 }
 
 // The split pass alone (partial results into `scratch`), each sequence's first shared[b] pages left out.

@@ -16,8 +16,9 @@
 // passed by more than 2^8.  Products and softmax of neighbouring pages overlap.
 //   warp 0        TMA producer (16-bit cache)         warp 1  issue of S, TMEM allocation      warp 2  issue of O += P V
 //   warps 4..11   queries, softmax, rescaling, partial results
-//   warps 12..19  8-bit cache only: codes from memory to halves in the swizzled operand layout, 16 bytes a load, the next page's
-//                 loads in flight while this page's are converted
+//   warps 12..19  8-bit cache only: codes, brought into shared memory as they are by warp 0, to halves in the swizzled operand layout
+// An item's partial results are gathered in the operands' memory and leave as one bulk copy (they are contiguous; 16-byte piece c of
+// row r lies at piece c ^ (r & 7), for the banks' sake).
 // In the 8-bit cache a key's factor multiplies its scores, a value's its weights, whose halves are kept relative to the largest
 // such weight (see attention_decode8.cu; the queries are scaled alike).
 // Bound by the prefix's bytes up to some 128 rows; then by the products.
@@ -35,8 +36,6 @@ int af_decode16_split(const void* q, long long q_stride, const void* kcache, con
                       const int* page_table, int max_pages, const int* slots, const int* lens, const int* shared, int batch, int nq,
                       int nkv, int hd, float scale, float cap, int n_splits, float* scratch, const int* plan, int* err,
                       cudaStream_t stream);
-int af_decode_plan_shared(int* plan, long long plan_ints, const int* page_table, int max_pages, const int* slots, const int* lens,
-                          const int* shared, int batch, int nq, int nkv, int n_splits, int bits, cudaStream_t stream);
 
 namespace {
 
@@ -66,11 +65,26 @@ __host__ __device__ inline ShPlan sh_layout(int batch, int nq, int nkv, int bloc
   return p;
 }
 
-// One block.  A group is the live rows of one `lead` that share at least a page; alone in it a row keeps its pages.  Fewer
+// Where the split kernel's plan begins.
+__host__ __device__ inline int sh_own_plan(const ShPlan& p) { return (p.total + 3) / 4 * 4; }
+
+// Items of a unit of `pages` shared pages, `units` of them and `rows` rows a kv head in its group: its share of the blocks, rounded
+// down, so that no block gets a second one; but no more than pay.  s items take pages / s of a page's time each (some 0.8 us with heads
+// of 256) and leave s partial results of every unit, written and read again at some 5 TB/s together: the sum is least for
+// s^2 = pages * time of a page * rate / (bytes of a partial result of all units).  (64 sequences of 2 heads a kv head of 256, 112 pages: 20 items
+// a unit instead of 37.)
+__device__ __forceinline__ int sh_items(int pages, int units, int rows, int hd, int blocks, long long total) {
+  const float page_us = 0.4f + 0.4f * (float)hd / 256.f;
+  const float bytes = (float)units * (float)min(rows, SH_ROWS) * (float)hd * 8.f;
+  const int pay = (int)ceilf(sqrtf((float)pages * page_us * 5.0e6f / bytes));
+  return max(1, min(min(pages, pay), (int)min((long long)pages, (long long)pages * blocks / total)));
+}
+
+// One block.  (Like attn_decode_plan_kernel it does not release its dependents early.)  A group is the live rows of one `lead` that share at least a page; alone in it a row keeps its pages.  Fewer
 // pages than a row claims are taken where another of the group shares fewer, and never the page of its new token.
 __global__ void __launch_bounds__(512)
-attn_shared_plan_kernel(int* __restrict__ plan, const int* __restrict__ lead, const int* __restrict__ pages, const int* __restrict__ slots,
-                        const int* __restrict__ lens, int batch, int nq, int nkv, int blocks) {
+attn_shared_plan_kernel(int* plan, const int* lead, const int* pages, const int* slots, const int* lens, const int* page_table, int max_pages,
+                        int batch, int nq, int nkv, int hd, int blocks, int own_room, int brk) {
   extern __shared__ int sp_smem[];
   int* gid = sp_smem;                  // [batch] the row's group, -1: none
   int* cnt = gid + batch;              // [batch] by group: members
@@ -79,7 +93,7 @@ attn_shared_plan_kernel(int* __restrict__ plan, const int* __restrict__ lead, co
   int* item0 = unit0 + batch;          //           first item
   int* memb0 = item0 + batch;          //           first place in `order`
   int* row0 = memb0 + batch;           //           first partial row
-  __shared__ long long total_s;
+  int* parts = row0 + batch;           //           items of a unit
   pdl_wait();
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int group = nq / nkv;
@@ -122,8 +136,7 @@ attn_shared_plan_kernel(int* __restrict__ plan, const int* __restrict__ lead, co
       const int g = base + lane;
       const bool on = g < batch && cnt[g] >= 2;
       const int c = on ? cnt[g] : 0, u = on ? nkv * ((c * group + SH_ROWS - 1) / SH_ROWS) : 0;
-      // items of a unit: its share of the blocks, rounded down, so that no block gets a second one
-      const int s = on ? (int)max(1ll, min((long long)few[g], (long long)few[g] * blocks / total)) : 0;
+      const int s = on ? sh_items(few[g], u, c * group, hd, blocks, total) : 0;
       int vi = u * s, vr = nkv * c * group * s;
       const int i1 = vi, r1 = vr;
 #pragma unroll
@@ -131,17 +144,15 @@ attn_shared_plan_kernel(int* __restrict__ plan, const int* __restrict__ lead, co
         const int a = __shfl_up_sync(0xffffffffu, vi, o), m = __shfl_up_sync(0xffffffffu, vr, o);
         if (lane >= o) vi += a, vr += m;
       }
-      if (on) item0[g] = items + vi - i1, row0[g] = rows + vr - r1;
+      if (on) item0[g] = items + vi - i1, row0[g] = rows + vr - r1, parts[g] = s;
       items += __shfl_sync(0xffffffffu, vi, 31);
       rows += __shfl_sync(0xffffffffu, vr, 31);
     }
     if (lane == 0) {
-      total_s = total;
       plan[0] = items, plan[1] = units, plan[2] = batch, plan[3] = nq, plan[4] = nkv, plan[5] = blocks;
     }
   }
   __syncthreads();
-  const long long total = total_s;
   for (int b = tid; b < batch; b += blockDim.x) {
     const int g = gid[b];
     const bool on = g >= 0 && cnt[g] >= 2;
@@ -165,7 +176,7 @@ attn_shared_plan_kernel(int* __restrict__ plan, const int* __restrict__ lead, co
       }
     }
     const int rows = c * group, tiles = (rows + SH_ROWS - 1) / SH_ROWS, u = nkv * tiles;
-    const int s = (int)max(1ll, min((long long)few[g], (long long)few[g] * blocks / total));
+    const int s = parts[g];
     for (int x = lane; x < u; x += 32) {
       int* r = plan + L.units + 8 * (unit0[g] + x);
       const int kvh = x / tiles, tile = x - kvh * tiles;
@@ -177,6 +188,9 @@ attn_shared_plan_kernel(int* __restrict__ plan, const int* __restrict__ lead, co
       plan[L.items + 2 * (item0[g] + x) + 1] = x - x / s * s;
     }
   }
+  __syncthreads();
+  da_write_plan(plan + sh_own_plan(L), slots, lens, page_table, max_pages, batch, nq, nkv, 0, 0, 0, own_room, blocks, plan + L.shared, brk,
+                parts + batch);
 }
 
 // ---------------------------------------------------------------- the prefix kernel
@@ -190,8 +204,12 @@ template <int HD, int BITS>
 struct Sh {
   static constexpr int WARPS = BITS == 8 ? 20 : 12, THREADS = WARPS * 32;
   static constexpr int TILE = AF_PAGE * HD * 2;                              // bytes of a page's keys, or values, as operand
-  static constexpr int STAGES = HD == 256 ? 3 : (HD == 128 ? 6 : 8);         // pages in flight
-  static constexpr int SMEM = 2 * STAGES * TILE + 1024;
+  // pages in flight (16 bits), or converted (8 bits; beside them RAW pages of codes are in flight)
+  static constexpr int STAGES = BITS == 16 ? (HD == 256 ? 3 : (HD == 128 ? 6 : 8)) : (HD == 256 ? 2 : (HD == 128 ? 4 : 6));
+  static constexpr int CODES = BITS == 8 ? AF_PAGE * HD : 0, RAW = HD == 256 ? 2 : (HD == 128 ? 4 : 8);
+  static constexpr int RAW_STAGE = 2 * CODES + (BITS == 8 ? 2 * AF_PAGE : 0);
+  static constexpr int SMEM = 2 * STAGES * TILE + RAW * RAW_STAGE + 1024;
+  static_assert(SH_ROWS * HD * 4 <= 2 * STAGES * TILE, "an item's results fit the operands' memory");
 };
 
 struct ShArgs {
@@ -212,6 +230,12 @@ __host__ __device__ constexpr uint32_t sh_idesc(int bn, bool f16, bool b_mn_majo
          ((uint32_t)(128 >> 4) << 24);
 }
 
+__device__ __forceinline__ void sh_bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(smem_u32(dst)),
+               "l"(src), "r"(bytes), "r"(smem_u32(bar))
+               : "memory");
+}
+
 // What an item is: every role reads it from the plan.
 struct ShItem {
   int rows, first, pages, row0, members0, group0, kvh, slot;      // rows of the tile; page range; partial row; ...
@@ -228,8 +252,9 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
   extern __shared__ unsigned char sh_raw[];
   unsigned char* k_s = (unsigned char*)(((uintptr_t)sh_raw + 1023) & ~(uintptr_t)1023);      // [stage][sub-tile][64 keys][128 B]
   unsigned char* v_s = k_s + STAGES * C::TILE;
+  unsigned char* raw_s = v_s + STAGES * C::TILE;     // [stage][codes of keys | of values | exponents of keys | of values]
   __shared__ uint64_t k_full[STAGES], k_empty[STAGES], v_full[STAGES], v_empty[STAGES], s_full[2], p_full[2], pv_done[2], m_ready[2], q_ready,
-      l_full;
+      l_full, staged, ring_free, raw_full[C::RAW], raw_empty[C::RAW];
   __shared__ float mref_s[2][SH_ROWS], l_s[2][SH_ROWS];
   __shared__ float wref_s[BITS == 8 ? 2 : 1][BITS == 8 ? SH_ROWS : 1];
   __shared__ __align__(16) float ks_s[BITS == 8 ? SH_EXPS : 1][AF_PAGE], lv_s[BITS == 8 ? SH_EXPS : 1][AF_PAGE];
@@ -265,6 +290,12 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
     }
     mbar_init(&q_ready, 8);
     mbar_init(&l_full, 8);
+    mbar_init(&staged, 8);
+    mbar_init(&ring_free, 1);
+    for (int s = 0; s < C::RAW; ++s) {
+      mbar_init(&raw_full[s], 1);
+      mbar_init(&raw_empty[s], 8);
+    }
     give_up_s = 0;
     mbar_fence_init();
   }
@@ -299,12 +330,28 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
 
   // Pages are counted through over the block's items (`jj`): a page's group, stage and phases follow from its count.
   if (warp == 0) {
-    // ---- the 16-bit cache's pages.  They are older than the kernels in front: nothing to wait for
-    if (BITS == 16 && lane == 0) {
-      int jj = 0;
-      for (int w = blockIdx.x; w < n_items && !*give_up; w += gridDim.x) {
+    // ---- the cache's pages, to the operands or (8 bits) as they are.  They are older than the kernels in front: nothing to wait for
+    if (lane == 0) {
+      int jj = 0, n = 0;
+      for (int w = blockIdx.x; w < n_items && !*give_up; w += gridDim.x, ++n) {
         const ShItem it = item_of(w);
         int next = page_id(it, 0);
+        if constexpr (BITS == 8) {
+          for (int j = 0; j < it.pages; ++j, ++jj) {
+            const int s = jj % C::RAW;
+            const size_t at = (size_t)(next * a.nkv + it.kvh) * AF_PAGE;
+            if (j + 1 < it.pages) next = page_id(it, j + 1);
+            if (!mbar_wait(&raw_empty[s], ((jj / C::RAW) & 1) ^ 1, give_up)) break;
+            unsigned char* st = raw_s + s * C::RAW_STAGE;
+            mbar_expect_tx(&raw_full[s], C::RAW_STAGE);
+            sh_bulk_load(st, a.k + at * HD, C::CODES, &raw_full[s]);
+            sh_bulk_load(st + C::CODES, a.v + at * HD, C::CODES, &raw_full[s]);
+            sh_bulk_load(st + 2 * C::CODES, a.k_exp + at, AF_PAGE, &raw_full[s]);
+            sh_bulk_load(st + 2 * C::CODES + AF_PAGE, a.v_exp + at, AF_PAGE, &raw_full[s]);
+          }
+          continue;
+        }
+        if (n > 0 && !mbar_wait(&ring_free, (n - 1) & 1, give_up)) break;      // (the item before has left the operands' memory)
         for (int j = 0; j < it.pages; ++j, ++jj) {
           const int s = jj % STAGES, row = (next * a.nkv + it.kvh) * AF_PAGE;
           const uint32_t ph = ((jj / STAGES) & 1) ^ 1;
@@ -536,8 +583,11 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
       }
       if (!ok) break;
       // ---- the item's partial results
+      // (First the page before the last: the group that does not own the last page has not seen that the barrier's phase before is
+      // complete, and a wait one phase ahead returns at once.  Its own page's scores were made after that phase.)
       const int last = jj - 1;
-      ok = mbar_wait(&pv_done[last & 1], (last >> 1) & 1, give_up);
+      ok = it.pages < 2 || mbar_wait(&pv_done[(last - 1) & 1], ((last - 1) >> 1) & 1, give_up);
+      ok = ok && mbar_wait(&pv_done[last & 1], (last >> 1) & 1, give_up);
       if (!ok) break;
       tc_fence_after();
       const float m_fin = any ? mref_s[last & 1][row] : 0.f;
@@ -549,7 +599,6 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
       if (any) {
         float f = 1.f;
         if constexpr (BITS == 8) f = fast_exp2(wref_s[last & 1][row] - SH_SHIFT - m_fin);
-        const size_t at = (size_t)it.row0 + row;
 #pragma unroll 1
         for (int c0 = 0; c0 < HD / 2; c0 += 32) {
           float o[32];
@@ -557,38 +606,50 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
           tmem_ld32(lane_addr + O_COL + col, o);
           tmem_wait_ld();
           if (live) {
+            unsigned char* dst = k_s + row * (HD * 4);
 #pragma unroll
             for (int c = 0; c < 32; c += 4)
-              *reinterpret_cast<float4*>(a.part_o + at * HD + col + c) = make_float4(o[c] * f, o[c + 1] * f, o[c + 2] * f, o[c + 3] * f);
+              *reinterpret_cast<float4*>(dst + ((((col + c) >> 2) ^ (row & 7)) << 4)) = make_float4(o[c] * f, o[c + 1] * f, o[c + 2] * f, o[c + 3] * f);
           }
         }
-        if (live && grp == 0) *reinterpret_cast<float2*>(a.part_ml + at * 2) = make_float2(m_fin, l_s[0][row] + l_s[1][row]);
+        if (live && grp == 0) *reinterpret_cast<float2*>(a.part_ml + ((size_t)it.row0 + row) * 2) = make_float2(m_fin, l_s[0][row] + l_s[1][row]);
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&staged);
+      if (warp == 4) {
+        ok = mbar_wait(&staged, n & 1, give_up);
+        if (ok && lane == 0) {
+          asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(a.part_o + (size_t)it.row0 * HD), "r"(smem_u32(k_s)),
+                       "r"(it.rows * HD * 4)
+                       : "memory");
+          asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+          if (w + (int)gridDim.x < n_items) {
+            asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+            mbar_arrive(&ring_free);
+          } else {
+            asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+          }
+        }
+        __syncwarp();
       }
     }
   } else if (BITS == 8 && warp >= 12) {
     // ---- codes to halves.  A page's keys (and values) are 64 rows of HD / 16 pieces of 16 codes; a thread takes PER of them
     constexpr int P_ROW = HD / 16, PER = AF_PAGE * P_ROW / 256;
     const int ct = threadIdx.x - 12 * 32;
-    int jj = 0;
+    int jj = 0, n = 0;
     bool ok = true;
-    uint4 kc[PER], vc[PER];
-    int ke = 0, ve = 0;
-    auto load = [&](const ShItem& it, int page) {
-      const size_t at = (size_t)(page * a.nkv + it.kvh) * AF_PAGE;
-      const uint4* kp = reinterpret_cast<const uint4*>(a.k + at * HD);
-      const uint4* vp = reinterpret_cast<const uint4*>(a.v + at * HD);
-#pragma unroll
-      for (int i = 0; i < PER; ++i) kc[i] = __ldg(kp + ct + i * 256), vc[i] = __ldg(vp + ct + i * 256);
-      if (ct < AF_PAGE) ke = a.k_exp[at + ct], ve = a.v_exp[at + ct];
-    };
-    auto convert = [&](unsigned char* tile, const uint4* codes) {
+    auto convert = [&](unsigned char* tile, const unsigned char* raw) {
 #pragma unroll
       for (int i = 0; i < PER; ++i) {
         const int x = ct + i * 256, r = x / P_ROW, p = x - r * P_ROW;
-        const uint32_t w[4] = {codes[i].x, codes[i].y, codes[i].z, codes[i].w};
+        const uint4 w = *reinterpret_cast<const uint4*>(raw + x * 16);
         uint4 h[2];
-        h[0] = make_uint4(c8_half2(w[0]), c8_half2(w[0] >> 16), c8_half2(w[1]), c8_half2(w[1] >> 16));
-        h[1] = make_uint4(c8_half2(w[2]), c8_half2(w[2] >> 16), c8_half2(w[3]), c8_half2(w[3] >> 16));
+        c8_half4(w.x, h[0].x, h[0].y);
+        c8_half4(w.y, h[0].z, h[0].w);
+        c8_half4(w.z, h[1].x, h[1].y);
+        c8_half4(w.w, h[1].z, h[1].w);
         unsigned char* base = tile + (p >> 2) * 8192 + r * 128;
         const int c = (p & 3) * 2, first = (p >> 2) & 1;      // (neighbouring sub-tiles begin with the other piece: other banks)
         *reinterpret_cast<uint4*>(base + (((c + first) ^ (r & 7)) << 4)) = first ? h[1] : h[0];
@@ -597,29 +658,28 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       __syncwarp();
     };
-    ShItem it = item_of(blockIdx.x);
-    load(it, page_id(it, 0));
-    for (int w = blockIdx.x; w < n_items && ok; w += gridDim.x) {
-      it = item_of(w);
-      if (w != (int)blockIdx.x) load(it, page_id(it, 0));
+    for (int w = blockIdx.x; w < n_items && ok; w += gridDim.x, ++n) {
+      const ShItem it = item_of(w);
+      if (n > 0) ok = mbar_wait(&ring_free, (n - 1) & 1, give_up);      // (the item before has left the operands' memory)
       for (int j = 0; j < it.pages && ok; ++j, ++jj) {
-        const int s = jj % STAGES;
+        const int s = jj % STAGES, rs = jj % C::RAW;
         const uint32_t ph = ((jj / STAGES) & 1) ^ 1;
-        const int next = j + 1 < it.pages ? page_id(it, j + 1) : -1;
-        ok = mbar_wait(&k_empty[s], ph, give_up);
+        const unsigned char* raw = raw_s + rs * C::RAW_STAGE;
+        ok = mbar_wait(&raw_full[rs], (jj / C::RAW) & 1, give_up) && mbar_wait(&k_empty[s], ph, give_up);
         if (!ok) break;
-        convert(k_s + s * C::TILE, kc);
         if (ct < AF_PAGE) {
-          ks_s[jj % SH_EXPS][ct] = __uint_as_float((uint32_t)ke << 23);
-          lv_s[jj % SH_EXPS][ct] = (float)(ve - 127);
+          ks_s[jj % SH_EXPS][ct] = __uint_as_float((uint32_t)raw[2 * C::CODES + ct] << 23);
+          lv_s[jj % SH_EXPS][ct] = (float)((int)raw[2 * C::CODES + AF_PAGE + ct] - 127);
         }
-        __syncwarp();
+        convert(k_s + s * C::TILE, raw);
         if (lane == 0) mbar_arrive(&k_full[s]);
         ok = mbar_wait(&v_empty[s], ph, give_up);
         if (!ok) break;
-        convert(v_s + s * C::TILE, vc);
-        if (lane == 0) mbar_arrive(&v_full[s]);
-        if (next >= 0) load(it, next);
+        convert(v_s + s * C::TILE, raw + C::CODES);
+        if (lane == 0) {
+          mbar_arrive(&v_full[s]);
+          mbar_arrive(&raw_empty[rs]);
+        }
       }
     }
   }
@@ -644,7 +704,7 @@ attn_shared_merge_kernel(__nv_bfloat16* __restrict__ out, long long out_stride, 
   const int group = nq / nkv, kvh = h / group, units_per_seq = nkv * ((group + 15) / 16);
   const ShPlan L = sh_layout(batch, nq, nkv, blocks);
   const int n_own = own_plan[DA_PLAN_HEAD + b * units_per_seq + kvh * ((group + 15) / 16) + (h % group) / 16];
-  int n_pre = 0, rows = 0;
+  int n_pre = 0, rows = 0, turn = 0;
   size_t pre0 = 0;
   const int unit0 = shared_plan[L.loc + 2 * b];
   if (unit0 >= 0) {
@@ -654,6 +714,7 @@ attn_shared_merge_kernel(__nv_bfloat16* __restrict__ out, long long out_stride, 
     rows = min(SH_ROWS, members * group - rr / SH_ROWS * SH_ROWS);
     n_pre = u[5];
     pre0 = (size_t)u[6] + rr % SH_ROWS;
+    turn = rr & 7;                     // (how the row's pieces lie)
   }
   const size_t own0 = ((size_t)b * nq + h) * own_room;
   __shared__ float f_s[SHM_MOST], l_s[SHM_MOST];
@@ -690,7 +751,7 @@ attn_shared_merge_kernel(__nv_bfloat16* __restrict__ out, long long out_stride, 
 #pragma unroll
       for (int u = 0; u < 8; ++u) {
         const int i = i0 + u * GROUPS, x = base + i;
-        v[u] = i < m ? __ldcg(reinterpret_cast<const float4*>((x < n_own ? own_o + (own0 + x) * HD : pre_o + (pre0 + (size_t)(x - n_own) * rows) * HD) + d))
+        v[u] = i < m ? __ldcg(reinterpret_cast<const float4*>(x < n_own ? own_o + (own0 + x) * HD + d : pre_o + (pre0 + (size_t)(x - n_own) * rows) * HD + (((d >> 2) ^ turn) << 2)))
                      : make_float4(0.f, 0.f, 0.f, 0.f);
       }
 #pragma unroll
@@ -743,7 +804,7 @@ AF_EXPORT long long af_attn_shared_plan_ints(int batch, int nq, int nkv) {
   if (batch <= 0 || batch > SH_MAX_BATCH || nq <= 0 || nkv <= 0 || nq % nkv) return 0;
   const int sms = af_sm_count();
   if (sms <= 0) return 0;
-  return (sh_layout(batch, nq, nkv, sms).total + 3) / 4 * 4 + af_attn_decode_plan_ints(batch, nq, nkv);
+  return sh_own_plan(sh_layout(batch, nq, nkv, sms)) + af_attn_decode_plan_ints(batch, nq, nkv);
 }
 
 // The most partial rows that the prefix kernel leaves (see af_attn_decode_shared).
@@ -757,25 +818,25 @@ AF_EXPORT long long af_attn_shared_rows(int batch, int nq, int nkv) {
 
 // The plans of a step: row b's first pages[b] cache pages are those of row lead[b].
 static int shared_plans(int* plan, long long plan_ints, const int* lead, const int* pages, const int* page_table, int max_pages,
-                        const int* slots, const int* lens, int batch, int nq, int nkv, int n_splits, int bits, cudaStream_t stream) {
+                        const int* slots, const int* lens, int batch, int nq, int nkv, int hd, int n_splits, int bits, cudaStream_t stream) {
   const long long need = af_attn_shared_plan_ints(batch, nq, nkv);
   AF_REQUIRE(need > 0, "af_attn_decode_shared: %d sequences (takes %d), %d heads in %d groups", batch, SH_MAX_BATCH, nq, nkv);
   AF_REQUIRE(plan_ints >= need, "af_attn_decode_shared: a plan of %lld integers", need);
-  const int sms = af_sm_count(), smem = 7 * batch * (int)sizeof(int);
+  const int sms = af_sm_count(), smem = (10 * batch + 2) * (int)sizeof(int);
   static bool configured[AF_MAX_DEVICES] = {};
   const int dev = af_current_device();
   if (dev < 0) return -1;
   if (!configured[dev]) {
-    const cudaError_t e = cudaFuncSetAttribute(attn_shared_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 7 * SH_MAX_BATCH * (int)sizeof(int));
+    const cudaError_t e = cudaFuncSetAttribute(attn_shared_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (10 * SH_MAX_BATCH + 2) * (int)sizeof(int));
     if (e != cudaSuccess) return af_fail((int)e, "af_attn_decode_shared: %s", cudaGetErrorString(e));
     configured[dev] = true;
   }
-  af_launch(attn_shared_plan_kernel, dim3(1), dim3(512), smem, stream, plan, lead, pages, slots, lens, batch, nq, nkv,
-            sms);
-  AF_COUNT_LAUNCH("af_attn_decode_shared (plan)");
-  const ShPlan L = sh_layout(batch, nq, nkv, sms);
-  const int at = (L.total + 3) / 4 * 4;
-  return af_decode_plan_shared(plan + at, plan_ints - at, page_table, max_pages, slots, lens, plan + L.shared, batch, nq, nkv, n_splits, bits, stream);
+  const int units_per_seq = nkv * ((nq / nkv + 15) / 16), brk = bits == 8 ? D8_BREAK_PAGES : DA_BREAK_PAGES;
+  AF_REQUIRE((long long)batch * (max_pages + 1 + brk) * units_per_seq < (1ll << 31), "af_attn_decode_shared: %d sequences of up to %d pages", batch,
+             max_pages);
+  af_launch(attn_shared_plan_kernel, dim3(1), dim3(512), smem, stream, plan, lead, pages, slots, lens, page_table, max_pages, batch, nq, nkv, hd,
+            sms, n_splits, brk);
+  AF_CHECK_LAUNCH("af_attn_decode_shared (plan)");
 }
 
 // What af_attn_decode_shared is given, as one block of 64-bit words.
@@ -814,12 +875,12 @@ AF_EXPORT int af_attn_decode_shared(const AfShared* c) {
   const int *page_table = (const int*)c->page_table, *slots = (const int*)c->slots, *lens = (const int*)c->lens;
   int rc;
   if (c->plan_ints > 0) {
-    rc = shared_plans(c->plan, c->plan_ints, (const int*)c->lead, (const int*)c->pages, page_table, max_pages, slots, lens, batch, nq, nkv, n_splits,
+    rc = shared_plans(c->plan, c->plan_ints, (const int*)c->lead, (const int*)c->pages, page_table, max_pages, slots, lens, batch, nq, nkv, hd, n_splits,
                       (int)c->bits, c->stream);
     if (rc) return rc;
   }
   const ShPlan L = sh_layout(batch, nq, nkv, sms);
-  const int at = (L.total + 3) / 4 * 4;
+  const int at = sh_own_plan(L);
   const long long rows = af_attn_shared_rows(batch, nq, nkv);
   ShArgs a{(const __nv_bfloat16*)c->q, c->q_stride, (const uint8_t*)c->k, (const uint8_t*)c->v, (const uint8_t*)c->k_exp, (const uint8_t*)c->v_exp,
            c->n_pages, page_table, c->plan, max_pages, batch, nq, nkv, (float)c->scale, (float)c->cap, c->pre_scratch, c->pre_scratch + rows * hd,

@@ -239,6 +239,60 @@ __host__ __device__ inline long long da_plan_records_at(int batch, int units_per
   return DA_PLAN_HEAD + (((long long)batch * units_per_seq + 3) / 4) * 4;
 }
 
+// Writes the plan, by a whole block; smem: 2 (batch + 1) integers.
+__device__ __forceinline__ void da_write_plan(int* plan, const int* slots, const int* lens, const int* page_table, int max_pages, int batch,
+                                              int nq, int nkv, int window, int keep, int ring_rows, int room, int grid_blocks,
+                                              const int* shared, int brk, int* dp_smem) {
+  int* pages_s = dp_smem;                 // [batch + 1]
+  int* splits_s = dp_smem + batch + 1;    // [batch + 1]
+  __shared__ DaPlan plan_s;
+  const int group = nq / nkv, tiles = (group + 15) / 16, units_per_seq = nkv * tiles;
+  if (threadIdx.x < 32) {
+    const DaPlan pl = da_plan(slots, lens, batch, window, keep, shared, brk, units_per_seq, grid_blocks, room, 0, pages_s, splits_s);
+    if (threadIdx.x == 0) plan_s = pl;
+  }
+  __syncthreads();
+  const DaPlan pl = plan_s;
+  if (threadIdx.x == 0) {
+    plan[0] = room;
+    plan[1] = da_plan_mark(grid_blocks, brk);
+    plan[2] = batch;
+    plan[3] = units_per_seq;
+    plan[4] = pl.even;
+    plan[5] = pl.share;
+    plan[6] = pl.n_blocks;
+    plan[7] = 0;
+  }
+  for (int u = threadIdx.x; u < batch * units_per_seq; u += blockDim.x) {
+    const int b = u / units_per_seq, y = u - b * units_per_seq;
+    const int width = pages_s[b + 1] - pages_s[b];      // (the run cut: with a break)
+    plan[DA_PLAN_HEAD + u] = pl.even ? da_even_splits(width, pl.share, room, pl.even)
+                                     : da_run_splits(pages_s[b] * units_per_seq + y * width, width - brk, pl.share, brk);
+  }
+  int* recs = plan + da_plan_records_at(batch, units_per_seq);
+  for (int w = threadIdx.x; w < grid_blocks; w += blockDim.x) {
+    const DaFirst fs = da_first_segment(pl, pages_s, splits_s, batch, units_per_seq, w);
+    int* r = recs + (size_t)w * DA_PLAN_REC;
+    int pos = 0, slot = 0, first = 0, ids[4] = {0, 0, 0, 0};
+    if (fs.n_pages >= 0) {
+      pos = lens[fs.b] - 1;
+      slot = slots[fs.b];
+      if (shared != nullptr) first = shared[fs.b];
+      const DaList l = da_list(pos, window, keep, first);
+      for (int i = 0; i < 4 && i < fs.n_pages; ++i) {
+        const int entry = af_cache_row(da_page_of(l.kept, l.skip, fs.p_in + i) * AF_PAGE, ring_rows, keep) / AF_PAGE;
+        int page = AF_INDEX_OK(entry < max_pages, entry) ? page_table[(size_t)slot * max_pages + entry] : 0;
+        if (!AF_INDEX_OK(page >= 0, page)) page = 0;
+        ids[i] = page;
+      }
+    }
+    reinterpret_cast<int4*>(r)[0] = make_int4(fs.n_pages, fs.b, fs.y, fs.z);
+    reinterpret_cast<int4*>(r)[1] = make_int4(fs.p_in, fs.run_left, pos, slot);
+    reinterpret_cast<int4*>(r)[2] = make_int4(ids[0], ids[1], ids[2], ids[3]);
+    reinterpret_cast<int4*>(r)[3] = make_int4(first, 0, 0, 0);
+  }
+}
+
 // ---------------------------------------------------------------- pass 2
 
 constexpr int DA_MERGE_FEW = 8;        // up to this many splits: 128 threads, every load at once

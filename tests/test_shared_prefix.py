@@ -248,6 +248,22 @@ def test_same_result_alone_and_on_another_stream(K):
         assert torch.equal(outs[0], outs[1]) and torch.equal(outs[0], outs[2])
 
 
+@pytest.mark.parametrize("bits", [16, 8])
+@pytest.mark.parametrize("hd,seqs", [(64, [(i % 40, 1 + i % 4, 300 + i) for i in range(120)]), (128, [(0, 40, 3000 + i) for i in range(20)]),
+                                     (256, [(i % 3, 40 + i % 3, 3000 + i) for i in range(24)])])
+def test_same_result_every_time(K, bits, hd, seqs):
+    """Blocks of several items, units of many items, several groups: fifty runs give the same bits."""
+    f = Family(seqs, 8, hd, bits)
+    q = (torch.randn(len(seqs), 16 * hd) * 2).to(torch.bfloat16).to(DEV)
+    l, p = f.lead()
+    first = None
+    for _ in range(50):
+        out = torch.empty(len(seqs), 16 * hd, dtype=torch.bfloat16, device=DEV)
+        K.attn_decode_shared(out, q, f, f.step(), 16, 8, hd, 0.1, 0.0, l, p, 43)
+        first = out if first is None else first
+        assert torch.equal(out, first)
+
+
 def test_other_paths(K):
     """Sizes that the shared kernels do not take (32 bits, odd head sizes) go to the ordinary attention; rings are refused."""
     f = Family([(0, 3, 200), (0, 3, 193)], 2, 64, 16)
