@@ -9,14 +9,14 @@
 //
 // The prefix kernel.  A block holds its 128 rows' queries in tensor memory and walks its pages, 64 keys at a time:
 //   S = Q K^T     tcgen05.mma, M = 128, N = 64, Q from TMEM, the K page from swizzled shared memory
-//   softmax       two groups of four warps take the pages in turn, a thread a row: all keys are visible (a shared page is full
-//                 and older than every member's token), so there is no mask; P goes back into its S columns of TMEM
+//   softmax       two groups of eight warps take the pages in turn, two threads a row (32 keys each): all keys are visible (a shared
+//                 page is full and older than every member's token), so there is no mask; P goes back into its S columns of TMEM
 //   O += P V      tcgen05.mma, P from TMEM, O (128 x head_dim, 32 bits) in TMEM for the whole item
 // The groups share O and its reference maximum, which a group hands to the other with every page and which moves only when it is
 // passed by more than 2^8.  Products and softmax of neighbouring pages overlap.
 //   warp 0        TMA producer (16-bit cache)         warp 1  issue of S, TMEM allocation      warp 2  issue of O += P V
-//   warps 4..11   queries, softmax, rescaling, partial results
-//   warps 12..19  8-bit cache only: codes, brought into shared memory as they are by warp 0, to halves in the swizzled operand layout
+//   warps 4..19   queries, softmax, rescaling, partial results
+//   warps 20..23  8-bit cache only: codes, brought into shared memory as they are by warp 0, to halves in the swizzled operand layout
 // An item's partial results are gathered in the operands' memory and leave as one bulk copy (they are contiguous; 16-byte piece c of
 // row r lies at piece c ^ (r & 7), for the banks' sake).
 // In the 8-bit cache a key's factor multiplies its scores, a value's its weights, whose halves are kept relative to the largest
@@ -202,7 +202,7 @@ constexpr int SH_EXPS = 16;              // (8 bits) pages whose factors are kep
 
 template <int HD, int BITS>
 struct Sh {
-  static constexpr int WARPS = BITS == 8 ? 20 : 12, THREADS = WARPS * 32;
+  static constexpr int WARPS = BITS == 8 ? 24 : 20, THREADS = WARPS * 32;
   static constexpr int TILE = AF_PAGE * HD * 2;                              // bytes of a page's keys, or values, as operand
   // pages in flight (16 bits), or converted (8 bits; beside them RAW pages of codes are in flight)
   static constexpr int STAGES = BITS == 16 ? (HD == 256 ? 3 : (HD == 128 ? 6 : 8)) : (HD == 256 ? 2 : (HD == 128 ? 4 : 6));
@@ -253,11 +253,14 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
   unsigned char* k_s = (unsigned char*)(((uintptr_t)sh_raw + 1023) & ~(uintptr_t)1023);      // [stage][sub-tile][64 keys][128 B]
   unsigned char* v_s = k_s + STAGES * C::TILE;
   unsigned char* raw_s = v_s + STAGES * C::TILE;     // [stage][codes of keys | of values | exponents of keys | of values]
-  __shared__ uint64_t k_full[STAGES], k_empty[STAGES], v_full[STAGES], v_empty[STAGES], s_full[2], p_full[2], pv_done[2], m_ready[2], q_ready,
+  __shared__ uint64_t k_full[STAGES], k_empty[STAGES], v_full[STAGES], v_empty[STAGES], s_full[2], p_full[2], pv_done[2], m_ready[2], x_full[2], q_ready,
       l_full, staged, ring_free, raw_full[C::RAW], raw_empty[C::RAW];
-  __shared__ float mref_s[2][SH_ROWS], l_s[2][SH_ROWS];
-  __shared__ float wref_s[BITS == 8 ? 2 : 1][BITS == 8 ? SH_ROWS : 1];
-  __shared__ __align__(16) float ks_s[BITS == 8 ? SH_EXPS : 1][AF_PAGE], lv_s[BITS == 8 ? SH_EXPS : 1][AF_PAGE];
+  constexpr int W_ROWS = BITS == 8 ? SH_ROWS : 1, W_PAGES = BITS == 8 ? SH_EXPS : 1;
+  // by group: the references after its page; by group and part: maxima of a page; by thread of a row: sums
+  __shared__ float mref_s[2][SH_ROWS], mx_s[2][2][SH_ROWS], l_s[4][SH_ROWS];
+  __shared__ float wref_s[2][W_ROWS], mw_s[2][2][W_ROWS];
+  // the keys' factors, the values' exponents, the values' factors
+  __shared__ __align__(16) float ks_s[W_PAGES][AF_PAGE], lv_s[W_PAGES][AF_PAGE], vs_s[W_PAGES][AF_PAGE];
   __shared__ uint32_t tmem_base_s;
   __shared__ int give_up_s;
   volatile int* give_up = &give_up_s;
@@ -277,24 +280,25 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
   }
   if (threadIdx.x == 0) {
     for (int s = 0; s < STAGES; ++s) {
-      mbar_init(&k_full[s], BITS == 8 ? 8 : 1);
+      mbar_init(&k_full[s], BITS == 8 ? 4 : 1);      // (one arrival a converting warp)
       mbar_init(&k_empty[s], 1);
-      mbar_init(&v_full[s], BITS == 8 ? 8 : 1);
+      mbar_init(&v_full[s], BITS == 8 ? 4 : 1);
       mbar_init(&v_empty[s], 1);
     }
     for (int s = 0; s < 2; ++s) {
       mbar_init(&s_full[s], 1);
-      mbar_init(&p_full[s], 4);
+      mbar_init(&p_full[s], 8);
       mbar_init(&pv_done[s], 1);
-      mbar_init(&m_ready[s], 4);
+      mbar_init(&m_ready[s], 8);
+      mbar_init(&x_full[s], 8);
     }
-    mbar_init(&q_ready, 8);
-    mbar_init(&l_full, 8);
-    mbar_init(&staged, 8);
+    mbar_init(&q_ready, 16);
+    mbar_init(&l_full, 16);
+    mbar_init(&staged, 16);
     mbar_init(&ring_free, 1);
     for (int s = 0; s < C::RAW; ++s) {
       mbar_init(&raw_full[s], 1);
-      mbar_init(&raw_empty[s], 8);
+      mbar_init(&raw_empty[s], 4);
     }
     give_up_s = 0;
     mbar_fence_init();
@@ -410,9 +414,11 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
         }
       }
     }
-  } else if (warp >= 4 && warp < 12) {
-    // ---- queries, softmax, partial results.  A thread has a row; group g takes the pages whose count is g modulo 2
-    const int grp = (warp - 4) >> 2, quarter = warp & 3, row = quarter * 32 + lane;
+  } else if (warp >= 4 && warp < 20) {
+    // ---- queries, softmax, partial results.  Group g takes the pages whose count is g modulo 2; two threads of a group have a row,
+    // each 32 of the page's keys
+    constexpr int W = AF_PAGE / 2;
+    const int grp = (warp - 4) >> 3, part = ((warp - 4) >> 2) & 1, quad = grp * 2 + part, quarter = warp & 3, row = quarter * 32 + lane;
     const uint32_t lane_addr = tmem + ((uint32_t)(quarter * 32) << 16);
     const float ecap = a.cap > 0.f ? 2.f * LOG2E / a.cap : 0.f, capl = a.cap * LOG2E;
     int jj = 0, n = 0;
@@ -424,14 +430,15 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
       const bool any = quarter * 32 < it.rows;             // (warps without a row only keep the barriers' count)
       float cs = a.cap > 0.f ? a.scale : a.scale * LOG2E;
       if (any) {
-        // ---- half of the row's query into TMEM, two elements a column
+        // ---- a quarter (heads of 64: half, by two threads) of the row's query into TMEM, two elements a column
         const int rr = it.group0 + row, member = rr / group;
         const int b = live ? a.plan[L.order + it.members0 + member] : 0;
         const __nv_bfloat16* qr = a.q + (size_t)b * a.q_stride + (size_t)(it.kvh * group + (live ? rr - member * group : 0)) * HD;
-        constexpr int HALF = HD / 2, PIECES = HALF / 8;
+        constexpr int SHARE = HD == 64 ? 32 : HD / 4, PIECES = SHARE / 8;
         float f1 = 1.f, f2 = 1.f;
         if constexpr (BITS == 8) {
           uint32_t top = 0;
+#pragma unroll 4
           for (int c = 0; c < HD / 8; ++c) {
             const uint4 x = live ? *reinterpret_cast<const uint4*>(qr + c * 8) : make_uint4(0u, 0u, 0u, 0u);
             const uint32_t ws[4] = {x.x, x.y, x.z, x.w};
@@ -445,24 +452,26 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
           f1 = c8_pow2(up / 2), f2 = c8_pow2(up - up / 2);
           cs *= c8_pow2(-(up / 2)) * c8_pow2(-(up - up / 2));
         }
+        if (quad * SHARE < HD) {
 #pragma unroll
-        for (int c0 = 0; c0 < PIECES; c0 += 4) {
-          uint32_t wd[16];
+          for (int c0 = 0; c0 < PIECES; c0 += 4) {
+            uint32_t wd[16];
 #pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            const uint4 x = live ? *reinterpret_cast<const uint4*>(qr + grp * HALF + (c0 + c) * 8) : make_uint4(0u, 0u, 0u, 0u);
-            wd[4 * c] = x.x, wd[4 * c + 1] = x.y, wd[4 * c + 2] = x.z, wd[4 * c + 3] = x.w;
-          }
-          if constexpr (BITS == 8) {
-#pragma unroll
-            for (int e = 0; e < 16; ++e) {
-              const __half2 h = __floats2half2_rn(__uint_as_float(wd[e] << 16) * f1 * f2, __uint_as_float(wd[e] & 0xffff0000u) * f1 * f2);
-              wd[e] = *reinterpret_cast<const uint32_t*>(&h);
+            for (int c = 0; c < 4; ++c) {
+              const uint4 x = live ? *reinterpret_cast<const uint4*>(qr + quad * SHARE + (c0 + c) * 8) : make_uint4(0u, 0u, 0u, 0u);
+              wd[4 * c] = x.x, wd[4 * c + 1] = x.y, wd[4 * c + 2] = x.z, wd[4 * c + 3] = x.w;
             }
+            if constexpr (BITS == 8) {
+#pragma unroll
+              for (int e = 0; e < 16; ++e) {
+                const __half2 h = __floats2half2_rn(__uint_as_float(wd[e] << 16) * f1 * f2, __uint_as_float(wd[e] & 0xffff0000u) * f1 * f2);
+                wd[e] = *reinterpret_cast<const uint32_t*>(&h);
+              }
+            }
+            tmem_st16(lane_addr + Q_COL + quad * (SHARE / 2) + c0 * 4, reinterpret_cast<const float*>(wd));
           }
-          tmem_st16(lane_addr + Q_COL + grp * (HALF / 2) + c0 * 4, reinterpret_cast<const float*>(wd));
+          tmem_wait_st();
         }
-        tmem_wait_st();
       }
       tc_fence_before();
       __syncwarp();
@@ -475,42 +484,59 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
         if (!ok) break;
         if (!any) {
           if (lane == 0) {
+            mbar_arrive(&x_full[grp]);
             mbar_arrive(&m_ready[grp]);
             mbar_arrive(&p_full[grp]);
           }
           continue;
         }
         tc_fence_after();
-        float s[AF_PAGE];
-        tmem_ld32(lane_addr + grp * 64, s);
-        tmem_ld32(lane_addr + grp * 64 + 32, s + 32);
+        float s[W];
+        tmem_ld32(lane_addr + grp * 64 + part * W, s);
         tmem_wait_ld();
-        const float* ksp = ks_s[BITS == 8 ? jj % SH_EXPS : 0];
-        const float* lvp = lv_s[BITS == 8 ? jj % SH_EXPS : 0];
-        float mx = SH_NONE, mw = SH_NONE;
+        const int fp = BITS == 8 ? jj % SH_EXPS : 0;
+        const float4* ksp = reinterpret_cast<const float4*>(ks_s[fp] + part * W);
+        const float4* lvp = reinterpret_cast<const float4*>(lv_s[fp] + part * W);
+        const float4* vsp = reinterpret_cast<const float4*>(vs_s[fp] + part * W);
         if constexpr (BITS == 8) {
 #pragma unroll
-          for (int c = 0; c < AF_PAGE; c += 4) {
-            const float4 f = *reinterpret_cast<const float4*>(ksp + c);
+          for (int c = 0; c < W; c += 4) {
+            const float4 f = ksp[c / 4];
             s[c] *= cs * f.x, s[c + 1] *= cs * f.y, s[c + 2] *= cs * f.z, s[c + 3] *= cs * f.w;
           }
         } else {
 #pragma unroll
-          for (int c = 0; c < AF_PAGE; ++c) s[c] *= cs;
+          for (int c = 0; c < W; ++c) s[c] *= cs;
         }
         if (a.cap > 0.f) {
 #pragma unroll
-          for (int c = 0; c < AF_PAGE; ++c) s[c] = capl - 2.f * capl * __fdividef(1.f, 1.f + fast_exp2(s[c] * ecap));
+          for (int c = 0; c < W; ++c) s[c] = capl - 2.f * capl * __fdividef(1.f, 1.f + fast_exp2(s[c] * ecap));
         }
+        float m4[4] = {SH_NONE, SH_NONE, SH_NONE, SH_NONE};
 #pragma unroll
-        for (int c = 0; c < AF_PAGE; ++c) mx = fmaxf(mx, s[c]);
+        for (int c = 0; c < W; ++c) m4[c & 3] = fmaxf(m4[c & 3], s[c]);
+        float mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])), mw = SH_NONE;
         if constexpr (BITS == 8) {
+          float w4[4] = {SH_NONE, SH_NONE, SH_NONE, SH_NONE};
 #pragma unroll
-          for (int c = 0; c < AF_PAGE; c += 4) {
-            const float4 f = *reinterpret_cast<const float4*>(lvp + c);
-            mw = fmaxf(mw, fmaxf(fmaxf(s[c] + f.x, s[c + 1] + f.y), fmaxf(s[c + 2] + f.z, s[c + 3] + f.w)));
+          for (int c = 0; c < W; c += 4) {
+            const float4 f = lvp[c / 4];
+            w4[0] = fmaxf(w4[0], s[c] + f.x), w4[1] = fmaxf(w4[1], s[c + 1] + f.y);
+            w4[2] = fmaxf(w4[2], s[c + 2] + f.z), w4[3] = fmaxf(w4[3], s[c + 3] + f.w);
           }
+          mw = fmaxf(fmaxf(w4[0], w4[1]), fmaxf(w4[2], w4[3]));
+          mw_s[grp][part][row] = mw;
         }
+        // the row's maxima over the group's two threads (both have read their scores: P may take the columns)
+        mx_s[grp][part][row] = mx;
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&x_full[grp]);
+        ok = mbar_wait(&x_full[grp], (jj >> 1) & 1, give_up);
+        if (!ok) break;
+        tc_fence_after();
+        mx = fmaxf(mx, mx_s[grp][part ^ 1][row]);
+        if constexpr (BITS == 8) mw = fmaxf(mw, mw_s[grp][part ^ 1][row]);
         // the references after the page before, published by the other group
         float m_prev = SH_NONE, w_prev = SH_NONE;
         if (j > 0) {
@@ -520,11 +546,11 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
           if constexpr (BITS == 8) w_prev = wref_s[grp ^ 1][row];
         }
         const float m_new = mx > m_prev + SH_MOVES ? mx : m_prev;
-        mref_s[grp][row] = m_new;
+        if (part == 0) mref_s[grp][row] = m_new;
         float w_new = m_new;                                // the reference of O
         if constexpr (BITS == 8) {
           w_new = mw > w_prev + SH_MOVES ? mw : w_prev;
-          wref_s[grp][row] = w_new;
+          if (part == 0) wref_s[grp][row] = w_new;
         } else {
           w_prev = m_prev;
         }
@@ -537,29 +563,32 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
           tc_fence_after();
           const float f = fast_exp2(w_prev - w_new);
 #pragma unroll 1
-          for (int c0 = 0; c0 < HD; c0 += 16) {
+          for (int c0 = 0; c0 < HD / 2; c0 += 16) {
             float o[16];
-            tmem_ld16(lane_addr + O_COL + c0, o);
+            tmem_ld16(lane_addr + O_COL + part * (HD / 2) + c0, o);
             tmem_wait_ld();
 #pragma unroll
             for (int c = 0; c < 16; ++c) o[c] *= f;
-            tmem_st16(lane_addr + O_COL + c0, o);
+            tmem_st16(lane_addr + O_COL + part * (HD / 2) + c0, o);
           }
           tmem_wait_st();
         }
         float sum4[4] = {0.f, 0.f, 0.f, 0.f};
-        uint32_t packed[AF_PAGE / 2];
+        uint32_t packed[W / 2];
         if constexpr (BITS == 8) {
+          // (a weight is its probability times 2^ev, brought to the weights' reference; a key more than 2^126 below the row's
+          // largest probability weighs nothing)
+          const float fw = fast_exp2(m_new - w_new + SH_SHIFT);
 #pragma unroll
-          for (int c = 0; c < AF_PAGE; c += 4) {
-            const float4 f = *reinterpret_cast<const float4*>(lvp + c);
-            float p[4];
+          for (int c = 0; c < W; c += 4) {
+            const float4 f = vsp[c / 4];
             const float fv[4] = {f.x, f.y, f.z, f.w};
+            float p[4];
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
               p[e] = fast_exp2(s[c + e] - m_new);
               sum4[e] += p[e];
-              p[e] = fast_exp2(s[c + e] + fv[e] - w_new + SH_SHIFT);
+              p[e] = p[e] * fv[e] * fw;
             }
             const __half2 h0 = __floats2half2_rn(p[0], p[1]), h1 = __floats2half2_rn(p[2], p[3]);
             packed[c / 2] = *reinterpret_cast<const uint32_t*>(&h0);
@@ -567,7 +596,7 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
           }
         } else {
 #pragma unroll
-          for (int c = 0; c < AF_PAGE; c += 2) {
+          for (int c = 0; c < W; c += 2) {
             const __nv_bfloat162 pb = __floats2bfloat162_rn(fast_exp2(s[c] - m_new), fast_exp2(s[c + 1] - m_new));
             sum4[(c >> 1) & 3] += __low2float(pb) + __high2float(pb);      // (of the rounded weights that the product sees)
             packed[c / 2] = *reinterpret_cast<const uint32_t*>(&pb);
@@ -575,7 +604,7 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
         }
         l = l * fast_exp2(m_known - m_new) + ((sum4[0] + sum4[1]) + (sum4[2] + sum4[3]));
         m_known = m_new;
-        tmem_st32(lane_addr + grp * 64, reinterpret_cast<const float*>(packed));
+        tmem_st16(lane_addr + grp * 64 + part * (W / 2), reinterpret_cast<const float*>(packed));
         tmem_wait_st();
         tc_fence_before();
         __syncwarp();
@@ -591,7 +620,7 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
       if (!ok) break;
       tc_fence_after();
       const float m_fin = any ? mref_s[last & 1][row] : 0.f;
-      if (any) l_s[grp][row] = l * fast_exp2(m_known - m_fin);
+      if (any) l_s[quad][row] = l * fast_exp2(m_known - m_fin);
       __syncwarp();
       if (lane == 0) mbar_arrive(&l_full);
       ok = mbar_wait(&l_full, n & 1, give_up);
@@ -600,19 +629,21 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
         float f = 1.f;
         if constexpr (BITS == 8) f = fast_exp2(wref_s[last & 1][row] - SH_SHIFT - m_fin);
 #pragma unroll 1
-        for (int c0 = 0; c0 < HD / 2; c0 += 32) {
-          float o[32];
-          const int col = grp * (HD / 2) + c0;
-          tmem_ld32(lane_addr + O_COL + col, o);
+        for (int c0 = 0; c0 < HD / 4; c0 += 16) {
+          float o[16];
+          const int col = quad * (HD / 4) + c0;
+          tmem_ld16(lane_addr + O_COL + col, o);
           tmem_wait_ld();
           if (live) {
             unsigned char* dst = k_s + row * (HD * 4);
 #pragma unroll
-            for (int c = 0; c < 32; c += 4)
+            for (int c = 0; c < 16; c += 4)
               *reinterpret_cast<float4*>(dst + ((((col + c) >> 2) ^ (row & 7)) << 4)) = make_float4(o[c] * f, o[c + 1] * f, o[c + 2] * f, o[c + 3] * f);
           }
         }
-        if (live && grp == 0) *reinterpret_cast<float2*>(a.part_ml + ((size_t)it.row0 + row) * 2) = make_float2(m_fin, l_s[0][row] + l_s[1][row]);
+        if (live && quad == 0)
+          *reinterpret_cast<float2*>(a.part_ml + ((size_t)it.row0 + row) * 2) =
+              make_float2(m_fin, (l_s[0][row] + l_s[1][row]) + (l_s[2][row] + l_s[3][row]));
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       }
       __syncwarp();
@@ -634,16 +665,16 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
         __syncwarp();
       }
     }
-  } else if (BITS == 8 && warp >= 12) {
+  } else if (BITS == 8 && warp >= 20) {
     // ---- codes to halves.  A page's keys (and values) are 64 rows of HD / 16 pieces of 16 codes; a thread takes PER of them
-    constexpr int P_ROW = HD / 16, PER = AF_PAGE * P_ROW / 256;
-    const int ct = threadIdx.x - 12 * 32;
+    constexpr int P_ROW = HD / 16, PER = AF_PAGE * P_ROW / 128;
+    const int ct = threadIdx.x - 20 * 32;
     int jj = 0, n = 0;
     bool ok = true;
     auto convert = [&](unsigned char* tile, const unsigned char* raw) {
 #pragma unroll
       for (int i = 0; i < PER; ++i) {
-        const int x = ct + i * 256, r = x / P_ROW, p = x - r * P_ROW;
+        const int x = ct + i * 128, r = x / P_ROW, p = x - r * P_ROW;
         const uint4 w = *reinterpret_cast<const uint4*>(raw + x * 16);
         uint4 h[2];
         c8_half4(w.x, h[0].x, h[0].y);
@@ -670,6 +701,7 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
         if (ct < AF_PAGE) {
           ks_s[jj % SH_EXPS][ct] = __uint_as_float((uint32_t)raw[2 * C::CODES + ct] << 23);
           lv_s[jj % SH_EXPS][ct] = (float)((int)raw[2 * C::CODES + AF_PAGE + ct] - 127);
+          vs_s[jj % SH_EXPS][ct] = __uint_as_float((uint32_t)raw[2 * C::CODES + AF_PAGE + ct] << 23);
         }
         convert(k_s + s * C::TILE, raw);
         if (lane == 0) mbar_arrive(&k_full[s]);
