@@ -19,8 +19,9 @@
 //   warps 20..23  8-bit cache only: codes, brought into shared memory as they are by warp 0, to halves in the swizzled operand layout
 // An item's partial results are gathered in the operands' memory and leave as one bulk copy (they are contiguous; 16-byte piece c of
 // row r lies at piece c ^ (r & 7), for the banks' sake).
-// In the 8-bit cache a key's factor multiplies its scores, a value's its weights, whose halves are kept relative to the largest
-// such weight (see attention_decode8.cu; the queries are scaled alike).
+// In the 8-bit cache a key's factor multiplies its scores, a value's (2^ev) its weights.  The one reference of a row is then the largest
+// s + max(ev, -60), so that the halves of the weights keep 2^-20 of the largest as normal numbers; sums and outputs are relative to it
+// less 6.  (Weights of values below 2^-60 * 448 may vanish, and of sums what is below 2^-20 even where values are of 2^110.)
 // Bound by the prefix's bytes up to some 128 rows; then by the products.
 // Every wait on a barrier is bounded in time; one that runs out sets the error word, and the block frees its TMEM and returns.
 #include "airframe_b200.h"
@@ -246,7 +247,10 @@ __global__ void __launch_bounds__(Sh<HD, BITS>::THREADS, 1)
 attn_shared_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, ShArgs a) {
   using C = Sh<HD, BITS>;
   constexpr int SUB = HD / 64, STAGES = C::STAGES;
-  constexpr uint32_t Q_COL = 128, O_COL = 256;       // TMEM columns: S (and P) [0, 64) [64, 128), Q [128, 128 + HD / 2), O [256, 256 + HD)
+  // TMEM columns: S of the two groups [0, 64) [64, 128); where there is room P apart from it, [128, 160) [160, 192), and Q from 192 on (the
+  // next scores are then made while a group's softmax still works); with heads of 256 P takes S's columns and Q is [128, 256); O from 256 on
+  constexpr bool APART = HD <= 128;
+  constexpr uint32_t P_COL = APART ? 128 : 0, P_STEP = APART ? 32 : 64, Q_COL = APART ? 192 : 128, O_COL = 256;
   constexpr uint32_t IDESC_S = sh_idesc(AF_PAGE, BITS == 8, false), IDESC_O = sh_idesc(HD, BITS == 8, true);
   constexpr float LOG2E = 1.4426950408889634f;
   extern __shared__ unsigned char sh_raw[];
@@ -255,11 +259,10 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
   unsigned char* raw_s = v_s + STAGES * C::TILE;     // [stage][codes of keys | of values | exponents of keys | of values]
   __shared__ uint64_t k_full[STAGES], k_empty[STAGES], v_full[STAGES], v_empty[STAGES], s_full[2], p_full[2], pv_done[2], m_ready[2], x_full[2], q_ready,
       l_full, staged, ring_free, raw_full[C::RAW], raw_empty[C::RAW];
-  constexpr int W_ROWS = BITS == 8 ? SH_ROWS : 1, W_PAGES = BITS == 8 ? SH_EXPS : 1;
-  // by group: the references after its page; by group and part: maxima of a page; by thread of a row: sums
+  constexpr int W_PAGES = BITS == 8 ? SH_EXPS : 1;
+  // by group: the reference after its page; by group and part: the maxima of a page; by thread of a row: sums
   __shared__ float mref_s[2][SH_ROWS], mx_s[2][2][SH_ROWS], l_s[4][SH_ROWS];
-  __shared__ float wref_s[2][W_ROWS], mw_s[2][2][W_ROWS];
-  // the keys' factors, the values' exponents, the values' factors
+  // the keys' factors, the values' exponents (no less than -60) and factors
   __shared__ __align__(16) float ks_s[W_PAGES][AF_PAGE], lv_s[W_PAGES][AF_PAGE], vs_s[W_PAGES][AF_PAGE];
   __shared__ uint32_t tmem_base_s;
   __shared__ int give_up_s;
@@ -382,7 +385,8 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
         for (int j = 0; j < it.pages && ok; ++j, ++jj) {
           const int s = jj % STAGES;
           ok = mbar_wait(&k_full[s], (jj / STAGES) & 1, give_up);
-          if (ok && j >= 2) ok = mbar_wait(&pv_done[jj & 1], ((jj - 2) >> 1) & 1, give_up);      // P of two pages before is consumed
+          // the scores of two pages before are in registers (or, in whose columns P lies, P is consumed)
+          if (ok && j >= 2) ok = mbar_wait(APART ? &x_full[jj & 1] : &pv_done[jj & 1], ((jj - 2) >> 1) & 1, give_up);
           if (!ok) break;
           tc_fence_after();
           const uint32_t kt = smem_u32(k_s + s * C::TILE);
@@ -408,7 +412,7 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
           const uint32_t vt = smem_u32(v_s + s * C::TILE);
 #pragma unroll
           for (int kk = 0; kk < AF_PAGE / 16; ++kk)
-            umma_f16_ts(tmem + O_COL, tmem + (jj & 1) * 64 + kk * 8, umma_desc_mn(vt + kk * 2048, 8192), IDESC_O, (j > 0 || kk > 0) ? 1u : 0u);
+            umma_f16_ts(tmem + O_COL, tmem + P_COL + (jj & 1) * P_STEP + kk * 8, umma_desc_mn(vt + kk * 2048, 8192), IDESC_O, (j > 0 || kk > 0) ? 1u : 0u);
           umma_commit(&v_empty[s]);
           umma_commit(&pv_done[jj & 1]);
         }
@@ -428,7 +432,8 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
       const ShItem it = item_of(w);
       const bool live = row < it.rows;
       const bool any = quarter * 32 < it.rows;             // (warps without a row only keep the barriers' count)
-      float cs = a.cap > 0.f ? a.scale : a.scale * LOG2E;
+      float cs = fabsf(a.cap > 0.f ? a.scale : a.scale * LOG2E);        // (a scale's sign goes to the query)
+      const uint32_t sign = a.scale < 0.f ? 0x80008000u : 0u;
       if (any) {
         // ---- a quarter (heads of 64: half, by two threads) of the row's query into TMEM, two elements a column
         const int rr = it.group0 + row, member = rr / group;
@@ -468,6 +473,8 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
                 wd[e] = *reinterpret_cast<const uint32_t*>(&h);
               }
             }
+#pragma unroll
+            for (int e = 0; e < 16; ++e) wd[e] ^= sign;
             tmem_st16(lane_addr + Q_COL + quad * (SHARE / 2) + c0 * 4, reinterpret_cast<const float*>(wd));
           }
           tmem_wait_st();
@@ -483,6 +490,9 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
         ok = mbar_wait(&s_full[grp], (jj >> 1) & 1, give_up);
         if (!ok) break;
         if (!any) {
+          // (not ahead of the group's other warps: their arrivals for the page before belong to the phase before)
+          if (j >= 2) ok = mbar_wait(&p_full[grp], ((jj - 2) >> 1) & 1, give_up);
+          if (!ok) break;
           if (lane == 0) {
             mbar_arrive(&x_full[grp]);
             mbar_arrive(&m_ready[grp]);
@@ -498,36 +508,37 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
         const float4* ksp = reinterpret_cast<const float4*>(ks_s[fp] + part * W);
         const float4* lvp = reinterpret_cast<const float4*>(lv_s[fp] + part * W);
         const float4* vsp = reinterpret_cast<const float4*>(vs_s[fp] + part * W);
+        // scores are s[c] * cx from here on
         if constexpr (BITS == 8) {
 #pragma unroll
           for (int c = 0; c < W; c += 4) {
             const float4 f = ksp[c / 4];
-            s[c] *= cs * f.x, s[c + 1] *= cs * f.y, s[c + 2] *= cs * f.z, s[c + 3] *= cs * f.w;
+            s[c] *= f.x, s[c + 1] *= f.y, s[c + 2] *= f.z, s[c + 3] *= f.w;
           }
-        } else {
-#pragma unroll
-          for (int c = 0; c < W; ++c) s[c] *= cs;
         }
+        float cx = cs;
         if (a.cap > 0.f) {
+          const float ec = ecap * cs;
 #pragma unroll
-          for (int c = 0; c < W; ++c) s[c] = capl - 2.f * capl * __fdividef(1.f, 1.f + fast_exp2(s[c] * ecap));
+          for (int c = 0; c < W; ++c) s[c] = capl - 2.f * capl * __fdividef(1.f, 1.f + fast_exp2(s[c] * ec));
+          cx = 1.f;
         }
         float m4[4] = {SH_NONE, SH_NONE, SH_NONE, SH_NONE};
-#pragma unroll
-        for (int c = 0; c < W; ++c) m4[c & 3] = fmaxf(m4[c & 3], s[c]);
-        float mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])), mw = SH_NONE;
+        float mx;
         if constexpr (BITS == 8) {
-          float w4[4] = {SH_NONE, SH_NONE, SH_NONE, SH_NONE};
 #pragma unroll
           for (int c = 0; c < W; c += 4) {
             const float4 f = lvp[c / 4];
-            w4[0] = fmaxf(w4[0], s[c] + f.x), w4[1] = fmaxf(w4[1], s[c + 1] + f.y);
-            w4[2] = fmaxf(w4[2], s[c + 2] + f.z), w4[3] = fmaxf(w4[3], s[c + 3] + f.w);
+            m4[0] = fmaxf(m4[0], fmaf(s[c], cx, f.x)), m4[1] = fmaxf(m4[1], fmaf(s[c + 1], cx, f.y));
+            m4[2] = fmaxf(m4[2], fmaf(s[c + 2], cx, f.z)), m4[3] = fmaxf(m4[3], fmaf(s[c + 3], cx, f.w));
           }
-          mw = fmaxf(fmaxf(w4[0], w4[1]), fmaxf(w4[2], w4[3]));
-          mw_s[grp][part][row] = mw;
+          mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
+        } else {
+#pragma unroll
+          for (int c = 0; c < W; ++c) m4[c & 3] = fmaxf(m4[c & 3], s[c]);
+          mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * cx;
         }
-        // the row's maxima over the group's two threads (both have read their scores: P may take the columns)
+        // the row's maximum over the group's two threads (both have read their scores: the columns may be written again)
         mx_s[grp][part][row] = mx;
         tc_fence_before();
         __syncwarp();
@@ -536,32 +547,26 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
         if (!ok) break;
         tc_fence_after();
         mx = fmaxf(mx, mx_s[grp][part ^ 1][row]);
-        if constexpr (BITS == 8) mw = fmaxf(mw, mw_s[grp][part ^ 1][row]);
-        // the references after the page before, published by the other group
-        float m_prev = SH_NONE, w_prev = SH_NONE;
+        // the reference after the page before, published by the other group; it moves only when it has to
+        float m_prev = SH_NONE;
         if (j > 0) {
           ok = mbar_wait(&m_ready[grp ^ 1], ((jj - 1) >> 1) & 1, give_up);
           if (!ok) break;
           m_prev = mref_s[grp ^ 1][row];
-          if constexpr (BITS == 8) w_prev = wref_s[grp ^ 1][row];
         }
         const float m_new = mx > m_prev + SH_MOVES ? mx : m_prev;
         if (part == 0) mref_s[grp][row] = m_new;
-        float w_new = m_new;                                // the reference of O
-        if constexpr (BITS == 8) {
-          w_new = mw > w_prev + SH_MOVES ? mw : w_prev;
-          if (part == 0) wref_s[grp][row] = w_new;
-        } else {
-          w_prev = m_prev;
-        }
         __syncwarp();
         if (lane == 0) mbar_arrive(&m_ready[grp]);
-        if (j > 0 && __any_sync(0xffffffffu, w_new != w_prev)) {
+        // the group's P of two pages before is consumed (waited for here: it also pins the phase that the wait below looks at)
+        if (APART && j >= 2) ok = mbar_wait(&pv_done[grp], ((jj - 2) >> 1) & 1, give_up);
+        if (!ok) break;
+        if (j > 0 && __any_sync(0xffffffffu, m_new != m_prev)) {
           // O is rescaled once the product of the page before is complete (the next one waits for this page's P)
           ok = mbar_wait(&pv_done[grp ^ 1], ((jj - 1) >> 1) & 1, give_up);
           if (!ok) break;
           tc_fence_after();
-          const float f = fast_exp2(w_prev - w_new);
+          const float f = fast_exp2(m_prev - m_new);
 #pragma unroll 1
           for (int c0 = 0; c0 < HD / 2; c0 += 16) {
             float o[16];
@@ -576,35 +581,28 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
         float sum4[4] = {0.f, 0.f, 0.f, 0.f};
         uint32_t packed[W / 2];
         if constexpr (BITS == 8) {
-          // (a weight is its probability times 2^ev, brought to the weights' reference; a key more than 2^126 below the row's
-          // largest probability weighs nothing)
-          const float fw = fast_exp2(m_new - w_new + SH_SHIFT);
+          const float ref = m_new - SH_SHIFT;
 #pragma unroll
           for (int c = 0; c < W; c += 4) {
             const float4 f = vsp[c / 4];
-            const float fv[4] = {f.x, f.y, f.z, f.w};
-            float p[4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              p[e] = fast_exp2(s[c + e] - m_new);
-              sum4[e] += p[e];
-              p[e] = p[e] * fv[e] * fw;
-            }
-            const __half2 h0 = __floats2half2_rn(p[0], p[1]), h1 = __floats2half2_rn(p[2], p[3]);
+            const float p0 = fast_exp2(fmaf(s[c], cx, -ref)), p1 = fast_exp2(fmaf(s[c + 1], cx, -ref));
+            const float p2 = fast_exp2(fmaf(s[c + 2], cx, -ref)), p3 = fast_exp2(fmaf(s[c + 3], cx, -ref));
+            sum4[0] += p0, sum4[1] += p1, sum4[2] += p2, sum4[3] += p3;
+            const __half2 h0 = __floats2half2_rn(p0 * f.x, p1 * f.y), h1 = __floats2half2_rn(p2 * f.z, p3 * f.w);
             packed[c / 2] = *reinterpret_cast<const uint32_t*>(&h0);
             packed[c / 2 + 1] = *reinterpret_cast<const uint32_t*>(&h1);
           }
         } else {
 #pragma unroll
           for (int c = 0; c < W; c += 2) {
-            const __nv_bfloat162 pb = __floats2bfloat162_rn(fast_exp2(s[c] - m_new), fast_exp2(s[c + 1] - m_new));
+            const __nv_bfloat162 pb = __floats2bfloat162_rn(fast_exp2(fmaf(s[c], cx, -m_new)), fast_exp2(fmaf(s[c + 1], cx, -m_new)));
             sum4[(c >> 1) & 3] += __low2float(pb) + __high2float(pb);      // (of the rounded weights that the product sees)
             packed[c / 2] = *reinterpret_cast<const uint32_t*>(&pb);
           }
         }
         l = l * fast_exp2(m_known - m_new) + ((sum4[0] + sum4[1]) + (sum4[2] + sum4[3]));
         m_known = m_new;
-        tmem_st16(lane_addr + grp * 64 + part * (W / 2), reinterpret_cast<const float*>(packed));
+        tmem_st16(lane_addr + P_COL + grp * P_STEP + part * (W / 2), reinterpret_cast<const float*>(packed));
         tmem_wait_st();
         tc_fence_before();
         __syncwarp();
@@ -613,7 +611,7 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
       if (!ok) break;
       // ---- the item's partial results
       // (First the page before the last: the group that does not own the last page has not seen that the barrier's phase before is
-      // complete, and a wait one phase ahead returns at once.  Its own page's scores were made after that phase.)
+      // complete, and a wait one phase ahead returns at once.  Of that page's barrier it has, or has waited for a product behind it.)
       const int last = jj - 1;
       ok = it.pages < 2 || mbar_wait(&pv_done[(last - 1) & 1], ((last - 1) >> 1) & 1, give_up);
       ok = ok && mbar_wait(&pv_done[last & 1], (last >> 1) & 1, give_up);
@@ -626,8 +624,6 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
       ok = mbar_wait(&l_full, n & 1, give_up);
       if (!ok) break;
       if (any) {
-        float f = 1.f;
-        if constexpr (BITS == 8) f = fast_exp2(wref_s[last & 1][row] - SH_SHIFT - m_fin);
 #pragma unroll 1
         for (int c0 = 0; c0 < HD / 4; c0 += 16) {
           float o[16];
@@ -638,12 +634,12 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
             unsigned char* dst = k_s + row * (HD * 4);
 #pragma unroll
             for (int c = 0; c < 16; c += 4)
-              *reinterpret_cast<float4*>(dst + ((((col + c) >> 2) ^ (row & 7)) << 4)) = make_float4(o[c] * f, o[c + 1] * f, o[c + 2] * f, o[c + 3] * f);
+              *reinterpret_cast<float4*>(dst + ((((col + c) >> 2) ^ (row & 7)) << 4)) = make_float4(o[c], o[c + 1], o[c + 2], o[c + 3]);
           }
         }
         if (live && quad == 0)
           *reinterpret_cast<float2*>(a.part_ml + ((size_t)it.row0 + row) * 2) =
-              make_float2(m_fin, (l_s[0][row] + l_s[1][row]) + (l_s[2][row] + l_s[3][row]));
+              make_float2(BITS == 8 ? m_fin - SH_SHIFT : m_fin, (l_s[0][row] + l_s[1][row]) + (l_s[2][row] + l_s[3][row]));
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       }
       __syncwarp();
@@ -700,7 +696,7 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
         if (!ok) break;
         if (ct < AF_PAGE) {
           ks_s[jj % SH_EXPS][ct] = __uint_as_float((uint32_t)raw[2 * C::CODES + ct] << 23);
-          lv_s[jj % SH_EXPS][ct] = (float)((int)raw[2 * C::CODES + AF_PAGE + ct] - 127);
+          lv_s[jj % SH_EXPS][ct] = (float)max((int)raw[2 * C::CODES + AF_PAGE + ct] - 127, -60);
           vs_s[jj % SH_EXPS][ct] = __uint_as_float((uint32_t)raw[2 * C::CODES + AF_PAGE + ct] << 23);
         }
         convert(k_s + s * C::TILE, raw);
