@@ -16,7 +16,8 @@
 // passed by more than 2^8.  Products and softmax of neighbouring pages overlap.
 //   warp 0        TMA producer (16-bit cache)         warp 1  issue of S, TMEM allocation      warp 2  issue of O += P V
 //   warps 4..19   queries, softmax, rescaling, partial results
-//   warps 20..23  8-bit cache only: codes, brought into shared memory as they are by warp 0, to halves in the swizzled operand layout
+//   warps 20..23  8-bit cache only: codes, brought into shared memory as they are by warp 0, to halves in the swizzled operand layout;
+//                 warp 3 the rows' factors
 // An item's partial results are gathered in the operands' memory and leave as one bulk copy (they are contiguous; 16-byte piece c of
 // row r lies at piece c ^ (r & 7), for the banks' sake).
 // In the 8-bit cache a key's factor multiplies its scores, a value's (2^ev) its weights.  The one reference of a row is then the largest
@@ -283,7 +284,7 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
   }
   if (threadIdx.x == 0) {
     for (int s = 0; s < STAGES; ++s) {
-      mbar_init(&k_full[s], BITS == 8 ? 4 : 1);      // (one arrival a converting warp)
+      mbar_init(&k_full[s], BITS == 8 ? 5 : 1);      // (one arrival a converting warp, and the factors')
       mbar_init(&k_empty[s], 1);
       mbar_init(&v_full[s], BITS == 8 ? 4 : 1);
       mbar_init(&v_empty[s], 1);
@@ -301,7 +302,7 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
     mbar_init(&ring_free, 1);
     for (int s = 0; s < C::RAW; ++s) {
       mbar_init(&raw_full[s], 1);
-      mbar_init(&raw_empty[s], 4);
+      mbar_init(&raw_empty[s], 5);
     }
     give_up_s = 0;
     mbar_fence_init();
@@ -662,28 +663,31 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
       }
     }
   } else if (BITS == 8 && warp >= 20) {
-    // ---- codes to halves.  A page's keys (and values) are 64 rows of HD / 16 pieces of 16 codes; a thread takes PER of them
+    // ---- codes to halves.  A page's keys (and values) are 64 rows of HD / 16 pieces of 16 codes; a thread takes PER of them, their
+    // codes read before the wait for the operand's place
     constexpr int P_ROW = HD / 16, PER = AF_PAGE * P_ROW / 128;
     const int ct = threadIdx.x - 20 * 32;
     int jj = 0, n = 0;
     bool ok = true;
-    auto convert = [&](unsigned char* tile, const unsigned char* raw) {
+    uint4 w4[PER];
+    auto take = [&](const unsigned char* raw) {
+#pragma unroll
+      for (int i = 0; i < PER; ++i) w4[i] = *reinterpret_cast<const uint4*>(raw + (ct + i * 128) * 16);
+    };
+    auto put = [&](unsigned char* tile) {
 #pragma unroll
       for (int i = 0; i < PER; ++i) {
         const int x = ct + i * 128, r = x / P_ROW, p = x - r * P_ROW;
-        const uint4 w = *reinterpret_cast<const uint4*>(raw + x * 16);
         uint4 h[2];
-        c8_half4(w.x, h[0].x, h[0].y);
-        c8_half4(w.y, h[0].z, h[0].w);
-        c8_half4(w.z, h[1].x, h[1].y);
-        c8_half4(w.w, h[1].z, h[1].w);
+        c8_half4(w4[i].x, h[0].x, h[0].y);
+        c8_half4(w4[i].y, h[0].z, h[0].w);
+        c8_half4(w4[i].z, h[1].x, h[1].y);
+        c8_half4(w4[i].w, h[1].z, h[1].w);
         unsigned char* base = tile + (p >> 2) * 8192 + r * 128;
-        const int c = (p & 3) * 2, first = (p >> 2) & 1;      // (neighbouring sub-tiles begin with the other piece: other banks)
+        const int c = (p & 3) * 2, first = (p >> 2) & 1;        // (neighbouring sub-tiles begin with the other piece: other banks)
         *reinterpret_cast<uint4*>(base + (((c + first) ^ (r & 7)) << 4)) = first ? h[1] : h[0];
         *reinterpret_cast<uint4*>(base + (((c + 1 - first) ^ (r & 7)) << 4)) = first ? h[0] : h[1];
       }
-      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-      __syncwarp();
     };
     for (int w = blockIdx.x; w < n_items && ok; w += gridDim.x, ++n) {
       const ShItem it = item_of(w);
@@ -692,20 +696,49 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
         const int s = jj % STAGES, rs = jj % C::RAW;
         const uint32_t ph = ((jj / STAGES) & 1) ^ 1;
         const unsigned char* raw = raw_s + rs * C::RAW_STAGE;
-        ok = mbar_wait(&raw_full[rs], (jj / C::RAW) & 1, give_up) && mbar_wait(&k_empty[s], ph, give_up);
+        ok = mbar_wait(&raw_full[rs], (jj / C::RAW) & 1, give_up);
         if (!ok) break;
-        if (ct < AF_PAGE) {
-          ks_s[jj % SH_EXPS][ct] = __uint_as_float((uint32_t)raw[2 * C::CODES + ct] << 23);
-          lv_s[jj % SH_EXPS][ct] = (float)max((int)raw[2 * C::CODES + AF_PAGE + ct] - 127, -60);
-          vs_s[jj % SH_EXPS][ct] = __uint_as_float((uint32_t)raw[2 * C::CODES + AF_PAGE + ct] << 23);
+        take(raw);
+        ok = mbar_wait(&k_empty[s], ph, give_up);
+        if (!ok) break;
+        put(k_s + s * C::TILE);
+        take(raw + C::CODES);
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncwarp();
+        if (lane == 0) {
+          mbar_arrive(&k_full[s]);
+          mbar_arrive(&raw_empty[rs]);
         }
-        convert(k_s + s * C::TILE, raw);
-        if (lane == 0) mbar_arrive(&k_full[s]);
         ok = mbar_wait(&v_empty[s], ph, give_up);
         if (!ok) break;
-        convert(v_s + s * C::TILE, raw + C::CODES);
+        put(v_s + s * C::TILE);
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&v_full[s]);
+      }
+    }
+  } else if (BITS == 8 && warp == 3) {
+    // ---- the factors of a page's rows
+    int jj = 0;
+    bool ok = true;
+    for (int w = blockIdx.x; w < n_items && ok; w += gridDim.x) {
+      const ShItem it = item_of(w);
+      for (int j = 0; j < it.pages && ok; ++j, ++jj) {
+        const int s = jj % STAGES, rs = jj % C::RAW;
+        const unsigned char* e = raw_s + rs * C::RAW_STAGE + 2 * C::CODES;
+        // (behind the S of STAGES pages before: SH_EXPS pages before nobody reads factors any more, and the arrival is its phase's)
+        ok = mbar_wait(&raw_full[rs], (jj / C::RAW) & 1, give_up) && mbar_wait(&k_empty[s], ((jj / STAGES) & 1) ^ 1, give_up);
+        if (!ok) break;
+#pragma unroll
+        for (int c = lane; c < AF_PAGE; c += 32) {
+          const uint32_t ke = e[c], ve = e[AF_PAGE + c];
+          ks_s[jj % SH_EXPS][c] = __uint_as_float(ke << 23);
+          vs_s[jj % SH_EXPS][c] = __uint_as_float(ve << 23);
+          lv_s[jj % SH_EXPS][c] = (float)max((int)ve - 127, -60);
+        }
+        __syncwarp();
         if (lane == 0) {
-          mbar_arrive(&v_full[s]);
+          mbar_arrive(&k_full[s]);
           mbar_arrive(&raw_empty[rs]);
         }
       }
