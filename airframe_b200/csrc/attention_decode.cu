@@ -634,25 +634,34 @@ AF_EXPORT long long af_attn_decode_plan_ints(int batch, int nq, int nkv) {
   return da_plan_records_at(batch, units_per_seq) + (long long)sms * DA_PLAN_REC;
 }
 
+// Blocks of af_attn_decode8's split kernel, and integers of its plan.
+AF_EXPORT long long af_attn_decode8_blocks(int, int nq, int nkv) {
+  const int sms = af_sm_count();
+  return sms <= 0 || nq <= 0 || nkv <= 0 || nq % nkv ? 0 : d8_blocks(sms, nq, nkv);
+}
+AF_EXPORT long long af_attn_decode8_plan_ints(int batch, int nq, int nkv) {
+  const long long n = af_attn_decode_plan_ints(batch, nq, nkv);
+  return n <= 0 ? 0 : n + (long long)(d8_blocks(af_sm_count(), nq, nkv) - af_sm_count()) * DA_PLAN_REC;
+}
+
 // Works out, once for a step, how af_attn_decode cuts the work of the layers that read the same caches the same
 // way (the same slots, lengths, page table, heads, window, ring and n_splits): pass `plan` to each of their calls.
 // It holds for these lengths alone: a step later it is made again.
 static int decode_plan_impl(int* plan, long long plan_ints, const int* page_table, int max_pages, const int* slots, const int* lens,
                             int batch, int nq, int nkv, int window, int keep, int ring_rows, int n_splits, int brk,
-                            cudaStream_t stream) {
+                            int blocks, cudaStream_t stream) {
   if (batch == 0) return 0;
   AF_REQUIRE(nq > 0 && nkv > 0 && nq % nkv == 0, "af_attn_decode_plan: heads %d, groups %d", nq, nkv);
-  AF_REQUIRE(plan != nullptr && ((uintptr_t)plan & 15) == 0 && plan_ints >= af_attn_decode_plan_ints(batch, nq, nkv),
-             "af_attn_decode_plan: a plan of %lld integers, 16-byte aligned, wanted", af_attn_decode_plan_ints(batch, nq, nkv));
+  AF_REQUIRE(plan != nullptr && ((uintptr_t)plan & 15) == 0 && plan_ints >= af_attn_decode8_plan_ints(batch, nq, nkv) - (long long)(d8_blocks(af_sm_count(), nq, nkv) - blocks) * DA_PLAN_REC,
+             "af_attn_decode_plan: a plan of %lld integers or more, 16-byte aligned, wanted", af_attn_decode_plan_ints(batch, nq, nkv));
   AF_REQUIRE(keep >= 0 && (keep == 0 || window != 0), "af_attn_decode_plan: %d kept tokens with window %d", keep, window);
   AF_REQUIRE(n_splits >= 1 && ring_rows % AF_PAGE == 0, "af_attn_decode_plan: splits %d, ring rows %d", n_splits, ring_rows);
   const int units_per_seq = nkv * ((nq / nkv + 15) / 16);
   AF_REQUIRE(batch <= DA_MAX_BATCH && (long long)batch * (max_pages + 1 + brk) * units_per_seq < (1ll << 31),
              "af_attn_decode_plan: %d sequences of up to %d pages (takes %d sequences)", batch, max_pages, DA_MAX_BATCH);
-  const int sms = af_sm_count();
-  if (sms <= 0) return -1;
+  if (blocks <= 0) return -1;
   af_launch(attn_decode_plan_kernel, dim3(1), dim3(256), (size_t)2 * (batch + 1) * sizeof(int), stream, plan, slots,
-            lens, page_table, max_pages, batch, nq, nkv, window, keep, ring_rows, n_splits, sms, brk);
+            lens, page_table, max_pages, batch, nq, nkv, window, keep, ring_rows, n_splits, blocks, brk);
   AF_CHECK_LAUNCH("af_attn_decode_plan");
 }
 
@@ -660,14 +669,14 @@ AF_EXPORT int af_attn_decode_plan_kept(int* plan, long long plan_ints, const int
                                   const int* slots, const int* lens, int batch, int nq, int nkv, int window,
                                   int keep, int ring_rows, int n_splits, cudaStream_t stream) {
   return decode_plan_impl(plan, plan_ints, page_table, max_pages, slots, lens, batch, nq, nkv, window, keep, ring_rows, n_splits,
-                          DA_BREAK_PAGES, stream);
+                          DA_BREAK_PAGES, af_sm_count(), stream);
 }
 
 // The same for af_attn_decode8 (attention_decode8.cu).
 int af_decode8_plan(int* plan, long long plan_ints, const int* page_table, int max_pages, const int* slots, const int* lens, int batch,
                     int nq, int nkv, int window, int keep, int ring_rows, int n_splits, cudaStream_t stream) {
   return decode_plan_impl(plan, plan_ints, page_table, max_pages, slots, lens, batch, nq, nkv, window, keep, ring_rows, n_splits,
-                          D8_BREAK_PAGES, stream);
+                          D8_BREAK_PAGES, d8_blocks(af_sm_count(), nq, nkv), stream);
 }
 
 // The split pass alone (partial results into `scratch`), each sequence's first shared[b] pages left out.

@@ -34,25 +34,27 @@ constexpr float D8_SHIFT = 6.f;          // weights are kept times 2^6
 
 template <int HD, int NT>
 struct D8 {
-  // Warps that compute (one more brings the pieces in; registers are dealt to four warps at a time): the accumulators of 16 heads
-  // of 256 take 128 registers, those of 8 heads 64 beside 32 of queries.
-  static constexpr int WARPS = HD * NT == 512 ? 7 : (HD * NT == 256 ? 11 : 15), THREADS = (WARPS + 1) * 32;
+  // Warps that compute (one more brings the pieces in) and blocks an SM (d8_blocks).  Groups of up to 8 heads: two blocks of eight warps,
+  // 128 registers a thread (heads of 256: 64 of them accumulators, 32 queries); more heads have twice those: one block.
+  static constexpr int BLOCKS = NT == 1 ? 2 : 1;
+  static constexpr int WARPS = NT == 1 ? 7 : (HD == 256 ? 7 : (HD == 128 ? 11 : 15)), THREADS = (WARPS + 1) * 32;
   // A stage holds a page.  What a warp takes at a time is a piece of it, 8 KB of keys and values: a page's pieces are worked side by
   // side, so that a stage is soon free again and as many bytes are on their way as are being worked.
   static constexpr int KEYS = 4096 / HD, TILES = KEYS / 16;              // keys of a piece, and its tiles of 16 keys
   static constexpr int AT_ONCE = NT == 2 && TILES == 4 ? 2 : TILES;      // tiles of a piece that are worked together
   static constexpr int CODES = AF_PAGE * HD;                             // bytes of a page's keys, and of its values
   static constexpr int SUB = AF_PAGE * 128;                              // bytes of a sub-tile of 128 dims
-  static constexpr int STAGES = HD == 256 ? 6 : (HD == 128 ? 12 : 20);
+  static constexpr int STAGES = (HD == 256 ? 6 : (HD == 128 ? 12 : 20)) / BLOCKS;
   // Barriers of the pages: the producer fills in order, so a page is only on its way when all pages STAGES before it are consumed; a
   // warp's next piece lies at most WARPS / (pieces of a page) + 1 pages behind its last one, and must not meet the barrier of a page
   // that is still on its way.
-  static constexpr int NBAR = 2 * STAGES;
+  static constexpr int NBAR = 2 * STAGES + (HD == 256 ? 2 : 0);
   static constexpr int RING = STAGES * 2 * CODES;
-  static constexpr int EXPS = 32;                                        // pages whose exponents are kept: eight more than stages
-  static constexpr int MERGE = 24 << 10, ROUND = MERGE / (WARPS * HD * 4);       // the merge's buffer, and the rows it takes at a time
+  static constexpr int EXPS = STAGES + 8 <= 16 ? 16 : 32;                // pages whose exponents are kept: eight more than stages
+  static constexpr int MERGE = (24 << 10) / BLOCKS, ROUND = MERGE / (WARPS * HD * 4);       // the merge's buffer, and the rows it takes at a time
   static constexpr int SMEM = RING + MERGE + EXPS * 2 * AF_PAGE + 1024;
-  static_assert(NBAR >= STAGES + WARPS * TILES / 4 + 2 && EXPS >= STAGES + 8 && ROUND >= 1, "barriers and buffers");
+  static_assert(NBAR >= STAGES + WARPS * TILES / 4 + 2 && EXPS >= STAGES + 8 && NBAR >= 8 && ROUND >= 1, "barriers and buffers");
+  static_assert(BLOCKS * (SMEM + 2304) <= 228 * 1024, "blocks an SM");
 };
 
 struct Decode8Args {
@@ -286,7 +288,7 @@ struct D8Segment {
 };
 
 template <int HD, int NT>
-__global__ void __launch_bounds__(D8<HD, NT>::THREADS, 1)
+__global__ void __launch_bounds__(D8<HD, NT>::THREADS, D8<HD, NT>::BLOCKS)
 decode8_split_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, Decode8Args a) {
   using C = D8<HD, NT>;
   constexpr int STAGES = C::STAGES, WARPS = C::WARPS, NBAR = C::NBAR, SEGS = 4;
@@ -399,8 +401,8 @@ decode8_split_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
         m = min(m, sg.n_pages - i0);
         const int here = id;
         bool late = !waited && is_last(i0 + m - 1);
-        const int at = stage + mine, my_stage = at >= 2 * STAGES ? at - 2 * STAGES : (at >= STAGES ? at - STAGES : at);
-        const uint32_t my_phase = (at >= 2 * STAGES ? phase : (at >= STAGES ? phase ^ 1 : phase)) ^ 1;
+        const int my_stage = (stage + mine) % STAGES;
+        const uint32_t my_phase = phase ^ (uint32_t)((stage + mine) / STAGES & 1) ^ 1;
         const int my_bar = bar + mine >= NBAR ? bar + mine - NBAR : bar + mine;
         int done = 0;
         while (done < m) {
@@ -434,9 +436,7 @@ decode8_split_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
             done = upto;
           } else if (done < most) {
             // nothing is free: the page's wait, bounded in time (every lane the same barrier)
-            const int w = stage + done;
-            ok = mbar_wait(&empty[w >= 2 * STAGES ? w - 2 * STAGES : (w >= STAGES ? w - STAGES : w)],
-                           (w >= 2 * STAGES ? phase : (w >= STAGES ? phase ^ 1 : phase)) ^ 1, give_up);
+            ok = mbar_wait(&empty[(stage + done) % STAGES], phase ^ (uint32_t)((stage + done) / STAGES & 1) ^ 1, give_up);
             ok = __all_sync(0xffffffffu, ok);
             if (!ok) break;
           }
@@ -689,17 +689,18 @@ int af_decode8_split(const void* q, long long q_stride, const void* k, const voi
   if (rc) return rc;
   const int sms = af_sm_count();
   if (sms <= 0) return -1;
+  const int blocks = d8_blocks(sms, nq, nkv);
   Decode8Args a{(const __nv_bfloat16*)q, q_stride, (const uint8_t*)k_exp, (const uint8_t*)v_exp, n_pages, page_table, slots, lens, shared, plan,
                 max_pages, nq, nkv, scale, cap, window, keep, ring_rows, n_splits, batch, scratch,
                 scratch + (size_t)batch * nq * n_splits * hd, err};
   if (group <= 8) {
-    if (hd == 64) return launch_decode8<64, 1>(mk, mv, a, sms, stream);
-    if (hd == 128) return launch_decode8<128, 1>(mk, mv, a, sms, stream);
-    return launch_decode8<256, 1>(mk, mv, a, sms, stream);
+    if (hd == 64) return launch_decode8<64, 1>(mk, mv, a, blocks, stream);
+    if (hd == 128) return launch_decode8<128, 1>(mk, mv, a, blocks, stream);
+    return launch_decode8<256, 1>(mk, mv, a, blocks, stream);
   }
-  if (hd == 64) return launch_decode8<64, 2>(mk, mv, a, sms, stream);
-  if (hd == 128) return launch_decode8<128, 2>(mk, mv, a, sms, stream);
-  return launch_decode8<256, 2>(mk, mv, a, sms, stream);
+  if (hd == 64) return launch_decode8<64, 2>(mk, mv, a, blocks, stream);
+  if (hd == 128) return launch_decode8<128, 2>(mk, mv, a, blocks, stream);
+  return launch_decode8<256, 2>(mk, mv, a, blocks, stream);
 }
 
 // What af_attn_decode8 is given, as one block of 64-bit words.

@@ -86,7 +86,7 @@ __device__ __forceinline__ int sh_items(int pages, int units, int rows, int hd, 
 // pages than a row claims are taken where another of the group shares fewer, and never the page of its new token.
 __global__ void __launch_bounds__(512)
 attn_shared_plan_kernel(int* plan, const int* lead, const int* pages, const int* slots, const int* lens, const int* page_table, int max_pages,
-                        int batch, int nq, int nkv, int hd, int blocks, int own_room, int brk) {
+                        int batch, int nq, int nkv, int hd, int blocks, int own_room, int own_blocks, int brk) {
   extern __shared__ int sp_smem[];
   int* gid = sp_smem;                  // [batch] the row's group, -1: none
   int* cnt = gid + batch;              // [batch] by group: members
@@ -191,7 +191,7 @@ attn_shared_plan_kernel(int* plan, const int* lead, const int* pages, const int*
     }
   }
   __syncthreads();
-  da_write_plan(plan + sh_own_plan(L), slots, lens, page_table, max_pages, batch, nq, nkv, 0, 0, 0, own_room, blocks, plan + L.shared, brk,
+  da_write_plan(plan + sh_own_plan(L), slots, lens, page_table, max_pages, batch, nq, nkv, 0, 0, 0, own_room, own_blocks, plan + L.shared, brk,
                 parts + batch);
 }
 
@@ -860,12 +860,15 @@ int launch_shared(const ShArgs& a, const void* k, const void* v, int blocks, cud
 
 }  // namespace
 
+// (attention_decode.cu)
+extern "C" long long af_attn_decode8_plan_ints(int batch, int nq, int nkv);
+
 // 32-bit integers of the two plans of a shared step (the prefix kernel's, then the split kernel's), 0 where the sizes are refused.
 AF_EXPORT long long af_attn_shared_plan_ints(int batch, int nq, int nkv) {
   if (batch <= 0 || batch > SH_MAX_BATCH || nq <= 0 || nkv <= 0 || nq % nkv) return 0;
   const int sms = af_sm_count();
   if (sms <= 0) return 0;
-  return sh_own_plan(sh_layout(batch, nq, nkv, sms)) + af_attn_decode_plan_ints(batch, nq, nkv);
+  return sh_own_plan(sh_layout(batch, nq, nkv, sms)) + af_attn_decode8_plan_ints(batch, nq, nkv);
 }
 
 // The most partial rows that the prefix kernel leaves (see af_attn_decode_shared).
@@ -896,7 +899,7 @@ static int shared_plans(int* plan, long long plan_ints, const int* lead, const i
   AF_REQUIRE((long long)batch * (max_pages + 1 + brk) * units_per_seq < (1ll << 31), "af_attn_decode_shared: %d sequences of up to %d pages", batch,
              max_pages);
   af_launch(attn_shared_plan_kernel, dim3(1), dim3(512), smem, stream, plan, lead, pages, slots, lens, page_table, max_pages, batch, nq, nkv, hd,
-            sms, n_splits, brk);
+            sms, n_splits, bits == 8 ? d8_blocks(sms, nq, nkv) : sms, brk);
   AF_CHECK_LAUNCH("af_attn_decode_shared (plan)");
 }
 

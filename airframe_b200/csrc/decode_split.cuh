@@ -66,6 +66,8 @@ __device__ __forceinline__ int da_even_splits(int P, int share, int room, int ho
 constexpr int DA_BREAK_PAGES = 2;
 // The same for the 8-bit cache, whose pages take half as long.
 constexpr int D8_BREAK_PAGES = 4;
+// Blocks of the 8-bit split kernel: two an SM (a block's end of a unit then falls into the other's work) where their registers fit.
+inline int d8_blocks(int sms, int nq, int nkv) { return nq / nkv <= 8 ? 2 * sms : sms; }
 __device__ __forceinline__ int da_plan_mark(int blocks, int brk) { return blocks | (brk << 16); }
 
 struct DaPlan {

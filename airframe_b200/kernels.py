@@ -1104,14 +1104,14 @@ def attn_decode8(out, q, kv, batch, nq: int, nkv: int, hd: int, scale: float, ca
     dev = _here("attn_decode8", out, q, table, slots, lens, kv.k, kv.v, kv.k_exp, kv.v_exp, *(() if sinks is None else (sinks,)))
     if B == 0:
         return
-    n = attn_decode_max_splits(B, nkv, batch.max_len_after, window, nq=nq, keep=keep)
+    n = attn_decode_max_splits(B, nkv, batch.max_len_after, window, _plan_ints("af_attn_decode8_blocks", 1, nq, nkv), nq, keep)
     # the plan of the step, made in front of its first layer's attention and shared by the layers that read alike
     aux = getattr(batch, "aux", None)
     key = ("attn_decode8_plan", table.data_ptr(), kv.ring_rows, nq, nkv, window, keep, n)
     plan = aux.get(key) if aux is not None else None
     ints = 0
     if plan is None:
-        ints = _plan_ints("af_attn_decode_plan_ints", B, nq, nkv)
+        ints = _plan_ints("af_attn_decode8_plan_ints", B, nq, nkv)
         plan = torch.empty(ints, dtype=torch.int32, device=q.device)
         if aux is not None:
             aux[key] = plan
@@ -1157,7 +1157,7 @@ def attn_decode_shared(out, q, kv, batch, nq: int, nkv: int, hd: int, scale: flo
                 *(() if sinks is None else (sinks,)))
     if B == 0:
         return
-    n = attn_decode_max_splits(B, nkv, batch.max_len_after, 0, nq=nq)
+    n = attn_decode_max_splits(B, nkv, batch.max_len_after, 0, _plan_ints("af_attn_decode8_blocks", 1, nq, nkv) if eight else 0, nq)
     aux = getattr(batch, "aux", None)
     key = ("attn_shared_plan", table.data_ptr(), nq, nkv, n, eight, lead.data_ptr(), pages.data_ptr())
     plan = aux.get(key) if aux is not None else None
