@@ -38,22 +38,23 @@ struct D8 {
   // 128 registers a thread (heads of 256: 64 of them accumulators, 32 queries); more heads have twice those: one block.
   static constexpr int BLOCKS = NT == 1 ? 2 : 1;
   static constexpr int WARPS = NT == 1 ? 7 : (HD == 256 ? 7 : (HD == 128 ? 11 : 15)), THREADS = (WARPS + 1) * 32;
-  // A stage holds a page.  What a warp takes at a time is a piece of it, 8 KB of keys and values: a page's pieces are worked side by
-  // side, so that a stage is soon free again and as many bytes are on their way as are being worked.
+  // A stage holds a page (heads of 256: half of one).  What a warp takes at a time is a piece of it, 8 KB of keys and values: a
+  // stage's pieces are worked side by side, so that it is soon free again and as many bytes are on their way as are being worked.
+  static constexpr int ROWS = HD == 256 ? 32 : 64, PER_PAGE = AF_PAGE / ROWS, STAGE_TILES = ROWS / 16;
   static constexpr int KEYS = 4096 / HD, TILES = KEYS / 16;              // keys of a piece, and its tiles of 16 keys
   static constexpr int AT_ONCE = NT == 2 && TILES == 4 ? 2 : TILES;      // tiles of a piece that are worked together
-  static constexpr int CODES = AF_PAGE * HD;                             // bytes of a page's keys, and of its values
-  static constexpr int SUB = AF_PAGE * 128;                              // bytes of a sub-tile of 128 dims
-  static constexpr int STAGES = (HD == 256 ? 6 : (HD == 128 ? 12 : 20)) / BLOCKS;
-  // Barriers of the pages: the producer fills in order, so a page is only on its way when all pages STAGES before it are consumed; a
-  // warp's next piece lies at most WARPS / (pieces of a page) + 1 pages behind its last one, and must not meet the barrier of a page
+  static constexpr int CODES = ROWS * HD;                                // bytes of a stage's keys, and of its values
+  static constexpr int SUB = ROWS * 128;                                 // bytes of a sub-tile of 128 dims
+  static constexpr int STAGES = (HD == 64 ? 20 : 12) / BLOCKS;
+  // Barriers of the stages' fillings: the producer fills in order, so one is only on its way when all STAGES before it are consumed; a
+  // warp's next piece lies at most WARPS / (pieces of a stage) + 1 fillings behind its last one, and must not meet the barrier of one
   // that is still on its way.
-  static constexpr int NBAR = 2 * STAGES + (HD == 256 ? 2 : 0);
+  static constexpr int NBAR = 2 * STAGES;
   static constexpr int RING = STAGES * 2 * CODES;
-  static constexpr int EXPS = STAGES + 8 <= 16 ? 16 : 32;                // pages whose exponents are kept: eight more than stages
+  static constexpr int EXPS = STAGES + 8 <= 16 ? 16 : 32;                // fillings whose exponents are kept: eight more than stages
   static constexpr int MERGE = (24 << 10) / BLOCKS, ROUND = MERGE / (WARPS * HD * 4);       // the merge's buffer, and the rows it takes at a time
-  static constexpr int SMEM = RING + MERGE + EXPS * 2 * AF_PAGE + 1024;
-  static_assert(NBAR >= STAGES + WARPS * TILES / 4 + 2 && EXPS >= STAGES + 8 && NBAR >= 8 && ROUND >= 1, "barriers and buffers");
+  static constexpr int SMEM = RING + MERGE + EXPS * 2 * ROWS + 1024;
+  static_assert(NBAR >= STAGES + WARPS * TILES / STAGE_TILES + 2 && EXPS >= STAGES + 8 && NBAR >= 8 && ROUND >= 1, "barriers and buffers");
   static_assert(BLOCKS * (SMEM + 2304) <= 228 * 1024, "blocks an SM");
 };
 
@@ -110,7 +111,7 @@ __device__ __forceinline__ bool d8_is_complete(uint64_t* bar, uint32_t parity) {
       : "memory");
   return ok != 0;
 }
-// All of a page's codes, keys or values: rows [row, row + 64) of every sub-tile of 128 dims (see d8_map).
+// All of a stage's codes, keys or values: its rows, from `row` on, of every sub-tile of 128 dims (see d8_map).
 __device__ __forceinline__ void d8_load(void* dst, const CUtensorMap* map, int row, uint64_t* bar, uint64_t policy) {
   asm volatile(
       "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes.L2::cache_hint [%0], [%1, {%3, %4, %3}], [%2], %5;" ::"r"(
@@ -119,12 +120,12 @@ __device__ __forceinline__ void d8_load(void* dst, const CUtensorMap* map, int r
       : "memory");
 }
 
-// S^T, softmax and O^T of N tiles of 16 keys, beginning with tile `t0` of a page.
+// S^T, softmax and O^T of N tiles of 16 keys, beginning with tile `t0` of a stage.
 template <int HD, int NT, int N>
 struct D8Step {
   using C = D8<HD, NT>;
-  // k_l, v_l, ke_l: this lane's addresses of the page's keys, values and exponents (tile 0); lo, hi, keep: the visible keys, counted
-  // from the page's first
+  // k_l, v_l, ke_l: this lane's addresses of the stage's keys, values and exponents (tile 0); lo, hi, keep: the visible keys, counted
+  // from the stage's first
   __device__ static __forceinline__ void run(uint32_t k_l, uint32_t v_l, uint32_t ke_l, int t0, bool whole, int lo, int hi, int keep,
                                              int g, int t, bool capped, float ecap, float capl, const uint32_t (&qf)[NT][HD / 16][2],
                                              const float (&cq)[NT][2], float (&o)[HD / 16][NT][4], float (&rs)[NT][2], float (&ra)[NT][2],
@@ -165,7 +166,7 @@ struct D8Step {
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         ks[h] = __uint_as_float((uint32_t)d8_lds_u8(ke_l + i * 16 + 8 * h) << 23);
-        lv[h] = (float)(d8_lds_u8(ke_l + AF_PAGE + i * 16 + 8 * h) - 127);
+        lv[h] = (float)(d8_lds_u8(ke_l + C::ROWS + i * 16 + 8 * h) - 127);
       }
 #pragma unroll
       for (int n = 0; n < NT; ++n)
@@ -291,13 +292,13 @@ template <int HD, int NT>
 __global__ void __launch_bounds__(D8<HD, NT>::THREADS, D8<HD, NT>::BLOCKS)
 decode8_split_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, Decode8Args a) {
   using C = D8<HD, NT>;
-  constexpr int STAGES = C::STAGES, WARPS = C::WARPS, NBAR = C::NBAR, SEGS = 4;
+  constexpr int STAGES = C::STAGES, WARPS = C::WARPS, NBAR = C::NBAR, PER = C::PER_PAGE, SEGS = 4;
   constexpr int ROWS = 8 * NT;
   constexpr float LOG2E = 1.4426950408889634f;
   extern __shared__ unsigned char d8_raw[];
   unsigned char* ring = (unsigned char*)(((uintptr_t)d8_raw + 1023) & ~(uintptr_t)1023);
   float* o_s = reinterpret_cast<float*>(ring + C::RING);       // the merge's buffer: [warp][row of the round][HD]
-  unsigned char* exps = ring + C::RING + C::MERGE;             // [page modulo EXPS][k exponents | v exponents]
+  unsigned char* exps = ring + C::RING + C::MERGE;             // [filling modulo EXPS][k exponents | v exponents]
   __shared__ uint64_t full[NBAR], empty[STAGES], seg_full[SEGS], seg_empty[SEGS];
   __shared__ D8Segment seg_s[SEGS];
   __shared__ float rs_s[WARPS][ROWS], ra_s[WARPS][ROWS], l_s[WARPS][ROWS];
@@ -314,7 +315,7 @@ decode8_split_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
   const int4 r0 = ld_keep_int4(rec, l2_policy_keep());
   if (warp == 0) {
     for (int s = lane; s < NBAR; s += 32) mbar_init(&full[s], 2);      // (the copies, and the exponents)
-    for (int s = lane; s < STAGES; s += 32) mbar_init(&empty[s], AF_PAGE / 16);
+    for (int s = lane; s < STAGES; s += 32) mbar_init(&empty[s], C::STAGE_TILES);
     if (lane < SEGS) {
       mbar_init(&seg_full[lane], 1);
       mbar_init(&seg_empty[lane], WARPS);
@@ -363,7 +364,7 @@ decode8_split_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
     y = r0.z;
     of_unit(r0.y, y, r1.x, r1.z, r1.w, r3.x);
     bool waited = false;                              // for the kernel in front
-    int ii = 0, stage = 0, bar = 0;                   // pages so far; their stage and barrier
+    int ii = 0, stage = 0, bar = 0;                   // fillings so far; their stage and barrier
     uint32_t phase = 0;
     for (int k = 0;; ++k) {
       sg.more = left > D8_BREAK_PAGES ? 1 : 0;        // (the even cut: one segment)
@@ -376,66 +377,71 @@ decode8_split_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
         asm volatile("prefetch.global.L1 [%0];" ::"l"(a.q + (size_t)sg.b * a.q_stride + (size_t)(sg.row_head0 + lane / (HD / 64)) * HD +
                                                        (lane % (HD / 64)) * 64));
       const int last_pp = sg.pos / AF_PAGE;           // the page of the new token, which the kernel in front wrote
-      // Eight pages at a time (of a block's first segment first the four whose ids are in the plan).  A lane has a quarter (16 bytes)
-      // of a page's exponents, asked for a round ahead, and sends its page's copies off when the stage is free: as many pages as are
-      // free in a row go out at once.  The page of the new token, a segment's last, was written by the kernel in front.
+      // Eight fillings at a time (of a block's first segment first four, whose pages' ids are in the plan).  Four lanes have the filling's
+      // exponents, 16 bytes each, asked for a round ahead; the first of them sends the copies off when the stage is free: as many
+      // fillings as are free in a row go out at once.  The page of the new token, a segment's last, was written by the kernel in front.
       const int quarter = lane & 3, mine = lane >> 2;
+      const bool has = quarter * 16 < C::ROWS;
       uint4 kx = make_uint4(0u, 0u, 0u, 0u), vx = kx;
-      auto is_last = [&](int i) { return da_page_of(sg.kept, sg.skip, sg.x_begin + i) == last_pp; };
-      auto load = [&](int page) {
-        const size_t at = (size_t)(page * a.nkv + sg.kvh) * AF_PAGE + quarter * 16;
-        kx = __ldcg(reinterpret_cast<const uint4*>(a.k_exp + at));
-        vx = __ldcg(reinterpret_cast<const uint4*>(a.v_exp + at));
+      auto is_last = [&](int i) { return da_page_of(sg.kept, sg.skip, sg.x_begin + i / PER) == last_pp; };
+      auto row_of = [&](int i, int page) { return (page * a.nkv + sg.kvh) * AF_PAGE + i % PER * C::ROWS; };
+      auto load = [&](int row) {
+        if (!has) return;
+        kx = __ldcg(reinterpret_cast<const uint4*>(a.k_exp + row + quarter * 16));
+        vx = __ldcg(reinterpret_cast<const uint4*>(a.v_exp + row + quarter * 16));
       };
-      int id = 0;
+      const int n = sg.n_pages * PER;
+      int row = 0;
       auto ask = [&](int i) {
-        if (i < sg.n_pages) {
-          id = k == 0 && i < 4 ? safe(i == 0 ? r2.x : (i == 1 ? r2.y : (i == 2 ? r2.z : r2.w))) : page_id(i);
-          if (waited || !is_last(i)) load(id);
+        if (i < n) {
+          const int p = i / PER;
+          row = row_of(i, k == 0 && p < 4 ? safe(p == 0 ? r2.x : (p == 1 ? r2.y : (p == 2 ? r2.z : r2.w))) : page_id(p));
+          if (waited || !is_last(i)) load(row);
         }
       };
       int m = k == 0 ? 4 : 8;
       if (mine < m) ask(mine);
       bool ok = true;
-      for (int i0 = 0; i0 < sg.n_pages && ok; i0 += m, m = 8) {
-        m = min(m, sg.n_pages - i0);
-        const int here = id;
-        bool late = !waited && is_last(i0 + m - 1);
+      for (int i0 = 0; i0 < n && ok; i0 += m, m = 8) {
+        m = min(m, n - i0);
+        const int here = row;
+        int late = 0;                                 // of the round, what lies in the new token's page
+        if (!waited)
+          while (late < min(m, PER) && is_last(i0 + m - 1 - late)) ++late;
         const int my_stage = (stage + mine) % STAGES;
         const uint32_t my_phase = phase ^ (uint32_t)((stage + mine) / STAGES & 1) ^ 1;
         const int my_bar = bar + mine >= NBAR ? bar + mine - NBAR : bar + mine;
         int done = 0;
         while (done < m) {
-          if (late && done == m - 1) {
+          if (late > 0 && done == m - late) {
             pdl_wait();
             waited = true;
-            late = false;
-            if (mine == done) load(here);
+            if (mine >= done && mine < m) load(here);
+            late = 0;
           }
           __syncwarp();
           const bool open = ii + mine < STAGES || d8_is_complete(&empty[my_stage], my_phase);
-          const int most = late ? m - 1 : m;
+          const int most = m - late;
           const uint32_t shut = __ballot_sync(0xffffffffu, mine >= done && !(open && mine < most));
           const int upto = shut ? (__ffs(shut) - 1) >> 2 : 8;
           if (upto > done) {
             if (quarter == 0 && mine >= done && mine < upto) {
-              const int row = (here * a.nkv + sg.kvh) * AF_PAGE;
               unsigned char* st = ring + (size_t)my_stage * 2 * C::CODES;
               mbar_expect_tx(&full[my_bar], 2 * C::CODES);
-              d8_load(st, &map_k, row, &full[my_bar], read_once);
-              d8_load(st + C::CODES, &map_v, row, &full[my_bar], read_once);
+              d8_load(st, &map_k, here, &full[my_bar], read_once);
+              d8_load(st + C::CODES, &map_v, here, &full[my_bar], read_once);
             }
-            // (and their exponents: the round's later pages may need these pages' stages)
-            if (mine >= done && mine < upto) {
-              uint4* e = reinterpret_cast<uint4*>(exps + ((ii + mine) % C::EXPS) * 2 * AF_PAGE) + quarter;
+            // (and their exponents: the round's later fillings may need these stages)
+            if (has && mine >= done && mine < upto) {
+              uint4* e = reinterpret_cast<uint4*>(exps + ((ii + mine) % C::EXPS) * 2 * C::ROWS) + quarter;
               e[0] = kx;
-              e[AF_PAGE / 16] = vx;
+              e[C::ROWS / 16] = vx;
             }
             __syncwarp();
             if (quarter == 0 && mine >= done && mine < upto) mbar_arrive(&full[my_bar]);
             done = upto;
           } else if (done < most) {
-            // nothing is free: the page's wait, bounded in time (every lane the same barrier)
+            // nothing is free: the stage's wait, bounded in time (every lane the same barrier)
             ok = mbar_wait(&empty[(stage + done) % STAGES], phase ^ (uint32_t)((stage + done) / STAGES & 1) ^ 1, give_up);
             ok = __all_sync(0xffffffffu, ok);
             if (!ok) break;
@@ -495,7 +501,7 @@ decode8_split_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
     const D8Segment sg = seg_s[k % SEGS];
     __syncwarp();
     if (lane == 0) mbar_arrive(&seg_empty[k % SEGS]);
-    const int n = sg.n_pages, n_rows = sg.n_rows, row_head0 = sg.row_head0;
+    const int n = sg.n_pages * PER, n_rows = sg.n_rows, row_head0 = sg.row_head0;
 
     // ---- the queries as B fragments (head g of every tile of 8), halves brought to [2^14, 2^15)
     uint32_t qf[NT][HD / 16][2];
@@ -547,16 +553,16 @@ decode8_split_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
     for (int n8 = 0; n8 < NT; ++n8) rs[n8][0] = rs[n8][1] = ra[n8][0] = ra[n8][1] = D8_NONE, l[n8][0] = l[n8][1] = 0.f;
 
     // A warp takes a piece at a time; where the keys are few, a tile of 16.
-    const int each = n * 4 <= 2 * WARPS ? 1 : C::TILES, items = n * 4 / each;
+    const int each = n * C::STAGE_TILES <= 2 * WARPS ? 1 : C::TILES, items = n * C::STAGE_TILES / each;
     bool ok = true;
     for (int x = warp; x < items; x += WARPS) {
-      const int tile = x * each & 3, i = x * each >> 2, ii = i_base + i, s = ii % STAGES;
+      const int tile = x * each % C::STAGE_TILES, i = x * each / C::STAGE_TILES, ii = i_base + i, s = ii % STAGES;
       ok = mbar_wait(&full[ii % NBAR], (ii / NBAR) & 1, give_up);
       if (!ok) break;
-      const uint32_t st = smem_u32(ring) + s * 2 * C::CODES, e_l = smem_u32(exps) + ii % C::EXPS * 2 * AF_PAGE + pg;
-      const int base = da_page_of(sg.kept, sg.skip, sg.x_begin + i) * AF_PAGE;
+      const uint32_t st = smem_u32(ring) + s * 2 * C::CODES, e_l = smem_u32(exps) + ii % C::EXPS * 2 * C::ROWS + pg;
+      const int base = da_page_of(sg.kept, sg.skip, sg.x_begin + i / PER) * AF_PAGE + i % PER * C::ROWS;
       const int lo = sg.lo - base, hi = sg.pos - base, keep = a.keep - base;       // (visible: [lo, hi] and what is before keep)
-      const bool whole = AF_PAGE - 1 <= hi && (lo <= 0 || AF_PAGE - 1 < keep);
+      const bool whole = C::ROWS - 1 <= hi && (lo <= 0 || C::ROWS - 1 < keep);
       if (C::AT_ONCE > 1 && each == 1) {
         D8Step<HD, NT, 1>::run(st + k_off, st + v_off, e_l, tile, whole, lo, hi, keep, g, t, a.cap > 0.f, ecap, capl, qf, cq, o, rs, ra, l);
       } else {
@@ -630,14 +636,14 @@ decode8_split_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
 }
 
 // Tensor map of the codes: [HD / 128 sub-tiles][rows][128 bytes] (HD 64: one of 64 bytes), the sub-tiles of a row beside one
-// another in memory; boxes of a page's rows in all sub-tiles, swizzled.
+// another in memory; boxes of a stage's rows in all sub-tiles, swizzled.
 int d8_map(CUtensorMap* map, const void* base, long long rows, int hd) {
   AfEncodeTiledFn enc = af_encode_tiled();
   if (enc == nullptr) return af_fail(-1, "the driver has no cuTensorMapEncodeTiled");
   const cuuint32_t width = hd < 128 ? 64u : 128u, subs = (cuuint32_t)hd / width;
   cuuint64_t dims[3] = {width, (cuuint64_t)rows, subs};
   cuuint64_t strides[2] = {(cuuint64_t)hd, width};
-  cuuint32_t box[3] = {width, (cuuint32_t)AF_PAGE, subs};
+  cuuint32_t box[3] = {width, hd == 256 ? 32u : 64u, subs};
   cuuint32_t estr[3] = {1, 1, 1};
   const CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
                          hd < 128 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
