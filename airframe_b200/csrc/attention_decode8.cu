@@ -134,11 +134,13 @@ struct D8Step {
     k_l += t0 * 16 * ROW;
     v_l += t0 * 16 * ROW;
     ke_l += t0 * 16;
-    float sc[N][NT][4], wt[N][NT][4];
+    constexpr int CHAINS = N * NT == 1 ? 2 : 1;            // (a product waits for the one before it in its sum)
+    float sc[N][NT][4], sc2[CHAINS == 2 ? N : 1][NT][4], wt[N][NT][4];
 #pragma unroll
     for (int i = 0; i < N; ++i)
 #pragma unroll
       for (int n = 0; n < NT; ++n) sc[i][n][0] = sc[i][n][1] = sc[i][n][2] = sc[i][n][3] = 0.f;
+    if constexpr (CHAINS == 2) sc2[0][0][0] = sc2[0][0][1] = sc2[0][0][2] = sc2[0][0][3] = 0.f;
     // ---- S^T = K Q^T
 #pragma unroll
     for (int c = 0; c < HD / 64; ++c) {
@@ -153,9 +155,17 @@ struct D8Step {
           c8_half4(xs[j], a0, a2);
           c8_half4(ys[j], a1, a3);
 #pragma unroll
-          for (int n = 0; n < NT; ++n) d8_mma(sc[i][n], a0, a1, a2, a3, qf[n][c * 4 + j][0], qf[n][c * 4 + j][1]);
+          for (int n = 0; n < NT; ++n) d8_mma(CHAINS == 2 && (j & 1) ? sc2[CHAINS == 2 ? i : 0][n] : sc[i][n], a0, a1, a2, a3, qf[n][c * 4 + j][0], qf[n][c * 4 + j][1]);
         }
       }
+    }
+    if constexpr (CHAINS == 2) {
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) sc[i][n][e] += sc2[CHAINS == 2 ? i : 0][n][e];
     }
     // ---- scale, softcap, mask; the weights' exponents; whether a reference moves
     const int kr = t0 * 16 + d8_perm(g);                  // this lane's keys: kr + 16 i, and 8 behind
