@@ -112,10 +112,10 @@ __device__ __forceinline__ uint32_t da_piece(uint32_t tile, int r, int c) {
 __global__ void __launch_bounds__(256)
 attn_decode_plan_kernel(int* __restrict__ plan, const int* __restrict__ slots, const int* __restrict__ lens,
                         const int* __restrict__ page_table, int max_pages, int batch, int nq, int nkv, int window,
-                        int keep, int ring_rows, int room, int grid_blocks, int brk) {
+                        int keep, int ring_rows, int room, int grid_blocks, int brk, bool counts) {
   extern __shared__ int dp_smem[];
   pdl_wait();
-  da_write_plan(plan, slots, lens, page_table, max_pages, batch, nq, nkv, window, keep, ring_rows, room, grid_blocks, nullptr, brk, dp_smem);
+  da_write_plan(plan, slots, lens, page_table, max_pages, batch, nq, nkv, window, keep, ring_rows, room, grid_blocks, nullptr, brk, dp_smem, counts);
 }
 
 // The heads of one kv group are the (up to 16) rows of an m16n8k16 tile; the
@@ -641,7 +641,7 @@ AF_EXPORT long long af_attn_decode8_blocks(int, int nq, int nkv) {
 }
 AF_EXPORT long long af_attn_decode8_plan_ints(int batch, int nq, int nkv) {
   const long long n = af_attn_decode_plan_ints(batch, nq, nkv);
-  return n <= 0 ? 0 : n + (long long)(d8_blocks(af_sm_count(), nq, nkv) - af_sm_count()) * DA_PLAN_REC;
+  return n <= 0 ? 0 : n + (long long)(d8_blocks(af_sm_count(), nq, nkv) - af_sm_count()) * DA_PLAN_REC + (long long)batch * nkv * ((nq / nkv + 15) / 16);
 }
 
 // Works out, once for a step, how af_attn_decode cuts the work of the layers that read the same caches the same
@@ -649,10 +649,10 @@ AF_EXPORT long long af_attn_decode8_plan_ints(int batch, int nq, int nkv) {
 // It holds for these lengths alone: a step later it is made again.
 static int decode_plan_impl(int* plan, long long plan_ints, const int* page_table, int max_pages, const int* slots, const int* lens,
                             int batch, int nq, int nkv, int window, int keep, int ring_rows, int n_splits, int brk,
-                            int blocks, cudaStream_t stream) {
+                            int blocks, bool counts, cudaStream_t stream) {
   if (batch == 0) return 0;
   AF_REQUIRE(nq > 0 && nkv > 0 && nq % nkv == 0, "af_attn_decode_plan: heads %d, groups %d", nq, nkv);
-  AF_REQUIRE(plan != nullptr && ((uintptr_t)plan & 15) == 0 && plan_ints >= af_attn_decode8_plan_ints(batch, nq, nkv) - (long long)(d8_blocks(af_sm_count(), nq, nkv) - blocks) * DA_PLAN_REC,
+  AF_REQUIRE(plan != nullptr && ((uintptr_t)plan & 15) == 0 && plan_ints >= (counts ? af_attn_decode8_plan_ints(batch, nq, nkv) : af_attn_decode_plan_ints(batch, nq, nkv)),
              "af_attn_decode_plan: a plan of %lld integers or more, 16-byte aligned, wanted", af_attn_decode_plan_ints(batch, nq, nkv));
   AF_REQUIRE(keep >= 0 && (keep == 0 || window != 0), "af_attn_decode_plan: %d kept tokens with window %d", keep, window);
   AF_REQUIRE(n_splits >= 1 && ring_rows % AF_PAGE == 0, "af_attn_decode_plan: splits %d, ring rows %d", n_splits, ring_rows);
@@ -661,7 +661,7 @@ static int decode_plan_impl(int* plan, long long plan_ints, const int* page_tabl
              "af_attn_decode_plan: %d sequences of up to %d pages (takes %d sequences)", batch, max_pages, DA_MAX_BATCH);
   if (blocks <= 0) return -1;
   af_launch(attn_decode_plan_kernel, dim3(1), dim3(256), (size_t)2 * (batch + 1) * sizeof(int), stream, plan, slots,
-            lens, page_table, max_pages, batch, nq, nkv, window, keep, ring_rows, n_splits, blocks, brk);
+            lens, page_table, max_pages, batch, nq, nkv, window, keep, ring_rows, n_splits, blocks, brk, counts);
   AF_CHECK_LAUNCH("af_attn_decode_plan");
 }
 
@@ -669,14 +669,14 @@ AF_EXPORT int af_attn_decode_plan_kept(int* plan, long long plan_ints, const int
                                   const int* slots, const int* lens, int batch, int nq, int nkv, int window,
                                   int keep, int ring_rows, int n_splits, cudaStream_t stream) {
   return decode_plan_impl(plan, plan_ints, page_table, max_pages, slots, lens, batch, nq, nkv, window, keep, ring_rows, n_splits,
-                          DA_BREAK_PAGES, af_sm_count(), stream);
+                          DA_BREAK_PAGES, af_sm_count(), false, stream);
 }
 
 // The same for af_attn_decode8 (attention_decode8.cu).
 int af_decode8_plan(int* plan, long long plan_ints, const int* page_table, int max_pages, const int* slots, const int* lens, int batch,
                     int nq, int nkv, int window, int keep, int ring_rows, int n_splits, cudaStream_t stream) {
   return decode_plan_impl(plan, plan_ints, page_table, max_pages, slots, lens, batch, nq, nkv, window, keep, ring_rows, n_splits,
-                          D8_BREAK_PAGES, d8_blocks(af_sm_count(), nq, nkv), stream);
+                          D8_BREAK_PAGES, d8_blocks(af_sm_count(), nq, nkv), true, stream);
 }
 
 // The split pass alone (partial results into `scratch`), each sequence's first shared[b] pages left out.

@@ -14,6 +14,9 @@
 // V (whose fragments pair two keys) a byte permutation of four rows.  P's fragments are transposed by movmatrix.
 //   The key with row r of a tile is r's permuted one (d8_perm), which keeps the 16-byte loads of both free of bank conflicts.
 //
+// The block that brings the last of a unit's splits merges them (a count per unit, which it puts back to zero for the next layer): the
+// others' partial results come out of L2, and no kernel has to start behind this one.  A unit of one split is finished as it is.
+//
 // Numbers.  Halves hold 11 bits (bfloat16: 8) but little range.  A head's query is brought to [2^14, 2^15) by a power of two
 // (exact down to 2^-29 of its largest element; 2^-39 of it is the most that is lost below).  A weight's half holds
 // 2^(s + ev) relative to the largest such sum of the warp's keys so far, times 2^6, which leaves 2^-20 of the largest weight a
@@ -69,6 +72,10 @@ struct Decode8Args {
   int window, keep, ring_rows, n_splits, batch;
   float *part_o, *part_ml;
   int* err;
+  __nv_bfloat16* out;              // null: the partial results are another kernel's to merge
+  long long out_stride;
+  int* counts;
+  const float* sinks;
 };
 
 __device__ __forceinline__ int d8_perm(int r) { return (r >> 1) | ((r & 1) << 2); }
@@ -293,9 +300,24 @@ struct D8Step {
   }
 };
 
+// Four outputs from their sums: v and L relative to 2^ref; a head's sink joins L.
+__device__ __forceinline__ void d8_finish(__nv_bfloat16* dst, float4 v, float ref, float L, const float* sinks, int head) {
+  if (ref == D8_NONE) ref = 0.f;
+  if (sinks != nullptr) {
+    // (the larger of the two is the reference, so that neither passes the range)
+    const float s = sinks[head] * 1.4426950408889634f, M = fmaxf(ref, s), f = fast_exp2(ref - M);
+    L = L * f + fast_exp2(s - M);
+    v.x *= f, v.y *= f, v.z *= f, v.w *= f;
+  }
+  const float inv = L == 0.f ? 0.f : 1.f / L;
+  const __nv_bfloat162 x = __floats2bfloat162_rn(v.x * inv, v.y * inv), y = __floats2bfloat162_rn(v.z * inv, v.w * inv);
+  reinterpret_cast<__nv_bfloat162*>(dst)[0] = x;
+  reinterpret_cast<__nv_bfloat162*>(dst)[1] = y;
+}
+
 // What a segment of a block's work is: some of the pages of one unit.  The producer warp works it out, the others read it.
 struct D8Segment {
-  int b, kvh, row_head0, n_rows, z, n_pages, x_begin, kept, skip, lo, pos, more;
+  int b, y, kvh, row_head0, n_rows, z, n_pages, x_begin, kept, skip, lo, pos, more;
 };
 
 template <int HD, int NT>
@@ -312,7 +334,7 @@ decode8_split_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
   __shared__ uint64_t full[NBAR], empty[STAGES], seg_full[SEGS], seg_empty[SEGS];
   __shared__ D8Segment seg_s[SEGS];
   __shared__ float rs_s[WARPS][ROWS], ra_s[WARPS][ROWS], l_s[WARPS][ROWS];
-  __shared__ int give_up_s;
+  __shared__ int give_up_s, last_s;
   volatile int* give_up = &give_up_s;
 
   pdl_launch_dependents();
@@ -338,8 +360,19 @@ decode8_split_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
     return;
   }
   __syncthreads();
+  // Units without a page give zeros.
+  auto zeros = [&]() {
+    if (a.out == nullptr) return;
+    for (int u = blockIdx.x; u < a.batch * units_per_seq; u += gridDim.x) {
+      if (a.plan[DA_PLAN_HEAD + u] != 0) continue;
+      const int b = u / units_per_seq, y = u - b * units_per_seq, h0 = y / tiles * group + y % tiles * 16, rows = min(16, y / tiles * group + group - h0);
+      for (int i = lane; i < rows * HD / 2; i += 32)
+        reinterpret_cast<uint32_t*>(a.out + (size_t)b * a.out_stride + (size_t)h0 * HD)[i] = 0u;
+    }
+  };
   if (r0.x < 0) {                                     // (no work; a grid without any must not end before the kernel in front)
-    if (blockIdx.x == 0) pdl_wait();
+    pdl_wait();
+    if (warp == WARPS) zeros();
     return;
   }
 
@@ -353,6 +386,7 @@ decode8_split_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
     int y;
     auto of_unit = [&](int b, int y, int p_in, int pos, int slot, int shared) {
       sg.b = b;
+      sg.y = y;
       sg.kvh = y / tiles;
       sg.row_head0 = sg.kvh * group + (y % tiles) * 16;
       sg.n_rows = min(16, sg.kvh * group + group - sg.row_head0);
@@ -481,6 +515,8 @@ decode8_split_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
       grace_period();
       if (a.err) atomicExch(a.err, 1);
     }
+    if (!waited) pdl_wait();
+    zeros();
     return;
   }
 
@@ -598,6 +634,8 @@ decode8_split_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
         const int row = n8 * 8 + 2 * t + h;
         if (g == 0) rs_s[warp][row] = rs[n8][h], ra_s[warp][row] = ra[n8][h], l_s[warp][row] = v;
       }
+    const int unit = sg.b * units_per_seq + sg.y;
+    const int n_parts = a.out != nullptr ? __ldcg(a.plan + DA_PLAN_HEAD + unit) : 0;       // (0: not merged here)
     bool going = true;
     for (int row0 = 0; row0 < n_rows; row0 += C::ROUND) {
       const int R = min(C::ROUND, n_rows - row0);
@@ -635,13 +673,69 @@ decode8_split_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
           L += l_s[w][row] * fast_exp2(rs_s[w][row] - M);
           v.x += x.x * f, v.y += x.y * f, v.z += x.z * f, v.w += x.w * f;
         }
-        const size_t pidx = ((size_t)sg.b * a.nq + row_head0 + row) * a.n_splits + sg.z;
-        *reinterpret_cast<float4*>(a.part_o + pidx * HD + d) = v;
-        if (d == 0) *reinterpret_cast<float2*>(a.part_ml + pidx * 2) = make_float2(M == D8_NONE ? -INFINITY : M, L);
+        if (n_parts == 1) {
+          d8_finish(a.out + (size_t)sg.b * a.out_stride + (size_t)(row_head0 + row) * HD + d, v, M, L, a.sinks, row_head0 + row);
+        } else {
+          const size_t pidx = ((size_t)sg.b * a.nq + row_head0 + row) * a.n_splits + sg.z;
+          *reinterpret_cast<float4*>(a.part_o + pidx * HD + d) = v;
+          if (d == 0) *reinterpret_cast<float2*>(a.part_ml + pidx * 2) = make_float2(M == D8_NONE ? -INFINITY : M, L);
+        }
       }
       if (row0 + C::ROUND < n_rows) all_of(true);      // (the buffer is written again; a segment's first vote does it for the next segment)
     }
-    if (!going || !sg.more) break;
+    if (!going) break;
+    if (n_parts > 1) {
+      // ---- the unit's last split merges them all
+      all_of(true);
+      if (tid == 0) {
+        __threadfence();
+        const int before = atomicAdd(a.counts + unit, 1);
+        last_s = before == n_parts - 1;
+        if (last_s) a.counts[unit] = 0;
+        __threadfence();
+      }
+      all_of(true);
+      if (last_s) {
+        constexpr int MOST = C::MERGE / 8;               // (maximum, sum) pairs that the buffer holds
+        float2* ml_s = reinterpret_cast<float2*>(o_s);
+        const int R = max(1, min(n_rows, MOST / n_parts));
+        for (int row0 = 0; row0 < n_rows; row0 += R) {
+          const int rows = min(R, n_rows - row0);
+          const size_t p0 = ((size_t)sg.b * a.nq + row_head0 + row0) * a.n_splits;
+          for (int i = tid; i < rows * n_parts && i < MOST; i += WARPS * 32) {
+            const int r = i / n_parts;
+            ml_s[i] = __ldcg(reinterpret_cast<const float2*>(a.part_ml) + p0 + (size_t)r * a.n_splits + (i - r * n_parts));
+          }
+          all_of(true);
+          for (int i = tid; i < rows * (HD / 4); i += WARPS * 32) {
+            const int r = i / (HD / 4), d = (i - r * (HD / 4)) * 4;
+            const float2* ml = ml_s + r * n_parts;
+            float M = -INFINITY;
+            for (int x = 0; x < n_parts; ++x) M = fmaxf(M, ml[x].x);
+            const float ref = M == -INFINITY ? 0.f : M;
+            float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+            float L = 0.f;
+            const float* src = a.part_o + (p0 + (size_t)r * a.n_splits) * HD + d;
+            for (int x0 = 0; x0 < n_parts; x0 += 8) {
+              float4 t8[8];
+#pragma unroll
+              for (int u = 0; u < 8; ++u)
+                t8[u] = x0 + u < n_parts ? __ldcg(reinterpret_cast<const float4*>(src + (size_t)(x0 + u) * HD)) : make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+              for (int u = 0; u < 8; ++u) {
+                const float2 m = x0 + u < n_parts ? ml[x0 + u] : make_float2(-INFINITY, 0.f);
+                const float f = fast_exp2(m.x - ref);
+                L += m.y * f;
+                v.x += t8[u].x * f, v.y += t8[u].y * f, v.z += t8[u].z * f, v.w += t8[u].w * f;
+              }
+            }
+            d8_finish(a.out + (size_t)sg.b * a.out_stride + (size_t)(row_head0 + row0 + r) * HD + d, v, ref, L, a.sinks, row_head0 + row0 + r);
+          }
+          all_of(true);
+        }
+      }
+    }
+    if (!sg.more) break;
   }
 }
 
@@ -678,12 +772,13 @@ int launch_decode8(const CUtensorMap& mk, const CUtensorMap& mv, const Decode8Ar
 
 }  // namespace
 
-// The split pass: partial results of every (sequence, head) into `scratch` (af_attn_decode_scratch(...) floats), as the
-// step's `plan` (af_attn_decode_plan_kept, or the shared one) cuts the work.
+// The attention into `out`, or where that is null the split pass alone: partial results of every (sequence, head) in `scratch`
+// (af_attn_decode_scratch(...) floats), as the step's `plan` (af_decode8_plan, or the shared one) cuts the work.
 int af_decode8_split(const void* q, long long q_stride, const void* k, const void* v, const void* k_exp, const void* v_exp,
                      long long n_pages, const int* page_table, int max_pages, const int* slots, const int* lens, const int* shared,
                      int batch, int nq, int nkv, int hd, float scale, float cap, int window, int keep, int ring_rows, int n_splits,
-                     float* scratch, const int* plan, int* err, cudaStream_t stream) {
+                     float* scratch, const int* plan, int* err, cudaStream_t stream, void* out, long long out_stride,
+                     const float* sinks) {
   AF_REQUIRE(nq > 0 && nkv > 0 && nq % nkv == 0, "af_attn_decode8: heads %d, groups %d", nq, nkv);
   AF_REQUIRE(hd == 64 || hd == 128 || hd == 256, "af_attn_decode8: head_dim %d (takes 64, 128, 256)", hd);
   AF_REQUIRE(keep >= 0 && (keep == 0 || window != 0), "af_attn_decode8: %d kept tokens with window %d", keep, window);
@@ -708,7 +803,8 @@ int af_decode8_split(const void* q, long long q_stride, const void* k, const voi
   const int blocks = d8_blocks(sms, nq, nkv);
   Decode8Args a{(const __nv_bfloat16*)q, q_stride, (const uint8_t*)k_exp, (const uint8_t*)v_exp, n_pages, page_table, slots, lens, shared, plan,
                 max_pages, nq, nkv, scale, cap, window, keep, ring_rows, n_splits, batch, scratch,
-                scratch + (size_t)batch * nq * n_splits * hd, err};
+                scratch + (size_t)batch * nq * n_splits * hd, err, (__nv_bfloat16*)out, out_stride,
+                (int*)plan + da_plan_records_at(batch, units_per_seq) + (size_t)blocks * DA_PLAN_REC, sinks};
   if (group <= 8) {
     if (hd == 64) return launch_decode8<64, 1>(mk, mv, a, blocks, stream);
     if (hd == 128) return launch_decode8<128, 1>(mk, mv, a, blocks, stream);
@@ -748,15 +844,7 @@ AF_EXPORT int af_attn_decode8(const AfDecode8* c) {
                                    (int)c->ring_rows, n_splits, c->stream);
     if (rc) return rc;
   }
-  const int rc = af_decode8_split(c->q, c->q_stride, c->k, c->v, c->k_exp, c->v_exp, c->n_pages, page_table, (int)c->max_pages, slots, lens,
-                                  nullptr, batch, nq, nkv, hd, (float)c->scale, (float)c->cap, (int)c->window, (int)c->keep, (int)c->ring_rows,
-                                  n_splits, c->scratch, c->plan, c->err, c->stream);
-  if (rc) return rc;
-  const int sms = af_sm_count();
-  const float* part_ml = c->scratch + (size_t)batch * nq * n_splits * hd;
-  const int threads = n_splits > DA_MERGE_FEW && batch * nq <= 32 ? DA_MERGE_THREADS : (hd < 128 ? hd : 128);
-  const auto merge = hd == 64 ? attn_decode_merge_kernel<64> : (hd == 128 ? attn_decode_merge_kernel<128> : attn_decode_merge_kernel<256>);
-  af_launch(merge, dim3(batch, nq), dim3(threads), 0, c->stream, (__nv_bfloat16*)c->out, c->out_stride, (const float*)c->scratch, part_ml, nq, nkv,
-            n_splits, slots, lens, (int)c->window, (int)c->keep, sms, (const int*)c->plan, (const float*)c->sinks);
-  AF_CHECK_LAUNCH("af_attn_decode8 (merge)");
+  return af_decode8_split(c->q, c->q_stride, c->k, c->v, c->k_exp, c->v_exp, c->n_pages, page_table, (int)c->max_pages, slots, lens, nullptr,
+                          batch, nq, nkv, hd, (float)c->scale, (float)c->cap, (int)c->window, (int)c->keep, (int)c->ring_rows, n_splits,
+                          c->scratch, c->plan, c->err, c->stream, c->out, c->out_stride, (const float*)c->sinks);
 }

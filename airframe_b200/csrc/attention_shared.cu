@@ -33,7 +33,8 @@
 int af_decode8_split(const void* q, long long q_stride, const void* k, const void* v, const void* k_exp, const void* v_exp,
                      long long n_pages, const int* page_table, int max_pages, const int* slots, const int* lens, const int* shared,
                      int batch, int nq, int nkv, int hd, float scale, float cap, int window, int keep, int ring_rows, int n_splits,
-                     float* scratch, const int* plan, int* err, cudaStream_t stream);
+                     float* scratch, const int* plan, int* err, cudaStream_t stream, void* out, long long out_stride,
+                     const float* sinks);
 int af_decode16_split(const void* q, long long q_stride, const void* kcache, const void* vcache, long long n_pages,
                       const int* page_table, int max_pages, const int* slots, const int* lens, const int* shared, int batch, int nq,
                       int nkv, int hd, float scale, float cap, int n_splits, float* scratch, const int* plan, int* err,
@@ -959,7 +960,7 @@ AF_EXPORT int af_attn_decode_shared(const AfShared* c) {
   if (rc) return rc;
   if (eight)
     rc = af_decode8_split(c->q, c->q_stride, c->k, c->v, c->k_exp, c->v_exp, c->n_pages, page_table, max_pages, slots, lens, c->plan + L.shared,
-                          batch, nq, nkv, hd, a.scale, a.cap, 0, 0, 0, n_splits, c->own_scratch, c->plan + at, c->err, c->stream);
+                          batch, nq, nkv, hd, a.scale, a.cap, 0, 0, 0, n_splits, c->own_scratch, c->plan + at, c->err, c->stream, nullptr, 0, nullptr);
   else
     rc = af_decode16_split(c->q, c->q_stride, c->k, c->v, c->n_pages, page_table, max_pages, slots, lens, c->plan + L.shared, batch, nq, nkv, hd,
                            a.scale, a.cap, n_splits, c->own_scratch, c->plan + at, c->err, c->stream);

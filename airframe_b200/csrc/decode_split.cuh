@@ -234,6 +234,7 @@ __device__ __forceinline__ int da_run_splits(int unit0, int P, int share, int br
 //   [8, 8 + sequences*units)  the splits of every unit, for the merge
 //   then 16 a block           n_pages (< 0: no work), b, y, z, p_in, run_left, position of the new token, slot,
 //                             the cache pages of the segment's first four pages, the sequence's pages left to another kernel
+//   then (the 8-bit cache)    a zero for every unit: how many of its splits are there in the layer at hand
 constexpr int DA_PLAN_HEAD = 8;
 constexpr int DA_PLAN_REC = 16;
 
@@ -244,7 +245,7 @@ __host__ __device__ inline long long da_plan_records_at(int batch, int units_per
 // Writes the plan, by a whole block; smem: 2 (batch + 1) integers.
 __device__ __forceinline__ void da_write_plan(int* plan, const int* slots, const int* lens, const int* page_table, int max_pages, int batch,
                                               int nq, int nkv, int window, int keep, int ring_rows, int room, int grid_blocks,
-                                              const int* shared, int brk, int* dp_smem) {
+                                              const int* shared, int brk, int* dp_smem, bool counts = false) {
   int* pages_s = dp_smem;                 // [batch + 1]
   int* splits_s = dp_smem + batch + 1;    // [batch + 1]
   __shared__ DaPlan plan_s;
@@ -272,6 +273,8 @@ __device__ __forceinline__ void da_write_plan(int* plan, const int* slots, const
                                      : da_run_splits(pages_s[b] * units_per_seq + y * width, width - brk, pl.share, brk);
   }
   int* recs = plan + da_plan_records_at(batch, units_per_seq);
+  if (counts)
+    for (int u = threadIdx.x; u < batch * units_per_seq; u += blockDim.x) recs[grid_blocks * DA_PLAN_REC + u] = 0;
   for (int w = threadIdx.x; w < grid_blocks; w += blockDim.x) {
     const DaFirst fs = da_first_segment(pl, pages_s, splits_s, batch, units_per_seq, w);
     int* r = recs + (size_t)w * DA_PLAN_REC;

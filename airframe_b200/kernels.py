@@ -1105,9 +1105,10 @@ def attn_decode8(out, q, kv, batch, nq: int, nkv: int, hd: int, scale: float, ca
     if B == 0:
         return
     n = attn_decode_max_splits(B, nkv, batch.max_len_after, window, _plan_ints("af_attn_decode8_blocks", 1, nq, nkv), nq, keep)
-    # the plan of the step, made in front of its first layer's attention and shared by the layers that read alike
+    # the plan of the step, made in front of its first layer's attention and shared by the layers that read alike, one after the
+    # other on one stream (it counts the parts of a layer's results)
     aux = getattr(batch, "aux", None)
-    key = ("attn_decode8_plan", table.data_ptr(), kv.ring_rows, nq, nkv, window, keep, n)
+    key = ("attn_decode8_plan", _raw_stream(dev), table.data_ptr(), kv.ring_rows, nq, nkv, window, keep, n)
     plan = aux.get(key) if aux is not None else None
     ints = 0
     if plan is None:
@@ -1159,7 +1160,7 @@ def attn_decode_shared(out, q, kv, batch, nq: int, nkv: int, hd: int, scale: flo
         return
     n = attn_decode_max_splits(B, nkv, batch.max_len_after, 0, _plan_ints("af_attn_decode8_blocks", 1, nq, nkv) if eight else 0, nq)
     aux = getattr(batch, "aux", None)
-    key = ("attn_shared_plan", table.data_ptr(), nq, nkv, n, eight, lead.data_ptr(), pages.data_ptr())
+    key = ("attn_shared_plan", _raw_stream(dev), table.data_ptr(), nq, nkv, n, eight, lead.data_ptr(), pages.data_ptr())
     plan = aux.get(key) if aux is not None else None
     ints = 0
     if plan is None:
