@@ -188,7 +188,10 @@ attn_decode_split_kernel(const __grid_constant__ CUtensorMap map_k, const __grid
       if (a.shared != nullptr) shared0 = a.shared[fs.b];
     }
   }
-  if (fs.n_pages < 0) return;                          // (nothing of the block's is in flight yet)
+  if (fs.n_pages < 0) {                                // (nothing of the block's is in flight yet)
+    if (a.shared != nullptr && blockIdx.x == 0) pdl_wait();
+    return;
+  }
   int left = fs.run_left;                              // what the block's run holds behind the segment's unit
   const float cs = a.cap > 0.f ? a.scale / a.cap : a.scale * LOG2E;
   const float cap2 = a.cap * LOG2E;
@@ -285,7 +288,8 @@ attn_decode_split_kernel(const __grid_constant__ CUtensorMap map_k, const __grid
       issued = issue_first(sg, 0, min(STAGES, sg.n_pages), 0, true);
     }
   }
-  pdl_wait();
+  // (with shared pages: behind the prefix kernel, which lets this one start when all before it is complete; it is waited for at the end)
+  if (a.shared == nullptr) pdl_wait();
   while (true) {
     const int b = sg.b, n_pages = sg.n_pages, n_rows = sg.n_rows, row_head0 = sg.row_head0, z = sg.z;
     const int lo = sg.lo, pos = sg.pos;
@@ -486,6 +490,7 @@ attn_decode_split_kernel(const __grid_constant__ CUtensorMap map_k, const __grid
     __syncthreads();       // (the buffer is one of the next segment's stages)
     sg = nx;
   }
+  if (a.shared != nullptr) pdl_wait();
   if (tid == 0 && give_up_s && a.err) atomicExch(a.err, 1);
 }
 

@@ -407,7 +407,7 @@ decode8_split_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
     sg.n_pages = r0.x;
     y = r0.z;
     of_unit(r0.y, y, r1.x, r1.z, r1.w, r3.x);
-    bool waited = false;                              // for the kernel in front
+    bool waited = a.shared != nullptr;                // for the kernel in front (see below)
     int ii = 0, stage = 0, bar = 0;                   // fillings so far; their stage and barrier
     uint32_t phase = 0;
     for (int k = 0;; ++k) {
@@ -515,7 +515,7 @@ decode8_split_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
       grace_period();
       if (a.err) atomicExch(a.err, 1);
     }
-    if (!waited) pdl_wait();
+    if (!waited || a.shared != nullptr) pdl_wait();
     zeros();
     return;
   }
@@ -540,7 +540,8 @@ decode8_split_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
         : "memory");
     return all != 0;
   };
-  pdl_wait();
+  // (behind the prefix kernel all that came before it is complete already: it is waited for at the producer's end alone)
+  if (a.shared == nullptr) pdl_wait();
   int i_base = 0;
   for (int k = 0;; ++k) {
     if (!all_of(mbar_wait(&seg_full[k % SEGS], (k / SEGS) & 1, give_up))) break;

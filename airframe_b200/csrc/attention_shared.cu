@@ -1,7 +1,9 @@
 // Decode attention of sequences that share a prefix (completions of one prompt, requests behind one system prompt): the
 // shared cache pages are read once for all of a group's sequences, and their products are one tensor-core product of many rows.
 //
-// Three kernels behind the step's plan (one small kernel a step for all layers):
+// Three kernels behind the step's plan (one small kernel a step for all layers), the first two of which run side by side where SMs are
+// left: the prefix kernel lets the next one start when its own wait is over, so that all that came before is complete, and the next
+// one waits for it at its end only:
 //   prefix  the rows of a unit are the query heads of one kv head of all members of a group (up to 128 of them, more in several
 //           units); the units' pages are cut into items, one a block; every row leaves (max, sum, output) of each item
 //   rest    the split kernel of the cache at hand over each sequence's own pages (its plan leaves the shared ones out)
@@ -83,7 +85,8 @@ __device__ __forceinline__ int sh_items(int pages, int units, int rows, int hd, 
   return max(1, min(min(pages, pay), (int)min((long long)pages, (long long)pages * blocks / total)));
 }
 
-// One block.  (Like attn_decode_plan_kernel it does not release its dependents early.)  A group is the live rows of one `lead` that share at least a page; alone in it a row keeps its pages.  Fewer
+// Two blocks: the first writes the prefix kernel's plan, the second the split kernel's.  (Like attn_decode_plan_kernel they do not
+// release their dependents early.)  A group is the live rows of one `lead` that share at least a page; alone in it a row keeps its pages.  Fewer
 // pages than a row claims are taken where another of the group shares fewer, and never the page of its new token.
 __global__ void __launch_bounds__(512)
 attn_shared_plan_kernel(int* plan, const int* lead, const int* pages, const int* slots, const int* lens, const int* page_table, int max_pages,
@@ -112,6 +115,14 @@ attn_shared_plan_kernel(int* plan, const int* lead, const int* pages, const int*
     }
   }
   __syncthreads();
+  if (blockIdx.x == 1) {
+    int* shared = unit0;
+    for (int b = tid; b < batch; b += blockDim.x) shared[b] = gid[b] >= 0 && cnt[gid[b]] >= 2 ? few[gid[b]] : 0;
+    __syncthreads();
+    da_write_plan(plan + sh_own_plan(L), slots, lens, page_table, max_pages, batch, nq, nkv, 0, 0, 0, own_room, own_blocks, shared, brk,
+                  parts + batch);
+    return;
+  }
   if (warp == 0) {
     // places of the groups: units first, then (their pages known) items and partial rows
     int units = 0, members = 0;
@@ -191,9 +202,6 @@ attn_shared_plan_kernel(int* plan, const int* lead, const int* pages, const int*
       plan[L.items + 2 * (item0[g] + x) + 1] = x - x / s * s;
     }
   }
-  __syncthreads();
-  da_write_plan(plan + sh_own_plan(L), slots, lens, page_table, max_pages, batch, nq, nkv, 0, 0, 0, own_room, own_blocks, plan + L.shared, brk,
-                parts + batch);
 }
 
 // ---------------------------------------------------------------- the prefix kernel
@@ -270,7 +278,6 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
   __shared__ int give_up_s;
   volatile int* give_up = &give_up_s;
 
-  pdl_launch_dependents();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int group = a.nq / a.nkv;
   const ShPlan L = sh_layout(a.batch, a.nq, a.nkv, (int)gridDim.x);
@@ -430,6 +437,7 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
     int jj = 0, n = 0;
     bool ok = true;
     pdl_wait();
+    pdl_launch_dependents();      // (now, not before: the split kernel behind takes everything in front of this kernel for complete)
     for (int w = blockIdx.x; w < n_items && ok; w += gridDim.x, ++n) {
       const ShItem it = item_of(w);
       const bool live = row < it.rows;
@@ -899,7 +907,7 @@ static int shared_plans(int* plan, long long plan_ints, const int* lead, const i
   const int units_per_seq = nkv * ((nq / nkv + 15) / 16), brk = bits == 8 ? D8_BREAK_PAGES : DA_BREAK_PAGES;
   AF_REQUIRE((long long)batch * (max_pages + 1 + brk) * units_per_seq < (1ll << 31), "af_attn_decode_shared: %d sequences of up to %d pages", batch,
              max_pages);
-  af_launch(attn_shared_plan_kernel, dim3(1), dim3(512), smem, stream, plan, lead, pages, slots, lens, page_table, max_pages, batch, nq, nkv, hd,
+  af_launch(attn_shared_plan_kernel, dim3(2), dim3(512), smem, stream, plan, lead, pages, slots, lens, page_table, max_pages, batch, nq, nkv, hd,
             sms, n_splits, bits == 8 ? d8_blocks(sms, nq, nkv) : sms, brk);
   AF_CHECK_LAUNCH("af_attn_decode_shared (plan)");
 }
