@@ -63,7 +63,7 @@ struct DecodeArgs {
   int window, ring_rows;
   int keep;        // a window's sequence keeps its first `keep` tokens in sight
   int n_splits;    // at most this many splits of a sequence's keys (the stride of the partial results)
-  int batch, n_sms;
+  int batch, n_blocks;
   float* part_o;   // [batch, nq, splits, HD]
   float* part_ml;  // [batch, nq, splits, 2]
   int* err;        // set to 1 when a bounded wait ran out
@@ -520,7 +520,7 @@ int launch_decode(DecodeArgs a, int batch, long long n_pages, bool merges, cudaS
   // (a sequence attends to at most max_pages + 1 pages: a window's first and last page may be the same of the ring)
   AF_REQUIRE(batch <= DA_MAX_BATCH && (long long)batch * (a.max_pages + 1 + DA_BREAK_PAGES) * units_per_seq < (1ll << 31),
              "af_attn_decode: %d sequences of up to %d pages (takes %d sequences)", batch, a.max_pages, DA_MAX_BATCH);
-  const int n_blocks = a.n_sms;   // one block an SM; the blocks work out among themselves which of them work
+  const int n_blocks = a.n_blocks;   // one block an SM; the blocks work out among themselves which of them work
   af_launch(attn_decode_split_kernel<HD>, dim3(n_blocks), dim3(DA_THREADS), smem, stream, mk, mv, a);
   AF_COUNT_LAUNCH("af_attn_decode (split)");
   if (!merges) return 0;
@@ -554,7 +554,7 @@ static int attn_decode_impl(const float* sinks, void* out, long long out_stride,
                              const void* kcache, const void* vcache, long long n_pages, const int* page_table,
                              int max_pages, const int* slots, const int* lens, int batch, int nq, int nkv, int hd,
                              float scale, float cap, int window, int keep, int ring_rows, int n_splits, float* scratch,
-                             const int* plan, int* err, cudaStream_t stream, const int* shared = nullptr, bool merges = true) {
+                             const int* plan, int* err, cudaStream_t stream, const int* shared = nullptr, bool merges = true, int blocks = 0) {
   if (batch == 0) return 0;
   AF_REQUIRE(keep >= 0 && (keep == 0 || window != 0), "af_attn_decode: %d kept tokens with window %d", keep, window);
   AF_REQUIRE(nq > 0 && nkv > 0 && nq % nkv == 0, "af_attn_decode: heads %d, groups %d", nq, nkv);
@@ -582,8 +582,8 @@ static int attn_decode_impl(const float* sinks, void* out, long long out_stride,
   a.keep = keep;
   a.n_splits = n_splits;
   a.batch = batch;
-  a.n_sms = af_sm_count();
-  if (a.n_sms <= 0) return -1;
+  a.n_blocks = blocks > 0 ? blocks : af_sm_count();
+  if (a.n_blocks <= 0) return -1;
   a.part_o = scratch;
   a.part_ml = scratch + (size_t)batch * nq * n_splits * hd;
   a.err = err;
@@ -687,10 +687,10 @@ int af_decode8_plan(int* plan, long long plan_ints, const int* page_table, int m
 // The split pass alone (partial results into `scratch`), each sequence's first shared[b] pages left out.
 int af_decode16_split(const void* q, long long q_stride, const void* kcache, const void* vcache, long long n_pages,
                       const int* page_table, int max_pages, const int* slots, const int* lens, const int* shared, int batch, int nq,
-                      int nkv, int hd, float scale, float cap, int n_splits, float* scratch, const int* plan, int* err,
+                      int nkv, int hd, float scale, float cap, int n_splits, float* scratch, const int* plan, int blocks, int* err,
                       cudaStream_t stream) {
   return attn_decode_impl(nullptr, nullptr, 0, q, q_stride, kcache, vcache, n_pages, page_table, max_pages, slots, lens, batch, nq, nkv, hd,
-                          scale, cap, 0, 0, 0, n_splits, scratch, plan, err, stream, shared, false);
+                          scale, cap, 0, 0, 0, n_splits, scratch, plan, err, stream, shared, false, blocks);
 }
 
 AF_EXPORT int af_attn_decode_plan(int* plan, long long plan_ints, const int* page_table, int max_pages,

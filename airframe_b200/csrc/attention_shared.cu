@@ -39,7 +39,7 @@ int af_decode8_split(const void* q, long long q_stride, const void* k, const voi
                      const float* sinks);
 int af_decode16_split(const void* q, long long q_stride, const void* kcache, const void* vcache, long long n_pages,
                       const int* page_table, int max_pages, const int* slots, const int* lens, const int* shared, int batch, int nq,
-                      int nkv, int hd, float scale, float cap, int n_splits, float* scratch, const int* plan, int* err,
+                      int nkv, int hd, float scale, float cap, int n_splits, float* scratch, const int* plan, int blocks, int* err,
                       cudaStream_t stream);
 
 namespace {
@@ -51,7 +51,7 @@ namespace {
 //   loc    [batch][2]   its group's first unit (-1: none), its place among the group's members
 //   order  [batch]      the groups' members, group after group
 //   units  [n][8]       where its members begin in `order`, members, kv head, tile of 128 rows; pages, items, first partial row, slot
-//   items  [n][2]       unit, part of its pages
+//   items  [n][8]       ShItem: what a block reads with two loads
 constexpr int SH_HEAD = 16, SH_ROWS = 128, SH_MAX_BATCH = DA_MAX_BATCH;
 
 __host__ __device__ inline int sh_max_units(int batch, int nq, int nkv) { return nkv * (batch * (nq / nkv) / SH_ROWS + batch / 2 + 1); }
@@ -64,9 +64,9 @@ __host__ __device__ inline ShPlan sh_layout(int batch, int nq, int nkv, int bloc
   p.shared = SH_HEAD;
   p.loc = p.shared + b4;
   p.order = p.loc + 2 * b4;
-  p.units = p.order + b4;
+  p.units = p.order + b4;       // (all of them multiples of four: read four integers at a time)
   p.items = p.units + 8 * units;
-  p.total = p.items + 2 * (blocks + units);
+  p.total = p.items + 8 * (blocks + units);
   return p;
 }
 
@@ -198,8 +198,11 @@ attn_shared_plan_kernel(int* plan, const int* lead, const int* pages, const int*
       r[4] = few[g], r[5] = s, r[6] = row0[g] + (kvh * rows + tile * SH_ROWS) * s, r[7] = slots[b];
     }
     for (int x = lane; x < u * s; x += 32) {
-      plan[L.items + 2 * (item0[g] + x)] = unit0[g] + x / s;
-      plan[L.items + 2 * (item0[g] + x) + 1] = x - x / s * s;
+      const int unit = x / s, z = x - unit * s, kvh = unit / tiles, tile = unit - kvh * tiles, r = min(SH_ROWS, rows - tile * SH_ROWS);
+      const int first = (int)((long long)z * few[g] / s), end = (int)((long long)(z + 1) * few[g] / s);
+      int4* it = reinterpret_cast<int4*>(plan + L.items + 8 * (item0[g] + x));
+      it[0] = make_int4(r, first, end - first, row0[g] + (kvh * rows + tile * SH_ROWS) * s + z * r);
+      it[1] = make_int4(memb0[g], tile * SH_ROWS, kvh, slots[b]);
     }
   }
 }
@@ -281,8 +284,12 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int group = a.nq / a.nkv;
   const ShPlan L = sh_layout(a.batch, a.nq, a.nkv, (int)gridDim.x);
-  const int n_items = a.plan[0];
-  if (a.plan[2] != a.batch || a.plan[3] != a.nq || a.plan[4] != a.nkv || a.plan[5] != (int)gridDim.x) {
+  const int4 head = *reinterpret_cast<const int4*>(a.plan);
+  // (the block's first item is read beside the head: the plan holds as many places for items as the grid has blocks)
+  const int4 it0 = *reinterpret_cast<const int4*>(a.plan + L.items + 8 * blockIdx.x);
+  const int4 it1 = *reinterpret_cast<const int4*>(a.plan + L.items + 8 * blockIdx.x + 4);
+  const int n_items = head.x;
+  if (head.z != a.batch || head.w != a.nq || a.plan[4] != a.nkv || a.plan[5] != (int)gridDim.x) {
     if (threadIdx.x == 0 && a.err) atomicExch(a.err, 1);      // (a plan made for another launch)
     return;
   }
@@ -325,18 +332,9 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
   const uint32_t tmem = tmem_base_s;
 
   auto item_of = [&](int w) {
-    const int u = a.plan[L.items + 2 * w], z = a.plan[L.items + 2 * w + 1];
-    const int4 x = *reinterpret_cast<const int4*>(a.plan + L.units + 8 * u), y = *reinterpret_cast<const int4*>(a.plan + L.units + 8 * u + 4);
-    ShItem it;
-    it.group0 = x.w * SH_ROWS;                                        // the tile's first row among the group's
-    it.rows = min(SH_ROWS, x.y * group - it.group0);
-    it.first = (int)((long long)z * y.x / y.y);
-    it.pages = (int)((long long)(z + 1) * y.x / y.y) - it.first;
-    it.row0 = y.z + z * it.rows;
-    it.members0 = x.x;
-    it.kvh = x.z;
-    it.slot = y.w;
-    return it;
+    const int4* r = reinterpret_cast<const int4*>(a.plan + L.items + 8 * w);
+    const int4 x = w == (int)blockIdx.x ? it0 : r[0], y = w == (int)blockIdx.x ? it1 : r[1];
+    return ShItem{x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
   };
   auto page_id = [&](const ShItem& it, int j) {
     const int entry = it.first + j;
@@ -869,15 +867,13 @@ int launch_shared(const ShArgs& a, const void* k, const void* v, int blocks, cud
 
 }  // namespace
 
-// (attention_decode.cu)
-extern "C" long long af_attn_decode8_plan_ints(int batch, int nq, int nkv);
 
 // 32-bit integers of the two plans of a shared step (the prefix kernel's, then the split kernel's), 0 where the sizes are refused.
 AF_EXPORT long long af_attn_shared_plan_ints(int batch, int nq, int nkv) {
   if (batch <= 0 || batch > SH_MAX_BATCH || nq <= 0 || nkv <= 0 || nq % nkv) return 0;
   const int sms = af_sm_count();
   if (sms <= 0) return 0;
-  return sh_own_plan(sh_layout(batch, nq, nkv, sms)) + af_attn_decode8_plan_ints(batch, nq, nkv);
+  return sh_own_plan(sh_layout(batch, nq, nkv, sms)) + af_attn_decode_plan_ints(batch, nq, nkv) + (long long)sms * DA_PLAN_REC;      // (own_blocks: 2 sms at most)
 }
 
 // The most partial rows that the prefix kernel leaves (see af_attn_decode_shared).
@@ -888,6 +884,9 @@ AF_EXPORT long long af_attn_shared_rows(int batch, int nq, int nkv) {
   const int rows = batch * (nq / nkv) < SH_ROWS ? batch * (nq / nkv) : SH_ROWS;
   return (long long)rows * sms + (long long)batch * nq;
 }
+
+// Blocks of the split kernel: of the 16-bit cache's two an SM, one after the other: those of SMs that the prefix kernel leaves take more.
+static int own_blocks(long long bits, int sms, int nq, int nkv) { return bits == 8 ? d8_blocks(sms, nq, nkv) : 2 * sms; }
 
 // The plans of a step: row b's first pages[b] cache pages are those of row lead[b].
 static int shared_plans(int* plan, long long plan_ints, const int* lead, const int* pages, const int* page_table, int max_pages,
@@ -908,7 +907,7 @@ static int shared_plans(int* plan, long long plan_ints, const int* lead, const i
   AF_REQUIRE((long long)batch * (max_pages + 1 + brk) * units_per_seq < (1ll << 31), "af_attn_decode_shared: %d sequences of up to %d pages", batch,
              max_pages);
   af_launch(attn_shared_plan_kernel, dim3(2), dim3(512), smem, stream, plan, lead, pages, slots, lens, page_table, max_pages, batch, nq, nkv, hd,
-            sms, n_splits, bits == 8 ? d8_blocks(sms, nq, nkv) : sms, brk);
+            sms, n_splits, own_blocks(bits, sms, nq, nkv), brk);
   AF_CHECK_LAUNCH("af_attn_decode_shared (plan)");
 }
 
@@ -971,7 +970,7 @@ AF_EXPORT int af_attn_decode_shared(const AfShared* c) {
                           batch, nq, nkv, hd, a.scale, a.cap, 0, 0, 0, n_splits, c->own_scratch, c->plan + at, c->err, c->stream, nullptr, 0, nullptr);
   else
     rc = af_decode16_split(c->q, c->q_stride, c->k, c->v, c->n_pages, page_table, max_pages, slots, lens, c->plan + L.shared, batch, nq, nkv, hd,
-                           a.scale, a.cap, n_splits, c->own_scratch, c->plan + at, c->err, c->stream);
+                           a.scale, a.cap, n_splits, c->own_scratch, c->plan + at, own_blocks(16, sms, nq, nkv), c->err, c->stream);
   if (rc) return rc;
   const auto merge = hd == 64 ? attn_shared_merge_kernel<64> : (hd == 128 ? attn_shared_merge_kernel<128> : attn_shared_merge_kernel<256>);
   af_launch(merge, dim3(batch, nq), dim3(SHM_THREADS), 0, c->stream, (__nv_bfloat16*)c->out, c->out_stride, (const float*)a.part_o,

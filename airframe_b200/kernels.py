@@ -1158,7 +1158,7 @@ def attn_decode_shared(out, q, kv, batch, nq: int, nkv: int, hd: int, scale: flo
                 *(() if sinks is None else (sinks,)))
     if B == 0:
         return
-    n = attn_decode_max_splits(B, nkv, batch.max_len_after, 0, _plan_ints("af_attn_decode8_blocks", 1, nq, nkv) if eight else 0, nq)
+    n = attn_decode_max_splits(B, nkv, batch.max_len_after, 0, _plan_ints("af_attn_decode8_blocks", 1, nq, nkv) if eight else 2 * sm_count(), nq)
     aux = getattr(batch, "aux", None)
     key = ("attn_shared_plan", _raw_stream(dev), table.data_ptr(), nq, nkv, n, eight, lead.data_ptr(), pages.data_ptr())
     plan = aux.get(key) if aux is not None else None
