@@ -216,7 +216,8 @@ constexpr int SH_EXPS = 16;              // (8 bits) pages whose factors are kep
 
 template <int HD, int BITS>
 struct Sh {
-  static constexpr int WARPS = BITS == 8 ? 24 : 20, THREADS = WARPS * 32;
+  static constexpr int CONV = BITS == 16 ? 0 : (HD == 256 ? 8 : 4);           // warps that convert: four keys and four values, or four both
+  static constexpr int WARPS = 20 + CONV, THREADS = WARPS * 32;
   static constexpr int TILE = AF_PAGE * HD * 2;                              // bytes of a page's keys, or values, as operand
   // pages in flight (16 bits), or converted (8 bits; beside them RAW pages of codes are in flight)
   static constexpr int STAGES = BITS == 16 ? (HD == 256 ? 3 : (HD == 128 ? 6 : 8)) : (HD == 256 ? 2 : (HD == 128 ? 4 : 6));
@@ -263,7 +264,7 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
   // TMEM columns: S of the two groups [0, 64) [64, 128); where there is room P apart from it, [128, 160) [160, 192), and Q from 192 on (the
   // next scores are then made while a group's softmax still works); with heads of 256 P takes S's columns and Q is [128, 256); O from 256 on
   constexpr bool APART = HD <= 128;
-  constexpr uint32_t P_COL = APART ? 128 : 0, P_STEP = APART ? 32 : 64, Q_COL = APART ? 192 : 128, O_COL = 256;
+  constexpr uint32_t P_COL = APART ? 128 : 0, P_STEP = APART ? 32 : 64, Q_COL = APART ? 192 : 128, O_COL = 256, O_STEP = APART ? HD : 0;
   constexpr uint32_t IDESC_S = sh_idesc(AF_PAGE, BITS == 8, false), IDESC_O = sh_idesc(HD, BITS == 8, true);
   constexpr float LOG2E = 1.4426950408889634f;
   extern __shared__ unsigned char sh_raw[];
@@ -273,8 +274,8 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
   __shared__ uint64_t k_full[STAGES], k_empty[STAGES], v_full[STAGES], v_empty[STAGES], s_full[2], p_full[2], pv_done[2], m_ready[2], x_full[2], q_ready,
       l_full, staged, ring_free, raw_full[C::RAW], raw_empty[C::RAW];
   constexpr int W_PAGES = BITS == 8 ? SH_EXPS : 1;
-  // by group: the reference after its page; by group and part: the maxima of a page; by thread of a row: sums
-  __shared__ float mref_s[2][SH_ROWS], mx_s[2][2][SH_ROWS], l_s[4][SH_ROWS];
+  // by group: the reference after its page; by group, turn and part: the maxima of a page; by thread of a row: sums
+  __shared__ float mref_s[2][SH_ROWS], mx_s[2][2][2][SH_ROWS], l_s[4][SH_ROWS];
   // the keys' factors, the values' exponents (no less than -60) and factors
   __shared__ __align__(16) float ks_s[W_PAGES][AF_PAGE], lv_s[W_PAGES][AF_PAGE], vs_s[W_PAGES][AF_PAGE];
   __shared__ uint32_t tmem_base_s;
@@ -317,7 +318,7 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
     mbar_init(&ring_free, 1);
     for (int s = 0; s < C::RAW; ++s) {
       mbar_init(&raw_full[s], 1);
-      mbar_init(&raw_empty[s], 5);
+      mbar_init(&raw_empty[s], C::CONV + 1);
     }
     give_up_s = 0;
     mbar_fence_init();
@@ -419,7 +420,7 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
           const uint32_t vt = smem_u32(v_s + s * C::TILE);
 #pragma unroll
           for (int kk = 0; kk < AF_PAGE / 16; ++kk)
-            umma_f16_ts(tmem + O_COL, tmem + P_COL + (jj & 1) * P_STEP + kk * 8, umma_desc_mn(vt + kk * 2048, 8192), IDESC_O, (j > 0 || kk > 0) ? 1u : 0u);
+            umma_f16_ts(tmem + O_COL + (jj & 1) * O_STEP, tmem + P_COL + (jj & 1) * P_STEP + kk * 8, umma_desc_mn(vt + kk * 2048, 8192), IDESC_O, (j > (APART ? 1 : 0) || kk > 0) ? 1u : 0u);
           umma_commit(&v_empty[s]);
           umma_commit(&pv_done[jj & 1]);
         }
@@ -503,7 +504,7 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
           if (!ok) break;
           if (lane == 0) {
             mbar_arrive(&x_full[grp]);
-            mbar_arrive(&m_ready[grp]);
+            if (!APART) mbar_arrive(&m_ready[grp]);
             mbar_arrive(&p_full[grp]);
           }
           continue;
@@ -547,42 +548,45 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
           mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * cx;
         }
         // the row's maximum over the group's two threads (both have read their scores: the columns may be written again)
-        mx_s[grp][part][row] = mx;
+        const int turn = (jj >> 1) & 1;      // (a thread may be at its next page before the other one has read)
+        mx_s[grp][turn][part][row] = mx;
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&x_full[grp]);
         ok = mbar_wait(&x_full[grp], (jj >> 1) & 1, give_up);
         if (!ok) break;
         tc_fence_after();
-        mx = fmaxf(mx, mx_s[grp][part ^ 1][row]);
+        mx = fmaxf(mx, mx_s[grp][turn][part ^ 1][row]);
         // the reference after the page before, published by the other group; it moves only when it has to
-        float m_prev = SH_NONE;
-        if (j > 0) {
+        float m_prev = APART ? m_known : SH_NONE;
+        if (!APART && j > 0) {
           ok = mbar_wait(&m_ready[grp ^ 1], ((jj - 1) >> 1) & 1, give_up);
           if (!ok) break;
           m_prev = mref_s[grp ^ 1][row];
         }
         const float m_new = mx > m_prev + SH_MOVES ? mx : m_prev;
-        if (part == 0) mref_s[grp][row] = m_new;
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&m_ready[grp]);
+        if constexpr (!APART) {
+          if (part == 0) mref_s[grp][row] = m_new;
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&m_ready[grp]);
+        }
         // the group's P of two pages before is consumed (waited for here: it also pins the phase that the wait below looks at)
         if (APART && j >= 2) ok = mbar_wait(&pv_done[grp], ((jj - 2) >> 1) & 1, give_up);
         if (!ok) break;
-        if (j > 0 && __any_sync(0xffffffffu, m_new != m_prev)) {
+        if (j > (APART ? 1 : 0) && __any_sync(0xffffffffu, m_new != m_prev)) {
           // O is rescaled once the product of the page before is complete (the next one waits for this page's P)
-          ok = mbar_wait(&pv_done[grp ^ 1], ((jj - 1) >> 1) & 1, give_up);
+          if (!APART) ok = mbar_wait(&pv_done[grp ^ 1], ((jj - 1) >> 1) & 1, give_up);
           if (!ok) break;
           tc_fence_after();
           const float f = fast_exp2(m_prev - m_new);
 #pragma unroll 1
           for (int c0 = 0; c0 < HD / 2; c0 += 16) {
             float o[16];
-            tmem_ld16(lane_addr + O_COL + part * (HD / 2) + c0, o);
+            tmem_ld16(lane_addr + O_COL + grp * O_STEP + part * (HD / 2) + c0, o);
             tmem_wait_ld();
 #pragma unroll
             for (int c = 0; c < 16; ++c) o[c] *= f;
-            tmem_st16(lane_addr + O_COL + part * (HD / 2) + c0, o);
+            tmem_st16(lane_addr + O_COL + grp * O_STEP + part * (HD / 2) + c0, o);
           }
           tmem_wait_st();
         }
@@ -625,19 +629,36 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
       ok = ok && mbar_wait(&pv_done[last & 1], (last >> 1) & 1, give_up);
       if (!ok) break;
       tc_fence_after();
-      const float m_fin = any ? mref_s[last & 1][row] : 0.f;
-      if (any) l_s[quad][row] = l * fast_exp2(m_known - m_fin);
+      if constexpr (APART) {
+        if (any) {
+          l_s[quad][row] = l;
+          if (part == 0) mref_s[grp][row] = m_known;      // (of a group without a page: SH_NONE)
+        }
+      } else if (any) {
+        l_s[quad][row] = l * fast_exp2(m_known - mref_s[last & 1][row]);
+      }
       __syncwarp();
       if (lane == 0) mbar_arrive(&l_full);
       ok = mbar_wait(&l_full, n & 1, give_up);
       if (!ok) break;
       if (any) {
+        // the groups' two references become one
+        const float m0 = mref_s[0][row], m1 = mref_s[1][row], m_fin = APART ? fmaxf(m0, m1) : mref_s[last & 1][row];
+        const float f0 = APART ? fast_exp2(m0 - m_fin) : 1.f, f1 = APART ? fast_exp2(m1 - m_fin) : 1.f;
+        const bool has0 = it.pages > 1 || (last & 1) == 0, has1 = it.pages > 1 || (last & 1) == 1;
 #pragma unroll 1
         for (int c0 = 0; c0 < HD / 4; c0 += 16) {
           float o[16];
           const int col = quad * (HD / 4) + c0;
           tmem_ld16(lane_addr + O_COL + col, o);
           tmem_wait_ld();
+          if constexpr (APART) {
+            float o1[16];
+            tmem_ld16(lane_addr + O_COL + O_STEP + col, o1);
+            tmem_wait_ld();
+#pragma unroll
+            for (int c = 0; c < 16; ++c) o[c] = (has0 ? o[c] * f0 : 0.f) + (has1 ? o1[c] * f1 : 0.f);
+          }
           if (live) {
             unsigned char* dst = k_s + row * (HD * 4);
 #pragma unroll
@@ -647,7 +668,7 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
         }
         if (live && quad == 0)
           *reinterpret_cast<float2*>(a.part_ml + ((size_t)it.row0 + row) * 2) =
-              make_float2(BITS == 8 ? m_fin - SH_SHIFT : m_fin, (l_s[0][row] + l_s[1][row]) + (l_s[2][row] + l_s[3][row]));
+              make_float2(BITS == 8 ? m_fin - SH_SHIFT : m_fin, (l_s[0][row] + l_s[1][row]) * f0 + (l_s[2][row] + l_s[3][row]) * f1);
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       }
       __syncwarp();
@@ -672,56 +693,45 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
   } else if (BITS == 8 && warp >= 20) {
     // ---- codes to halves.  A page's keys (and values) are 64 rows of HD / 16 pieces of 16 codes; a thread takes PER of them, their
     // codes read before the wait for the operand's place
-    constexpr int P_ROW = HD / 16, PER = AF_PAGE * P_ROW / 128;
-    const int ct = threadIdx.x - 20 * 32;
+    constexpr int P_ROW = HD / 16, PER = AF_PAGE * P_ROW / 128, KINDS = C::CONV == 8 ? 1 : 2;
+    const int ct = (threadIdx.x - 20 * 32) & 127, kind0 = C::CONV == 8 ? (warp - 20) >> 2 : 0;
     int jj = 0, n = 0;
     bool ok = true;
-    uint4 w4[PER];
-    auto take = [&](const unsigned char* raw) {
-#pragma unroll
-      for (int i = 0; i < PER; ++i) w4[i] = *reinterpret_cast<const uint4*>(raw + (ct + i * 128) * 16);
-    };
-    auto put = [&](unsigned char* tile) {
-#pragma unroll
-      for (int i = 0; i < PER; ++i) {
-        const int x = ct + i * 128, r = x / P_ROW, p = x - r * P_ROW;
-        uint4 h[2];
-        c8_half4(w4[i].x, h[0].x, h[0].y);
-        c8_half4(w4[i].y, h[0].z, h[0].w);
-        c8_half4(w4[i].z, h[1].x, h[1].y);
-        c8_half4(w4[i].w, h[1].z, h[1].w);
-        unsigned char* base = tile + (p >> 2) * 8192 + r * 128;
-        const int c = (p & 3) * 2, first = (p >> 2) & 1;        // (neighbouring sub-tiles begin with the other piece: other banks)
-        *reinterpret_cast<uint4*>(base + (((c + first) ^ (r & 7)) << 4)) = first ? h[1] : h[0];
-        *reinterpret_cast<uint4*>(base + (((c + 1 - first) ^ (r & 7)) << 4)) = first ? h[0] : h[1];
-      }
-    };
     for (int w = blockIdx.x; w < n_items && ok; w += gridDim.x, ++n) {
       const ShItem it = item_of(w);
       if (n > 0) ok = mbar_wait(&ring_free, (n - 1) & 1, give_up);      // (the item before has left the operands' memory)
       for (int j = 0; j < it.pages && ok; ++j, ++jj) {
         const int s = jj % STAGES, rs = jj % C::RAW;
-        const uint32_t ph = ((jj / STAGES) & 1) ^ 1;
-        const unsigned char* raw = raw_s + rs * C::RAW_STAGE;
         ok = mbar_wait(&raw_full[rs], (jj / C::RAW) & 1, give_up);
-        if (!ok) break;
-        take(raw);
-        ok = mbar_wait(&k_empty[s], ph, give_up);
-        if (!ok) break;
-        put(k_s + s * C::TILE);
-        take(raw + C::CODES);
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-        __syncwarp();
-        if (lane == 0) {
-          mbar_arrive(&k_full[s]);
-          mbar_arrive(&raw_empty[rs]);
+#pragma unroll
+        for (int kind = kind0; kind < kind0 + KINDS && ok; ++kind) {      // 0: keys, 1: values
+          const unsigned char* raw = raw_s + rs * C::RAW_STAGE + kind * C::CODES;
+          uint4 w4[PER];
+#pragma unroll
+          for (int i = 0; i < PER; ++i) w4[i] = *reinterpret_cast<const uint4*>(raw + (ct + i * 128) * 16);
+          ok = mbar_wait(kind ? &v_empty[s] : &k_empty[s], ((jj / STAGES) & 1) ^ 1, give_up);
+          if (!ok) break;
+          unsigned char* tile = (kind ? v_s : k_s) + s * C::TILE;
+#pragma unroll
+          for (int i = 0; i < PER; ++i) {
+            const int x = ct + i * 128, r = x / P_ROW, p = x - r * P_ROW;
+            uint4 h[2];
+            c8_half4(w4[i].x, h[0].x, h[0].y);
+            c8_half4(w4[i].y, h[0].z, h[0].w);
+            c8_half4(w4[i].z, h[1].x, h[1].y);
+            c8_half4(w4[i].w, h[1].z, h[1].w);
+            unsigned char* base = tile + (p >> 2) * 8192 + r * 128;
+            const int c = (p & 3) * 2, first = (p >> 2) & 1;        // (neighbouring sub-tiles begin with the other piece: other banks)
+            *reinterpret_cast<uint4*>(base + (((c + first) ^ (r & 7)) << 4)) = first ? h[1] : h[0];
+            *reinterpret_cast<uint4*>(base + (((c + 1 - first) ^ (r & 7)) << 4)) = first ? h[0] : h[1];
+          }
+          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+          __syncwarp();
+          if (lane == 0) {
+            mbar_arrive(kind ? &v_full[s] : &k_full[s]);
+            if (kind == kind0 + KINDS - 1) mbar_arrive(&raw_empty[rs]);
+          }
         }
-        ok = mbar_wait(&v_empty[s], ph, give_up);
-        if (!ok) break;
-        put(v_s + s * C::TILE);
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&v_full[s]);
       }
     }
   } else if (BITS == 8 && warp == 3) {
