@@ -251,6 +251,33 @@ __device__ __forceinline__ void sh_bulk_load(void* dst, const void* src, uint32_
                : "memory");
 }
 
+// Two products (and sums) at a time.
+struct ShPair {
+  float x, y;
+};
+__device__ __forceinline__ ShPair sh_mul2(ShPair a, ShPair b) {
+  ShPair d;
+  asm("{\n\t.reg .b64 a, b, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmul.rn.f32x2 d, a, b;\n\tmov.b64 {%0, %1}, d;\n\t}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
+__device__ __forceinline__ ShPair sh_add2(ShPair a, ShPair b) {
+  ShPair d;
+  asm("{\n\t.reg .b64 a, b, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tadd.rn.f32x2 d, a, b;\n\tmov.b64 {%0, %1}, d;\n\t}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
+__device__ __forceinline__ ShPair sh_fma2(ShPair a, ShPair b, ShPair c) {
+  ShPair d;
+  asm("{\n\t.reg .b64 a, b, c, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmov.b64 c, {%6, %7};\n\tfma.rn.f32x2 d, a, b, c;\n\t"
+      "mov.b64 {%0, %1}, d;\n\t}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return d;
+}
+
 // What an item is: every role reads it from the plan.
 struct ShItem {
   int rows, first, pages, row0, members0, group0, kvh, slot;      // rows of the tile; page range; partial row; ...
@@ -522,7 +549,8 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
 #pragma unroll
           for (int c = 0; c < W; c += 4) {
             const float4 f = ksp[c / 4];
-            s[c] *= f.x, s[c + 1] *= f.y, s[c + 2] *= f.z, s[c + 3] *= f.w;
+            const ShPair t0 = sh_mul2({s[c], s[c + 1]}, {f.x, f.y}), t1 = sh_mul2({s[c + 2], s[c + 3]}, {f.z, f.w});
+            s[c] = t0.x, s[c + 1] = t0.y, s[c + 2] = t1.x, s[c + 3] = t1.y;
           }
         }
         float cx = cs;
@@ -538,8 +566,8 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
 #pragma unroll
           for (int c = 0; c < W; c += 4) {
             const float4 f = lvp[c / 4];
-            m4[0] = fmaxf(m4[0], fmaf(s[c], cx, f.x)), m4[1] = fmaxf(m4[1], fmaf(s[c + 1], cx, f.y));
-            m4[2] = fmaxf(m4[2], fmaf(s[c + 2], cx, f.z)), m4[3] = fmaxf(m4[3], fmaf(s[c + 3], cx, f.w));
+            const ShPair t0 = sh_fma2({s[c], s[c + 1]}, {cx, cx}, {f.x, f.y}), t1 = sh_fma2({s[c + 2], s[c + 3]}, {cx, cx}, {f.z, f.w});
+            m4[0] = fmaxf(m4[0], t0.x), m4[1] = fmaxf(m4[1], t0.y), m4[2] = fmaxf(m4[2], t1.x), m4[3] = fmaxf(m4[3], t1.y);
           }
           mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
         } else {
@@ -590,29 +618,32 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
           }
           tmem_wait_st();
         }
-        float sum4[4] = {0.f, 0.f, 0.f, 0.f};
+        ShPair sum0 = {0.f, 0.f}, sum1 = {0.f, 0.f};
         uint32_t packed[W / 2];
         if constexpr (BITS == 8) {
           const float ref = m_new - SH_SHIFT;
 #pragma unroll
           for (int c = 0; c < W; c += 4) {
             const float4 f = vsp[c / 4];
-            const float p0 = fast_exp2(fmaf(s[c], cx, -ref)), p1 = fast_exp2(fmaf(s[c + 1], cx, -ref));
-            const float p2 = fast_exp2(fmaf(s[c + 2], cx, -ref)), p3 = fast_exp2(fmaf(s[c + 3], cx, -ref));
-            sum4[0] += p0, sum4[1] += p1, sum4[2] += p2, sum4[3] += p3;
-            const __half2 h0 = __floats2half2_rn(p0 * f.x, p1 * f.y), h1 = __floats2half2_rn(p2 * f.z, p3 * f.w);
+            const ShPair t0 = sh_fma2({s[c], s[c + 1]}, {cx, cx}, {-ref, -ref}), t1 = sh_fma2({s[c + 2], s[c + 3]}, {cx, cx}, {-ref, -ref});
+            const ShPair p0 = {fast_exp2(t0.x), fast_exp2(t0.y)}, p1 = {fast_exp2(t1.x), fast_exp2(t1.y)};
+            sum0 = sh_add2(sum0, p0), sum1 = sh_add2(sum1, p1);
+            const ShPair w0 = sh_mul2(p0, {f.x, f.y}), w1 = sh_mul2(p1, {f.z, f.w});
+            const __half2 h0 = __floats2half2_rn(w0.x, w0.y), h1 = __floats2half2_rn(w1.x, w1.y);
             packed[c / 2] = *reinterpret_cast<const uint32_t*>(&h0);
             packed[c / 2 + 1] = *reinterpret_cast<const uint32_t*>(&h1);
           }
         } else {
 #pragma unroll
           for (int c = 0; c < W; c += 2) {
-            const __nv_bfloat162 pb = __floats2bfloat162_rn(fast_exp2(fmaf(s[c], cx, -m_new)), fast_exp2(fmaf(s[c + 1], cx, -m_new)));
-            sum4[(c >> 1) & 3] += __low2float(pb) + __high2float(pb);      // (of the rounded weights that the product sees)
+            const ShPair t = sh_fma2({s[c], s[c + 1]}, {cx, cx}, {-m_new, -m_new});
+            const __nv_bfloat162 pb = __floats2bfloat162_rn(fast_exp2(t.x), fast_exp2(t.y));
+            ShPair& sum = (c >> 1) & 1 ? sum1 : sum0;
+            sum = sh_add2(sum, {__low2float(pb), __high2float(pb)});      // (of the rounded weights that the product sees)
             packed[c / 2] = *reinterpret_cast<const uint32_t*>(&pb);
           }
         }
-        l = l * fast_exp2(m_known - m_new) + ((sum4[0] + sum4[1]) + (sum4[2] + sum4[3]));
+        l = l * fast_exp2(m_known - m_new) + ((sum0.x + sum0.y) + (sum1.x + sum1.y));
         m_known = m_new;
         tmem_st16(lane_addr + P_COL + grp * P_STEP + part * (W / 2), reinterpret_cast<const float*>(packed));
         tmem_wait_st();
