@@ -300,25 +300,26 @@ class SequenceCache:
         return new
 
     def shared_claims(self, slots):
-        """For the rows of a step (slots, -1 or None: none): (lead, pages, most): row i's first ``pages[i]`` pages are those of row
-        ``lead[i]`` in every group that keeps all keys, ``most`` the most pages that are read again and again without: a group's shared
-        pages times its rows but one.  None where no two rows share a page."""
-        if not self._family:
+        """For the rows of a step (slots, -1 or None: none): (lead, pages, families, need): row i's first ``pages[i]`` pages are those
+        of row ``lead[i]`` in every group that keeps all keys; by family (rows, shared pages); and such a group's KVNeed (the one with the
+        longest rows).  None where no two rows share a page or no group keeps all keys."""
+        needs = [g.need for g in self.groups.values() if not g.need.window]
+        if not self._family or not needs:
             return None
         rows: dict = {}
         for i, s in enumerate(slots):
             f = self._family.get(s)
             if f is not None:
                 rows.setdefault(f[0], []).append((i, min(f[1], self.lens[s] // PAGE)))
-        lead, pages, saved = list(range(len(slots))), [0] * len(slots), 0
+        lead, pages, families = list(range(len(slots))), [0] * len(slots), []
         for members in rows.values():
             n = min(p for _, p in members)
             if len(members) < 2 or n == 0:
                 continue
             for i, _ in members:
                 lead[i], pages[i] = members[0][0], n
-            saved += n * (len(members) - 1)
-        return (lead, pages, saved) if saved else None
+            families.append((len(members), n))
+        return (lead, pages, families, max(needs, key=lambda n: n.num_kv_heads * n.head_dim)) if families else None
 
     def length(self, slot: int) -> int:
         if not self.slots.is_held(slot):

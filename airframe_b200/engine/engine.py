@@ -74,7 +74,10 @@ class Engine:
     def _claims(self, slots):
         """(lead, pages) of a decode step whose shared pages are worth the shared kernels, else None."""
         claims = self.cache.shared_claims(slots)
-        return claims[:2] if claims is not None and claims[2] >= kernels.SHARED_PAGES_FROM else None
+        if claims is None:
+            return None
+        lead, pages, groups, need = claims
+        return (lead, pages) if kernels.attn_decode_shared_pays(groups, need.num_kv_heads, need.head_dim, need.eight_bits) else None
 
     def length(self, slot: int) -> int:
         return self.cache.length(slot)

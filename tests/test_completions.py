@@ -120,15 +120,37 @@ def test_shared_claims():
     d = c.fork(a)                                    # shares 6 with a, 3 with b
     e = c.fork(b)                                    # 3
     y = c.fork(z)                                    # another family: 4
-    assert c.shared_claims([a, b]) == ([0, 0], [3, 3], 3)
-    assert c.shared_claims([z, d, a]) == ([0, 1, 1], [0, 6, 6], 6)
-    assert c.shared_claims([y, b, -1, d, z, e, None]) == ([0, 1, 2, 1, 0, 1, 6], [4, 3, 0, 3, 4, 3, 0], 3 * 2 + 4)
+    assert c.shared_claims([a, b])[:3] == ([0, 0], [3, 3], [(2, 3)])
+    assert c.shared_claims([z, d, a])[:3] == ([0, 1, 1], [0, 6, 6], [(2, 6)])
+    assert c.shared_claims([y, b, -1, d, z, e, None])[:3] == ([0, 1, 2, 1, 0, 1, 6], [4, 3, 0, 3, 4, 3, 0], [(2, 4), (3, 3)])
     assert c.shared_claims([a, z]) is None
     held = c.groups[KVNeed(1, 8)].held
     assert held[a][:6] == held[d][:6] and held[a][:3] == held[b][:3] == held[e][:3]
     c.free_slot(a)                                   # its slot is another sequence's now
     n = c.take_slot()
-    assert n == a and c.shared_claims([n, b, e]) == ([0, 1, 1], [0, 3, 3], 3)
+    assert n == a and c.shared_claims([n, b, e])[:3] == ([0, 1, 1], [0, 3, 3], [(2, 3)])
+
+
+def test_claims_are_of_the_groups_that_keep_all_keys():
+    """Their longest rows decide; without such a group nothing is read once."""
+    ring, small, large = KVNeed(1, 8, 64), KVNeed(1, 8), KVNeed(2, 8, eight_bits=True)
+    for needs, want in (([ring], None), ([ring, small], small), ([large, ring, small], large)):
+        c = SequenceCache([(n, None, None) for n in needs], 64 * 100, 2000, torch.float32, "cpu", max_sequences=4)
+        a = c.take_slot()
+        c.reserve({a: 200})
+        c.commit({a: 200})
+        claims = c.shared_claims([a, c.fork(a)])
+        assert claims is None if want is None else claims[3] == want
+
+
+def test_shared_pages_pay_where_enough_is_read_again():
+    from airframe_b200.kernels import attn_decode_shared_pays as pays
+    for eight in (False, True):
+        assert not pays([(2, 16)], 4, 256, eight) and not pays([(64, 1)], 8, 128, eight)
+        assert pays([(32, 64)], 4, 256, eight) and pays([(8, 256)], 8, 128, eight)
+        assert pays([(32, 256), (2, 16)], 4, 128, eight)
+    assert pays([(3, 1024)], 4, 256) and not pays([(3, 1024)], 4, 256, True)
+    assert not pays([], 4, 256)
 
 
 def test_fits_counts_shared_pages_once():
@@ -233,7 +255,7 @@ def _forked(rt, prompt, tails, graphs=True):
 def test_forks_go_on_like_separate_sequences(tmp_path, monkeypatch, name, dtype, kv, graphs):
     """Forks with other tails (shared pages, copied begun pages and rings; one ends early) against sequences of their own."""
     from airframe_b200 import kernels
-    monkeypatch.setattr(kernels, "SHARED_PAGES_FROM", 1)
+    monkeypatch.setattr(kernels, "attn_decode_shared_pays", lambda *a: True)
     cfg = dict(CONFIGS[name], max_position_embeddings=512)
     rt = _runtime(tmp_path, cfg, dtype, kv_dtype=kv)
     shared = []
@@ -302,7 +324,7 @@ def test_completions_of_a_prompt(tmp_path, monkeypatch):
     from airframe_b200 import kernels
     from airframe_b200.engine import GpuRuntime
     from airframe_b200.sampling import SamplingParams
-    monkeypatch.setattr(kernels, "SHARED_PAGES_FROM", 1)
+    monkeypatch.setattr(kernels, "attn_decode_shared_pays", lambda *a: True)
     cfg = dict(CONFIGS["A"], max_position_embeddings=512)
     rt = GpuRuntime.load(make_folder(cfg, seed=5, store_dtype="float32", root=tmp_path), dtype="float32", max_tokens=64 * 60)
     prompts = [replay.random_ids(256, 130, 1), replay.random_ids(256, 7, 2)]

@@ -171,9 +171,7 @@ def test_far_from_the_first_page(K):
         q = torch.zeros(2, nq * hd)
         q[:, ::hd] = 200.0
         q = q.to(torch.bfloat16)
-        for i, held in enumerate(f.held):           # the first channel of the key at position p: p / 64, exact in the codes' range
-            pass
-        ramp = torch.arange(30 * PAGE, dtype=torch.float32) / 128
+        ramp = torch.arange(30 * PAGE, dtype=torch.float32) / 128      # (the first channel of the key at each position)
         for page in range(30):
             pid = int(f.table[f.order[0], page])
             rows = torch.zeros(1, PAGE, hd)
