@@ -1,9 +1,16 @@
 // Decode attention over the 8-bit cache (cache8.cuh): one new token per sequence, bound by the bytes of codes it reads (every
 // byte is read once; half of the 16-bit cache's).
 //
-// The work is cut as for the 16-bit cache (decode_split.cuh): one block an SM, units of a (sequence, kv head), their pages in
-// equal splits or runs, by the step's plan.  A page's codes come in by TMA (swizzled) and its exponents by two bulk copies,
-// through a ring of shared-memory stages; groups of four warps take the pages in turn, a warp 16 of a page's 64 keys.
+// The work is cut as for the 16-bit cache (decode_split.cuh): units of a (sequence, kv head), their pages in equal splits or runs, by the
+// step's plan.  A block has a warp that brings codes in (TMA, swizzled, through a ring of stages; a row's exponents by plain loads) and
+// warps that compute, each 8 KB of keys and values at a time, its running maximum, sum and output its own until the unit's end.  A
+// warp's 8 KB are many products (of 16 keys by 8 heads, 16 by 16 by 8 at a time) in a dependent chain from score to output, so it is
+// the number of warps with a chain at work that feeds the memory: two blocks of seven computing warps an SM, as the registers
+// allow.  Measured (1 sequence of 131,072 tokens, 8 kv heads of 128, 4 heads each; 64 sequences of up to 8,192 tokens and a window of
+// 4,096, 8 kv heads of 256, 2 heads each): 53.2 and 76.3 us, 5.1 and 4.1 TB/s; with one such block an SM 59.7 and 105.  Bound by the memory's rate at long lengths; below some
+// 1,000 tokens by the plan and the two launches (13.0 us at 700 tokens).
+// Groups of 9 to 16 heads take twice the accumulators and one block an SM: 8 sequences of 16,384 tokens, 2 kv heads of 16 heads each: 31% of
+// a copy's rate with heads of 128, 40% with 256.
 //
 // Products.  With a query group of few heads the keys are the rows of the m16n8k16 tiles and the heads their 8 columns:
 //   S^T = K Q^T (16 keys x 8 heads), O^T += V^T P^T (16 dims x 8 heads)

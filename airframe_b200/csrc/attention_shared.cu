@@ -14,18 +14,24 @@
 //   softmax       two groups of eight warps take the pages in turn, two threads a row (32 keys each): all keys are visible (a shared
 //                 page is full and older than every member's token), so there is no mask; P goes back into its S columns of TMEM
 //   O += P V      tcgen05.mma, P from TMEM, O (128 x head_dim, 32 bits) in TMEM for the whole item
-// The groups share O and its reference maximum, which a group hands to the other with every page and which moves only when it is
-// passed by more than 2^8.  Products and softmax of neighbouring pages overlap.
+// A reference maximum moves only when it is passed by more than 2^8.  With heads of 64 and 128 each group has a reference and an O of its own
+// (two of 128 columns), joined at the item's end; with heads of 256 TMEM holds one O, whose reference a group hands to the other with
+// every page.  Products and softmax of neighbouring pages overlap.
 //   warp 0        TMA producer (16-bit cache)         warp 1  issue of S, TMEM allocation      warp 2  issue of O += P V
 //   warps 4..19   queries, softmax, rescaling, partial results
-//   warps 20..23  8-bit cache only: codes, brought into shared memory as they are by warp 0, to halves in the swizzled operand layout;
-//                 warp 3 the rows' factors
+//   warps 20..    8-bit cache only: codes, brought into shared memory as they are by warp 0, to halves in the swizzled operand layout (four
+//                 warps keys and values; with heads of 256, whose pages take twice the conversions, four the keys and four the values); warp 3 the
+//                 rows' factors
 // An item's partial results are gathered in the operands' memory and leave as one bulk copy (they are contiguous; 16-byte piece c of
 // row r lies at piece c ^ (r & 7), for the banks' sake).
 // In the 8-bit cache a key's factor multiplies its scores, a value's (2^ev) its weights.  The one reference of a row is then the largest
 // s + max(ev, -60), so that the halves of the weights keep 2^-20 of the largest as normal numbers; sums and outputs are relative to it
 // less 6.  (Weights of values below 2^-60 * 448 may vanish, and of sums what is below 2^-20 even where values are of 2^110.)
-// Bound by the prefix's bytes up to some 128 rows; then by the products.
+// Measured, a layer of 2 sequences behind 131,072 tokens: 8 kv heads of 128, bfloat16, 87.5 us (6.1 TB/s with all that belongs to it), bound by
+// the prefix's bytes; 8 bits 118.9 us, 0.85 us a page and block, bound by the chain scores - softmax - weights of the two groups (a group's
+// page takes some 3,400 cycles, of which 900 are waits on barriers that are complete); 4 kv heads of 256 96 us and 122 (8 bits: by the conversion
+// and the single O).  32 sequences of 8 kv heads of 128, 4 heads each, behind 32,768 tokens in 8 bits: the kernel 46.7 us, 1.3 us a page with
+// all 128 rows at work (half of the issue slots).  64 sequences of 4 kv heads of 256, 2 heads each, behind 7,168 tokens: the kernel 24 us.
 // Every wait on a barrier is bounded in time; one that runs out sets the error word, and the block frees its TMEM and returns.
 #include "airframe_b200.h"
 #include "cache8.cuh"
@@ -50,7 +56,7 @@ namespace {
 //   shared [batch]      the pages of each sequence that the prefix kernel takes (0: none)
 //   loc    [batch][2]   its group's first unit (-1: none), its place among the group's members
 //   order  [batch]      the groups' members, group after group
-//   units  [n][8]       where its members begin in `order`, members, kv head, tile of 128 rows; pages, items, first partial row, slot
+//   units  [n][4]       members of its group, items, first partial row, 0
 //   items  [n][8]       ShItem: what a block reads with two loads
 constexpr int SH_HEAD = 16, SH_ROWS = 128, SH_MAX_BATCH = DA_MAX_BATCH;
 
@@ -65,7 +71,7 @@ __host__ __device__ inline ShPlan sh_layout(int batch, int nq, int nkv, int bloc
   p.loc = p.shared + b4;
   p.order = p.loc + 2 * b4;
   p.units = p.order + b4;       // (all of them multiples of four: read four integers at a time)
-  p.items = p.units + 8 * units;
+  p.items = p.units + 4 * units;
   p.total = p.items + 8 * (blocks + units);
   return p;
 }
@@ -85,7 +91,7 @@ __device__ __forceinline__ int sh_items(int pages, int units, int rows, int hd, 
   return max(1, min(min(pages, pay), (int)min((long long)pages, (long long)pages * blocks / total)));
 }
 
-// Two blocks: the first writes the prefix kernel's plan, the second the split kernel's.  (Like attn_decode_plan_kernel they do not
+// Some 7 us a step, for all layers.  Two blocks: the first writes the prefix kernel's plan, the second the split kernel's.  (Like attn_decode_plan_kernel they do not
 // release their dependents early.)  A group is the live rows of one `lead` that share at least a page; alone in it a row keeps its pages.  Fewer
 // pages than a row claims are taken where another of the group shares fewer, and never the page of its new token.
 __global__ void __launch_bounds__(512)
@@ -192,10 +198,8 @@ attn_shared_plan_kernel(int* plan, const int* lead, const int* pages, const int*
     const int rows = c * group, tiles = (rows + SH_ROWS - 1) / SH_ROWS, u = nkv * tiles;
     const int s = parts[g];
     for (int x = lane; x < u; x += 32) {
-      int* r = plan + L.units + 8 * (unit0[g] + x);
       const int kvh = x / tiles, tile = x - kvh * tiles;
-      r[0] = memb0[g], r[1] = c, r[2] = kvh, r[3] = tile;
-      r[4] = few[g], r[5] = s, r[6] = row0[g] + (kvh * rows + tile * SH_ROWS) * s, r[7] = slots[b];
+      reinterpret_cast<int4*>(plan + L.units)[unit0[g] + x] = make_int4(c, s, row0[g] + (kvh * rows + tile * SH_ROWS) * s, 0);
     }
     for (int x = lane; x < u * s; x += 32) {
       const int unit = x / s, z = x - unit * s, kvh = unit / tiles, tile = unit - kvh * tiles, r = min(SH_ROWS, rows - tile * SH_ROWS);
@@ -800,7 +804,10 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
 
 // ---------------------------------------------------------------- merge
 
-constexpr int SHM_THREADS = 256, SHM_MOST = 1024;     // partial results of a (sequence, head) that the block weighs
+// Two warps: a thread has up to eight loads of partial results on their way, and more threads a block only keep other blocks out.  (A layer of 128
+// sequences of 32 heads of 128, 4 items each: with 256, 128 and 64 threads 67.3, 58.6 and 58.6 us in all; 64 sequences of 8 heads of 256, 20
+// items: 44.3, 46.0 and 44.5.)
+constexpr int SHM_THREADS = 64, SHM_MOST = 1024;     // partial results of a (sequence, head) that the block weighs
 
 // out[b, h] from the items of the shared pages and the splits of the sequence's own.
 template <int HD>
@@ -818,11 +825,11 @@ attn_shared_merge_kernel(__nv_bfloat16* __restrict__ out, long long out_stride, 
   const int unit0 = shared_plan[L.loc + 2 * b];
   if (unit0 >= 0) {
     const int rr = shared_plan[L.loc + 2 * b + 1] * group + h % group;
-    const int members = shared_plan[L.units + 8 * unit0 + 1], tiles = (members * group + SH_ROWS - 1) / SH_ROWS;
-    const int* u = shared_plan + L.units + 8 * (unit0 + kvh * tiles + rr / SH_ROWS);
+    const int members = shared_plan[L.units + 4 * unit0], tiles = (members * group + SH_ROWS - 1) / SH_ROWS;
+    const int* u = shared_plan + L.units + 4 * (unit0 + kvh * tiles + rr / SH_ROWS);
     rows = min(SH_ROWS, members * group - rr / SH_ROWS * SH_ROWS);
-    n_pre = u[5];
-    pre0 = (size_t)u[6] + rr % SH_ROWS;
+    n_pre = u[1];
+    pre0 = (size_t)u[2] + rr % SH_ROWS;
     turn = rr & 7;                     // (how the row's pieces lie)
   }
   const size_t own0 = ((size_t)b * nq + h) * own_room;
