@@ -117,10 +117,13 @@ class KVGroup:
         self.held[dst] = self.held[src][:whole] + new
         self.table_host[dst, :n] = torch.tensor(self.held[dst], dtype=torch.int32)
         self.dirty.add(dst)
+        if not new or self.k is None:
+            return
+        pages = torch.tensor([self.held[src][whole:n], new], device=self.k.device)      # (a ring's pages, many of them, move together)
         for t in (self.k, self.v, self.k_exp, self.v_exp):
             if t is not None:
-                for a, b in zip(self.held[src][whole:n], new):
-                    t[:, b].copy_(t[:, a])
+                t = t.view(torch.uint8)
+                t.index_copy_(1, pages[1], t.index_select(1, pages[0]))
 
     def release(self, slot: int) -> None:
         for p in self.held[slot]:

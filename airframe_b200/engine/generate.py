@@ -117,8 +117,8 @@ class GenerationLoop:
         batches, cur, cur_pages = [], [], 0
 
         def shares(i, batch):
-            """Tokens of request i whose pages an earlier completion of the same prompt in the batch holds."""
-            return len(prompts[i]) if fits is not None and any(j // completions == i // completions for j in batch if j < i) else 0
+            """Tokens of request i whose pages an earlier completion of the same prompt in the batch (requests in order) holds."""
+            return len(prompts[i]) if fits is not None and batch and i % completions and i > batch[0] else 0
 
         def together(batch):
             if completions == 1:

@@ -135,6 +135,8 @@ class Attention(Mixer):
             if ctx.compute_dtype != torch.bfloat16 or size not in kernels.CACHE8_HEAD_SIZES or value != size:
                 raise ConfigError(f"attention: a cache of 8 bits goes with bfloat16 and keys and values of one size in "
                                   f"{kernels.CACHE8_HEAD_SIZES}, not with {ctx.compute_dtype}, {size} and {value}")
+            if type(self.position).score_slopes is not PositionEncoding.score_slopes:
+                raise ConfigError(f"attention: a cache of 8 bits does not serve the score slopes of '{self.position.kind}'")
         self.q_norm_w = self.k_norm_w = self.bias = self.sinks = None
         self.w_qkv = None
         self.w_o = None

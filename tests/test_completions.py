@@ -153,6 +153,44 @@ def test_shared_pages_pay_where_enough_is_read_again():
     assert not pays([], 4, 256)
 
 
+def test_a_fork_of_a_ring_has_its_rows():
+    """Every page of a window, the kept first tokens' and the begun page of all keys are copied, in every layer of a group."""
+    ring, kept, full = KVNeed(1, 8, 192), KVNeed(2, 4, 128, keep_first=3), KVNeed(1, 8)
+    c = SequenceCache([(ring, None, None), (kept, None, None), (full, None, None), (ring, None, None)], 64 * 100, 2000, torch.float32, "cpu", max_sequences=4)
+    a = c.take_slot()
+    c.reserve({a: 700})
+    c.commit({a: 700})
+    for g in c.groups.values():
+        g.k.copy_(torch.randn(g.k.shape))
+        g.v.copy_(torch.randn(g.v.shape))
+    before = {n: (g.k.clone(), g.v.clone()) for n, g in c.groups.items()}
+    b = c.fork(a)
+    for n, g in c.groups.items():
+        assert len(g.held[b]) == len(g.held[a]) and (n.window is None or not set(g.held[a]) & set(g.held[b]))
+        for t, old in ((g.k, before[n][0]), (g.v, before[n][1])):
+            assert torch.equal(t[:, g.held[b]], old[:, g.held[a]]) and torch.equal(t[:, g.held[a]], old[:, g.held[a]])
+            others = [p for p in range(t.shape[1]) if p not in g.held[b]]
+            assert torch.equal(t[:, others], old[:, others])
+
+
+def test_batches_of_completions_share_only_what_is_in_the_batch():
+    """Requests of one prompt that fall into two batches: the second batch's first one holds the whole prompt again."""
+    from airframe_b200.engine import GenerationLoop
+    from airframe_b200.sampling import SamplingParams
+
+    class Eng:
+        cache = SequenceCache([(KVNeed(1, 8), None, None)], 64 * 12, 2000, torch.float32, None, max_sequences=8)
+        max_context = 2000
+        vocab_size = 100
+    loop = GenerationLoop(Eng(), None)
+    params = SamplingParams(max_tokens=65)
+    prompts = [[1] * 256] * 6 + [[2] * 256] * 6          # 4 whole pages each, one page of their own: 4 + 6 and 4 + 6 of 12
+    got = loop.plan_batches(prompts, params, 6)
+    assert got == [list(range(6)), list(range(6, 12))]
+    got = loop.plan_batches([[1] * 320] * 9, params, 9)   # 5 whole pages: 5 + 7 fit
+    assert got == [list(range(7)), [7, 8]]
+
+
 def test_fits_counts_shared_pages_once():
     full, ring = KVNeed(1, 8), KVNeed(1, 8, 64)
     c = SequenceCache([(full, None, None), (ring, None, None)], 64 * 10, 2000, torch.float32, None, max_sequences=4)
@@ -168,6 +206,18 @@ def test_refused_builds():
         Model(spec("D"), torch.float32, "cpu", F8)
     with pytest.raises(ConfigError, match="kv_dtype"):
         Model(spec("D"), torch.bfloat16, "cpu", torch.float8_e5m2)
+    import test_toy_parts
+    from airframe_b200.config import PartSpec
+    from airframe_b200.parts import unregister_part
+    test_toy_parts._register()
+    try:
+        slopes = spec("D")
+        slopes.layers[0].mixer.params["position"] = PartSpec("toy_distance_slopes", {"base": 2.0, "heads": slopes.layers[0].mixer.params["num_heads"]})
+        with pytest.raises(ConfigError, match="slopes"):
+            Model(slopes, torch.bfloat16, "cpu", F8)
+    finally:
+        for kind in (("feed_forward", "toy_top1_experts"), ("position", "toy_learned_offset"), ("position", "toy_distance_slopes")):
+            unregister_part(*kind)
     needs = Model(spec("D"), torch.bfloat16, "cpu", F8).cache_needs()
     assert all(n[0].eight_bits for n in needs)
     from airframe_b200.engine.runtime import _kv_dtype

@@ -195,6 +195,46 @@ def test_far_from_the_first_page(K):
 
 
 @pytest.mark.parametrize("bits", [16, 8])
+@pytest.mark.parametrize("hd", [64, 128, 256])
+def test_long_items(K, bits, hd):
+    """A block's item of several pages, in which the reference maximum moves with every page, with every second one, once and never:
+    20 groups of 2 with 8 kv heads are more units than SMs, so that no unit is cut."""
+    pages, nq, nkv = 11, 8, 8
+    f = Family([(i % 20, pages, pages * PAGE + 3 + i) for i in range(40)], nkv, hd, bits)
+    q = torch.randn(40, nq * hd) * 0.1
+    q[:, ::hd] = 200.0
+    q = q.to(torch.bfloat16)
+    for g in range(20):
+        up = torch.arange(pages * PAGE).float() / 128
+        ramp = (up, -up, torch.where(torch.arange(pages * PAGE) // PAGE % 2 == 0, up, -up), up * (torch.arange(pages * PAGE) // PAGE == 6))[g % 4]
+        for page in range(pages):
+            pid = int(f.table[f.order[g], page])
+            if bits == 8:
+                rows = values(f.codes["k"][0][pid], f.codes["k"][1][pid]).float()
+            else:
+                rows = f.k[pid].float().cpu()
+            rows[..., 0] = ramp[page * PAGE:(page + 1) * PAGE]
+            rows = rows.to(torch.bfloat16)
+            if bits == 8:
+                c, e = quantise(rows)
+                f.k.view(torch.uint8)[pid], f.k_exp[pid] = c.to(DEV), e.to(DEV)
+                rows = values(c, e)
+            else:
+                f.k[pid] = rows.to(DEV)
+                rows = rows.double()
+            for held in (f.held[g], f.held[g + 20]):
+                for r in range(PAGE):
+                    held[page * PAGE + r] = torch.stack([rows[:, r], held[page * PAGE + r][1]])
+    ref, mag, big = plain_attention(q, f.held, f.lens, nq, nkv, hd, 0.1, 0.0, 0, "window", 0, None)
+    out = torch.empty(40, nq * hd, dtype=torch.bfloat16, device=DEV)
+    l, p = f.lead()
+    K.attn_decode_shared(out, q.to(DEV), f, f.step(), nq, nkv, hd, 0.1, 0.0, l, p, pages)
+    got, lim = out.double().cpu().view(40, nq, hd), bound(ref, mag, big, hd)
+    assert bool(((got - ref).abs() <= lim).all()), float(((got - ref).abs() / lim).max())
+    K.check_device_errors(DEV)
+
+
+@pytest.mark.parametrize("bits", [16, 8])
 def test_captured_and_replayed(K, bits):
     """A captured step replayed with other groups and lengths: the plan is made anew on the device."""
     nq, nkv, hd = 4, 2, 128
