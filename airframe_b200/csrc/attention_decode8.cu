@@ -556,6 +556,8 @@ decode8_split_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
     __syncwarp();
     if (lane == 0) mbar_arrive(&seg_empty[k % SEGS]);
     const int n = sg.n_pages * PER, n_rows = sg.n_rows, row_head0 = sg.row_head0;
+    const int unit = sg.b * units_per_seq + sg.y;
+    const int n_parts = a.out != nullptr ? __ldcg(a.plan + DA_PLAN_HEAD + unit) : 0;       // (0: not merged here)
 
     // ---- the queries as B fragments (head g of every tile of 8), halves brought to [2^14, 2^15)
     uint32_t qf[NT][HD / 16][2];
@@ -567,10 +569,12 @@ decode8_split_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
       uint32_t top = 0;
 #pragma unroll
       for (int c = 0; c < HD / 64; ++c) {
+        const uint4* p = reinterpret_cast<const uint4*>(qr + c * 64);
+        const uint4 q0 = on ? p[0] : make_uint4(0u, 0u, 0u, 0u), q1 = on ? p[1] : make_uint4(0u, 0u, 0u, 0u);
+        const uint32_t words[8] = {q0.x, q0.y, q0.z, q0.w, q1.x, q1.y, q1.z, q1.w};
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          const uint32_t* p = reinterpret_cast<const uint32_t*>(qr + c * 64 + j * 4);
-          const uint32_t x = on ? p[0] : 0u, y = on ? p[1] : 0u;
+          const uint32_t x = words[2 * j], y = words[2 * j + 1];
           qf[n8][c * 4 + j][0] = x;
           qf[n8][c * 4 + j][1] = y;
 #pragma unroll
@@ -642,8 +646,6 @@ decode8_split_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
         const int row = n8 * 8 + 2 * t + h;
         if (g == 0) rs_s[warp][row] = rs[n8][h], ra_s[warp][row] = ra[n8][h], l_s[warp][row] = v;
       }
-    const int unit = sg.b * units_per_seq + sg.y;
-    const int n_parts = a.out != nullptr ? __ldcg(a.plan + DA_PLAN_HEAD + unit) : 0;       // (0: not merged here)
     bool going = true;
     for (int row0 = 0; row0 < n_rows; row0 += C::ROUND) {
       const int R = min(C::ROUND, n_rows - row0);
@@ -696,14 +698,40 @@ decode8_split_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
       // ---- the unit's last split merges them all
       all_of(true);
       if (tid == 0) {
-        __threadfence();
-        const int before = atomicAdd(a.counts + unit, 1);
+        int before;
+        asm volatile("atom.add.acq_rel.gpu.global.s32 %0, [%1], 1;" : "=r"(before) : "l"(a.counts + unit) : "memory");
         last_s = before == n_parts - 1;
         if (last_s) a.counts[unit] = 0;
-        __threadfence();
       }
       all_of(true);
-      if (last_s) {
+      constexpr int FEW = 16;
+      if (last_s && n_parts <= FEW) {
+        // few of them: maxima, sums and outputs all asked for at once
+        for (int i = tid; i < n_rows * (HD / 4); i += WARPS * 32) {
+          const int r = i / (HD / 4), d = (i - r * (HD / 4)) * 4;
+          const size_t p0 = ((size_t)sg.b * a.nq + row_head0 + r) * a.n_splits;
+          float2 ml[FEW];
+          float4 x[FEW];
+#pragma unroll
+          for (int u = 0; u < FEW; ++u) {
+            ml[u] = u < n_parts ? __ldcg(reinterpret_cast<const float2*>(a.part_ml) + p0 + u) : make_float2(-INFINITY, 0.f);
+            x[u] = u < n_parts ? __ldcg(reinterpret_cast<const float4*>(a.part_o + (p0 + u) * HD + d)) : make_float4(0.f, 0.f, 0.f, 0.f);
+          }
+          float M = -INFINITY;
+#pragma unroll
+          for (int u = 0; u < FEW; ++u) M = fmaxf(M, ml[u].x);
+          const float ref = M == -INFINITY ? 0.f : M;
+          float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+          float L = 0.f;
+#pragma unroll
+          for (int u = 0; u < FEW; ++u) {
+            const float f = fast_exp2(ml[u].x - ref);
+            L += ml[u].y * f;
+            v.x += x[u].x * f, v.y += x[u].y * f, v.z += x[u].z * f, v.w += x[u].w * f;
+          }
+          d8_finish(a.out + (size_t)sg.b * a.out_stride + (size_t)(row_head0 + r) * HD + d, v, ref, L, a.sinks, row_head0 + r);
+        }
+      } else if (last_s) {
         constexpr int MOST = C::MERGE / 8;               // (maximum, sum) pairs that the buffer holds
         float2* ml_s = reinterpret_cast<float2*>(o_s);
         const int R = max(1, min(n_rows, MOST / n_parts));
