@@ -53,9 +53,9 @@ __device__ __forceinline__ int da_blocks_used(int n_blocks, int room, int units_
   return max(1, min(n_blocks, (room - 2) * units_per_seq));
 }
 
-// Splits of a unit of P pages in the even cut: pages / share, rounded to the nearest (how 1) or down (how 2).
+// Splits of a unit of P pages in the even cut: pages / share, rounded to the nearest (how 1), down (how 2) or up (how 3).
 __device__ __forceinline__ int da_even_splits(int P, int share, int room, int how) {
-  return P > 0 ? max(1, min(room, (P + (how == 1 ? share / 2 : 0)) / share)) : 0;
+  return P > 0 ? max(1, min(room, (P + (how == 1 ? share / 2 : (how == 3 ? share - 1 : 0))) / share)) : 0;
 }
 
 // What a block loses at the end of a unit inside its run (merging, the next unit's queries, the first page's
@@ -111,18 +111,25 @@ __device__ __forceinline__ DaPlan da_plan(const int* slots, const int* lens, int
   const int total = carry * units_per_seq;
   pl.n_blocks = da_blocks_used(grid_blocks, room, units_per_seq, most);
   pl.share = max(1, (total + pl.n_blocks - 1) / pl.n_blocks);
-  // the even cut, rounding either way: how many splits in all, and the most pages of one
-  int items1 = 0, worst1 = 0, items2 = 0, worst2 = 0;
+  // the even cut, rounding either way: how many splits in all, and the most pages of one.  (Rounding up is the 8-bit cache's alone: its
+  // blocks are small and many, so that where the splits still fit them no block has more than its share.  8 sequences of 2,049 tokens, 4 kv
+  // heads, 296 blocks: 9 splits of up to 4 pages instead of 8 of up to 5,
+  // a layer 15.1 -> 14.3 us.)
+  const bool up = brk == D8_BREAK_PAGES;
+  int items1 = 0, worst1 = 0, items2 = 0, worst2 = 0, items3 = 0, worst3 = 0;
   for (int base = 0; base < batch; base += 32) {
     const int i = base + lane;
     const int P = base == 0 ? P_first : (i < batch ? da_pages(slots, lens, i, window, keep, shared) : 0);
     const int sp1 = da_even_splits(P, pl.share, room, 1), sp2 = da_even_splits(P, pl.share, room, 2);
+    const int sp3 = up ? da_even_splits(P, pl.share, room, 3) : 0;
     if (P > 0) {
       worst1 = max(worst1, (P + sp1 - 1) / sp1);
       worst2 = max(worst2, (P + sp2 - 1) / sp2);
+      if (up) worst3 = max(worst3, (P + sp3 - 1) / sp3);
     }
     items1 += sp1;
     items2 += sp2;
+    items3 += sp3;
   }
   items1 = __reduce_add_sync(0xffffffffu, items1);
   items2 = __reduce_add_sync(0xffffffffu, items2);
@@ -132,6 +139,11 @@ __device__ __forceinline__ DaPlan da_plan(const int* slots, const int* lens, int
   int how = 0, worst = 0;
   if (fits1 && (!fits2 || worst1 <= worst2)) how = 1, worst = worst1;
   else if (fits2) how = 2, worst = worst2;
+  if (up) {
+    items3 = __reduce_add_sync(0xffffffffu, items3);
+    worst3 = __reduce_max_sync(0xffffffffu, worst3);
+    if (items3 * units_per_seq <= grid_blocks && (how == 0 || worst3 < worst)) how = 3, worst = worst3;
+  }
   pl.even = (how != 0 && worst <= pl.share + brk) ? how : 0;
   if (!pl.even) {
     live = __reduce_add_sync(0xffffffffu, live);
