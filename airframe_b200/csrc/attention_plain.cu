@@ -6,6 +6,7 @@
 // for V.  A sequence's page table maps row / AF_PAGE to a page.  A layer with
 // a window keeps rows modulo `ring_rows` (a multiple of AF_PAGE, >= window), behind the pages of the sequence's
 // first `keep` tokens if the window keeps those in sight.
+#include "cache8.cuh"
 #include "common.cuh"
 
 #define AF_MAX_HD 640
@@ -33,14 +34,22 @@ __device__ __forceinline__ float rope_src(const T* row, const float* parts, int 
   return v;
 }
 
-template <typename T>
+// An 8-bit cache's pages (cache8.cuh).
+struct Rope8 {
+  uint8_t *k, *v, *k_exp, *v_exp;
+  long long n_pages;
+};
+
+// EIGHT (bfloat16 rows, blocks of hd / 2 threads): k and v go to the 8-bit cache as store_kv8 keeps them; a thread has at most a pair and
+// two elements beyond the rotary part.
+template <typename T, bool EIGHT>
 __global__ void rope_cache_kernel(T* __restrict__ qkv, int row_stride, const float* __restrict__ parts,
                                   int n_parts, size_t part_stride, const int* __restrict__ positions,
                                   const int* __restrict__ seq_of_token, const int* __restrict__ slots,
                                   const int* __restrict__ len_after, const float* __restrict__ inv_freq,
                                   int nq, int nkv, int hd, int rot_dim, int pairing,
                                   T* __restrict__ kcache, T* __restrict__ vcache,
-                                  const int* __restrict__ page_table, int max_pages, int ring_rows, int keep) {
+                                  const int* __restrict__ page_table, int max_pages, int ring_rows, int keep, Rope8 c8) {
   pdl_launch_dependents();
   // Positions, slots, lengths, the page table and the frequencies are inputs of the step, not
   // results of the kernel before: the row's place in the cache and the first pair's sine and
@@ -52,18 +61,23 @@ __global__ void rope_cache_kernel(T* __restrict__ qkv, int row_stride, const flo
   const int half = rot_dim / 2;
   // where this head's row goes in the cache (k and v heads only)
   T* dst = nullptr;
-  if (kcache != nullptr && head >= nq) {
+  long long row8 = -1;
+  if ((EIGHT || kcache != nullptr) && head >= nq) {
     const int seq = seq_of_token[t];
     const int slot = slots[seq];
     // of the tokens of this step that share a ring row only the last is kept; padding rows are skipped
     if (slot >= 0 && af_cache_stores(pos, len_after[seq], ring_rows, keep)) {
       const int r = af_cache_row(pos, ring_rows, keep);
-      if (AF_INDEX_OK(pos >= 0 && r / AF_PAGE < max_pages, r)) {
+      if (AF_INDEX_OK(pos >= 0 && r / AF_PAGE < max_pages, r) && (!EIGHT || (pos >= 0 && r / AF_PAGE < max_pages))) {
         const int page = page_table[(size_t)slot * max_pages + r / AF_PAGE];
         const bool is_v = head >= nq + nkv;
         const int h = head - nq - (is_v ? nkv : 0);
-        if (AF_INDEX_OK(page >= 0, page))
+        if constexpr (EIGHT) {
+          if (AF_INDEX_OK(page >= 0 && page < c8.n_pages, page) && page >= 0 && page < c8.n_pages)      // (a bad page is not written)
+            row8 = ((long long)page * nkv + h) * AF_PAGE + r % AF_PAGE;
+        } else if (AF_INDEX_OK(page >= 0, page)) {
           dst = (is_v ? vcache : kcache) + (((size_t)page * nkv + h) * AF_PAGE + r % AF_PAGE) * hd;
+        }
       }
     }
   }
@@ -73,6 +87,8 @@ __global__ void rope_cache_kernel(T* __restrict__ qkv, int row_stride, const flo
   pdl_wait();
   pr = pdl_fresh(pr);
   row = pdl_fresh(row);
+  uint32_t el[4] = {0, 0, 0, 0};      // (EIGHT) this thread's elements of the row, and which they are
+  int at[4] = {-1, -1, -1, -1};
   // rotary pairs
   for (int p = threadIdx.x; p < half; p += blockDim.x) {
     const int i0 = pairing == AF_PAIR_HALF ? p : 2 * p;
@@ -91,6 +107,10 @@ __global__ void rope_cache_kernel(T* __restrict__ qkv, int row_stride, const flo
       row[i0] = ta;
       row[i1] = tb;
     }
+    if constexpr (EIGHT) {
+      el[0] = *reinterpret_cast<const uint16_t*>(&ta), el[1] = *reinterpret_cast<const uint16_t*>(&tb);
+      at[0] = i0, at[1] = i1;
+    }
     if (dst != nullptr) {
       dst[i0] = ta;
       dst[i1] = tb;
@@ -101,6 +121,38 @@ __global__ void rope_cache_kernel(T* __restrict__ qkv, int row_stride, const flo
     const T v = from_f32<T>(rope_src(row, pr, n_parts, part_stride, i));
     if (pr != nullptr) row[i] = v;
     if (dst != nullptr) dst[i] = v;
+    if constexpr (EIGHT) {
+      const int x = at[2] < 0 ? 2 : 3;
+      el[x] = *reinterpret_cast<const uint16_t*>(&v);
+      at[x] = i;
+    }
+  }
+  if constexpr (EIGHT) {
+    if (head < nq) return;
+    // the row's largest finite magnitude, its exponent, the codes
+    __shared__ uint32_t top_s[8];
+    uint32_t top = 0;
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {
+      const uint32_t m = el[x] & 0x7fffu;
+      top = max(top, m < 0x7f80u ? m : 0u);
+    }
+    top = __reduce_max_sync(0xffffffffu, top);
+    if ((threadIdx.x & 31) == 0) top_s[threadIdx.x >> 5] = top;
+    __syncthreads();
+    for (int w = 0; w < (int)blockDim.x >> 5; ++w) top = max(top, top_s[w]);
+    if (row8 < 0) return;
+    const bool is_v = head >= nq + nkv;
+    const int e = c8_exponent(top << 16);
+    const float inv = c8_pow2(-e);
+    uint8_t* codes = (is_v ? c8.v : c8.k) + (size_t)row8 * hd;
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {
+      if (at[x] < 0) continue;
+      const float f = __uint_as_float(el[x] << 16) * inv;
+      codes[at[x]] = (uint8_t)c8_pack2(isfinite(f) ? f : __uint_as_float(0x7fc00000u), 0.f);
+    }
+    if (threadIdx.x == 0) (is_v ? c8.v_exp : c8.k_exp)[row8] = (uint8_t)(e + 127);
   }
 }
 
@@ -307,12 +359,42 @@ AF_EXPORT int af_rope_cache_write(void* qkv, int dtype, int row_stride, const fl
     AF_CHECK_LAUNCH("af_rope_cache_write");
   }
   AF_DISPATCH_DTYPE(dtype, T,
-                    af_launch(rope_cache_kernel<T>, dim3(dim3(n_tokens, nq + 2 * nkv)), dim3(hd / 2 < 32 ? 32 : (hd / 2 > 256 ? 256 : hd / 2)), 0, stream, 
+                    af_launch(rope_cache_kernel<T, false>, dim3(dim3(n_tokens, nq + 2 * nkv)), dim3(hd / 2 < 32 ? 32 : (hd / 2 > 256 ? 256 : hd / 2)), 0, stream, 
                         (T*)qkv, row_stride, parts, n_parts, (size_t)part_stride, positions, seq_of_token,
                         slots, len_after, inv_freq, nq,
                         nkv, hd, rot_dim, pairing, (T*)kcache, (T*)vcache, page_table, max_pages,
-                        ring_rows, keep));
+                        ring_rows, keep, Rope8{}));
   AF_CHECK_LAUNCH("af_rope_cache_write");
+}
+
+// What af_rope_store_kv8 is given, as one block of 64-bit words.
+struct AfRopeStore8 {
+  void* qkv;
+  const float* parts;
+  const int *positions, *seq_of_token, *slots, *len_after;
+  const float* inv_freq;
+  const int* page_table;
+  uint8_t *k, *v, *k_exp, *v_exp;
+  cudaStream_t stream;
+  long long row_stride, n_parts, part_stride, n_tokens, nq, nkv, hd, rot_dim, pairing, max_pages, n_pages, ring_rows, keep;
+};
+
+// af_rope_cache_write of bfloat16 rows and af_store_kv8 in one kernel, for the few rows of decode steps: the same rows, codes and exponents.
+AF_EXPORT int af_rope_store_kv8(const AfRopeStore8* c) {
+  if (c->n_tokens == 0) return 0;
+  AF_REQUIRE(c->n_tokens > 0 && c->n_tokens < (1ll << 31) && c->nq > 0 && c->nkv > 0 && c->nq + 2 * c->nkv < 65536,
+             "af_rope_store_kv8: %lld tokens, %lld heads, %lld kv heads", c->n_tokens, c->nq, c->nkv);
+  AF_REQUIRE(c->hd == 64 || c->hd == 128 || c->hd == 256, "af_rope_store_kv8: head_dim %lld (takes 64, 128, 256)", c->hd);
+  AF_REQUIRE(c->rot_dim >= 0 && c->rot_dim <= c->hd && c->rot_dim % 2 == 0, "af_rope_store_kv8: rotary dim %lld must be even and <= head_dim", c->rot_dim);
+  AF_REQUIRE(c->pairing == AF_PAIR_HALF || c->pairing == AF_PAIR_ADJACENT, "af_rope_store_kv8: pairing");
+  AF_REQUIRE(c->ring_rows >= 0 && c->ring_rows % AF_PAGE == 0 && c->keep >= 0 && c->max_pages > 0 && c->n_pages > 0,
+             "af_rope_store_kv8: ring rows %lld, %lld kept, %lld page entries", c->ring_rows, c->keep, c->max_pages);
+  af_launch(rope_cache_kernel<__nv_bfloat16, true>, dim3((unsigned)c->n_tokens, (unsigned)(c->nq + 2 * c->nkv)), dim3((unsigned)c->hd / 2), 0, c->stream,
+            (__nv_bfloat16*)c->qkv, (int)c->row_stride, c->parts, (int)c->n_parts, (size_t)c->part_stride, c->positions, c->seq_of_token, c->slots,
+            c->len_after, c->inv_freq, (int)c->nq, (int)c->nkv, (int)c->hd, (int)c->rot_dim, (int)c->pairing, (__nv_bfloat16*)nullptr,
+            (__nv_bfloat16*)nullptr, c->page_table, (int)c->max_pages, (int)c->ring_rows, (int)c->keep,
+            Rope8{c->k, c->v, c->k_exp, c->v_exp, c->n_pages});
+  AF_CHECK_LAUNCH("af_rope_store_kv8");
 }
 
 // ---------------------------------------------------------------- tables of a step

@@ -338,6 +338,7 @@ CACHE8_HEAD_SIZES = (64, 128, 256)     # head sizes that the 8-bit cache takes
 # What the entry points below take as one block of 64-bit words (pointers, whole numbers, then 64-bit floats): a ctypes argument
 # costs the host some 0.3 us, a packed one 0.05.
 _STORE8 = struct.Struct("<12Q10q")
+_ROPE_STORE8 = struct.Struct("<13Q13q")
 _DECODE8 = struct.Struct("<14Q13q2d")
 _SHARED = struct.Struct("<17Q11q2d")
 
@@ -393,6 +394,32 @@ def store_kv8(qkv, batch, nq: int, nkv: int, hd: int, kv, rounded=None) -> None:
         qkv.data_ptr(), 0 if rounded is None else rounded.data_ptr(), positions.data_ptr(), seq.data_ptr(), slots.data_ptr(), lens.data_ptr(),
         table.data_ptr(), kv.k.data_ptr(), kv.v.data_ptr(), kv.k_exp.data_ptr(), kv.v_exp.data_ptr(), _raw_stream(dev),
         _rows(qkv, "qkv"), 0 if rounded is None else _rows(rounded, "rounded"), n_pages, table.shape[1], kv.ring_rows, kv_keep(kv), T, nq, nkv, hd)))
+
+
+def rope_store_kv8(qkv, batch, inv_freq, nq: int, nkv: int, hd: int, rot_dim: int, pairing: str, kv, parts=None) -> None:
+    """:func:`rope_cache_write` of bfloat16 rows (without a cache) and :func:`store_kv8` in one kernel, for the few rows of a decode
+    step: the same rows, codes and exponents."""
+    T = qkv.shape[0]
+    width = (nq + 2 * nkv) * hd
+    if qkv.dtype != torch.bfloat16 or qkv.shape != (T, width):
+        raise KernelError(f"rope_store_kv8: bfloat16 rows of (nq + 2 nkv) * head_dim = {width}, got {qkv.dtype} {tuple(qkv.shape)}")
+    if pairing not in PAIRINGS or inv_freq.numel() != rot_dim // 2 or rot_dim % 2:
+        raise KernelError(f"rope_store_kv8: pairing '{pairing}', {inv_freq.numel()} frequencies for a rotation of {rot_dim}")
+    if parts is not None and (parts.dtype != torch.float32 or parts.shape[1:] != (T, width) or len(parts) < 1 or not parts[0].is_contiguous()):
+        raise KernelError(f"rope_store_kv8: parts must be float32 [splits, {T}, {width}]")
+    positions, seq, slots, lens, table = batch.positions, batch.seq_of_token, batch.slots, batch.len_after, kv.page_table
+    if positions.numel() != T or seq.numel() != T or slots.numel() != lens.numel():
+        raise KernelError(f"rope_store_kv8: {T} rows, {positions.numel()} positions, {seq.numel()} places of sequences")
+    n_pages = _cache8_pages(kv, nkv, hd, "rope_store_kv8")
+    _typed("rope_store_kv8", torch.int32, positions=positions, seq_of_token=seq, slots=slots, len_after=lens, page_table=table)
+    _typed("rope_store_kv8", torch.float32, inv_freq=inv_freq)
+    dev = _here("rope_store_kv8", qkv, positions, seq, slots, lens, table, inv_freq, kv.k, kv.v, kv.k_exp, kv.v_exp,
+                *(() if parts is None else (parts,)))
+    _check(_lib().af_rope_store_kv8(_ROPE_STORE8.pack(
+        qkv.data_ptr(), 0 if parts is None else parts.data_ptr(), positions.data_ptr(), seq.data_ptr(), slots.data_ptr(), lens.data_ptr(),
+        inv_freq.data_ptr(), table.data_ptr(), kv.k.data_ptr(), kv.v.data_ptr(), kv.k_exp.data_ptr(), kv.v_exp.data_ptr(), _raw_stream(dev),
+        _rows(qkv, "qkv"), 0 if parts is None else parts.shape[0], 0 if parts is None else parts.stride(0), T, nq, nkv, hd, rot_dim,
+        PAIRINGS[pairing], table.shape[1], n_pages, kv.ring_rows, kv_keep(kv))))
 
 
 def sum_parts(qkv, parts, batch, nq: int, nkv: int, hd: int) -> None:

@@ -286,6 +286,7 @@ class Attention(Mixer):
         nq, nkv, hd = self.nq, self.nkv, self.hd
         kv = view.kv
         gate = None
+        stored = False
         if self.packs:
             qkv, gate = self._project_norm_pack(x, batch, view)
         elif self.rope_epilogue:
@@ -298,11 +299,12 @@ class Attention(Mixer):
                 qkv = torch.empty(x.shape[0], (nq + 2 * nkv) * hd, dtype=x.dtype, device=x.device)
             # positions into q and k, then k and v into the cache: the store is this mixer's; an encoding
             # that can do both in one kernel says so
-            if not view.writes or self.eight_bits:
+            if view.writes and (not self.eight_bits or (self.position.stores_eight_bits and not batch.is_prefill)):
+                stored = self.position.encode_and_store(qkv, batch, nq, nkv, hd, kv, parts=parts)
+            if not stored:
                 self.position.encode(qkv, batch, nq, nkv, hd, parts=parts)
-            elif not self.position.encode_and_store(qkv, batch, nq, nkv, hd, kv, parts=parts):
-                self.position.encode(qkv, batch, nq, nkv, hd, parts=parts)
-                kernels.store_kv(qkv, batch, nq, nkv, hd, kv)
+                if view.writes and not self.eight_bits:
+                    kernels.store_kv(qkv, batch, nq, nkv, hd, kv)
         slopes = self.position.score_slopes(nq)
         dv = self.dv
         if self.pad:                 # (from here on the heads are what the packing kernel made of them)
@@ -310,7 +312,7 @@ class Attention(Mixer):
         q = qkv[:, : nq * hd]
         k = qkv[:, nq * hd: (nq + nkv) * hd]
         v = qkv[:, (nq + nkv) * hd:]
-        if self.eight_bits and view.writes:
+        if self.eight_bits and view.writes and not stored:
             rounded = torch.empty(x.shape[0], 2 * nkv * hd, dtype=x.dtype, device=x.device) if batch.is_prefill else None
             kernels.store_kv8(qkv, batch, nq, nkv, hd, kv, rounded=rounded)
             if batch.is_prefill:

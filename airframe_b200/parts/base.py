@@ -200,6 +200,9 @@ class PositionEncoding(Part):
         (kept in ``batch.aux``) for all layers that rotate alike."""
         raise NotImplementedError
 
+    # whether encode_and_store knows caches of 8 bits too (``kv.k_exp``), for decode steps
+    stores_eight_bits = False
+
     def encode_and_store(self, qkv, batch, nq: int, nkv: int, hd: int, kv, parts=None) -> bool:
         """Optional fast path: :meth:`encode` and the mixer's cache store in one
         kernel.  Returns False when the encoding has none (the mixer then calls

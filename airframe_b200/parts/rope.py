@@ -134,12 +134,17 @@ class Rope(PositionEncoding):
             return self.rotary_table(batch, hd)
         return None
 
+    stores_eight_bits = True
+
     def encode_and_store(self, qkv, batch, nq, nkv, hd, kv, parts=None) -> bool:
         """The rotation and the mixer's cache store as one kernel (the rotated
         k rows are what the cache keeps)."""
         self._plain_only()
         if self.rotary_dim > hd:
             raise ConfigError(f"rope: rotary_dim {self.rotary_dim} exceeds head_dim {hd}")
+        if kv.k_exp is not None:
+            kernels.rope_store_kv8(qkv, batch, self.inv_freq, nq, nkv, hd, self.rotary_dim, self.pairing, kv, parts=parts)
+            return True
         table = self._prompt_table(qkv, batch, hd, parts)
         kernels.rope_cache_write(qkv, batch.positions, self.inv_freq, nq, nkv, hd, self.rotary_dim,
                                  self.pairing, seq_of_token=batch.seq_of_token, slots=batch.slots,

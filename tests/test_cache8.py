@@ -168,6 +168,44 @@ def test_store(K, hd, nq, nkv, before, new, ring, keep, rounded):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("hd,nq,nkv", [(64, 3, 3), (128, 8, 2), (256, 8, 4)])
+@pytest.mark.parametrize("rot,pairing", [(1.0, "half"), (1.0, "adjacent"), (0.25, "half"), (0.0, "half")])
+@pytest.mark.parametrize("splits", [0, 1, 19])
+def test_rotate_and_store(K, hd, nq, nkv, rot, pairing, splits):
+    """One kernel gives the rows, codes and exponents that the rotation and the store give, to the bit: a ring with kept tokens, padding
+    rows, rows of zeros and of infinities."""
+    before, ring, keep = [0, 63, 64, 700, 129, 5, 8], 192, 5
+    lens = [n + 1 for n in before]
+    rot_dim = int(hd * rot) // 2 * 2
+    width = (nq + 2 * nkv) * hd
+    src = hard_rows(len(lens) + 2, width).to(DEV)
+    parts = (src.float()[None] * torch.rand(splits, 1, 1, device=DEV)).contiguous() if splits else None
+    inv = (10000.0 ** (-torch.arange(rot_dim // 2).float() / max(1, rot_dim // 2))).to(DEV)
+    got = []
+    for fused in (False, True):
+        torch.manual_seed(3)
+        view = View(lens, nkv, hd, ring, keep)
+        b = store_batch(view, before, [1] * len(lens), DEV)
+        pad = lambda t, v: torch.cat([t, torch.full((2,), v, dtype=torch.int32, device=DEV)])
+        b.positions, b.slots, b.len_after = pad(b.positions, 0), pad(b.slots, -1), pad(b.len_after, 0)
+        b.seq_of_token = torch.arange(len(lens) + 2, dtype=torch.int32, device=DEV)
+        view.to(DEV)
+        wide = torch.full((len(lens) + 2, width + 8), 7.0, dtype=torch.bfloat16, device=DEV)
+        qkv = wide[:, :width]
+        if not splits:
+            qkv.copy_(src)
+        if fused:
+            K.rope_store_kv8(qkv, b, inv, nq, nkv, hd, rot_dim, pairing, view, parts=parts)
+        else:
+            K.rope_cache_write(qkv, b.positions, inv, nq, nkv, hd, rot_dim, pairing, parts=parts)
+            K.store_kv8(qkv, b, nq, nkv, hd, view)
+        got.append([wide.view(torch.int16), *(t.view(torch.uint8) for t in (view.k, view.v, view.k_exp, view.v_exp))])
+    for x, y in zip(*got):
+        assert torch.equal(x, y)
+    K.check_device_errors(DEV)
+
+
+@pytest.mark.gpu
 def test_store_extremes(K):
     """The largest and the smallest bfloat16 values: no code overflows, exponents stay in range."""
     hd, nkv = 64, 1
@@ -461,6 +499,14 @@ def test_refusals(K):
         K.store_kv8(x, b, nq, nkv, hd, view, rounded=torch.zeros(70, 3, dtype=torch.bfloat16))
     with pytest.raises(K.KernelError, match="CUDA device"):
         K.store_kv8(x, b, nq, nkv, hd, view)
+    inv = torch.ones(hd // 2)
+    for bad, match in ((dict(qkv=x.float()), "bfloat16 rows"), (dict(pairing="none"), "pairing"), (dict(rot_dim=32), "frequencies"),
+                       (dict(qkv=x[:5]), "positions"), (dict(parts=torch.zeros(0, 70, x.shape[1])), "parts"),
+                       (dict(parts=torch.zeros(2, 70, x.shape[1], dtype=torch.bfloat16)), "parts"), (dict(inv_freq=inv.double()), "inv_freq"),
+                       ({}, "CUDA device")):
+        args = dict(dict(qkv=x, inv_freq=inv, rot_dim=hd, pairing="half", parts=None), **bad)
+        with pytest.raises(K.KernelError, match=match):
+            K.rope_store_kv8(args["qkv"], b, args["inv_freq"], nq, nkv, hd, args["rot_dim"], args["pairing"], view, parts=args["parts"])
     d = step(view, [70], "cpu")
     q, out = torch.zeros(1, nq * hd, dtype=torch.bfloat16), torch.zeros(1, nq * hd, dtype=torch.bfloat16)
     with pytest.raises(K.KernelError, match="slopes"):
