@@ -122,7 +122,8 @@ class KVGroup:
         pages = torch.tensor([self.held[src][whole:n], new], device=self.k.device)      # (a ring's pages, many of them, move together)
         for t in (self.k, self.v, self.k_exp, self.v_exp):
             if t is not None:
-                t = t.view(torch.uint8)
+                row = t.shape[-1] * t.element_size()      # (moved in the widest words that a row is made of)
+                t = t.view(next(d for d, b in ((torch.int64, 8), (torch.int32, 4), (torch.int16, 2), (torch.uint8, 1)) if row % b == 0))
                 t.index_copy_(1, pages[1], t.index_select(1, pages[0]))
 
     def release(self, slot: int) -> None:
