@@ -804,14 +804,16 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
 
 // ---------------------------------------------------------------- merge
 
-// Two warps: a thread has up to eight loads of partial results on their way, and more threads a block only keep other blocks out.  (A layer of 128
-// sequences of 32 heads of 128, 4 items each: with 256, 128 and 64 threads 67.3, 58.6 and 58.6 us in all; 64 sequences of 8 heads of 256, 20
-// items: 44.3, 46.0 and 44.5.)
-constexpr int SHM_THREADS = 64, SHM_MOST = 1024;     // partial results of a (sequence, head) that the block weighs
+// Threads: four rows of partial results side by side (heads of 256: 256 threads, of 128: 128), with up to eight loads a thread on their way; with more
+// blocks than the SMs hold of the large ones two side by side.  (A layer in all, us, 256 / 128 / 64 threads: 64 sequences of 8 heads of 256, 20 items each
+// 45.4 / 46.0 / 48.2, 128 sequences of them 47.3 / 44.3 / -; 32 sequences of 32 heads of 128, 18 items 64.3 / 61.4 / 63.3, 128 sequences of
+// them 67.3 / 58.6 / -.)
+constexpr int SHM_LARGE_AN_SM = 4;
+constexpr int SHM_MOST = 1024;     // partial results of a (sequence, head) that the block weighs
 
 // out[b, h] from the items of the shared pages and the splits of the sequence's own.
-template <int HD>
-__global__ void __launch_bounds__(SHM_THREADS)
+template <int HD, int THREADS>
+__global__ void __launch_bounds__(THREADS)
 attn_shared_merge_kernel(__nv_bfloat16* __restrict__ out, long long out_stride, const float* pre_o, const float* pre_ml, const float* own_o,
                          const float* own_ml, int nq, int nkv, int own_room, const int* __restrict__ shared_plan, const int* __restrict__ own_plan,
                          int blocks, const float* __restrict__ sinks) {
@@ -834,11 +836,11 @@ attn_shared_merge_kernel(__nv_bfloat16* __restrict__ out, long long out_stride, 
   }
   const size_t own0 = ((size_t)b * nq + h) * own_room;
   __shared__ float f_s[SHM_MOST], l_s[SHM_MOST];
-  __shared__ float4 red_s[SHM_THREADS];
+  __shared__ float4 red_s[THREADS];
   pdl_wait();
   pre_o = pdl_fresh(pre_o), pre_ml = pdl_fresh(pre_ml), own_o = pdl_fresh(own_o), own_ml = pdl_fresh(own_ml);
   const int n = n_own + n_pre;         // (own splits first)
-  constexpr int ROW = HD / 4, GROUPS = SHM_THREADS / ROW;
+  constexpr int ROW = HD / 4, GROUPS = THREADS / ROW;
   const int grp = tid / ROW, d = (tid - grp * ROW) * 4;
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
   float M = sinks ? sinks[h] * 1.4426950408889634f : -INFINITY, Ls = sinks ? 1.f : 0.f;
@@ -847,7 +849,7 @@ attn_shared_merge_kernel(__nv_bfloat16* __restrict__ out, long long out_stride, 
     const int m = min(SHM_MOST, n - base);
     __syncthreads();
     float mine = -INFINITY;
-    for (int i = tid; i < m; i += SHM_THREADS) {
+    for (int i = tid; i < m; i += THREADS) {
       const int x = base + i;
       const float2 ml = __ldcg(reinterpret_cast<const float2*>(x < n_own ? own_ml + (own0 + x) * 2 : pre_ml + (pre0 + (size_t)(x - n_own) * rows) * 2));
       f_s[i] = ml.x;
@@ -1020,8 +1022,12 @@ AF_EXPORT int af_attn_decode_shared(const AfShared* c) {
     rc = af_decode16_split(c->q, c->q_stride, c->k, c->v, c->n_pages, page_table, max_pages, slots, lens, c->plan + L.shared, batch, nq, nkv, hd,
                            a.scale, a.cap, n_splits, c->own_scratch, c->plan + at, own_blocks(16, sms, nq, nkv), c->err, c->stream);
   if (rc) return rc;
-  const auto merge = hd == 64 ? attn_shared_merge_kernel<64> : (hd == 128 ? attn_shared_merge_kernel<128> : attn_shared_merge_kernel<256>);
-  af_launch(merge, dim3(batch, nq), dim3(SHM_THREADS), 0, c->stream, (__nv_bfloat16*)c->out, c->out_stride, (const float*)a.part_o,
+  const bool large = hd == 256 && (long long)batch * nq <= (long long)SHM_LARGE_AN_SM * sms;
+  const auto merge = hd == 64    ? attn_shared_merge_kernel<64, 128>
+                     : hd == 128 ? attn_shared_merge_kernel<128, 128>
+                     : large     ? attn_shared_merge_kernel<256, 256>
+                                 : attn_shared_merge_kernel<256, 128>;
+  af_launch(merge, dim3(batch, nq), dim3(large ? 256 : 128), 0, c->stream, (__nv_bfloat16*)c->out, c->out_stride, (const float*)a.part_o,
             (const float*)a.part_ml, (const float*)c->own_scratch, (const float*)c->own_scratch + (size_t)batch * nq * n_splits * hd, nq, nkv,
             n_splits, (const int*)c->plan, (const int*)c->plan + at, sms, (const float*)c->sinks);
   AF_CHECK_LAUNCH("af_attn_decode_shared (merge)");
