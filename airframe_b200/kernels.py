@@ -1157,12 +1157,12 @@ def attn_decode_shared_pays(groups, nkv: int, hd: int, eight_bits: bool = False)
     sequences but one, and in the 8-bit cache, whose codes the shared kernel converts (0.9 us a page and block, of which the
     tensor-core products and the softmax take most) and the ordinary one reads at the memory's rate, but four.  Measured a layer of steps that make their
     plan once (ordinary / shared, us), kv heads x head size 4 x 256 and 8 x 128:
-    bfloat16, 8 sequences: 32 pages 13.1 / 17.0 and 14.6 / 19.6, 64 pages 19.4 / 18.2 and 23.5 / 21.2, 128 pages 32.0 / 21.2 and
-    38.2 / 23.5; 64 sequences: 8 pages 26.9 / 27.2 and 35.1 / 39.9, 16 pages 37.8 / 30.3 and 49.2 / 41.9; 2 sequences: 512 pages 33.7 / 37.8
-    and 38.2 / 35.4, 2,048 pages 159 / 96 and 158 / 88.
-    8 bits, 8 sequences: 64 pages 22.8 / 27.6 and 18.7 / 23.0, 128 pages 30.0 / 29.9 and 26.9 / 25.1, 256 pages 46.1 / 37.6 and
-    43.0 / 31.7; 128 sequences: 8 pages 45.9 / 52.2 and 45.6 / 60.1, 16 pages 62.3 / 55.1 and 60.2 / 61.8; 4 sequences: 512 pages 47.2 / 52.1
-    and 40.1 / 47.1."""
+    bfloat16, 8 sequences: 32 pages 12.7 / 16.9 and 14.6 / 19.4, 64 pages 19.2 / 17.9 and 23.3 / 20.7, 128 pages 31.8 / 21.1 and
+    37.8 / 23.3; 64 sequences: 8 pages 27.1 / 27.3 and 35.3 / 35.1, 16 pages 37.9 / 30.2 and 49.1 / 36.1; 2 sequences: 512 pages 32.8 / 37.3
+    and 38.4 / 33.8, 2,048 pages 157 / 96 and 158 / 88.
+    8 bits, 8 sequences: 64 pages 20.1 / 26.9 and 18.2 / 22.3, 128 pages 28.5 / 29.7 and 26.6 / 25.3, 256 pages 45.1 / 37.1 and
+    43.1 / 32.3; 128 sequences: 8 pages 44.6 / 48.4 and 45.8 / 51.5, 16 pages 61.2 / 51.4 and 60.4 / 53.0; 4 sequences: 512 pages 47.0 / 49.1
+    and 40.2 / 44.3."""
     members = sum(m for m, _ in groups)
     spared = sum(n * (m - (4 if eight_bits else 1)) for m, n in groups)
     return spared * nkv * hd >= 1024 * (512 + 10 * members if eight_bits else 384 + 4 * members)
