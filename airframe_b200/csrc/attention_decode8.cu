@@ -7,8 +7,9 @@
 // warp's 8 KB are many products (of 16 keys by 8 heads, 16 by 16 by 8 at a time) in a dependent chain from score to output, so it is
 // the number of warps with a chain at work that feeds the memory: two blocks of seven computing warps an SM, as the registers
 // allow.  Measured (1 sequence of 131,072 tokens, 8 kv heads of 128, 4 heads each; 64 sequences of up to 8,192 tokens and a window of
-// 4,096, 8 kv heads of 256, 2 heads each): 53.2 and 76.3 us, 5.1 and 4.1 TB/s; with one such block an SM 59.7 and 105.  Bound by the memory's rate at long lengths; below some
-// 1,000 tokens by the plan and the two launches (13.0 us at 700 tokens).
+// 4,096, 8 kv heads of 256, 2 heads each): 53 and 74 us, 5.1 and 4.2 TB/s; with one such block an SM 60 and 105.  Bound by the memory's rate at long lengths.  At short ones by the
+// chain of a block: 8 sequences of 2,049 tokens, 4 kv heads of 256, take 14.3 us a layer of a step that has its plan (queries 1, four pages 4.5, the
+// warps' join 2.3, the count of a unit's splits 1.5, their join 0.8, the boundary to the kernel before), 1 of 701 8.5.
 // Groups of 9 to 16 heads take twice the accumulators and one block an SM: 8 sequences of 16,384 tokens, 2 kv heads of 16 heads each: 31% of
 // a copy's rate with heads of 128, 40% with 256.
 //
