@@ -41,6 +41,8 @@ class Engine:
         self.cache = SequenceCache(model.cache_needs(), max_tokens, self.max_context,
                                    dtype=model.ctx.compute_dtype, device=self.device,
                                    max_sequences=max_sequences)
+        # the most sequences that a step may carry (None: any number): what the 8-bit cache's attention plans for
+        self.max_step_sequences = (kernels.ATTN_DECODE_MAX_SEQS if any(g.need.eight_bits for g in self.cache.groups.values()) else None)
         self.vocab_size = model.spec.vocab_size
         # decode steps of models whose parts allow it are captured into CUDA graphs,
         # one per padded batch size
@@ -88,6 +90,7 @@ class Engine:
         """Validate a step; returns each sequence's length before it."""
         if not entries:
             raise StepError("a step needs at least one sequence")
+        self._check_rows(len(entries))
         seen = set()
         lens = []
         for e in entries:
@@ -112,6 +115,10 @@ class Engine:
         if not all(starting) and any(len(e.tokens) != 1 for e in entries):
             raise StepError("sequences that go on bring one token each")
         return lens
+
+    def _check_rows(self, n: int) -> None:
+        if self.max_step_sequences is not None and n > self.max_step_sequences:
+            raise StepError(f"a step of this model carries up to {self.max_step_sequences} sequences (its cache is in 8 bits), not {n}")
 
     fused_greedy = True     # step(..., greedy=True) and decode_rows(..., greedy=True) give tokens instead of logits
 
@@ -167,6 +174,7 @@ class Engine:
         live = [s for s in slots if s is not None]
         if not live or len(set(live)) != len(live):
             raise StepError("decode_rows needs at least one sequence, each slot once")
+        self._check_rows(len(slots))
         try:
             lens = [self.cache.length(s) if s is not None else 0 for s in slots]
         except PoolError as err:

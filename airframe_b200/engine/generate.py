@@ -110,6 +110,9 @@ class GenerationLoop:
         whole pages once, where the cache says so)."""
         total_pages = self.engine.cache.total_pages
         limit = self.engine.cache.n_slots
+        most = getattr(self.engine, "max_step_sequences", None)
+        if most is not None:
+            limit = min(limit, most)
         if self.max_batch:
             limit = min(limit, self.max_batch)
         # a cache whose groups of layers have storage of their own answers for each of them

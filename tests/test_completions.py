@@ -189,6 +189,33 @@ def test_batches_of_completions_share_only_what_is_in_the_batch():
     assert got == [list(range(6)), list(range(6, 12))]
     got = loop.plan_batches([[1] * 320] * 9, params, 9)   # 5 whole pages: 5 + 7 fit
     assert got == [list(range(7)), [7, 8]]
+    Eng.max_step_sequences = 3
+    assert loop.plan_batches([[1] * 64] * 7, SamplingParams(max_tokens=1), 7) == [[0, 1, 2], [3, 4, 5], [6]]
+
+
+@pytest.mark.gpu
+def test_a_step_of_too_many_sequences_is_refused(tmp_path):
+    """The 8-bit cache's attention plans for a number of sequences: more are refused before anything changes, and a loop makes batches."""
+    from airframe_b200.engine import StepEntry, StepError
+    from airframe_b200.sampling import SamplingParams
+    cfg = dict(CONFIGS["D"], max_position_embeddings=512)
+    rt = _runtime(tmp_path, cfg, "bfloat16", kv_dtype="float8_e4m3")
+    eng = rt.engine
+    assert eng.max_step_sequences == 2048 and _runtime(tmp_path, cfg, "bfloat16").engine.max_step_sequences is None
+    eng.max_step_sequences = 2
+    slots = [eng.take_slot() for _ in range(3)]
+    with pytest.raises(StepError, match="up to 2 sequences"):
+        eng.step([StepEntry(s, [1, 2, 3], [2]) for s in slots])
+    assert [eng.length(s) for s in slots] == [0, 0, 0]
+    eng.step([StepEntry(s, [1, 2, 3], [2]) for s in slots[:2]])
+    eng.step([StepEntry(slots[2], [1, 2, 3], [2])])
+    with pytest.raises(StepError, match="up to 2 sequences"):
+        eng.decode_rows(slots, torch.ones(3, dtype=torch.int32, device=eng.device))
+    assert [eng.length(s) for s in slots] == [3, 3, 3]
+    for s in slots:
+        eng.free_slot(s)
+    outs = rt.generate([[1, 2], [3], [4, 5, 6], [7]], SamplingParams(max_tokens=3, temperature=0.0, ignore_eos=True))
+    assert [len(o) for o in outs] == [3] * 4
 
 
 def test_fits_counts_shared_pages_once():
