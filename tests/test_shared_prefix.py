@@ -318,3 +318,36 @@ def test_other_paths(K):
     f.ring_rows = 0
     with pytest.raises(K.KernelError, match="lead"):
         K.attn_decode_shared(out, q.float().to(DEV), f, f.step(), 4, 2, 64, 0.125, 0.0, l[:1], p, 3)
+
+
+@pytest.mark.parametrize("bits", [16, 8])
+def test_two_streams_at_once(K, bits):
+    """Steps of two batches (shared prefixes, and sequences on their own) that run side by side give what each gives alone."""
+    jobs = []
+    for hd, seqs in ((128, [(0, 20, 1400 + 9 * i) for i in range(12)]), (256, [(i % 3, 6, 500 + 31 * i) for i in range(9)])):
+        nq, nkv = 8, 4
+        f = Family(seqs, nkv, hd, bits)
+        q = torch.randn(len(seqs), nq * hd).to(torch.bfloat16).to(DEV)
+        lead, pages = f.lead()
+
+        def run(f=f, q=q, lead=lead, pages=pages, hd=hd, most=max(p for _, p, _ in seqs)):
+            outs = [torch.empty_like(q) for _ in range(3)]
+            for layer in range(2):                   # (the second with the first one's plan)
+                if layer == 0:
+                    b = f.step()
+                K.attn_decode_shared(outs[layer], q, f, b, 8, 4, hd, 0.1, 0.0, lead, pages, most)
+                K.attn_decode(outs[2], q, f, b, 8, 4, hd, 0.1, 0.0, 0)
+            return outs
+
+        jobs.append((run, run(), torch.cuda.Stream()))
+    torch.cuda.synchronize()
+    got = []
+    for _ in range(15):
+        for run, _, stream in jobs:
+            with torch.cuda.stream(stream):
+                got.append(run())
+    torch.cuda.synchronize()
+    for i, outs in enumerate(got):
+        for x, y in zip(outs, jobs[i % 2][1]):
+            assert torch.equal(x, y)
+    K.check_device_errors(DEV)
