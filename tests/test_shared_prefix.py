@@ -351,3 +351,47 @@ def test_two_streams_at_once(K, bits):
         for x, y in zip(outs, jobs[i % 2][1]):
             assert torch.equal(x, y)
     K.check_device_errors(DEV)
+
+
+@pytest.mark.parametrize("bits", [16, 8])
+def test_far_pages(K, bits):
+    """Shared pages, and the sequences' own, whose bytes lie beyond 2^32 (16 bits) and 2^31 (8 bits) from the cache's first."""
+    nq, nkv, hd = 8, 4, 256
+    f = Family([(0, 5, 400), (0, 5, 321), (0, 5, 350)], nkv, hd, bits)
+    n = (1 << 31) // (nkv * PAGE * hd) + 70
+    shift = n - f.k.shape[0]
+    for name in ("k", "v", "k_exp", "v_exp") if bits == 8 else ("k", "v"):
+        t = getattr(f, name)
+        plain = t.view(torch.uint8) if bits == 8 else t
+        far = torch.zeros(n, *t.shape[1:], dtype=plain.dtype, device=DEV)
+        far[shift:] = plain
+        setattr(f, name, far.view(F8) if t.dtype == F8 else far)
+    f.page_table = torch.where(f.page_table >= 0, f.page_table + shift, f.page_table)
+    q = torch.randn(3, nq * hd).to(torch.bfloat16)
+    ref, mag, big = plain_attention(q, f.held, f.lens, nq, nkv, hd, 0.0625, 0.0, 0, "window", 0, None)
+    out = torch.empty(3, nq * hd, dtype=torch.bfloat16, device=DEV)
+    l, p = f.lead()
+    K.attn_decode_shared(out, q.to(DEV), f, f.step(), nq, nkv, hd, 0.0625, 0.0, l, p, 5)
+    assert bool(((out.double().cpu().view(3, nq, hd) - ref).abs() <= bound(ref, mag, big, hd)).all())
+    K.check_device_errors(DEV)
+
+
+@pytest.mark.parametrize("bits", [16, 8])
+def test_prefix_of_what_is_not_finite(K, bits):
+    """NaN in a group's shared pages reaches that group's outputs and no other's."""
+    nq, nkv, hd = 4, 2, 64
+    f = Family([(0, 3, 200), (1, 3, 230), (0, 3, 250), (1, 3, 199)], nkv, hd, bits)
+    ref, mag, big = plain_attention(q := torch.randn(4, nq * hd).to(torch.bfloat16), f.held, f.lens, nq, nkv, hd, 0.1, 0.0, 0, "window", 0, None)
+    page = int(f.table[f.order[0], 1])
+    if bits == 8:
+        f.v.view(torch.uint8)[page, 1, 7, 3] = 0x7f           # (a NaN code)
+    else:
+        f.v[page, 1, 7, 3] = float("nan")
+    out = torch.empty(4, nq * hd, dtype=torch.bfloat16, device=DEV)
+    l, p = f.lead()
+    K.attn_decode_shared(out, q.to(DEV), f, f.step(), nq, nkv, hd, 0.1, 0.0, l, p, 3)
+    got, lim = out.double().cpu().view(4, nq, hd), bound(ref, mag, big, hd)
+    struck = torch.zeros(4, nq, hd, dtype=torch.bool)
+    struck[0::2, nq // 2:, 3] = True                          # (the second kv head's query heads of the first group, that dim)
+    assert bool(got[struck].isnan().all()) and bool(((got - ref).abs() <= lim)[~struck].all())
+    K.check_device_errors(DEV)
