@@ -220,7 +220,9 @@ constexpr int SH_EXPS = 16;              // (8 bits) pages whose factors are kep
 
 template <int HD, int BITS>
 struct Sh {
-  static constexpr int CONV = BITS == 16 ? 0 : (HD == 256 ? 8 : 4);           // warps that convert: four keys and four values, or four both
+  // Warps that convert: four keys and four values, or four both.  (2 sequences behind 131,072 tokens: heads of 256 124 us with eight, 146 with four; heads of
+  // 128 123 and 119: what the softmax loses in registers.)
+  static constexpr int CONV = BITS == 16 ? 0 : (HD == 256 ? 8 : 4);
   static constexpr int WARPS = 20 + CONV, THREADS = WARPS * 32;
   static constexpr int TILE = AF_PAGE * HD * 2;                              // bytes of a page's keys, or values, as operand
   // pages in flight (16 bits), or converted (8 bits; beside them RAW pages of codes are in flight)
