@@ -809,13 +809,10 @@ int launch_decode8(const CUtensorMap& mk, const CUtensorMap& mv, const Decode8Ar
 
 }  // namespace
 
-// The attention into `out`, or where that is null the split pass alone: partial results of every (sequence, head) in `scratch`
-// (af_attn_decode_scratch(...) floats), as the step's `plan` (af_decode8_plan, or the shared one) cuts the work.
-int af_decode8_split(const void* q, long long q_stride, const void* k, const void* v, const void* k_exp, const void* v_exp,
-                     long long n_pages, const int* page_table, int max_pages, const int* slots, const int* lens, const int* shared,
-                     int batch, int nq, int nkv, int hd, float scale, float cap, int window, int keep, int ring_rows, int n_splits,
-                     float* scratch, const int* plan, int* err, cudaStream_t stream, void* out, long long out_stride,
-                     const float* sinks) {
+// What the kernel cannot take, refused before anything is launched.
+static int d8_refuses(const void* q, long long q_stride, const void* k, const void* v, const void* k_exp, const void* v_exp,
+                      long long n_pages, int max_pages, int batch, int nq, int nkv, int hd, int window, int keep, int ring_rows,
+                      int n_splits, const float* scratch, const int* plan) {
   AF_REQUIRE(nq > 0 && nkv > 0 && nq % nkv == 0, "af_attn_decode8: heads %d, groups %d", nq, nkv);
   AF_REQUIRE(hd == 64 || hd == 128 || hd == 256, "af_attn_decode8: head_dim %d (takes 64, 128, 256)", hd);
   AF_REQUIRE(keep >= 0 && (keep == 0 || window != 0), "af_attn_decode8: %d kept tokens with window %d", keep, window);
@@ -825,13 +822,27 @@ int af_decode8_split(const void* q, long long q_stride, const void* k, const voi
              "af_attn_decode8: splits %d, scratch and a 16-byte aligned plan", n_splits);
   AF_REQUIRE((((uintptr_t)k | (uintptr_t)v | (uintptr_t)k_exp | (uintptr_t)v_exp | (uintptr_t)scratch) & 15) == 0,
              "af_attn_decode8: cache and scratch alignment");
-  AF_REQUIRE(q_stride % 2 == 0 && ((uintptr_t)q & 3) == 0, "af_attn_decode8: queries must be 4-byte aligned");
+  // (a row of queries is read in loads of 16 bytes)
+  AF_REQUIRE((batch == 1 || q_stride % 8 == 0) && ((uintptr_t)q & 15) == 0, "af_attn_decode8: rows of queries must be 16-byte aligned");
   AF_REQUIRE(n_pages > 0 && n_pages * nkv * AF_PAGE < (1ll << 31), "af_attn_decode8: %lld cache pages", n_pages);
   const int group = nq / nkv, units_per_seq = nkv * ((group + 15) / 16);
   AF_REQUIRE(batch <= DA_MAX_BATCH && (long long)batch * (max_pages + 1 + D8_BREAK_PAGES) * units_per_seq < (1ll << 31),
              "af_attn_decode8: %d sequences of up to %d pages (takes %d sequences)", batch, max_pages, DA_MAX_BATCH);
+  return 0;
+}
+
+// The attention into `out`, or where that is null the split pass alone: partial results of every (sequence, head) in `scratch`
+// (af_attn_decode_scratch(...) floats), as the step's `plan` (af_decode8_plan, or the shared one) cuts the work.
+int af_decode8_split(const void* q, long long q_stride, const void* k, const void* v, const void* k_exp, const void* v_exp,
+                     long long n_pages, const int* page_table, int max_pages, const int* slots, const int* lens, const int* shared,
+                     int batch, int nq, int nkv, int hd, float scale, float cap, int window, int keep, int ring_rows, int n_splits,
+                     float* scratch, const int* plan, int* err, cudaStream_t stream, void* out, long long out_stride,
+                     const float* sinks) {
+  int rc = d8_refuses(q, q_stride, k, v, k_exp, v_exp, n_pages, max_pages, batch, nq, nkv, hd, window, keep, ring_rows, n_splits, scratch, plan);
+  if (rc) return rc;
+  const int group = nq / nkv, units_per_seq = nkv * ((group + 15) / 16);
   CUtensorMap mk, mv;
-  int rc = d8_map(&mk, k, n_pages * nkv * AF_PAGE, hd);
+  rc = d8_map(&mk, k, n_pages * nkv * AF_PAGE, hd);
   if (rc) return rc;
   rc = d8_map(&mv, v, n_pages * nkv * AF_PAGE, hd);
   if (rc) return rc;
@@ -876,8 +887,11 @@ AF_EXPORT int af_attn_decode8(const AfDecode8* c) {
   AF_REQUIRE(c->batch > 0 && c->batch <= DA_MAX_BATCH, "af_attn_decode8: %lld sequences (takes %d)", c->batch, DA_MAX_BATCH);
   const int batch = (int)c->batch, nq = (int)c->nq, nkv = (int)c->nkv, hd = (int)c->hd, n_splits = (int)c->n_splits;
   const int *page_table = (const int*)c->page_table, *slots = (const int*)c->slots, *lens = (const int*)c->lens;
+  int rc = d8_refuses(c->q, c->q_stride, c->k, c->v, c->k_exp, c->v_exp, c->n_pages, (int)c->max_pages, batch, nq, nkv, hd, (int)c->window,
+                      (int)c->keep, (int)c->ring_rows, n_splits, c->scratch, c->plan);
+  if (rc) return rc;
   if (c->plan_ints > 0) {
-    const int rc = af_decode8_plan(c->plan, c->plan_ints, page_table, (int)c->max_pages, slots, lens, batch, nq, nkv, (int)c->window, (int)c->keep,
+    rc = af_decode8_plan(c->plan, c->plan_ints, page_table, (int)c->max_pages, slots, lens, batch, nq, nkv, (int)c->window, (int)c->keep,
                                    (int)c->ring_rows, n_splits, c->stream);
     if (rc) return rc;
   }

@@ -1123,7 +1123,7 @@ def _decode_rows(who: str, out, q, batch, nq: int, hd: int, sinks) -> int:
 def attn_decode8(out, q, kv, batch, nq: int, nkv: int, hd: int, scale: float, cap: float, window: int, sinks=None,
                  keep: int = 0) -> None:
     """Decode attention over a cache of 8 bits (``window`` < 0: a chunk of that many positions; ``keep``: beside a window,
-    the first tokens that stay visible)."""
+    the first tokens that stay visible).  Rows of queries that do not begin on 16 bytes are copied first."""
     B = _decode_rows("attn_decode8", out, q, batch, nq, hd, sinks)
     n_pages = _cache8_pages(kv, nkv, hd, "attn_decode8")
     table, slots, lens = kv.page_table, batch.slots, batch.len_after
@@ -1131,6 +1131,8 @@ def attn_decode8(out, q, kv, batch, nq: int, nkv: int, hd: int, scale: float, ca
     dev = _here("attn_decode8", out, q, table, slots, lens, kv.k, kv.v, kv.k_exp, kv.v_exp, *(() if sinks is None else (sinks,)))
     if B == 0:
         return
+    if q.data_ptr() % 16 or (B > 1 and q.stride(0) % 8):      # (the kernel loads 16 bytes at a time)
+        q = torch.empty_like(out, memory_format=torch.contiguous_format).copy_(q[:, : nq * hd])
     n = attn_decode_max_splits(B, nkv, batch.max_len_after, window, _plan_ints("af_attn_decode8_blocks", 1, nq, nkv), nq, keep)
     # the plan of the step, made in front of its first layer's attention and shared by the layers that read alike, one after the
     # other on one stream (it counts the parts of a layer's results)

@@ -1,0 +1,77 @@
+"""Limits of the 8-bit cache's attention and of shared prefixes: rows and pages of odd addresses, refusals that come before any
+launch, plans of calls that were refused, positions and lengths beyond a page table."""
+import ctypes
+import math
+from types import SimpleNamespace
+
+import pytest
+import torch
+
+from test_cache8 import F8, PAGE, View, fill, step
+
+DEV = "cuda:0"
+
+
+@pytest.fixture(scope="module")
+def K():
+    from airframe_b200 import kernels
+    return kernels
+
+
+def refusal(K, entry, block):
+    """What the library says to a call that it must not let reach the device (there is none here, or nothing to read at these addresses)."""
+    lib = K._lib()
+    lib.af_last_error.restype = ctypes.c_char_p
+    assert getattr(lib, entry)(block) != 0
+    return lib.af_last_error().decode()
+
+
+# ---------------------------------------------------------------------------------------------- rows of queries
+
+def decode8_block(K, **over):
+    """The argument block of af_attn_decode8 for one step of two sequences, 4 heads in 2 groups of 64."""
+    a = dict(out=0x10000, q=0x20000, k=0x30000, v=0x40000, k_exp=0x50000, v_exp=0x60000, table=0x70000, slots=0x80000, lens=0x90000,
+             scratch=0xa0000, plan=0xb0000, sinks=0, err=0xc0000, stream=0, out_stride=256, q_stride=256, n_pages=4, max_pages=2, batch=2,
+             nq=4, nkv=2, hd=64, window=0, keep=0, ring_rows=0, n_splits=4, plan_ints=1 << 20, scale=1.0, cap=0.0)
+    assert set(over) <= set(a)
+    return K._DECODE8.pack(*dict(a, **over).values())
+
+
+@pytest.mark.skipif(torch.cuda.is_available(), reason="addresses of nothing: only where there is no device to send them to")
+@pytest.mark.parametrize("over,match", [
+    (dict(q=0x20004), "16-byte"), (dict(q=0x20008), "16-byte"), (dict(q_stride=258), "16-byte"), (dict(q_stride=260), "16-byte"),
+    (dict(k_exp=0x50008), "alignment"), (dict(v=0x40004), "alignment"), (dict(nq=3), "heads"), (dict(hd=96), "head_dim 96"),
+    (dict(keep=3), "kept"), (dict(ring_rows=128), "ring"), (dict(n_splits=0), "splits"), (dict(n_pages=1 << 26), "pages")])
+def test_decode8_refuses_before_a_launch(K, over, match):
+    said = refusal(K, "af_attn_decode8", decode8_block(K, **over))
+    assert "af_attn_decode8:" in said and match in said
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("hd,nq,nkv", [(64, 4, 2), (128, 8, 2), (256, 16, 1)])
+@pytest.mark.parametrize("offset,pad", [(0, 2), (2, 0), (4, 4), (1, 7), (8, 16)])
+def test_decode8_rows_that_begin_anywhere(K, hd, nq, nkv, offset, pad):
+    """Queries whose rows begin on 2, 4 or 8 bytes (a slice, an odd stride) give the bits that aligned rows give, and so do one
+    sequence's rows and those that the shared kernels do not take."""
+    lens = [130, 1, 70]
+    view = View(lens, nkv, hd)
+    fill(view, lens, nkv, hd)
+    view.to(DEV)
+    q = torch.randn(3, nq * hd, dtype=torch.bfloat16, device=DEV)
+    odd = torch.empty(3, offset + nq * hd + pad, dtype=torch.bfloat16, device=DEV)[:, offset: offset + nq * hd]
+    odd.copy_(q)
+    want, got = torch.empty_like(q), torch.empty_like(q)
+    K.attn_decode(want, q, view, step(view, lens, DEV), nq, nkv, hd, 0.1, 0.0, 0)
+    K.attn_decode(got, odd, view, step(view, lens, DEV), nq, nkv, hd, 0.1, 0.0, 0)
+    assert torch.equal(got, want)
+    lead, pages = (torch.tensor(x, dtype=torch.int32, device=DEV) for x in ([0, 1, 2], [0, 0, 0]))
+    if offset * 2 % 16 or odd.stride(0) % 8:
+        K.attn_decode_shared(got.zero_(), odd, view, step(view, lens, DEV), nq, nkv, hd, 0.1, 0.0, lead, pages, 1)
+        assert torch.equal(got, want)
+    one = View([130], nkv, hd)
+    fill(one, [130], nkv, hd)
+    one.to(DEV)
+    K.attn_decode(want[:1], q[:1], one, step(one, [130], DEV), nq, nkv, hd, 0.1, 0.0, 0)
+    K.attn_decode(got[:1], odd[:1], one, step(one, [130], DEV), nq, nkv, hd, 0.1, 0.0, 0)
+    assert torch.equal(got[:1], want[:1])
+    K.check_device_errors(DEV)
