@@ -991,7 +991,11 @@ AF_EXPORT int af_attn_decode_shared(const AfShared* c) {
                   15) == 0 &&
                  ((uintptr_t)c->out & 3) == 0,
              "af_attn_decode_shared: rows must be 16-byte aligned (out: 4)");
+  // (an 8-bit cache's exponents come into shared memory by copies of 16 bytes)
+  AF_REQUIRE(c->bits == 16 || (c->k_exp != nullptr && c->v_exp != nullptr && (((uintptr_t)c->k_exp | (uintptr_t)c->v_exp) & 15) == 0),
+             "af_attn_decode_shared: exponents must be 16-byte aligned");
   AF_REQUIRE(c->own_scratch != nullptr && c->pre_scratch != nullptr && c->plan != nullptr, "af_attn_decode_shared: scratch and plan");
+  AF_REQUIRE(c->n_splits >= 1 && c->n_splits <= 65535, "af_attn_decode_shared: splits %lld", c->n_splits);
   AF_REQUIRE(c->n_pages > 0 && c->n_pages * c->nkv * AF_PAGE < (1ll << 31), "af_attn_decode_shared: %lld cache pages", c->n_pages);
   const int sms = af_sm_count();
   if (sms <= 0) return -1;

@@ -47,6 +47,25 @@ def test_decode8_refuses_before_a_launch(K, over, match):
     assert "af_attn_decode8:" in said and match in said
 
 
+def shared_block(K, **over):
+    """The argument block of af_attn_decode_shared for the same step."""
+    a = dict(out=0x10000, q=0x20000, k=0x30000, v=0x40000, k_exp=0x50000, v_exp=0x60000, table=0x70000, slots=0x80000, lens=0x90000,
+             lead=0xd0000, pages=0xe0000, own=0xa0000, pre=0xf0000, plan=0xb0000, sinks=0, err=0xc0000, stream=0, out_stride=256,
+             q_stride=256, n_pages=4, max_pages=2, batch=2, nq=4, nkv=2, hd=64, n_splits=4, plan_ints=1 << 20, bits=8, scale=1.0, cap=0.0)
+    assert set(over) <= set(a)
+    return K._SHARED.pack(*dict(a, **over).values())
+
+
+@pytest.mark.skipif(torch.cuda.is_available(), reason="addresses of nothing: only where there is no device to send them to")
+@pytest.mark.parametrize("over,match", [
+    (dict(k_exp=0x50004), "exponents"), (dict(v_exp=0x60008), "exponents"), (dict(v_exp=0), "exponents"), (dict(q=0x20008), "16-byte"),
+    (dict(q_stride=260), "16-byte"), (dict(n_splits=0), "splits"), (dict(bits=4), "bits"), (dict(hd=96), "head_dim 96"), (dict(nq=3), "heads"),
+    (dict(pre=0), "scratch"), (dict(bits=16, k=0x30008), "16-byte")])
+def test_shared_refuses_before_a_launch(K, over, match):
+    said = refusal(K, "af_attn_decode_shared", shared_block(K, **over))
+    assert "af_attn_decode_shared:" in said and match in said
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("hd,nq,nkv", [(64, 4, 2), (128, 8, 2), (256, 16, 1)])
 @pytest.mark.parametrize("offset,pad", [(0, 2), (2, 0), (4, 4), (1, 7), (8, 16)])
@@ -74,4 +93,28 @@ def test_decode8_rows_that_begin_anywhere(K, hd, nq, nkv, offset, pad):
     K.attn_decode(want[:1], q[:1], one, step(one, [130], DEV), nq, nkv, hd, 0.1, 0.0, 0)
     K.attn_decode(got[:1], odd[:1], one, step(one, [130], DEV), nq, nkv, hd, 0.1, 0.0, 0)
     assert torch.equal(got[:1], want[:1])
+    K.check_device_errors(DEV)
+
+
+@pytest.mark.gpu
+def test_exponents_of_an_odd_address_are_refused(K):
+    """Pages' exponents that do not begin on 16 bytes: an error by both attentions, and the next call works."""
+    nq, nkv, hd, lens = 4, 2, 64, [200, 193]
+    view = View(lens, nkv, hd)
+    fill(view, lens, nkv, hd)
+    view.to(DEV)
+    q, out = torch.randn(2, nq * hd, dtype=torch.bfloat16, device=DEV), torch.zeros(2, nq * hd, dtype=torch.bfloat16, device=DEV)
+    lead, pages = torch.arange(2, dtype=torch.int32, device=DEV), torch.zeros(2, dtype=torch.int32, device=DEV)
+    whole = view.v_exp
+    room = torch.zeros(whole.numel() + 16, dtype=torch.uint8, device=DEV)
+    view.v_exp = room[4: 4 + whole.numel()].view(whole.shape).copy_(whole)
+    b = step(view, lens, DEV)
+    with pytest.raises(K.KernelError, match="exponents"):
+        K.attn_decode_shared(out, q, view, b, nq, nkv, hd, 0.1, 0.0, lead, pages, 1)
+    with pytest.raises(K.KernelError, match="alignment"):
+        K.attn_decode(out, q, view, step(view, lens, DEV), nq, nkv, hd, 0.1, 0.0, 0)
+    assert not out.any()
+    view.v_exp = whole
+    K.attn_decode_shared(out, q, view, step(view, lens, DEV), nq, nkv, hd, 0.1, 0.0, lead, pages, 1)
+    assert bool(out.any())
     K.check_device_errors(DEV)
