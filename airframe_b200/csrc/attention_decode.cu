@@ -564,6 +564,9 @@ static int attn_decode_impl(const float* sinks, void* out, long long out_stride,
   AF_REQUIRE(n_splits >= 1 && n_splits <= 65535 && scratch != nullptr, "af_attn_decode: splits %d", n_splits);
   AF_REQUIRE(((uintptr_t)kcache & 15) == 0 && ((uintptr_t)vcache & 15) == 0 && ((uintptr_t)plan & 15) == 0,
              "af_attn_decode: cache and plan alignment");
+  // (queries are read, and many splits' outputs written, two elements at a time)
+  AF_REQUIRE((batch == 1 || (q_stride % 2 == 0 && out_stride % 2 == 0)) && (((uintptr_t)q | (uintptr_t)out) & 3) == 0,
+             "af_attn_decode: rows of queries and out must be 4-byte aligned");
   DecodeArgs a;
   a.q = (const __nv_bfloat16*)q;
   a.q_stride = q_stride;

@@ -981,8 +981,17 @@ def attn_decode_split(out, q, kcache, vcache, page_table, slots, lens, nq, nkv, 
     results into ``scratch``, then their merge).  ``n_splits`` is the most
     splits a (sequence, kv head) unit gets: the kernel cuts the units' pages so
     that all blocks get about the same number of them (with less room than
-    :func:`attn_decode_max_splits` fewer blocks work).  ``keep``: with a window, the first tokens that stay visible."""
+    :func:`attn_decode_max_splits` fewer blocks work).  ``keep``: with a window, the first tokens that stay visible.  Rows
+    of ``q`` or ``out`` that do not begin on 4 bytes go through a copy."""
     B = q.shape[0]
+    if q.data_ptr() % 4 or (B > 1 and q.stride(0) % 2):      # (the kernel loads two elements at a time, and stores them so)
+        q = torch.empty(B, nq * hd, dtype=q.dtype, device=q.device).copy_(q[:, : nq * hd])
+    if out.data_ptr() % 4 or (B > 1 and out.stride(0) % 2):
+        whole = torch.empty(B, nq * hd, dtype=out.dtype, device=out.device)
+        attn_decode_split(whole, q, kcache, vcache, page_table, slots, lens, nq, nkv, hd, scale, cap, window, ring_rows, n_splits, scratch, plan,
+                          sinks, keep)
+        out[:, : nq * hd] = whole
+        return
     lib = _lib()
     lib.af_attn_decode_scratch.restype = ctypes.c_longlong
     need = lib.af_attn_decode_scratch(c_int(B), c_int(nq), c_int(hd), c_int(n_splits))

@@ -47,6 +47,19 @@ def test_decode8_refuses_before_a_launch(K, over, match):
     assert "af_attn_decode8:" in said and match in said
 
 
+@pytest.mark.skipif(torch.cuda.is_available(), reason="addresses of nothing: only where there is no device to send them to")
+@pytest.mark.parametrize("q,q_stride,out,out_stride", [(0x20002, 256, 0x10000, 256), (0x20000, 257, 0x10000, 256), (0x20000, 256, 0x10002, 256),
+                                                       (0x20000, 256, 0x10000, 257)])
+def test_decode_of_16_bits_refuses_odd_rows(K, q, q_stride, out, out_stride):
+    """The 16-bit split kernel, which takes what the shared one leaves, reads queries and writes outputs in words of 4 bytes."""
+    I, P, L, F = ctypes.c_int, ctypes.c_void_p, ctypes.c_longlong, ctypes.c_float
+    lib = K._lib()
+    lib.af_last_error.restype = ctypes.c_char_p
+    assert lib.af_attn_decode_kept(P(out), L(out_stride), P(q), L(q_stride), P(0x30000), P(0x40000), L(4), P(0x70000), I(2), P(0x80000), P(0x90000),
+                                   I(2), I(4), I(2), I(64), F(1.0), F(0.0), I(0), I(0), I(0), I(4), P(0xa0000), P(0xb0000), P(0), P(0xc0000), P(0)) != 0
+    assert "4-byte" in lib.af_last_error().decode()
+
+
 def shared_block(K, **over):
     """The argument block of af_attn_decode_shared for the same step."""
     a = dict(out=0x10000, q=0x20000, k=0x30000, v=0x40000, k_exp=0x50000, v_exp=0x60000, table=0x70000, slots=0x80000, lens=0x90000,
@@ -117,4 +130,35 @@ def test_exponents_of_an_odd_address_are_refused(K):
     view.v_exp = whole
     K.attn_decode_shared(out, q, view, step(view, lens, DEV), nq, nkv, hd, 0.1, 0.0, lead, pages, 1)
     assert bool(out.any())
+    K.check_device_errors(DEV)
+
+
+class Pages16:
+    """A layer's view of a bfloat16 cache, slots and pages in order."""
+
+    def __init__(self, lens, nkv, hd):
+        self.pages_per_seq = -(-max(lens) // PAGE)
+        n = len(lens) * self.pages_per_seq
+        self.k, self.v = (torch.randn(n, nkv, PAGE, hd, device=DEV).to(torch.bfloat16) for _ in range(2))
+        self.page_table = torch.arange(n, dtype=torch.int32, device=DEV).view(len(lens), -1).contiguous()
+        self.ring_rows, self.keep_first, self.order = 0, 0, list(range(len(lens)))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("offset,pad", [(1, 0), (0, 1), (3, 4), (2, 2)])
+@pytest.mark.parametrize("lens", [[130, 1, 70], [3000, 1500, 5000]])
+def test_decode_of_16_bits_with_odd_rows(K, offset, pad, lens):
+    """Queries and outputs in rows that begin on 2 or 4 bytes: the aligned rows' bits, also through the shared entry."""
+    nq, nkv, hd = 8, 2, 128
+    view = Pages16(lens, nkv, hd)
+    odd = lambda: torch.zeros(3, offset + nq * hd + pad, dtype=torch.bfloat16, device=DEV)[:, offset: offset + nq * hd]
+    q = torch.randn(3, nq * hd, dtype=torch.bfloat16, device=DEV)
+    want, q2, got = torch.empty_like(q), odd().copy_(q), odd()
+    K.attn_decode(want, q, view, step(view, lens, DEV), nq, nkv, hd, 0.1, 0.0, 0)
+    K.attn_decode(got, q2, view, step(view, lens, DEV), nq, nkv, hd, 0.1, 0.0, 0)
+    assert torch.equal(got, want)
+    lead, pages = (torch.tensor(x, dtype=torch.int32, device=DEV) for x in ([0, 1, 2], [0, 0, 0]))
+    got.zero_()
+    K.attn_decode_shared(got, q2, view, step(view, lens, DEV), nq, nkv, hd, 0.1, 0.0, lead, pages, 1)
+    assert torch.equal(got, want)
     K.check_device_errors(DEV)
