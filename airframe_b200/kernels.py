@@ -1152,14 +1152,14 @@ def attn_decode8(out, q, kv, batch, nq: int, nkv: int, hd: int, scale: float, ca
     if plan is None:
         ints = _plan_ints("af_attn_decode8_plan_ints", B, nq, nkv)
         plan = torch.empty(ints, dtype=torch.int32, device=q.device)
-        if aux is not None:
-            aux[key] = plan
     scratch = torch.empty(B * nq * n * (hd + 2), dtype=torch.float32, device=q.device)
     _check(_lib().af_attn_decode8(_DECODE8.pack(
         out.data_ptr(), q.data_ptr(), kv.k.data_ptr(), kv.v.data_ptr(), kv.k_exp.data_ptr(), kv.v_exp.data_ptr(), table.data_ptr(),
         slots.data_ptr(), lens.data_ptr(), scratch.data_ptr(), plan.data_ptr(), 0 if sinks is None else sinks.data_ptr(),
         _error_pointer(dev), _raw_stream(dev), _rows(out, "out"), _rows(q, "q"), n_pages, table.shape[1], B, nq, nkv, hd, window, keep,
         kv.ring_rows, n, ints, scale, cap)))
+    if ints and aux is not None:
+        aux[key] = plan              # (now, not before: a refused call has made none)
 
 
 def attn_decode_shared_pays(groups, nkv: int, hd: int, eight_bits: bool = False) -> bool:
@@ -1216,8 +1216,6 @@ def attn_decode_shared(out, q, kv, batch, nq: int, nkv: int, hd: int, scale: flo
     if plan is None:
         ints = _plan_ints("af_attn_shared_plan_ints", B, nq, nkv)
         plan = torch.empty(ints, dtype=torch.int32, device=q.device)
-        if aux is not None:
-            aux[key] = plan
     n_own = (B * nq * n * (hd + 2) + 3) // 4 * 4
     scratch = torch.empty(n_own + _plan_ints("af_attn_shared_rows", B, nq, nkv) * (hd + 2), dtype=torch.float32, device=q.device)
     _check(_lib().af_attn_decode_shared(_SHARED.pack(
@@ -1225,6 +1223,8 @@ def attn_decode_shared(out, q, kv, batch, nq: int, nkv: int, hd: int, scale: flo
         table.data_ptr(), slots.data_ptr(), lens.data_ptr(), lead.data_ptr(), pages.data_ptr(), scratch.data_ptr(),
         scratch.data_ptr() + 4 * n_own, plan.data_ptr(), 0 if sinks is None else sinks.data_ptr(), _error_pointer(dev), _raw_stream(dev),
         _rows(out, "out"), _rows(q, "q"), n_pages, table.shape[1], B, nq, nkv, hd, n, ints, 8 if eight else 16, scale, cap)))
+    if ints and aux is not None:
+        aux[key] = plan
     if gate is not None:
         head_gate(out, gate, nq, hd)
 

@@ -162,3 +162,45 @@ def test_decode_of_16_bits_with_odd_rows(K, offset, pad, lens):
     K.attn_decode_shared(got, q2, view, step(view, lens, DEV), nq, nkv, hd, 0.1, 0.0, lead, pages, 1)
     assert torch.equal(got, want)
     K.check_device_errors(DEV)
+
+
+# ---------------------------------------------------------------------------------------------- plans
+
+class Refusing:
+    """A library that refuses its first call and records whether each call was to make a plan."""
+
+    def __init__(self, plan_word):
+        self.made, self.word = [], plan_word
+
+    def __getattr__(self, name):
+        def entry(block):
+            self.made.append(ctypes.cast(block, ctypes.POINTER(ctypes.c_longlong))[self.word] > 0)
+            return -1 if len(self.made) == 1 else 0
+        return (lambda: b"no") if name == "af_last_error" else entry
+
+
+@pytest.mark.parametrize("shared", [False, True])
+def test_a_refused_call_leaves_no_plan(K, monkeypatch, shared):
+    """A step's plan is made by its first call that the library takes: one that was refused has made none for the next to read."""
+    nq, nkv, hd = 4, 2, 64
+    lib = Refusing(26)               # (the word that says how long a plan to make, in both blocks)
+    for name, fake in (("_lib", lambda: lib), ("_here", lambda *a: 0), ("_current_device", lambda: 0), ("_raw_stream", lambda d: 0),
+                       ("_error_pointer", lambda d: 0), ("_plan_ints", lambda *a: 64), ("sm_count", lambda: 148)):
+        monkeypatch.setattr(K, name, fake)
+    view = View([200, 200], nkv, hd).to("cpu")
+    b = step(view, [200, 200], "cpu")
+    q = torch.zeros(2, nq * hd, dtype=torch.bfloat16)
+    out, lead, pages = torch.empty_like(q), torch.zeros(2, dtype=torch.int32), torch.full((2,), 3, dtype=torch.int32)
+
+    def call():
+        if shared:
+            K.attn_decode_shared(out, q, view, b, nq, nkv, hd, 0.1, 0.0, lead, pages, 3)
+        else:
+            K.attn_decode8(out, q, view, b, nq, nkv, hd, 0.1, 0.0, 0)
+
+    with pytest.raises(K.KernelError):
+        call()
+    assert not b.aux
+    call()
+    call()
+    assert lib.made == [True, True, False] and len(b.aux) == 1
