@@ -289,11 +289,17 @@ class SequenceCache:
                 raise CacheFull(f"{g.pages_to_fork(n)} more cache pages wanted, {g.pages.n_free} of {g.n_pages} free "
                                 f"(window {g.need.window})")
         new = self.slots.take()
-        for g in self.groups.values():
-            g.fork(slot, new, n)
-        for st in self.states.values():
-            if st is not None:
-                st[new].copy_(st[slot])
+        try:
+            for g in self.groups.values():
+                g.fork(slot, new, n)
+            for st in self.states.values():
+                if st is not None:
+                    st[new].copy_(st[slot])
+        except BaseException:             # (no memory for a copy, for one)
+            for g in self.groups.values():
+                g.release(new)
+            self.slots.give_back(new)
+            raise
         self.lens[new] = n
         self.room[new] = min((g.room(new) for g in self.groups.values()), default=self.max_context)
         if slot not in self._family:

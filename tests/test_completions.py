@@ -107,6 +107,38 @@ def test_fork_refusals_change_nothing():
     assert c.groups[need].pages.n_held == 0
 
 
+@pytest.mark.parametrize("broken", ["index_copy_", "index_select", "copy_"])
+def test_a_fork_whose_copy_fails_changes_nothing(monkeypatch, broken):
+    """No memory for a page's copy or a state's: the slot and the pages taken so far go back, owners and claims are as before."""
+    full, ring = KVNeed(2, 16), KVNeed(1, 8, 100)
+    c = SequenceCache([(full, None, None), (ring, StateNeed((3,)), None)], 64 * 40, 1024, torch.float32, "cpu", max_sequences=4)
+    a = c.take_slot()
+    c.reserve({a: 150})
+    c.commit({a: 150})
+    b = c.fork(a)
+    held = {n: ([list(h) for h in g.held], g.table_host.clone(), g.pages.n_free) for n, g in c.groups.items()}
+    whole, calls = getattr(torch.Tensor, broken), []
+
+    def fails(self, *args, **kw):
+        calls.append(1)
+        if len(calls) == (1 if broken == "copy_" else 3):        # (of the second group of layers, or its state)
+            raise torch.OutOfMemoryError("no memory")
+        return whole(self, *args, **kw)
+
+    with monkeypatch.context() as m:
+        m.setattr(torch.Tensor, broken, fails)
+        with pytest.raises(torch.OutOfMemoryError):
+            c.fork(a)
+    assert c.slots.n_held == 2
+    for n, g in c.groups.items():
+        assert g.held == held[n][0] and torch.equal(g.table_host, held[n][1]) and g.pages.n_free == held[n][2]
+    assert c.groups[full].pages.owners(c.groups[full].held[a][0]) == 2 and c.shared_claims([a, b])[:2] == ([0, 0], [2, 2])
+    d = c.fork(a)
+    for s in (a, b, d):
+        c.free_slot(s)
+    assert c.slots.n_held == 0 and all(g.pages.n_held == 0 for g in c.groups.values())
+
+
 def test_shared_claims():
     c = SequenceCache([(KVNeed(1, 8), None, None)], 64 * 100, 2000, torch.float32, "cpu", max_sequences=8)
     a, z = c.take_slot(), c.take_slot()
