@@ -309,11 +309,11 @@ class SequenceCache:
         self._family[new] = (family, min(pages, n // PAGE))
         return new
 
-    def shared_claims(self, slots):
+    def shared_claims(self, slots, among=None):
         """For the rows of a step (slots, -1 or None: none): (lead, pages, families, need): row i's first ``pages[i]`` pages are those
         of row ``lead[i]`` in every group that keeps all keys; by family (rows, shared pages); and such a group's KVNeed (the one with the
-        longest rows).  None where no two rows share a page or no group keeps all keys."""
-        needs = [g.need for g in self.groups.values() if not g.need.window]
+        longest rows; with ``among``, one of these).  None where no two rows share a page or there is no such group."""
+        needs = [g.need for g in self.groups.values() if not g.need.window and (among is None or g.need in among)]
         if not self._family or not needs:
             return None
         rows: dict = {}

@@ -43,6 +43,7 @@ class Engine:
                                    max_sequences=max_sequences)
         # the most sequences that a step may carry (None: any number): what the 8-bit cache's attention plans for
         self.max_step_sequences = (kernels.ATTN_DECODE_MAX_SEQS if any(g.need.eight_bits for g in self.cache.groups.values()) else None)
+        self._shared_needs = model.shared_needs()
         self.vocab_size = model.spec.vocab_size
         # decode steps of models whose parts allow it are captured into CUDA graphs,
         # one per padded batch size
@@ -74,12 +75,13 @@ class Engine:
         return new
 
     def _claims(self, slots):
-        """(lead, pages) of a decode step whose shared pages are worth the shared kernels, else None."""
-        claims = self.cache.shared_claims(slots)
+        """(lead, pages) of a decode step whose shared pages are worth the shared kernels in the layers that can take them, else None."""
+        claims = self.cache.shared_claims(slots, self._shared_needs)
         if claims is None:
             return None
         lead, pages, groups, need = claims
-        return (lead, pages) if kernels.attn_decode_shared_pays(groups, need.num_kv_heads, need.head_dim, need.eight_bits) else None
+        pays = kernels.attn_decode_shared_pays(groups, need.num_kv_heads, need.head_dim, need.eight_bits, self.model.ctx.compute_dtype, len(slots))
+        return (lead, pages) if pays else None
 
     def length(self, slot: int) -> int:
         return self.cache.length(slot)

@@ -96,6 +96,11 @@ class Model:
             out.append((b.mixer.kv_need(), b.mixer.state_need(), e.cache_from, b.state_need()))
         return out
 
+    def shared_needs(self) -> set:
+        """The KVNeeds of the runs whose decode steps read pages that sequences share once (see :meth:`Mixer.reads_shared`)."""
+        mixers = [self.blocks[e.layer].mixer for e in self.spec.schedule]
+        return {m.kv_need() for m in mixers if m.reads_shared()}
+
     # ------------------------------------------------------------------ what a step costs
 
     def decode_bytes(self, lens) -> int:

@@ -1162,9 +1162,9 @@ def attn_decode8(out, q, kv, batch, nq: int, nkv: int, hd: int, scale: float, ca
         aux[key] = plan              # (now, not before: a refused call has made none)
 
 
-def attn_decode_shared_pays(groups, nkv: int, hd: int, eight_bits: bool = False) -> bool:
-    """Whether a decode step is faster with :func:`attn_decode_shared` than with :func:`attn_decode`: ``groups`` are (sequences, shared
-    pages) of the step.  A rule on the pages that need not be read again, which come out of L2 at some 12 TB/s: a group's pages times its
+def attn_decode_shared_pays(groups, nkv: int, hd: int, eight_bits: bool = False, dtype=torch.bfloat16, n_seqs: int = 0) -> bool:
+    """Whether a decode step (of ``n_seqs`` sequences and activations of ``dtype``, where the shared kernels take these) is faster with
+    :func:`attn_decode_shared` than with :func:`attn_decode`: ``groups`` are (sequences, shared pages) of the step.  A rule on the pages that need not be read again, which come out of L2 at some 12 TB/s: a group's pages times its
     sequences but one, and in the 8-bit cache, whose codes the shared kernel converts (0.9 us a page and block, of which the
     tensor-core products and the softmax take most) and the ordinary one reads at the memory's rate, but four.  Measured a layer of steps that make their
     plan once (ordinary / shared, us), kv heads x head size 4 x 256 and 8 x 128:
@@ -1174,6 +1174,8 @@ def attn_decode_shared_pays(groups, nkv: int, hd: int, eight_bits: bool = False)
     8 bits, 8 sequences: 64 pages 20.1 / 26.9 and 18.2 / 22.3, 128 pages 28.5 / 29.7 and 26.6 / 25.3, 256 pages 45.1 / 37.1 and
     43.1 / 32.3; 128 sequences: 8 pages 44.6 / 48.4 and 45.8 / 51.5, 16 pages 61.2 / 51.4 and 60.4 / 53.0; 4 sequences: 512 pages 47.0 / 49.1
     and 40.2 / 44.3."""
+    if not attn_decode_shared_supported(dtype, hd, n_seqs):
+        return False
     members = sum(m for m, _ in groups)
     spared = sum(n * (m - (4 if eight_bits else 1)) for m, n in groups)
     return spared * nkv * hd >= 1024 * (512 + 10 * members if eight_bits else 384 + 4 * members)

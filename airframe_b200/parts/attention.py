@@ -148,6 +148,11 @@ class Attention(Mixer):
             return KVNeed(self.nkv, self.pad, self.window, keep_first=self.keep, eight_bits=self.eight_bits)
         return KVNeed(self.nkv, self.hd, self.window, None if self.dv == self.hd else self.dv, self.keep, self.eight_bits)
 
+    def reads_shared(self) -> bool:
+        # (all keys visible, no score slopes, values of the keys' size in the cache)
+        return (not self.window and (bool(self.pad) or self.dv == self.hd)
+                and type(self.position).score_slopes is PositionEncoding.score_slopes)
+
     def weight_decls(self):
         q, k, v, o = self.names
         decls = [WeightDecl(q, (self.nq * self.hd, self.hidden)),
@@ -327,7 +332,7 @@ class Attention(Mixer):
                 batch.step_kv[view.cache_id] = (k.clone(), v.clone())
             kernels.attn_prefill(ctx, q, k, v, batch, nq, nkv, hd, self.scale, self.softcap, window, slopes,
                                  keep=self.keep, **more)
-        elif batch.shared is not None and not window and slopes is None and dv == hd:
+        elif batch.shared is not None and self.reads_shared():
             s = batch.shared
             kernels.attn_decode_shared(ctx, q, kv, batch, nq, nkv, hd, self.scale, self.softcap, s.lead, s.pages, s.most_pages,
                                        sinks=self.sinks, gate=gate)

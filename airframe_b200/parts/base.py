@@ -220,6 +220,10 @@ class Mixer(Part):
         """None, a :class:`StateNeed`, or a tuple of them (the run's view then has a tuple of tensors)."""
         return None
 
+    def reads_shared(self) -> bool:
+        """Whether a decode step of this mixer reads the cache pages that its sequences share (``batch.shared``) once for all of them."""
+        return False
+
     def forward(self, x, batch, view):
         """x [T, H] in the compute dtype (normalised) -> [T, H] in the compute
         dtype, or a :class:`~airframe_b200.parts.linear.PartialSums` or

@@ -42,6 +42,9 @@ class ParallelMixers(Mixer):
     def state_need(self):
         return next((m.state_need() for m, _ in self.branches if m.state_need() is not None), None)
 
+    def reads_shared(self) -> bool:
+        return any(m.reads_shared() for m, _ in self.branches)
+
     def weight_decls(self):
         return [d for m, _ in self.branches for d in m.weight_decls()]
 

@@ -175,6 +175,52 @@ def test_claims_are_of_the_groups_that_keep_all_keys():
         assert claims is None if want is None else claims[3] == want
 
 
+def _claims_of(spec, dtype=torch.bfloat16):
+    """What an engine of this model claims for 40 forks of 64 pages each (far beyond what the rule asks for)."""
+    from airframe_b200.engine import Engine
+    model = Model(spec, dtype, "cpu")
+    model.loaded = True
+    eng = Engine(model, 64 * 6000, 64 * 70, max_sequences=60)
+    s = eng.take_slot()
+    eng.cache.reserve({s: 64 * 64})
+    eng.cache.commit({s: 64 * 64})
+    eng.cache._family[s] = (0, 64)
+    slots = [s]
+    for _ in range(39):                  # (the bookkeeping of forks alone: the pages are not copied)
+        t = eng.take_slot()
+        eng.cache.lens[t], eng.cache._family[t] = 64 * 64, (0, 64)
+        slots.append(t)
+    return eng._claims(slots)
+
+
+def test_a_model_without_a_layer_that_shares_claims_nothing():
+    """Shared steps have graphs of their own: a model whose kernels would be the ordinary ones again makes none (32 bits, head sizes
+    that the shared kernels do not take, latent attention, score slopes, windows alone)."""
+    import test_toy_parts
+    import tiny_banitar
+    from airframe_b200.config import PartSpec
+    from airframe_b200.parts import unregister_part
+    big = lambda size=256: config_from_dict(dict(CONFIGS["D"], max_position_embeddings=64 * 70, num_attention_heads=8, num_key_value_heads=8,
+                                                head_dim=size)).model_spec()
+    assert _claims_of(big()) == ([0] * 40, [64] * 40)
+    assert _claims_of(big(), torch.float32) is None and _claims_of(big(96)) is None
+    windows = big()
+    for layer in windows.layers:
+        layer.mixer.params["window"] = 128
+    assert _claims_of(windows) is None
+    test_toy_parts._register()
+    try:
+        slopes = big()
+        for layer in slopes.layers:
+            layer.mixer.params["position"] = PartSpec("toy_distance_slopes", {"base": 2.0, "heads": 8})
+        assert _claims_of(slopes) is None
+    finally:
+        for kind in (("feed_forward", "toy_top1_experts"), ("position", "toy_learned_offset"), ("position", "toy_distance_slopes")):
+            unregister_part(*kind)
+    latent = config_from_dict(tiny_banitar.CONFIGS[next(iter(tiny_banitar.CONFIGS))]).model_spec()
+    assert Model(latent, torch.bfloat16, "cpu").shared_needs() == set()
+
+
 def test_shared_pages_pay_where_enough_is_read_again():
     from airframe_b200.kernels import attn_decode_shared_pays as pays
     for eight in (False, True):
