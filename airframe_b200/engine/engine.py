@@ -75,13 +75,22 @@ class Engine:
         return new
 
     def _claims(self, slots):
-        """(lead, pages) of a decode step whose shared pages are worth the shared kernels in the layers that can take them, else None."""
+        """(lead, pages) of a decode step whose shared pages are worth the shared kernels in the layers that can take them, else None.
+        A family that gains nothing by them shares no pages in the step (its sequences are read one by one)."""
         claims = self.cache.shared_claims(slots, self._shared_needs)
         if claims is None:
             return None
         lead, pages, groups, need = claims
-        pays = kernels.attn_decode_shared_pays(groups, need.num_kv_heads, need.head_dim, need.eight_bits, self.model.ctx.compute_dtype, len(slots))
-        return (lead, pages) if pays else None
+        step = (need.num_kv_heads, need.head_dim, need.eight_bits, self.model.ctx.compute_dtype, len(slots))
+        if not kernels.attn_decode_shared_pays(groups, *step):
+            return None
+        gains = {g: kernels.attn_decode_shared_pays([g], *step, True) for g in set(groups)}
+        if not all(gains.values()):
+            members = [0] * len(slots)
+            for r, n in zip(lead, pages):
+                members[r] += n > 0
+            pages = [n if n and gains[members[r], n] else 0 for r, n in zip(lead, pages)]
+        return lead, pages
 
     def length(self, slot: int) -> int:
         return self.cache.length(slot)

@@ -1162,9 +1162,13 @@ def attn_decode8(out, q, kv, batch, nq: int, nkv: int, hd: int, scale: float, ca
         aux[key] = plan              # (now, not before: a refused call has made none)
 
 
-def attn_decode_shared_pays(groups, nkv: int, hd: int, eight_bits: bool = False, dtype=torch.bfloat16, n_seqs: int = 0) -> bool:
+def attn_decode_shared_pays(groups, nkv: int, hd: int, eight_bits: bool = False, dtype=torch.bfloat16, n_seqs: int = 0,
+                            beside: bool = False) -> bool:
     """Whether a decode step (of ``n_seqs`` sequences and activations of ``dtype``, where the shared kernels take these) is faster with
-    :func:`attn_decode_shared` than with :func:`attn_decode`: ``groups`` are (sequences, shared pages) of the step.  A rule on the pages that need not be read again, which come out of L2 at some 12 TB/s: a group's pages times its
+    :func:`attn_decode_shared` than with :func:`attn_decode`: ``groups`` are (sequences, shared pages) of the step, of which those that
+    gain nothing are left to themselves (``beside``: whether these gain in a step that is shared anyway).
+
+    A rule on the pages that need not be read again, which come out of L2 at some 12 TB/s: a group's pages times its
     sequences but one, and in the 8-bit cache, whose codes the shared kernel converts (0.9 us a page and block, of which the
     tensor-core products and the softmax take most) and the ordinary one reads at the memory's rate, but four.  Measured a layer of steps that make their
     plan once (ordinary / shared, us), kv heads x head size 4 x 256 and 8 x 128:
@@ -1176,9 +1180,10 @@ def attn_decode_shared_pays(groups, nkv: int, hd: int, eight_bits: bool = False,
     and 40.2 / 44.3."""
     if not attn_decode_shared_supported(dtype, hd, n_seqs):
         return False
-    members = sum(m for m, _ in groups)
-    spared = sum(n * (m - (4 if eight_bits else 1)) for m, n in groups)
-    return spared * nkv * hd >= 1024 * (512 + 10 * members if eight_bits else 384 + 4 * members)
+    once, a_seq, free = (512, 10, 4) if eight_bits else (384, 4, 1)
+    gains = [n * (m - free) * nkv * hd / 1024 - a_seq * m for m, n in groups]
+    gain = sum(g for g in gains if g > 0)
+    return gain > 0 and (beside or gain >= once)
 
 
 def attn_decode_shared_supported(dtype, hd: int, n_seqs: int) -> bool:

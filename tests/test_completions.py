@@ -175,22 +175,25 @@ def test_claims_are_of_the_groups_that_keep_all_keys():
         assert claims is None if want is None else claims[3] == want
 
 
+def _claiming(spec, dtype=torch.bfloat16, kv_dtype=None):
+    from airframe_b200.engine import Engine
+    model = Model(spec, dtype, "cpu", kv_dtype)
+    model.loaded = True
+    return Engine(model, 64 * 600, 64 * 70, max_sequences=60)
+
+
+def _family(eng, family, n, pages):
+    """n forks of one sequence (the bookkeeping alone: nothing is copied)."""
+    slots = [eng.take_slot() for _ in range(n)]
+    for s in slots:
+        eng.cache.lens[s], eng.cache._family[s] = 64 * pages, (family, pages)
+    return slots
+
+
 def _claims_of(spec, dtype=torch.bfloat16):
     """What an engine of this model claims for 40 forks of 64 pages each (far beyond what the rule asks for)."""
-    from airframe_b200.engine import Engine
-    model = Model(spec, dtype, "cpu")
-    model.loaded = True
-    eng = Engine(model, 64 * 6000, 64 * 70, max_sequences=60)
-    s = eng.take_slot()
-    eng.cache.reserve({s: 64 * 64})
-    eng.cache.commit({s: 64 * 64})
-    eng.cache._family[s] = (0, 64)
-    slots = [s]
-    for _ in range(39):                  # (the bookkeeping of forks alone: the pages are not copied)
-        t = eng.take_slot()
-        eng.cache.lens[t], eng.cache._family[t] = 64 * 64, (0, 64)
-        slots.append(t)
-    return eng._claims(slots)
+    eng = _claiming(spec, dtype)
+    return eng._claims(_family(eng, 0, 40, 64))
 
 
 def test_a_model_without_a_layer_that_shares_claims_nothing():
@@ -229,6 +232,21 @@ def test_shared_pages_pay_where_enough_is_read_again():
         assert pays([(32, 256), (2, 16)], 4, 128, eight)
     assert pays([(3, 1024)], 4, 256) and not pays([(3, 1024)], 4, 256, True)
     assert not pays([], 4, 256)
+
+
+def test_groups_that_gain_nothing_are_left_to_themselves():
+    """A pair in 8 bits costs more together than apart: it neither joins nor keeps a large group from being read once."""
+    from airframe_b200.kernels import attn_decode_shared_pays as pays
+    assert pays([(32, 256)], 8, 128, True) and pays([(32, 256), (2, 4096)], 8, 128, True) and not pays([(2, 4096)], 8, 128, True)
+    assert pays([(4, 64)], 8, 128, False, torch.bfloat16, 40, True) and not pays([(2, 4096)], 8, 128, True, torch.bfloat16, 40, True)
+    eng = _claiming(config_from_dict(dict(CONFIGS["D"], max_position_embeddings=64 * 70, num_attention_heads=8, num_key_value_heads=8, head_dim=128)).model_spec(),
+                    kv_dtype=F8)
+    many = _family(eng, 0, 40, 64)
+    pair, other = _family(eng, 1, 2, 60), _family(eng, 2, 2, 60)
+    slots = [pair[0], many[0], other[0], other[1], *many[1:], pair[1]]
+    lead, pages = eng._claims(slots)
+    assert pages == [0, 64, 0, 0] + [64] * 39 + [0] and lead[4:-1] == [1] * 39
+    assert eng._claims(pair + other) is None
 
 
 def test_a_fork_of_a_ring_has_its_rows():
