@@ -1168,20 +1168,26 @@ def attn_decode_shared_pays(groups, nkv: int, hd: int, eight_bits: bool = False,
     :func:`attn_decode_shared` than with :func:`attn_decode`: ``groups`` are (sequences, shared pages) of the step, of which those that
     gain nothing are left to themselves (``beside``: whether these gain in a step that is shared anyway).
 
-    A rule on the pages that need not be read again, which come out of L2 at some 12 TB/s: a group's pages times its
-    sequences but one, and in the 8-bit cache, whose codes the shared kernel converts (0.9 us a page and block, of which the
-    tensor-core products and the softmax take most) and the ordinary one reads at the memory's rate, but four.  Measured a layer of steps that make their
-    plan once (ordinary / shared, us), kv heads x head size 4 x 256 and 8 x 128:
-    bfloat16, 8 sequences: 32 pages 12.7 / 16.9 and 14.6 / 19.4, 64 pages 19.2 / 17.9 and 23.3 / 20.7, 128 pages 31.8 / 21.1 and
-    37.8 / 23.3; 64 sequences: 8 pages 27.1 / 27.3 and 35.3 / 35.1, 16 pages 37.9 / 30.2 and 49.1 / 36.1; 2 sequences: 512 pages 32.8 / 37.3
-    and 38.4 / 33.8, 2,048 pages 157 / 96 and 158 / 88.
-    8 bits, 8 sequences: 64 pages 20.1 / 26.9 and 18.2 / 22.3, 128 pages 28.5 / 29.7 and 26.6 / 25.3, 256 pages 45.1 / 37.1 and
-    43.1 / 32.3; 128 sequences: 8 pages 44.6 / 48.4 and 45.8 / 51.5, 16 pages 61.2 / 51.4 and 60.4 / 53.0; 4 sequences: 512 pages 47.0 / 49.1
-    and 40.2 / 44.3."""
+    A group of m sequences spares the reading of its pages m - 1 times, out of L2 at some 12 TB/s.  The prefix kernel takes longer for a
+    page than the ordinary one, the more the larger the heads (one accumulator with heads of 256), and in 8 bits, where it converts
+    the codes: less than 1.4 (heads of 128), 1.7 (256) or 3.5 (8 bits) sequences pay nothing.  Against it stand the plans and two
+    more kernels a step, a block's start and partial results for every kv head of a group, and the merge of every sequence; the unit is a page
+    of 1,024 elements (kv heads x head size).
+
+    Measured, a layer of steps that make their plan once for 13 (ordinary / shared, us), kv heads x head size 4 x 256 and 8 x 128:
+    bfloat16, one group of 8 sequences: 32 pages 12.2 / 15.5 and 14.2 / 18.4, 64 pages 18.6 / 16.5 and 23.2 / 19.5, 128 pages 31.5 / 19.7 and
+    38.3 / 21.7; of 64: 8 pages 27.5 / 26.2 and 35.0 / 33.6, 16 pages 37.3 / 28.5 and 48.8 / 34.6; of 2: 512 pages 33.4 / 35.4 and
+    37.8 / 32.0, 1,024 pages 60.4 / 55.1 and 78.9 / 49.6; 16 groups of 2: 64 pages 56.2 / 75.7 and 61.5 / 53.7, 128 pages 124 / 112 and
+    129 / 92; 64 groups of 2: 16 pages 29.1 / 42.1 and 42.8 / 65.4; 64 groups of 8: 8 pages 88.1 / 99.8 and 141 / 168.
+    8 bits, one group of 8: 64 pages 18.4 / 25.2 and 16.5 / 20.3, 128 pages 26.7 / 27.8 and 25.0 / 23.4, 256 pages 43.6 / 34.9 and 40.8 / 30.0; of
+    128: 8 pages 42.7 / 46.1 and 43.3 / 49.8, 16 pages 59.3 / 49.3 and 58.1 / 51.1; of 4: 512 pages 45.5 / 47.2 and 38.0 / 42.1; 32 groups of 8: 24 pages
+    66.1 / 78.1 and 72.7 / 95.6.
+    Of 1,833 such steps (1 to 64 groups of 2 to 128, 4 to 2,048 pages, 2 to 16 kv heads of 64, 128 and 256) the rule chooses the slower one for 171, all but
+    12 of them within a fifth: what is left between it and the times is the order in which the ordinary kernel's blocks meet shared pages in L2."""
     if not attn_decode_shared_supported(dtype, hd, n_seqs):
         return False
-    once, a_seq, free = (512, 10, 4) if eight_bits else (384, 4, 1)
-    gains = [n * (m - free) * nkv * hd / 1024 - a_seq * m for m, n in groups]
+    once, a_seq, a_head, free = (400, 10, 16, 3.5) if eight_bits else (200, 2, 5, 1.1 + 0.6 * hd / 256)
+    gains = [n * (m - free) * nkv * hd / 1024 - a_seq * m - a_head * nkv for m, n in groups]
     gain = sum(g for g in gains if g > 0)
     return gain > 0 and (beside or gain >= once)
 

@@ -249,6 +249,14 @@ def test_groups_that_gain_nothing_are_left_to_themselves():
     assert eng._claims(pair + other) is None
 
 
+def test_the_faster_way_of_pairs_and_of_many_groups():
+    """Where both ways were measured, the faster one: pairs of long prompts by head size, many small groups of short ones."""
+    from airframe_b200.kernels import attn_decode_shared_pays as pays
+    assert not pays([(2, 512)], 4, 256) and pays([(2, 1024)], 4, 256) and pays([(2, 512)], 8, 128)
+    assert not pays([(2, 16)] * 64, 4, 256) and not pays([(2, 16)] * 64, 8, 128) and not pays([(2, 64)] * 16, 4, 256) and pays([(4, 128)] * 4, 4, 256)
+    assert not pays([(8, 8)] * 64, 8, 128) and not pays([(8, 24)] * 32, 8, 128, True) and not pays([(8, 32)] * 64, 4, 256, True)
+
+
 def test_a_fork_of_a_ring_has_its_rows():
     """Every page of a window, the kept first tokens' and the begun page of all keys are copied, in every layer of a group."""
     ring, kept, full = KVNeed(1, 8, 192), KVNeed(2, 4, 128, keep_first=3), KVNeed(1, 8)
