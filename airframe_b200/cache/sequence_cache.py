@@ -370,6 +370,15 @@ class SequenceCache:
         for g in self.groups.values():
             g.flush()
 
+    def pages_wanted(self, tokens: int, shared: int = 0) -> list:
+        """Pages that a sequence which comes to hold these many tokens takes in every group; ``shared``: its first tokens whose whole
+        pages are another's (a fork)."""
+        return [pages_for(g.rows_held(tokens)) - (0 if g.ring_rows else shared // PAGE) for g in self.groups.values()]
+
+    def pages_there(self) -> list:
+        """Pages of every group, in the order of :meth:`pages_wanted`."""
+        return [g.n_pages for g in self.groups.values()]
+
     def fits(self, token_counts, shared=None) -> bool:
         """Whether sequences that come to hold these many tokens fit together:
         a slot each, and in every group the pages they hold there (a group with
@@ -379,8 +388,8 @@ class SequenceCache:
             return False
         if shared is None:
             shared = [0] * len(token_counts)
-        return all(sum(pages_for(g.rows_held(n)) - (0 if g.ring_rows else s // PAGE) for n, s in zip(token_counts, shared)) <= g.n_pages
-                   for g in self.groups.values())
+        wanted = [self.pages_wanted(n, s) for n, s in zip(token_counts, shared)]
+        return all(sum(each) <= there for each, there in zip(zip(*wanted), self.pages_there()))
 
     # ------------------------------------------------------------------ figures
 

@@ -115,31 +115,33 @@ class GenerationLoop:
             limit = min(limit, most)
         if self.max_batch:
             limit = min(limit, self.max_batch)
-        # a cache whose groups of layers have storage of their own answers for each of them
-        fits = getattr(self.engine.cache, "fits", None)
-        batches, cur, cur_pages = [], [], 0
-
-        def shares(i, batch):
-            """Tokens of request i whose pages an earlier completion of the same prompt in the batch (requests in order) holds."""
-            return len(prompts[i]) if fits is not None and batch and i % completions and i > batch[0] else 0
-
-        def together(batch):
-            if completions == 1:
-                return fits([self.tokens_held(len(prompts[j]), params) for j in batch])
-            return fits([self.tokens_held(len(prompts[j]), params) for j in batch], [shares(j, batch) for j in batch])
-
+        # a cache whose groups of layers have storage of their own answers for each of them (one that cannot count says whether a batch fits)
+        wanted = getattr(self.engine.cache, "pages_wanted", None)
+        fits = getattr(self.engine.cache, "fits", None) if wanted is None else None
+        there = self.engine.cache.pages_there() if wanted is not None else []
+        batches, cur = [], []
+        cur_pages, taken = 0, [0] * len(there)        # of the batch at hand: in all, and by group
         for i, p in enumerate(prompts):
             held = self.tokens_held(len(p), params)
             need = _pages(held)
-            if need > total_pages or (fits is not None and not fits([held])):
+            each = wanted(held) if wanted is not None else []
+            if need > total_pages or any(n > t for n, t in zip(each, there)) or (fits is not None and not fits([held])):
                 raise RequestError(f"request {i} needs {need} cache pages, the cache has {total_pages}")
-            need -= shares(i, cur) // PAGE
-            if cur and (len(cur) >= limit or cur_pages + need > total_pages or (fits is not None and not together(cur + [i]))):
-                batches.append(cur)
-                cur, cur_pages = [], 0
-                need = _pages(held)
+            if cur:
+                # (requests in order: one of a prompt's later completions has the one before it in the batch, and its whole pages)
+                mine, less = each, 0
+                if wanted is not None and i % completions:
+                    mine, less = wanted(held, len(p)), len(p) // PAGE
+                if (len(cur) < limit and cur_pages + need - less <= total_pages
+                        and all(n + m <= t for n, m, t in zip(taken, mine, there))
+                        and (fits is None or fits([self.tokens_held(len(prompts[j]), params) for j in cur] + [held]))):
+                    need, each = need - less, mine
+                else:
+                    batches.append(cur)
+                    cur, cur_pages, taken = [], 0, [0] * len(there)
             cur.append(i)
             cur_pages += need
+            taken = [n + m for n, m in zip(taken, each)]
         if cur:
             batches.append(cur)
         return batches

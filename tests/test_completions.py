@@ -257,6 +257,40 @@ def test_the_faster_way_of_pairs_and_of_many_groups():
     assert not pays([(8, 8)] * 64, 8, 128) and not pays([(8, 24)] * 32, 8, 128, True) and not pays([(8, 32)] * 64, 4, 256, True)
 
 
+def test_batches_are_planned_in_linear_time(monkeypatch):
+    """A request is asked about a bounded number of times, however many are in its batch, and the batches are those that ``fits`` allows."""
+    import random
+    from airframe_b200.sampling import SamplingParams
+    rng = random.Random(5)
+    asked = []
+    whole = SequenceCache.pages_wanted
+    monkeypatch.setattr(SequenceCache, "pages_wanted", lambda self, *a: (asked.append(1), whole(self, *a))[1])
+    monkeypatch.setattr(SequenceCache, "fits", None)
+    for completions in (1, 3, 700):
+        class Eng:
+            cache = SequenceCache([(KVNeed(1, 8), None, None), (KVNeed(1, 8, 200, keep_first=3), None, None)], 64 * 900, 4000, torch.float32, None,
+                                  max_sequences=800)
+            max_context = 4000
+            vocab_size = 100
+        prompts = [p for p in ([1] * rng.randint(1, 700) for _ in range(2100 // completions)) for _ in range(completions)]
+        params = SamplingParams(max_tokens=90)
+        asked.clear()
+        batches = GenerationLoop(Eng(), None).plan_batches(prompts, params, completions)
+        assert len(asked) <= 2 * len(prompts)
+        assert [i for b in batches for i in b] == list(range(len(prompts)))
+        monkeypatch.undo()
+        held = lambda b: [min(len(prompts[i]) + 89, 4000) for i in b]
+        shared = lambda b: [len(prompts[i]) if i % completions and i > b[0] else 0 for i in b]
+        for k, b in enumerate(batches):
+            assert Eng.cache.fits(held(b), shared(b))
+            if k + 1 < len(batches):                      # (and none could have taken the next request too)
+                more = b + [batches[k + 1][0]]
+                pages = sum((n + 63) // 64 - s // 64 for n, s in zip(held(more), shared(more)))
+                assert not Eng.cache.fits(held(more), shared(more)) or pages > Eng.cache.total_pages
+        monkeypatch.setattr(SequenceCache, "pages_wanted", lambda self, *a: (asked.append(1), whole(self, *a))[1])
+        monkeypatch.setattr(SequenceCache, "fits", None)
+
+
 def test_a_fork_of_a_ring_has_its_rows():
     """Every page of a window, the kept first tokens' and the begun page of all keys are copied, in every layer of a group."""
     ring, kept, full = KVNeed(1, 8, 192), KVNeed(2, 4, 128, keep_first=3), KVNeed(1, 8)
