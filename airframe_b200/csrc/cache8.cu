@@ -57,7 +57,8 @@ __global__ void __launch_bounds__(S8_THREADS) store_kv8_kernel(Store8Args a) {
     long long row = -1;
     if (slot >= 0 && af_cache_stores(pos, a.len_after[s], a.ring_rows, a.keep)) {
       const int cr = af_cache_row(pos, a.ring_rows, a.keep), entry = cr / AF_PAGE;
-      const int page = AF_INDEX_OK(entry < a.max_pages, entry) && entry < a.max_pages ? a.page_table[(size_t)slot * a.max_pages + entry] : -1;
+      const bool inside = pos >= 0 && entry < a.max_pages;
+      const int page = AF_INDEX_OK(inside, pos) && inside ? a.page_table[(size_t)slot * a.max_pages + entry] : -1;
       if (AF_INDEX_OK(page >= 0 && page < a.n_pages, page) && page >= 0 && page < a.n_pages)      // (a bad page is not written)
         row = (long long)page * a.nkv * AF_PAGE + cr % AF_PAGE;
     }

@@ -1,13 +1,12 @@
 """Limits of the 8-bit cache's attention and of shared prefixes: rows and pages of odd addresses, refusals that come before any
 launch, plans of calls that were refused, positions and lengths beyond a page table."""
 import ctypes
-import math
 from types import SimpleNamespace
 
 import pytest
 import torch
 
-from test_cache8 import F8, PAGE, View, fill, step
+from test_cache8 import PAGE, View, fill, step
 
 DEV = "cuda:0"
 
@@ -204,3 +203,38 @@ def test_a_refused_call_leaves_no_plan(K, monkeypatch, shared):
     call()
     call()
     assert lib.made == [True, True, False] and len(b.aux) == 1
+
+
+# ---------------------------------------------------------------------------------------------- beyond the page table
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("pos", [-1, -64, -65, -1000, 128, 1000, 2 ** 31 - 1])
+def test_store_of_positions_outside_the_table(K, pos):
+    """A token whose position lies before the first or behind the table's last page is not stored; its neighbours are, and other
+    sequences' pages stay as they were."""
+    hd, nkv, nq = 128, 2, 2
+    view = View([128, 128, 128], nkv, hd).to(DEV)
+    order = view.order
+    x = torch.randn(3, (nq + 2 * nkv) * hd, device=DEV).to(torch.bfloat16)
+    t = lambda v: torch.tensor(v, dtype=torch.int32, device=DEV)
+
+    def stored(places):
+        for name in "kv":
+            getattr(view, name).view(torch.uint8).copy_(view.codes[name])
+            getattr(view, name + "_exp").copy_(view.exps[name])
+        b = SimpleNamespace(positions=t([places[i] for i in range(3)]), seq_of_token=t([0, 1, 2]), slots=t(order), len_after=t([128] * 3))
+        rounded = torch.empty(3, 2 * nkv * hd, dtype=torch.bfloat16, device=DEV)
+        K.store_kv8(x, b, nq, nkv, hd, view, rounded=rounded)
+        return [view.k.view(torch.uint8).clone(), view.v.view(torch.uint8).clone(), view.k_exp.clone(), view.v_exp.clone(), rounded]
+
+    whole, got = stored([5, 70, 127]), stored([5, pos, 127])
+    page = int(view.table_host[order[1], 1])
+    for w, g, name in zip(whole[:4], got[:4], ("k", "v", "k", "v")):
+        was = (view.codes if w.dim() == 4 else view.exps)[name].to(DEV)
+        w[page, :, 6] = was[page, :, 6]                    # (what position 70 wrote)
+        assert torch.equal(w, g)
+    assert torch.equal(whole[4], got[4])
+    inv = torch.ones(hd // 2, device=DEV)
+    b = SimpleNamespace(positions=t([pos] * 3), seq_of_token=t([0, 1, 2]), slots=t(order), len_after=t([128] * 3))
+    K.rope_store_kv8(x.clone(), b, inv, nq, nkv, hd, hd, "half", view)
+    assert torch.equal(view.k.view(torch.uint8), got[0]) and torch.equal(view.v_exp, got[3])
