@@ -300,8 +300,8 @@ __device__ __forceinline__ void da_write_plan(int* plan, const int* slots, const
       const DaList l = da_list(pos, window, keep, first);
       for (int i = 0; i < 4 && i < fs.n_pages; ++i) {
         const int entry = af_cache_row(da_page_of(l.kept, l.skip, fs.p_in + i) * AF_PAGE, ring_rows, keep) / AF_PAGE;
-        int page = AF_INDEX_OK(entry < max_pages, entry) ? page_table[(size_t)slot * max_pages + entry] : 0;
-        if (!AF_INDEX_OK(page >= 0, page)) page = 0;
+        int page = AF_INDEX_OK(entry < max_pages, entry) && entry < max_pages ? page_table[(size_t)slot * max_pages + entry] : 0;
+        if (!AF_INDEX_OK(page >= 0, page) || page < 0) page = 0;
         ids[i] = page;
       }
     }

@@ -6,7 +6,7 @@ from types import SimpleNamespace
 import pytest
 import torch
 
-from test_cache8 import PAGE, View, fill, step
+from test_cache8 import PAGE, View, bound, fill, plain_attention, step
 
 DEV = "cuda:0"
 
@@ -238,3 +238,25 @@ def test_store_of_positions_outside_the_table(K, pos):
     b = SimpleNamespace(positions=t([pos] * 3), seq_of_token=t([0, 1, 2]), slots=t(order), len_after=t([128] * 3))
     K.rope_store_kv8(x.clone(), b, inv, nq, nkv, hd, hd, "half", view)
     assert torch.equal(view.k.view(torch.uint8), got[0]) and torch.equal(view.v_exp, got[3])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("hd", [64, 256])
+def test_lengths_beyond_the_table(K, hd):
+    """A length that the page table has no entries for reads no page of its own; the step's other sequences are as they should be."""
+    nq, nkv = 4, 2
+    lens = [128, 100, 128]
+    view = View(lens, nkv, hd)
+    held = fill(view, lens, nkv, hd)
+    view.to(DEV)
+    q = torch.randn(3, nq * hd).to(torch.bfloat16)
+    ref, mag, big = plain_attention(q, held, lens, nq, nkv, hd, 0.1, 0.0, 0, "window", 0, None)
+    ok = lambda out: bool(((out.double().cpu().view(3, nq, hd) - ref).abs() <= bound(ref, mag, big, hd))[0::2].all())
+    lead, pages = (torch.tensor(v, dtype=torch.int32, device=DEV) for v in ([0, 1, 2], [0, 0, 0]))
+    for long in (129, 64 * 60, 64 * 3000 + 7):
+        out = torch.empty(3, nq * hd, dtype=torch.bfloat16, device=DEV)
+        K.attn_decode(out, q.to(DEV), view, step(view, [128, long, 128], DEV), nq, nkv, hd, 0.1, 0.0, 0)
+        assert ok(out)
+        K.attn_decode_shared(out.zero_(), q.to(DEV), view, step(view, [128, long, 128], DEV), nq, nkv, hd, 0.1, 0.0, lead, pages, 1)
+        assert ok(out)
+    K.check_device_errors(DEV)
