@@ -146,6 +146,8 @@ class Engine:
         head can find the best without them)."""
         entries = [e if isinstance(e, StepEntry) else StepEntry(*e) for e in entries]
         lens = self.check(entries)
+        if lens[0] > 0:
+            self._check_rows(pad_to)
         growth = {e.slot: n + len(e.tokens) for e, n in zip(entries, lens)}
         self.cache.reserve(growth)
         self.cache.flush()

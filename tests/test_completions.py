@@ -196,6 +196,19 @@ def _claims_of(spec, dtype=torch.bfloat16):
     return eng._claims(_family(eng, 0, 40, 64))
 
 
+def test_padding_counts_as_rows_of_a_step():
+    """More rows than the 8-bit cache's attention plans for are refused before anything changes, padding or not."""
+    from airframe_b200.engine import StepError
+    eng = _claiming(config_from_dict(CONFIGS["D"]).model_spec(), kv_dtype=F8)
+    s = eng.take_slot()
+    eng.cache.reserve({s: 64})
+    eng.cache.commit({s: 64})
+    held = eng.cache.pages_held()
+    with pytest.raises(StepError, match="up to 2048 sequences"):
+        eng.step([StepEntry(s, [1], [0])], pad_to=2049)
+    assert eng.length(s) == 64 and eng.cache.pages_held() == held
+
+
 def test_a_model_without_a_layer_that_shares_claims_nothing():
     """Shared steps have graphs of their own: a model whose kernels would be the ordinary ones again makes none (32 bits, head sizes
     that the shared kernels do not take, latent attention, score slopes, windows alone)."""
