@@ -142,7 +142,7 @@ class Rope(PositionEncoding):
         self._plain_only()
         if self.rotary_dim > hd:
             raise ConfigError(f"rope: rotary_dim {self.rotary_dim} exceeds head_dim {hd}")
-        if kv.k_exp is not None:
+        if getattr(kv, "k_exp", None) is not None:
             kernels.rope_store_kv8(qkv, batch, self.inv_freq, nq, nkv, hd, self.rotary_dim, self.pairing, kv, parts=parts)
             return True
         table = self._prompt_table(qkv, batch, hd, parts)

@@ -196,6 +196,21 @@ def _claims_of(spec, dtype=torch.bfloat16):
     return eng._claims(_family(eng, 0, 40, 64))
 
 
+def test_rope_stores_into_views_without_exponents(monkeypatch):
+    """A view of cache pages that knows nothing of 8 bits goes to the rotation and store of the compute dtype, as it did."""
+    from types import SimpleNamespace
+    from airframe_b200 import kernels
+    from airframe_b200.config import PartSpec
+    from airframe_b200.parts import BuildContext, build_part
+    rope = build_part("position", PartSpec("rope", {"theta": 10000.0, "rotary_dim": 16, "pairing": "half"}), BuildContext(torch.bfloat16, torch.device("cpu")))
+    went = []
+    monkeypatch.setattr(kernels, "rope_cache_write", lambda *a, **k: went.append(k["kcache"]))
+    t = torch.zeros(3, dtype=torch.int32)
+    batch = SimpleNamespace(positions=t, seq_of_token=t, slots=t, len_after=t, aux={})
+    kv = SimpleNamespace(k="pages", v="pages", page_table=t.view(1, 3), ring_rows=0, keep_first=0)
+    assert rope.encode_and_store(torch.zeros(3, 4 * 16, dtype=torch.bfloat16), batch, 2, 1, 16, kv) and went == ["pages"]
+
+
 def test_padding_counts_as_rows_of_a_step():
     """More rows than the 8-bit cache's attention plans for are refused before anything changes, padding or not."""
     from airframe_b200.engine import StepError
