@@ -517,6 +517,46 @@ def test_forks_go_on_like_separate_sequences(tmp_path, monkeypatch, name, dtype,
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("kv", [None, "float8_e4m3"])
+def test_the_rule_in_the_engine(tmp_path, monkeypatch, kv):
+    """Twenty forks behind 45 pages go through the shared kernels by the rule's own word, three behind 2 pages and a pair beside the
+    twenty do not; all of them give what sequences of their own give."""
+    from airframe_b200 import kernels
+    from airframe_b200.engine import GpuRuntime
+    cfg = dict(CONFIGS["D"], max_position_embeddings=4096)
+    rt = GpuRuntime.load(make_folder(cfg, seed=5, store_dtype="bfloat16", root=tmp_path), max_tokens=64 * 160, kv_dtype=kv)
+    eng, V, shared = rt.engine, cfg["vocab_size"], []
+    whole = kernels.attn_decode_shared
+    monkeypatch.setattr(kernels, "attn_decode_shared", lambda *a, **k: (shared.append(a), whole(*a, **k))[1])
+
+    def forks(prompt, n):
+        s = eng.take_slot()
+        rt.step([StepEntry(s, prompt, [])])
+        return [s] + eng.fork(s, n - 1)
+
+    few = replay.random_ids(V, 140, 5)
+    tails = [replay.random_ids(V, 3, 100 + i) for i in range(20)]
+    _forked(rt, few, tails[:3])
+    assert not shared
+    prompt, other = replay.random_ids(V, 64 * 45 + 10, 6), replay.random_ids(V, 64 * 3 + 5, 7)
+    many, pair = forks(prompt, 20), forks(other, 2)
+    slots, mine = [pair[0], *many, pair[1]], [tails[0], *tails, tails[1]]
+    eng.use_graphs = True
+    got = torch.stack([rt.step([StepEntry(s, [t[i]], [0]) for s, t in zip(slots, mine)]).cpu() for i in range(3)])
+    assert shared
+    graph = next(g for k, g in eng._graphs.items() if isinstance(k, tuple) and k[-1] == "shared")
+    Bp = eng.padded_batch(22)
+    pages = graph["dynamic"][5 * Bp: 5 * Bp + 22].tolist()
+    assert pages == [0] + [45] * 20 + [0]
+    for s in slots:
+        eng.free_slot(s)
+    eng.use_graphs = False
+    for r, ids in ((0, other), (1, prompt), (9, prompt), (21, other)):
+        ref = replay.run_tail(rt, ids + mine[r], 3)[-3:]
+        assert rel_err(got[:, r], ref) < BF16_SPLITS
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("make,cfg", [(tiny_fiferax.make_folder, tiny_fiferax.CONFIGS["A"]), (tiny_retudra.make_folder, tiny_retudra.CONFIGS["A"])])
 def test_forks_of_sequences_with_states(tmp_path, make, cfg):
     from airframe_b200.engine import GpuRuntime
