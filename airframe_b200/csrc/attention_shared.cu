@@ -91,7 +91,8 @@ __device__ __forceinline__ int sh_items(int pages, int units, int rows, int hd, 
   return max(1, min(min(pages, pay), (int)min((long long)pages, (long long)pages * blocks / total)));
 }
 
-// Some 7 us a step, for all layers.  Two blocks: the first writes the prefix kernel's plan, the second the split kernel's.  (Like attn_decode_plan_kernel they do not
+// A step's, for all layers: some 7 us with up to 64 sequences, 24 with 64 groups of 4, 50 to 70 with one of 2,048, 170 with 512 of 4 (a group's units and
+// items by one warp).  Two blocks: the first writes the prefix kernel's plan, the second the split kernel's.  (Like attn_decode_plan_kernel they do not
 // release their dependents early.)  A group is the live rows of one `lead` that share at least a page; alone in it a row keeps its pages.  Fewer
 // pages than a row claims are taken where another of the group shares fewer, and never the page of its new token.
 __global__ void __launch_bounds__(512)
@@ -106,11 +107,13 @@ attn_shared_plan_kernel(int* plan, const int* lead, const int* pages, const int*
   int* memb0 = item0 + batch;          //           first place in `order`
   int* row0 = memb0 + batch;           //           first partial row
   int* parts = row0 + batch;           //           items of a unit
+  int* seen = parts + batch;           //           members met so far
+  int* lead_row = seen + batch;        //           the first member
   pdl_wait();
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int group = nq / nkv;
   const ShPlan L = sh_layout(batch, nq, nkv, blocks);
-  for (int b = tid; b < batch; b += blockDim.x) cnt[b] = 0, few[b] = 0x7fffffff;
+  for (int b = tid; b < batch; b += blockDim.x) cnt[b] = 0, few[b] = 0x7fffffff, seen[b] = 0;
   __syncthreads();
   for (int b = tid; b < batch; b += blockDim.x) {
     const int len = lens[b], p = slots[b] >= 0 && len > 0 ? min(pages[b], (len - 1) / AF_PAGE) : 0, g = lead[b];
@@ -171,30 +174,33 @@ attn_shared_plan_kernel(int* plan, const int* lead, const int* pages, const int*
     if (lane == 0) {
       plan[0] = items, plan[1] = units, plan[2] = batch, plan[3] = nq, plan[4] = nkv, plan[5] = blocks;
     }
+  } else if (warp == 1) {
+    // each row's place among its group's members, in the order of the rows: 32 rows at a time, a lane counts those of its group before it
+    for (int base = 0; base < batch; base += 32) {
+      const int b = base + lane, g = b < batch ? gid[b] : -1;
+      const uint32_t same = __match_any_sync(0xffffffffu, g);
+      const int place = g >= 0 ? seen[g] + __popc(same & ((1u << lane) - 1)) : 0;
+      __syncwarp();
+      if (g >= 0) {
+        if (place == 0) lead_row[g] = b;
+        if (lane == __ffs(same) - 1) seen[g] += __popc(same);
+      }
+      if (b < batch) plan[L.loc + 2 * b + 1] = place;
+      __syncwarp();
+    }
   }
   __syncthreads();
   for (int b = tid; b < batch; b += blockDim.x) {
     const int g = gid[b];
     const bool on = g >= 0 && cnt[g] >= 2;
-    int place = 0;
-    if (on)
-      for (int j = 0; j < b; ++j) place += gid[j] == g ? 1 : 0;
     plan[L.shared + b] = on ? few[g] : 0;
     plan[L.loc + 2 * b] = on ? unit0[g] : -1;
-    plan[L.loc + 2 * b + 1] = place;
-    if (on) plan[L.order + memb0[g] + place] = b;
+    if (on) plan[L.order + memb0[g] + plan[L.loc + 2 * b + 1]] = b;
   }
   for (int g = warp; g < batch; g += (int)blockDim.x >> 5) {
     const int c = cnt[g];
     if (c < 2) continue;
-    int b = 0;                                            // a member's slot: its page table holds the shared pages
-    for (int base = 0; base < batch; base += 32) {
-      const uint32_t with = __ballot_sync(0xffffffffu, base + lane < batch && gid[min(base + lane, batch - 1)] == g);
-      if (with) {
-        b = base + __ffs(with) - 1;
-        break;
-      }
-    }
+    const int b = lead_row[g];                            // a member's slot: its page table holds the shared pages
     const int rows = c * group, tiles = (rows + SH_ROWS - 1) / SH_ROWS, u = nkv * tiles;
     const int s = parts[g];
     for (int x = lane; x < u; x += 32) {

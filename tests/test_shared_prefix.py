@@ -395,3 +395,20 @@ def test_prefix_of_what_is_not_finite(K, bits):
     struck[0::2, nq // 2:, 3] = True                          # (the second kv head's query heads of the first group, that dim)
     assert bool(got[struck].isnan().all()) and bool(((got - ref).abs() <= lim)[~struck].all())
     K.check_device_errors(DEV)
+
+
+@pytest.mark.parametrize("bits", [16, 8])
+def test_many_groups_in_any_order(K, bits):
+    """Hundreds of rows whose groups' members lie among one another in no order, rows alone between them: a row's place is its own."""
+    nq, nkv, hd = 2, 1, 64
+    rng = torch.Generator().manual_seed(3)
+    groups = torch.randint(0, 60, (333,), generator=rng).tolist()
+    seqs = [(g, 2, 129 + (7 * i) % 60) for i, g in enumerate(groups)]
+    f = Family(seqs, nkv, hd, bits)
+    q = torch.randn(len(seqs), nq * hd).to(torch.bfloat16)
+    ref, mag, big = plain_attention(q, f.held, f.lens, nq, nkv, hd, 0.125, 0.0, 0, "window", 0, None)
+    lead, pages = f.lead()
+    out = torch.empty(len(seqs), nq * hd, dtype=torch.bfloat16, device=DEV)
+    K.attn_decode_shared(out, q.to(DEV), f, f.step(), nq, nkv, hd, 0.125, 0.0, lead, pages, 2)
+    assert bool(((out.double().cpu().view(-1, nq, hd) - ref).abs() <= bound(ref, mag, big, hd)).all())
+    K.check_device_errors(DEV)
