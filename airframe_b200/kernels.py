@@ -1176,13 +1176,13 @@ def attn_decode_shared_pays(groups, nkv: int, hd: int, eight_bits: bool = False,
 
     Measured, a layer of steps that make their plan once for 13 (ordinary / shared, us), kv heads x head size 4 x 256 and 8 x 128:
     bfloat16, one group of 8 sequences: 32 pages 12.2 / 15.5 and 14.2 / 18.4, 64 pages 18.6 / 16.5 and 23.2 / 19.5, 128 pages 31.5 / 19.7 and
-    38.3 / 21.7; of 64: 8 pages 27.5 / 26.2 and 35.0 / 33.6, 16 pages 37.3 / 28.5 and 48.8 / 34.6; of 2: 512 pages 33.4 / 35.4 and
-    37.8 / 32.0, 1,024 pages 60.4 / 55.1 and 78.9 / 49.6; 16 groups of 2: 64 pages 56.2 / 75.7 and 61.5 / 53.7, 128 pages 124 / 112 and
-    129 / 92; 64 groups of 2: 16 pages 29.1 / 42.1 and 42.8 / 65.4; 64 groups of 8: 8 pages 88.1 / 99.8 and 141 / 168.
+    38.3 / 21.7; of 64: 8 pages 27.5 / 26.2 and 35.0 / 33.6, 16 pages 37.3 / 28.5 and 48.8 / 34.6; of 2: 512 pages 33.5 / 35.1 and
+    38.0 / 32.1, 1,024 pages 56.9 / 55.0 and 78.9 / 49.7; 16 groups of 2: 64 pages 56.2 / 75.9 and 61.6 / 53.2, 128 pages 124 / 116 and
+    130 / 96; 64 groups of 2: 16 pages 29.1 / 41.9 and 42.9 / 65.2; 64 groups of 8: 8 pages 88.1 / 98.0 and 141 / 166.
     8 bits, one group of 8: 64 pages 18.4 / 25.2 and 16.5 / 20.3, 128 pages 26.7 / 27.8 and 25.0 / 23.4, 256 pages 43.6 / 34.9 and 40.8 / 30.0; of
     128: 8 pages 42.7 / 46.1 and 43.3 / 49.8, 16 pages 59.3 / 49.3 and 58.1 / 51.1; of 4: 512 pages 45.5 / 47.2 and 38.0 / 42.1; 32 groups of 8: 24 pages
-    66.1 / 78.1 and 72.7 / 95.6.
-    Of 1,833 such steps (1 to 64 groups of 2 to 128, 4 to 2,048 pages, 2 to 16 kv heads of 64, 128 and 256) the rule chooses the slower one for 171, all but
+    65.9 / 77.5 and 72.7 / 94.9.
+    Of 1,765 such steps (1 to 64 groups of 2 to 128, 4 to 2,048 pages, 2 to 16 kv heads of 64, 128 and 256) the rule chooses the slower one for 168, all but
     12 of them within a fifth: what is left between it and the times is the order in which the ordinary kernel's blocks meet shared pages in L2."""
     if not attn_decode_shared_supported(dtype, hd, n_seqs):
         return False
