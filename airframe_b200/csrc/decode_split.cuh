@@ -70,6 +70,7 @@ constexpr int D8_BREAK_PAGES = 4;
 // Blocks of the 8-bit split kernel: two an SM (a block's end of a unit then falls into the other's work) where their registers fit.  (The same step
 // with one an SM: 105 us.)
 inline int d8_blocks(int sms, int nq, int nkv) { return nq / nkv <= 8 ? 2 * sms : sms; }
+static_assert(DA_BREAK_PAGES != D8_BREAK_PAGES, "da_plan and the plans' marks tell the two caches apart by their breaks");
 __device__ __forceinline__ int da_plan_mark(int blocks, int brk) { return blocks | (brk << 16); }
 
 struct DaPlan {

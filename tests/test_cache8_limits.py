@@ -260,3 +260,39 @@ def test_lengths_beyond_the_table(K, hd):
         K.attn_decode_shared(out.zero_(), q.to(DEV), view, step(view, [128, long, 128], DEV), nq, nkv, hd, 0.1, 0.0, lead, pages, 1)
         assert ok(out)
     K.check_device_errors(DEV)
+
+
+# ---------------------------------------------------------------------------------------------- what is beside the 8-bit cache
+
+@pytest.mark.gpu
+def test_heads_that_are_no_multiple_are_refused(K):
+    nq, nkv, hd = 3, 2, 64
+    view = View([70], nkv, hd).to(DEV)
+    q = torch.zeros(1, nq * hd, dtype=torch.bfloat16, device=DEV)
+    with pytest.raises(K.KernelError, match="heads"):
+        K.attn_decode(torch.empty_like(q), q, view, step(view, [70], DEV), nq, nkv, hd, 1.0, 0.0, 0)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("tokens", [63, 64, 300, 1200])
+def test_rotation_of_prompts_alone_has_the_bits_of_the_rotation_with_its_store(K, dtype, tokens):
+    """A rotary encoding reads the step's table of cosines and sines from so many rows on whether or not it stores: the same rows as
+    without the table, and as with the store."""
+    from airframe_b200.config import PartSpec
+    from airframe_b200.parts import BuildContext, build_part
+    nq, nkv, hd = 4, 2, 128
+    rope = build_part("position", PartSpec("rope", {"theta": 10000.0, "rotary_dim": hd, "pairing": "half"}), BuildContext(dtype, torch.device(DEV)))
+    rope.load({})
+    x = torch.randn(tokens, (nq + 2 * nkv) * hd, device=DEV).to(dtype)
+    pos = torch.arange(tokens, dtype=torch.int32, device=DEV) * 7
+    n_pages = -(-int(tokens) * 7 // PAGE)
+    kv = SimpleNamespace(k=torch.zeros(n_pages, nkv, PAGE, hd, dtype=dtype, device=DEV), v=torch.zeros(n_pages, nkv, PAGE, hd, dtype=dtype, device=DEV),
+                         page_table=torch.arange(n_pages, dtype=torch.int32, device=DEV)[None], ring_rows=0, keep_first=0)
+    batch = lambda: SimpleNamespace(positions=pos, seq_of_token=torch.zeros_like(pos), slots=torch.zeros(1, dtype=torch.int32, device=DEV),
+                                    len_after=torch.full((1,), tokens * 7, dtype=torch.int32, device=DEV), aux={})
+    alone, stored, plain = x.clone(), x.clone(), x.clone()
+    rope.encode(alone, batch(), nq, nkv, hd)
+    assert rope.encode_and_store(stored, batch(), nq, nkv, hd, kv)
+    K.rope_cache_write(plain, pos, rope.inv_freq, nq, nkv, hd, hd, "half")
+    assert torch.equal(alone, plain) and torch.equal(alone, stored)
