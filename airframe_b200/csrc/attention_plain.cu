@@ -38,6 +38,7 @@ __device__ __forceinline__ float rope_src(const T* row, const float* parts, int 
 struct Rope8 {
   uint8_t *k, *v, *k_exp, *v_exp;
   long long n_pages;
+  bool late;      // more tokens than sequences: the kernel behind may not start before earlier pages are written (see cache8.cu)
 };
 
 // EIGHT (bfloat16 rows, blocks of hd / 2 threads): k and v go to the 8-bit cache as store_kv8 keeps them; a thread has at most a pair and
@@ -50,7 +51,7 @@ __global__ void rope_cache_kernel(T* __restrict__ qkv, int row_stride, const flo
                                   int nq, int nkv, int hd, int rot_dim, int pairing,
                                   T* __restrict__ kcache, T* __restrict__ vcache,
                                   const int* __restrict__ page_table, int max_pages, int ring_rows, int keep, Rope8 c8) {
-  pdl_launch_dependents();
+  if (!EIGHT || !c8.late) pdl_launch_dependents();
   // Positions, slots, lengths, the page table and the frequencies are inputs of the step, not
   // results of the kernel before: the row's place in the cache and the first pair's sine and
   // cosine are worked out before the wait for that kernel.
@@ -376,7 +377,7 @@ struct AfRopeStore8 {
   const int* page_table;
   uint8_t *k, *v, *k_exp, *v_exp;
   cudaStream_t stream;
-  long long row_stride, n_parts, part_stride, n_tokens, nq, nkv, hd, rot_dim, pairing, max_pages, n_pages, ring_rows, keep;
+  long long row_stride, n_parts, part_stride, n_tokens, nq, nkv, hd, rot_dim, pairing, max_pages, n_pages, ring_rows, keep, n_seqs;
 };
 
 // af_rope_cache_write of bfloat16 rows and af_store_kv8 in one kernel, for the few rows of decode steps: the same rows, codes and exponents.
@@ -393,7 +394,7 @@ AF_EXPORT int af_rope_store_kv8(const AfRopeStore8* c) {
             (__nv_bfloat16*)c->qkv, (int)c->row_stride, c->parts, (int)c->n_parts, (size_t)c->part_stride, c->positions, c->seq_of_token, c->slots,
             c->len_after, c->inv_freq, (int)c->nq, (int)c->nkv, (int)c->hd, (int)c->rot_dim, (int)c->pairing, (__nv_bfloat16*)nullptr,
             (__nv_bfloat16*)nullptr, c->page_table, (int)c->max_pages, (int)c->ring_rows, (int)c->keep,
-            Rope8{c->k, c->v, c->k_exp, c->v_exp, c->n_pages});
+            Rope8{c->k, c->v, c->k_exp, c->v_exp, c->n_pages, c->n_tokens > c->n_seqs});
   AF_CHECK_LAUNCH("af_rope_store_kv8");
 }
 

@@ -25,6 +25,7 @@ struct Store8Args {
   int max_pages, T, nq, nkv, ring_rows, keep;
   long long n_pages;
   uint8_t *k, *v, *k_exp, *v_exp;
+  int n_seqs;
   uint32_t by_token;           // 2^32 / (2 nkv), rounded up: x / (2 nkv) is the high word of x times it (x below 2^16)
 };
 
@@ -32,7 +33,9 @@ struct Store8Args {
 // threads work out where its tokens' rows go (a chain of four loads a token).
 template <int HD, int U>
 __global__ void __launch_bounds__(S8_THREADS) store_kv8_kernel(Store8Args a) {
-  pdl_launch_dependents();
+  // (the attention behind a decode step's store reads all pages but the new tokens' before it waits for this kernel: more tokens than
+  // sequences fill earlier pages too, and it may not start before they are there)
+  if (a.T <= a.n_seqs) pdl_launch_dependents();
   pdl_wait();
   constexpr int LANES = HD / 8, ROWS = S8_THREADS / LANES;       // rows that the block takes at a time
   __shared__ long long row_s[U * ROWS / 2 + 2];                  // the block's tokens' rows of a page's first head (-1: not stored)
@@ -150,7 +153,7 @@ AF_EXPORT int af_cache8_supported(int hd) { return hd == 64 || hd == 128 || hd =
 struct AfStore8 {
   const void *qkv, *rounded, *positions, *seq_of_token, *slots, *len_after, *page_table, *k, *v, *k_exp, *v_exp;
   cudaStream_t stream;
-  long long ld, rounded_ld, n_pages, max_pages, ring_rows, keep, T, nq, nkv, hd;
+  long long ld, rounded_ld, n_pages, max_pages, ring_rows, keep, T, nq, nkv, hd, n_seqs;
 };
 
 // The k and v heads of the packed bfloat16 rows [q | k | v] (T of them, ld elements apart) into the 8-bit pages of their
@@ -167,7 +170,7 @@ AF_EXPORT int af_store_kv8(const AfStore8* c) {
   Store8Args a{(const __nv_bfloat16*)c->qkv, c->ld, (__nv_bfloat16*)c->rounded, c->rounded_ld, (const int*)c->positions,
                (const int*)c->seq_of_token, (const int*)c->slots, (const int*)c->len_after, (const int*)c->page_table, (int)c->max_pages,
                (int)c->T, (int)c->nq, (int)c->nkv, (int)c->ring_rows, (int)c->keep, c->n_pages, (uint8_t*)c->k, (uint8_t*)c->v,
-               (uint8_t*)c->k_exp, (uint8_t*)c->v_exp, (uint32_t)(((1ull << 32) + 2 * c->nkv - 1) / (2 * c->nkv))};
+               (uint8_t*)c->k_exp, (uint8_t*)c->v_exp, (int)c->n_seqs, (uint32_t)(((1ull << 32) + 2 * c->nkv - 1) / (2 * c->nkv))};
   if (c->hd == 64) return launch_store8<64>(a, c->stream);
   if (c->hd == 128) return launch_store8<128>(a, c->stream);
   return launch_store8<256>(a, c->stream);

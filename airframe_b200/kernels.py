@@ -337,8 +337,8 @@ CACHE8_HEAD_SIZES = (64, 128, 256)     # head sizes that the 8-bit cache takes
 
 # What the entry points below take as one block of 64-bit words (pointers, whole numbers, then 64-bit floats): a ctypes argument
 # costs the host some 0.3 us, a packed one 0.05.
-_STORE8 = struct.Struct("<12Q10q")
-_ROPE_STORE8 = struct.Struct("<13Q13q")
+_STORE8 = struct.Struct("<12Q11q")
+_ROPE_STORE8 = struct.Struct("<13Q14q")
 _DECODE8 = struct.Struct("<14Q13q2d")
 _SHARED = struct.Struct("<17Q11q2d")
 
@@ -393,7 +393,8 @@ def store_kv8(qkv, batch, nq: int, nkv: int, hd: int, kv, rounded=None) -> None:
     _check(_lib().af_store_kv8(_STORE8.pack(
         qkv.data_ptr(), 0 if rounded is None else rounded.data_ptr(), positions.data_ptr(), seq.data_ptr(), slots.data_ptr(), lens.data_ptr(),
         table.data_ptr(), kv.k.data_ptr(), kv.v.data_ptr(), kv.k_exp.data_ptr(), kv.v_exp.data_ptr(), _raw_stream(dev),
-        _rows(qkv, "qkv"), 0 if rounded is None else _rows(rounded, "rounded"), n_pages, table.shape[1], kv.ring_rows, kv_keep(kv), T, nq, nkv, hd)))
+        _rows(qkv, "qkv"), 0 if rounded is None else _rows(rounded, "rounded"), n_pages, table.shape[1], kv.ring_rows, kv_keep(kv), T, nq, nkv, hd,
+        slots.numel())))
 
 
 def rope_store_kv8(qkv, batch, inv_freq, nq: int, nkv: int, hd: int, rot_dim: int, pairing: str, kv, parts=None) -> None:
@@ -419,7 +420,7 @@ def rope_store_kv8(qkv, batch, inv_freq, nq: int, nkv: int, hd: int, rot_dim: in
         qkv.data_ptr(), 0 if parts is None else parts.data_ptr(), positions.data_ptr(), seq.data_ptr(), slots.data_ptr(), lens.data_ptr(),
         inv_freq.data_ptr(), table.data_ptr(), kv.k.data_ptr(), kv.v.data_ptr(), kv.k_exp.data_ptr(), kv.v_exp.data_ptr(), _raw_stream(dev),
         _rows(qkv, "qkv"), 0 if parts is None else parts.shape[0], 0 if parts is None else parts.stride(0), T, nq, nkv, hd, rot_dim,
-        PAIRINGS[pairing], table.shape[1], n_pages, kv.ring_rows, kv_keep(kv))))
+        PAIRINGS[pairing], table.shape[1], n_pages, kv.ring_rows, kv_keep(kv), slots.numel())))
 
 
 def sum_parts(qkv, parts, batch, nq: int, nkv: int, hd: int) -> None:
@@ -1132,7 +1133,9 @@ def _decode_rows(who: str, out, q, batch, nq: int, hd: int, sinks) -> int:
 def attn_decode8(out, q, kv, batch, nq: int, nkv: int, hd: int, scale: float, cap: float, window: int, sinks=None,
                  keep: int = 0) -> None:
     """Decode attention over a cache of 8 bits (``window`` < 0: a chunk of that many positions; ``keep``: beside a window,
-    the first tokens that stay visible).  Rows of queries that do not begin on 16 bytes are copied first."""
+    the first tokens that stay visible).  Rows of queries that do not begin on 16 bytes are copied first.  Pages but the one of a
+    sequence's newest token are read before the kernel in front is complete: no earlier row may be among what that one writes
+    (:func:`store_kv8` of more tokens than sequences is complete before anything behind it starts)."""
     B = _decode_rows("attn_decode8", out, q, batch, nq, hd, sinks)
     n_pages = _cache8_pages(kv, nkv, hd, "attn_decode8")
     table, slots, lens = kv.page_table, batch.slots, batch.len_after
@@ -1200,7 +1203,8 @@ def attn_decode_shared_supported(dtype, hd: int, n_seqs: int) -> bool:
 def attn_decode_shared(out, q, kv, batch, nq: int, nkv: int, hd: int, scale: float, cap: float, lead, pages, most_pages: int,
                        sinks=None, gate=None) -> None:
     """Decode attention (all keys visible) of sequences that share their first pages: row b's first ``pages[b]`` cache pages
-    are those of row ``lead[b]`` (int32 [B] each; rows that share nothing: 0 pages), ``most_pages`` the most that any row shares."""
+    are those of row ``lead[b]`` (int32 [B] each; rows that share nothing: 0 pages), ``most_pages`` the most that any row shares.  As in :func:`attn_decode8`, rows
+    but the newest are read before the kernel in front is complete."""
     B = batch.n_seqs
     if lead.numel() != B or pages.numel() != B or most_pages < 0:
         raise KernelError(f"attn_decode_shared: a lead and a number of pages for each of {B} rows")

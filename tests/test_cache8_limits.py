@@ -205,6 +205,66 @@ def test_a_refused_call_leaves_no_plan(K, monkeypatch, shared):
     assert lib.made == [True, True, False] and len(b.aux) == 1
 
 
+# ---------------------------------------------------------------------------------------------- one behind the other
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rotates", [False, True])
+def test_layers_of_stores_of_many_tokens_and_attention(K, rotates):
+    """A store of many tokens directly in front of the attention that reads them, in layers that share one step's plan: the bits that
+    the same calls give one at a time (a store of more tokens than sequences is complete before the attention starts)."""
+    nq, nkv, hd, layers, lens = 4, 2, 128, 8, [1500, 700, 64, 2000]
+    T = sum(lens)
+    t = lambda v: torch.tensor(v, dtype=torch.int32, device=DEV)
+    views = [View(lens, nkv, hd).to(DEV) for _ in range(layers)]
+    for v in views:                                       # (one group of layers: the same table and slots)
+        v.page_table, v.order = views[0].page_table, views[0].order
+    store = SimpleNamespace(positions=t([p for n in lens for p in range(n)]), seq_of_token=t([i for i, n in enumerate(lens) for _ in range(n)]),
+                            slots=t(views[0].order), len_after=t(lens))
+    x = [torch.randn(T, (nq + 2 * nkv) * hd, device=DEV).to(torch.bfloat16) for _ in range(layers)]
+    q = torch.randn(4, nq * hd, device=DEV).to(torch.bfloat16)
+    inv = torch.zeros(hd // 2, device=DEV)                # (a rotation by nothing)
+
+    def run(apart):
+        outs = torch.empty(layers, 4, nq * hd, dtype=torch.bfloat16, device=DEV)
+        b = step(views[0], lens, DEV)
+        for v in views:
+            v.k.view(torch.uint8).zero_(), v.v.view(torch.uint8).zero_(), v.k_exp.fill_(100), v.v_exp.fill_(100)
+        K.attn_decode(outs[0], q, views[0], b, nq, nkv, hd, 0.1, 0.0, 0)          # (the plan)
+        for i, v in enumerate(views):
+            if rotates:
+                K.rope_store_kv8(x[i].clone(), store, inv, nq, nkv, hd, hd, "half", v)
+            else:
+                K.store_kv8(x[i], store, nq, nkv, hd, v)
+            if apart:
+                torch.cuda.synchronize()
+            K.attn_decode(outs[i], q, v, b, nq, nkv, hd, 0.1, 0.0, 0)
+        return outs
+
+    want = run(True)
+    for _ in range(30):
+        assert torch.equal(run(False), want)
+    K.check_device_errors(DEV)
+
+
+def test_stores_say_how_many_sequences_they_are_of(K, monkeypatch):
+    """The entries learn the number of sequences, by which a store of more tokens lets nothing start before it is complete."""
+    said = []
+
+    class Lib:
+        def __getattr__(self, name):
+            return lambda block: said.append(ctypes.cast(block, ctypes.POINTER(ctypes.c_longlong))[{"af_store_kv8": 22, "af_rope_store_kv8": 26}[name]]) or 0
+
+    for name, fake in (("_lib", Lib), ("_here", lambda *a: 0), ("_raw_stream", lambda d: 0)):
+        monkeypatch.setattr(K, name, fake)
+    view = View([70, 5, 9], 2, 64).to("cpu")
+    t = lambda v: torch.tensor(v, dtype=torch.int32)
+    b = SimpleNamespace(positions=t([1] * 7), seq_of_token=t([0] * 7), slots=t(view.order), len_after=t([70, 5, 9]))
+    x = torch.zeros(7, 8 * 64, dtype=torch.bfloat16)
+    K.store_kv8(x, b, 4, 2, 64, view)
+    K.rope_store_kv8(x, b, torch.ones(32), 4, 2, 64, 64, "half", view)
+    assert said == [3, 3]
+
+
 # ---------------------------------------------------------------------------------------------- beyond the page table
 
 @pytest.mark.gpu
