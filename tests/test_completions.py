@@ -602,6 +602,38 @@ def test_engine_with_a_cache_of_8_bits(tmp_path, monkeypatch, name):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("module,name", [("banitar", "B"), ("banitar", "C"), ("banitar", "F"), ("fiferax", "B"), ("fiferax", "C"), ("retudra", "B"),
+                                         ("retudra", "E"), ("zatasun", "B")])
+def test_the_other_architectures_with_a_cache_of_8_bits(tmp_path, monkeypatch, module, name):
+    """Attention with norms of queries and keys, gates, sinks, biases, chunks, kept first tokens, padded heads and stretched rotations, beside
+    latent attention and states: a prompt in one step against single tokens, captured steps against ones kernel by kernel, and forks (shared
+    pages where a layer keeps all keys).  A router may choose other experts for a token whose row differs in its last bit: a tenth of the
+    positions may be such."""
+    import importlib
+    from airframe_b200 import kernels
+    from airframe_b200.engine import GpuRuntime
+    mod = importlib.import_module("tiny_" + module)
+    rt = GpuRuntime.load(mod.make_folder(mod.CONFIGS[name], seed=5, root=tmp_path), max_tokens=64 * 40, kv_dtype="float8_e4m3")
+    eng = rt.engine
+    assert any(g.need.eight_bits for g in eng.cache.groups.values())
+    ids = replay.random_ids(rt.model.spec.vocab_size, 330, 3)
+    whole = replay.run_whole(rt, ids)
+    tail = replay.run_tail(rt, ids, 100)
+
+    def near(got, ref):
+        each = (got.double() - ref.double()).abs().amax(1) / ref.double().abs().max()
+        assert float(each.quantile(0.9)) < BF16_SPLITS
+
+    near(tail, whole)
+    eng.use_graphs = False
+    assert torch.equal(replay.run_tail(rt, ids, 100), tail)
+    eng.use_graphs = rt.model.graph_safe
+    monkeypatch.setattr(kernels, "attn_decode_shared_pays", lambda *a: True)
+    for g in _forked(rt, ids[:200], [ids[200:230], ids[200:260], ids[200:]]):
+        near(g, whole[200: 200 + len(g)])
+
+
+@pytest.mark.gpu
 def test_completions_of_a_prompt(tmp_path, monkeypatch):
     """The same tokens as so many requests of their own (whose generators are seeded alike), greedy and drawn; prompt steps once."""
     from airframe_b200 import kernels
