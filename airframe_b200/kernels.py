@@ -1059,7 +1059,8 @@ def attn_decode(out, q, kv, batch, nq, nkv, hd, scale, cap, window, slopes=None,
     """Attention of a decode step over the cache: the split kernel for
     bfloat16 and head sizes it takes (a chunked mask goes to it as a negative window, a gate follows it as a
     kernel of its own), else the plain kernel (which also serves scores with a per-head slope, values of another
-    size than the keys or inside them, and sinks).  A cache of 8 bits has its own (:func:`attn_decode8`)."""
+    size than the keys or inside them, and sinks).  A cache of 8 bits has its own (:func:`attn_decode8`).  The split kernel
+    reads all pages but the newest token's before the kernel in front is complete: that one may write no earlier row."""
     # values that lie inside their key rows: the split kernel takes the key pages for the value pages too and gives
     # whole key-sized rows back, of which the caller (who asked for it with an `out` that wide) reads the values' part
     keep = kv_keep(kv)
